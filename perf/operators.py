@@ -330,7 +330,9 @@ def _plain_route(s):
     # ranked by score + bias; without a bias by the logit, which orders alike
     choice = x if s["bias"] is None else torch.where(x == NEG, NEG, score + s["bias"])
     if g > 1:
-        best = choice.view(t, g, e // g).sort(dim=2, descending=True).values[:, :, :c["best"]]
+        # a group's worth is its best choice, or its two best scores (+ bias) together
+        value = choice if c["best"] == 1 or s["bias"] is not None else torch.where(x == NEG, NEG, score)
+        best = value.view(t, g, e // g).sort(dim=2, descending=True).values[:, :, :c["best"]]
         rank = torch.where(best[:, :, 0] == NEG, NEG, torch.where(best == NEG, 0.0, best).sum(dim=2))
         keep = rank.sort(dim=1, descending=True, stable=True).indices[:, :c["top_groups"]]
         kept = torch.zeros((t, g), dtype=torch.bool, device=DEV).scatter_(1, keep, True)
@@ -474,7 +476,8 @@ def _exact_route(s, c):
     rank = z if s["bias"] is None else prob + s["bias"].double()
     rank = rank.masked_fill(dead, NEG)
     if c["groups"] > 1:
-        parts = rank.reshape(z.shape[0], c["groups"], -1)
+        parts = prob.masked_fill(dead, NEG) if c["best"] == 2 and s["bias"] is None else rank
+        parts = parts.reshape(z.shape[0], c["groups"], -1)
         best = parts.topk(c["best"], dim=2).values
         total = best.masked_fill(best == NEG, 0.0).sum(dim=2).masked_fill(best[..., 0] == NEG, NEG)
         # lowest group first among equal ones: as many groups beat it as rank before it
