@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define MXGG_ABI_VERSION 13
+#define MXGG_ABI_VERSION 14
 
 typedef enum mxgg_status {
   MXGG_OK = 0,
@@ -552,6 +552,49 @@ int mxgg_combine(const void* y, int64_t rows, int64_t cols, int64_t ldy, const i
 int mxgg_combine_score_grad(const void* grad_out, int64_t ldg, const void* y, int64_t rows,
                             int64_t cols, int64_t ldy, const int32_t* perm, int64_t tokens,
                             int64_t topk, float* grad_scores, void* stream);
+
+/*
+ * Routing decision of a MoE layer (the expert ids that mxgg_route_plan sorts and
+ * the weights that mxgg_combine applies), from the router's logits x [tokens,
+ * experts] (row-major without gaps, element type `dtype`; an mxgg_out_dtype):
+ *   s = 1 / (1 + exp(-x)) (SIGMOID) or softmax(x) over the row (SOFTMAX), fp32
+ *   c = s + bias[e]; without a bias c = x, which orders the experts as s does
+ *   With groups > 1, `groups` runs of experts/groups experts: a group's worth is
+ *   its best c (group_best 1) or the sum of its two best s (+ bias)
+ *   (group_best 2; of its only one left, that one); only experts of the
+ *   top_groups best groups can be chosen.
+ *   expert_idx[t][k] : the expert of the k-th largest c; equal c, and equal
+ *                      groups, in index order; a NaN ranks above every number
+ *   weights[t][k]    : scale * s, with `renormalize` scale * s / sum over the
+ *                      row's chosen s (0 where that sum is 0)
+ * An expert with x = -inf or c = -inf cannot be chosen; a slot with no expert
+ * left has id -1 (dropped by mxgg_route_plan) and weight 0.
+ *   selected         : fp32 [tokens, topk] for mxgg_route_topk_grad, or NULL
+ * experts <= 1024, topk <= 32 and <= experts, groups <= 64 dividing experts.
+ * `options` is host memory, read during the call.
+ */
+typedef enum mxgg_route_score { MXGG_SCORE_SOFTMAX = 0, MXGG_SCORE_SIGMOID = 1 } mxgg_route_score;
+
+typedef struct mxgg_route_options {
+  int64_t experts, topk, groups, top_groups;
+  int32_t score, dtype, group_best, renormalize;
+  float scale;
+} mxgg_route_options;
+
+int mxgg_route_topk(const void* logits, int64_t tokens, const float* bias,
+                    const mxgg_route_options* options, int32_t* expert_idx, float* weights,
+                    float* selected, void* stream);
+
+/*
+ * Gradient of mxgg_route_topk's weights with respect to the logits: from
+ * grad_weights fp32 [tokens, topk] and the forward's expert_idx and selected,
+ * grad_logits [tokens, experts] (element type `dtype`, every element written).
+ * The choice itself and the bias have no gradient.  logits are read for SOFTMAX
+ * without `renormalize` only (NULL otherwise allowed).
+ */
+int mxgg_route_topk_grad(const float* grad_weights, const int32_t* expert_idx,
+                         const float* selected, const void* logits, int64_t tokens,
+                         const mxgg_route_options* options, void* grad_logits, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1008,4 +1008,85 @@ int mxgg_combine_score_grad(const void* grad_out, int64_t ldg, const void* y, in
       "combine_score_grad");
 }
 
+static int check_route_options(const char* what, int64_t tokens, const mxgg_route_options* o) {
+  if (!o) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null options", what);
+  if (tokens < 0 || o->experts < 1 || o->topk < 1 || o->topk > o->experts)
+    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld, experts=%lld, topk=%lld", what,
+                     (long long)tokens, (long long)o->experts, (long long)o->topk);
+  if (o->experts > kMaxGroupsAbi || o->topk > 32)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: experts=%lld above %lld or topk=%lld above 32",
+                     what, (long long)o->experts, (long long)kMaxGroupsAbi, (long long)o->topk);
+  if (o->groups < 1 || o->groups > 64 || o->experts % o->groups != 0 || o->top_groups < 1 ||
+      o->top_groups > o->groups)
+    return set_error(MXGG_ERR_SHAPE,
+                     "%s: groups=%lld must divide the experts, with 1 <= top_groups=%lld <= groups "
+                     "<= 64",
+                     what, (long long)o->groups, (long long)o->top_groups);
+  if ((o->score != MXGG_SCORE_SOFTMAX && o->score != MXGG_SCORE_SIGMOID) ||
+      (o->dtype != MXGG_OUT_BF16 && o->dtype != MXGG_OUT_F32) ||
+      (o->group_best != 1 && o->group_best != 2))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: score=%d, dtype=%d, group_best=%d", what,
+                     o->score, o->dtype, o->group_best);
+  // one workgroup per token at worst, below the grid's 2^32 work-items; element
+  // offsets are 64-bit
+  if (tokens >= INT64_C(1) << 24)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: tokens above 2^24", what);
+  return MXGG_OK;
+}
+
+int mxgg_route_topk(const void* logits, int64_t tokens, const float* bias,
+                    const mxgg_route_options* options, int32_t* expert_idx, float* weights,
+                    float* selected, void* stream) {
+  const int rc = check_route_options("route_topk", tokens, options);
+  if (rc != MXGG_OK) return rc;
+  if (tokens == 0) return MXGG_OK;
+  if (!logits || !expert_idx || !weights)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "route_topk: null pointer");
+  const mxgg_route_options& o = *options;
+  RouteTopkArgs a{};
+  a.logits = logits;
+  a.bias = bias;
+  a.idx = expert_idx;
+  a.weights = weights;
+  a.sel = selected;
+  a.tokens = tokens;
+  a.E = (int32_t)o.experts;
+  a.K = (int32_t)o.topk;
+  a.groups = (int32_t)o.groups;
+  a.top_groups = (int32_t)o.top_groups;
+  a.group_best = o.group_best;
+  a.softmax = o.score == MXGG_SCORE_SOFTMAX;
+  a.renorm = o.renormalize != 0;
+  a.bf16 = o.dtype == MXGG_OUT_BF16;
+  a.scale = o.scale;
+  return check_launch(launch_route_topk(a, static_cast<hipStream_t>(stream)), "route_topk");
+}
+
+int mxgg_route_topk_grad(const float* grad_weights, const int32_t* expert_idx,
+                         const float* selected, const void* logits, int64_t tokens,
+                         const mxgg_route_options* options, void* grad_logits, void* stream) {
+  const int rc = check_route_options("route_topk_grad", tokens, options);
+  if (rc != MXGG_OK) return rc;
+  if (tokens == 0) return MXGG_OK;
+  const mxgg_route_options& o = *options;
+  const bool whole = o.score == MXGG_SCORE_SOFTMAX && !o.renormalize;
+  if (!grad_weights || !expert_idx || !selected || !grad_logits || (whole && !logits))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "route_topk_grad: null pointer");
+  RouteTopkGradArgs a{};
+  a.logits = logits;
+  a.idx = expert_idx;
+  a.sel = selected;
+  a.dweights = grad_weights;
+  a.dlogits = grad_logits;
+  a.tokens = tokens;
+  a.E = (int32_t)o.experts;
+  a.K = (int32_t)o.topk;
+  a.softmax = o.score == MXGG_SCORE_SOFTMAX;
+  a.renorm = o.renormalize != 0;
+  a.bf16 = o.dtype == MXGG_OUT_BF16;
+  a.scale = o.scale;
+  return check_launch(launch_route_topk_grad(a, static_cast<hipStream_t>(stream)),
+                      "route_topk_grad");
+}
+
 }  // extern "C"

@@ -112,6 +112,35 @@ hipError_t launch_combine_score_grad(const uint16_t* dout, int64_t ldd, const ui
                                      int64_t tokens, int topk, int64_t cols, float* dscore,
                                      hipStream_t stream);
 
+// Routing decision (topk.hip).  The launchers fill in the fields after `scale`.
+struct RouteTopkArgs {
+  const void* logits;  // [tokens][E], fp32 or bf16
+  const float* bias;   // [E] or nullptr
+  int32_t* idx;        // [tokens][K]
+  float* weights;      // [tokens][K]
+  float* sel;          // [tokens][K] or nullptr: what the gradient needs of the scores
+  int64_t tokens;
+  int32_t E, K, groups, top_groups, group_best;
+  int32_t softmax, renorm, bf16;
+  float scale;
+  int32_t lanes, lanes_group;  // lanes of a token and of a group (powers of two)
+  uint32_t k_recip;
+};
+hipError_t launch_route_topk(RouteTopkArgs args, hipStream_t stream);
+struct RouteTopkGradArgs {
+  const void* logits;  // [tokens][E], read for softmax without renormalisation only
+  const int32_t* idx;
+  const float* sel;
+  const float* dweights;
+  void* dlogits;       // [tokens][E]
+  int64_t tokens;
+  int32_t E, K, softmax, renorm, bf16;
+  float scale;
+  int32_t tokens_wave;
+  uint32_t k_recip;
+};
+hipError_t launch_route_topk_grad(RouteTopkGradArgs args, hipStream_t stream);
+
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,
                                int32_t* ends, hipStream_t stream);

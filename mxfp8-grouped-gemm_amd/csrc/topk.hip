@@ -1,0 +1,469 @@
+// Routing decision of a MoE layer: which experts every token goes to, with
+// which weights, and the gradient of the weights with respect to the logits.
+//
+//   s = 1 / (1 + exp(-x))  or  softmax(x) over the token's experts (fp32)
+//   c = s + bias; without a bias c = x, which orders experts as s does
+//   groups of experts/groups consecutive experts: a group's worth is its best c,
+//   or the sum of its two best s (+ bias); the top_groups best groups stay
+//   the topk experts of largest c in them, largest first, ties (also between
+//   groups) to the lowest index; a NaN c ranks above every number
+//   weights: scale * s, or scale * s / (sum of the selected s); for softmax the
+//   latter is the softmax over the selected logits alone (the row's sum cancels)
+// An expert with c = -inf (or x = -inf) is out of the choice; a slot that no
+// expert is left for gets id -1 and weight 0.
+//
+// Selection: c becomes a sortable 32-bit integer, packed with the inverted
+// expert index into the mantissa of a double in [1, 2): one v_max_f64 then
+// compares key and index together, at the full rate of the vector unit, and no
+// two keys are equal.  A token is held by 2^k lanes of VPL experts each; every
+// lane sorts its keys in registers down to the L largest and log2(lanes)
+// butterfly steps merge the sorted lists (L max and a bitonic clean each).
+#include <algorithm>
+
+#include "mx_device.h"
+#include "mxgg_internal.h"
+
+namespace mxgg {
+namespace {
+
+constexpr int kTopkThreads = 256;
+constexpr int kTopkWaves = kTopkThreads / 64;
+constexpr int kGradTile = 2048;  // gradients of a wave's tile, at most
+
+// LDS index with one word of padding every 32: lanes that walk rows of 32 words
+// in step fall on different banks.
+__host__ __device__ constexpr int pad32(int i) { return i + (i >> 5); }
+
+// LDS writes of this wave's lanes before, reads of other lanes' words after.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr float kNegInf = -__builtin_inff();
+
+// Order of fp32 values as unsigned integers; NaN above all, -0 with +0.
+__device__ __forceinline__ uint32_t sortable(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 0xFFFFFFFFu : k;
+}
+__device__ __forceinline__ float unsortable(uint32_t k) {
+  return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
+}
+
+// Key and index as a double in [1, 2); 0.0 = absent.
+constexpr uint32_t kIndexMask = 1023u;
+static_assert(kMaxGroups <= (int)kIndexMask + 1, "an expert index takes ten bits");
+__device__ __forceinline__ double pack_key(uint32_t key, uint32_t idx) {
+  const uint64_t b =
+      ((uint64_t)(0x3FF00000u | (key >> 12)) << 32) | (key << 20) | (kIndexMask - idx);
+  return __builtin_bit_cast(double, b);
+}
+__device__ __forceinline__ uint32_t key_of(double d) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, d);
+  return (uint32_t)(b >> 32) << 12 | (uint32_t)b >> 20;
+}
+__device__ __forceinline__ int index_of(double d) {
+  return (int)(kIndexMask - ((uint32_t)__builtin_bit_cast(uint64_t, d) & kIndexMask));
+}
+
+// Plain v_max_f64 / v_min_f64: the keys are ordinary numbers, so the
+// canonicalising steps that fmax would add are left out.
+__device__ __forceinline__ double dmax(double a, double b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ double dmin(double a, double b) {
+  double r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ void exchange(double& hi, double& lo) {
+  const double a = dmax(hi, lo);
+  lo = dmin(hi, lo);
+  hi = a;
+}
+
+// Batcher's odd-even merge sort of a[LO .. LO + N), descending: N = 8 takes 19
+// exchanges, 16 63, 32 191.
+template <int LO, int N, int R, int TOTAL>
+__device__ __forceinline__ void merge_net(double (&a)[TOTAL]) {
+  if constexpr (2 * R < N) {
+    merge_net<LO, N, 2 * R>(a);
+    merge_net<LO + R, N, 2 * R>(a);
+#pragma unroll
+    for (int i = LO + R; i + R < LO + N; i += 2 * R) exchange(a[i], a[i + R]);
+  } else {
+    exchange(a[LO], a[LO + R]);
+  }
+}
+template <int LO, int N, int TOTAL>
+__device__ __forceinline__ void sort_net(double (&a)[TOTAL]) {
+  if constexpr (N > 1) {
+    sort_net<LO, N / 2>(a);
+    sort_net<LO + N / 2, N / 2>(a);
+    merge_net<LO, N, 1>(a);
+  }
+}
+// The L largest of two descending lists, descending.
+template <int L>
+__device__ __forceinline__ void merge_top(double (&a)[L], const double (&b)[L]) {
+#pragma unroll
+  for (int i = 0; i < L; ++i) a[i] = dmax(a[i], b[L - 1 - i]);
+#pragma unroll
+  for (int k = L / 2; k >= 1; k >>= 1)
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if ((i & k) == 0) exchange(a[i], a[i + k]);
+}
+
+__device__ __forceinline__ double shfl_xor_f64(double v, int off) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, off);
+  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(b >> 32), off);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+// The list of the L largest over this lane and lane ^ off.
+template <int L>
+__device__ __forceinline__ void merge_lanes(double (&a)[L], int off) {
+  double b[L];
+#pragma unroll
+  for (int i = 0; i < L; ++i) b[i] = shfl_xor_f64(a[i], off);
+  merge_top<L>(a, b);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const uint16_t* p) { return bf16_bits_to_f32(*p); }
+__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(uint16_t* p, float v) {
+  *p = (uint16_t)pack_bf16x2(v, 0.0f);
+}
+
+// Four consecutive values, at any alignment of an element.
+struct RawF32 {
+  float v[4];
+  __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 16); }
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+};
+struct RawBf16 {
+  uint32_t v[2];
+  __device__ __forceinline__ void load(const uint16_t* p) { __builtin_memcpy(v, p, 8); }
+  __device__ __forceinline__ float get(int i) const {
+    return (i & 1) ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]);
+  }
+};
+__device__ __forceinline__ RawF32 raw4(const float*) { return RawF32{}; }
+__device__ __forceinline__ RawBf16 raw4(const uint16_t*) { return RawBf16{}; }
+__device__ __forceinline__ void store4(float* p, const float4& q) { __builtin_memcpy(p, &q, 16); }
+__device__ __forceinline__ void store4(uint16_t* p, const float4& q) {
+  const uint32_t w[2] = {pack_bf16x2(q.x, q.y), pack_bf16x2(q.z, q.w)};
+  __builtin_memcpy(p, w, 8);
+}
+
+// n <= MAX consecutive logits into a wave's padded LDS tile: all loads first.
+template <int MAX, typename T>
+__device__ __forceinline__ void load_tile(const T* __restrict__ x, int n, float* tile) {
+  const int lane = threadIdx.x & 63;
+  constexpr int kLoads = (MAX + 255) / 256;
+  decltype(raw4(x)) c[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int i = 4 * (lane + 64 * j);
+    if (i + 4 <= n) c[j].load(x + i);
+  }
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int i = 4 * (lane + 64 * j);
+    if (i + 4 <= n) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) tile[pad32(i) + u] = c[j].get(u);  // within one run of 32
+    } else {
+      for (int u = i; u < n; ++u) tile[pad32(u)] = load_one(x + u);
+    }
+  }
+}
+
+// p / K for p < 2048 and K <= 32, from recip = ceil(2^20 / K).
+__device__ __forceinline__ int div_k(int p, uint32_t recip) {
+  return (int)(((uint32_t)p * recip) >> 20);
+}
+
+template <int VPL, int L, typename T>
+__global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
+  static_assert(VPL >= L, "a lane's list is cut from its own experts");
+  __shared__ float tiles[kTopkWaves][pad32(64 * VPL)];
+  __shared__ float bias_s[pad32(kMaxGroups)];
+  __shared__ float2 stats[kTopkWaves][64];       // softmax maximum and sum of a token
+  __shared__ int32_t picked[kTopkWaves][64 * L];
+  __shared__ float value[kTopkWaves][64 * L];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per_wave = 64 / a.lanes;
+  const int64_t t0 = ((int64_t)blockIdx.x * kTopkWaves + wave) * per_wave;
+  const int nt = (int)std::min<int64_t>(per_wave, std::max<int64_t>(0, a.tokens - t0));
+  float* tile = tiles[wave];
+  load_tile<64 * VPL, T>(static_cast<const T*>(a.logits) + t0 * a.E, nt * a.E, tile);
+  if (a.bias != nullptr)
+    for (int e = tid; e < a.E; e += kTopkThreads) bias_s[pad32(e)] = a.bias[e];
+  __syncthreads();
+  if (nt == 0) return;
+
+  // this lane's experts: VPL of group g, from offset o in it
+  const int tok = lane / a.lanes, sub = lane & (a.lanes - 1);
+  const int per = a.E / a.groups;
+  const int g = sub / a.lanes_group, o = (sub & (a.lanes_group - 1)) * VPL;
+  const int count = tok < nt && g < a.groups ? min(max(per - o, 0), VPL) : 0;
+  const int e0 = g * per + o;
+  float x[VPL];
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) x[v] = v < count ? tile[pad32(tok * a.E + e0 + v)] : kNegInf;
+
+  // softmax statistics of the whole row, where the choice or the weights need them
+  float top = 0.0f, total = 1.0f;
+  const bool sums = a.groups > 1 && a.group_best == 2;
+  if (a.softmax && (a.bias != nullptr || !a.renorm || sums)) {
+    top = kNegInf;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) top = __builtin_fmaxf(top, x[v]);
+    for (int off = 1; off < a.lanes; off <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, off));
+    if (top == kNegInf) top = 0.0f;
+    total = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) total += expf(x[v] - top);
+    for (int off = 1; off < a.lanes; off <<= 1) total += __shfl_xor(total, off);
+    if (total == 0.0f) total = 1.0f;  // every expert is out
+    if (sub == 0) stats[wave][tok] = make_float2(top, total);
+  }
+
+  // choice keys, and the L largest of the lane
+  double list[L];
+  {
+    double key[VPL];
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      float c = x[v];
+      if (a.bias != nullptr && v < count) {
+        const float s = a.softmax ? expf(c - top) / total : sigmoid(c);
+        c = c == kNegInf ? c : s + bias_s[pad32(e0 + v)];
+      }
+      key[v] = c == kNegInf ? 0.0 : pack_key(sortable(c), (uint32_t)(e0 + v));
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i) list[i] = key[i];
+    sort_net<0, L>(list);
+#pragma unroll
+    for (int v0 = L; v0 < VPL; v0 += L) {
+      double more[L];
+#pragma unroll
+      for (int i = 0; i < L; ++i) more[i] = key[v0 + i];
+      sort_net<0, L>(more);
+      merge_top<L>(list, more);
+    }
+  }
+  for (int off = 1; off < a.lanes_group; off <<= 1) merge_lanes<L>(list, off);
+
+  // groups: the list now holds the group's best; rank its worth among the token's
+  if (a.groups > 1) {
+    uint32_t worth = key_of(list[0]);
+    if (sums) {
+      float w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[i] = unsortable(key_of(list[i]));
+        if (a.bias == nullptr) w[i] = a.softmax ? expf(w[i] - top) / total : sigmoid(w[i]);
+        if (list[i] == 0.0) w[i] = 0.0f;
+      }
+      worth = sortable(w[0] + w[1]);
+    }
+    const double mine = list[0] == 0.0 ? 0.0 : pack_key(worth, (uint32_t)g);
+    int above = 0;
+    for (int off = a.lanes_group; off < a.lanes; off += a.lanes_group)
+      above += shfl_xor_f64(mine, off) > mine ? 1 : 0;
+    if (above >= a.top_groups) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) list[i] = 0.0;
+    }
+    for (int off = a.lanes_group; off < a.lanes; off <<= 1) merge_lanes<L>(list, off);
+  }
+
+  // weights: one (token, slot) a lane, sums over a token's slots in slot order
+  int32_t* pk = picked[wave];
+  float* val = value[wave];
+  if (sub == 0 && tok < nt) {
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (i < a.K) pk[tok * a.K + i] = list[i] == 0.0 ? -1 : index_of(list[i]);
+  }
+  wave_sync();
+  const int slots = nt * a.K;
+  for (int p = lane; p < slots; p += 64) {
+    const int t = div_k(p, a.k_recip), e = pk[p];
+    const float* row_x = tile;
+    float s = 0.0f;
+    if (e >= 0) {
+      const float xe = row_x[pad32(t * a.E + e)];
+      if (!a.softmax) {
+        s = sigmoid(xe);
+      } else if (!a.renorm) {
+        s = expf(xe - stats[wave][t].x) / stats[wave][t].y;
+      } else {
+        // relative to the largest selected logit: the first slot's without a bias
+        float m = row_x[pad32(t * a.E + pk[t * a.K])];
+        if (a.bias != nullptr)
+          for (int j = 1; j < a.K; ++j) {
+            const int ej = pk[t * a.K + j];
+            if (ej >= 0) m = __builtin_fmaxf(m, row_x[pad32(t * a.E + ej)]);
+          }
+        s = expf(xe - m);
+      }
+    }
+    val[p] = s;
+  }
+  wave_sync();
+  for (int p = lane; p < slots; p += 64) {
+    const int t = div_k(p, a.k_recip);
+    float w = val[p], s = w;
+    if (a.renorm) {
+      float sum = 0.0f;
+      for (int j = 0; j < a.K; ++j) sum += val[t * a.K + j];
+      w = sum == 0.0f ? 0.0f : w / sum;
+      if (a.softmax) s = w;
+    }
+    const int64_t at = t0 * a.K + p;
+    a.idx[at] = pk[p];
+    a.weights[at] = a.scale * w;
+    if (a.sel != nullptr) a.sel[at] = s;
+  }
+}
+
+// Gradient of the weights: dw [tokens][K] -> d logits [tokens][E].
+//   sigmoid        : dx = ds s (1 - s), zero for experts not selected
+//   softmax, renorm: dx = p (dp - sum p dp) over the selected, zero elsewhere
+//   softmax alone  : dx = p (dp - sum p dp) over the whole row (p from the logits)
+// with ds = scale dw, or scale (dw - sum dw s / S) / S where s is divided by its
+// sum S over the slots.  A wave takes NT whole tokens: the rows are put together
+// in LDS from the slots and leave as one run of memory.
+template <typename T>
+__global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradArgs a) {
+  __shared__ float grad_s[kTopkWaves][kGradTile];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t0 = ((int64_t)blockIdx.x * kTopkWaves + wave) * a.tokens_wave;
+  const int nt = (int)std::min<int64_t>(a.tokens_wave, std::max<int64_t>(0, a.tokens - t0));
+  if (nt == 0) return;
+  float* grad = grad_s[wave];
+  const int n = nt * a.E, slots = nt * a.K;
+  for (int i = 4 * lane; i < n; i += 256)
+    *reinterpret_cast<float4*>(grad + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  wave_sync();
+  const int32_t* idx = a.idx + t0 * a.K;
+  const float* sel = a.sel + t0 * a.K;
+  const float* dw = a.dweights + t0 * a.K;
+  for (int p = lane; p < slots; p += 64) {
+    const int t = div_k(p, a.k_recip), e = idx[p];
+    if ((uint32_t)e >= (uint32_t)a.E) continue;
+    const float s = sel[p];
+    float d = dw[p], g;
+    if (a.renorm || a.softmax) {
+      float dot = 0.0f, sum = 0.0f;
+      for (int j = 0; j < a.K; ++j) {
+        const int q = t * a.K + j;
+        if ((uint32_t)idx[q] < (uint32_t)a.E) {
+          dot += sel[q] * dw[q];
+          sum += sel[q];
+        }
+      }
+      if (a.softmax)
+        g = a.scale * (a.renorm ? s * (d - dot) : d);
+      else
+        g = sum == 0.0f ? 0.0f : a.scale * (d - dot / sum) / sum * s * (1.0f - s);
+    } else {
+      g = a.scale * d * s * (1.0f - s);
+    }
+    grad[t * a.E + e] = g;
+  }
+  wave_sync();
+  if (a.softmax && !a.renorm) {
+    const int lanes = 64 / a.tokens_wave, t = lane / lanes, sub = lane & (lanes - 1);
+    const T* x = static_cast<const T*>(a.logits) + (t0 + t) * a.E;
+    if (t < nt) {
+      float top = kNegInf, total = 0.0f, dot = 0.0f;
+      for (int e = sub; e < a.E; e += lanes) top = __builtin_fmaxf(top, load_one(x + e));
+      for (int off = 1; off < lanes; off <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, off));
+      if (top == kNegInf) top = 0.0f;
+      for (int e = sub; e < a.E; e += lanes) total += expf(load_one(x + e) - top);
+      for (int off = 1; off < lanes; off <<= 1) total += __shfl_xor(total, off);
+      if (total == 0.0f) total = 1.0f;
+      for (int j = 0; j < a.K; ++j) {
+        const int q = t * a.K + j;
+        if ((uint32_t)idx[q] < (uint32_t)a.E) dot += sel[q] * a.scale * dw[q];
+      }
+      for (int e = sub; e < a.E; e += lanes) {
+        const float p = expf(load_one(x + e) - top) / total;
+        grad[t * a.E + e] = p * (grad[t * a.E + e] - dot);
+      }
+    }
+    wave_sync();
+  }
+  T* out = static_cast<T*>(a.dlogits) + t0 * a.E;
+  for (int i = 4 * lane; i < n; i += 256) {
+    if (i + 4 <= n)
+      store4(out + i, *reinterpret_cast<const float4*>(grad + i));
+    else
+      for (int u = i; u < n; ++u) store_one(out + u, grad[u]);
+  }
+}
+
+int next_pow2(int v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+
+template <int VPL, int L, typename T>
+hipError_t run_topk(RouteTopkArgs a, hipStream_t stream) {
+  const int per = a.E / a.groups;
+  a.lanes_group = next_pow2((per + VPL - 1) / VPL);
+  a.lanes = a.lanes_group * next_pow2(a.groups);
+  const int64_t tokens = (int64_t)kTopkWaves * (64 / a.lanes);
+  hipLaunchKernelGGL((k_route_topk<VPL, L, T>), dim3((unsigned)((a.tokens + tokens - 1) / tokens)),
+                     dim3(kTopkThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_topk_list(const RouteTopkArgs& a, hipStream_t stream) {
+  if (a.K <= 8) return run_topk<32, 8, T>(a, stream);
+  if (a.K <= 16) return run_topk<32, 16, T>(a, stream);
+  return run_topk<32, 32, T>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_route_topk(RouteTopkArgs a, hipStream_t stream) {
+  if (a.tokens == 0) return hipSuccess;
+  a.k_recip = (uint32_t)(((1u << 20) + a.K - 1) / a.K);
+  return a.bf16 ? run_topk_list<uint16_t>(a, stream) : run_topk_list<float>(a, stream);
+}
+
+hipError_t launch_route_topk_grad(RouteTopkGradArgs a, hipStream_t stream) {
+  if (a.tokens == 0) return hipSuccess;
+  a.k_recip = (uint32_t)(((1u << 20) + a.K - 1) / a.K);
+  // whole tokens a wave: as many as its LDS tile holds, a power of two
+  a.tokens_wave = 64;
+  while (a.tokens_wave * a.E > kGradTile) a.tokens_wave >>= 1;
+  const int64_t tokens = (int64_t)kTopkWaves * a.tokens_wave;
+  const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens));
+  if (a.bf16)
+    hipLaunchKernelGGL((k_route_topk_grad<uint16_t>), grid, dim3(kTopkThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_route_topk_grad<float>), grid, dim3(kTopkThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace mxgg

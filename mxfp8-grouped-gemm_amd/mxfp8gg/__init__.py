@@ -43,12 +43,14 @@ from .autograd import (
 )
 from .routing import (
     RoutePlan,
+    RouteTopK,
     combine,
     combine_score_grad,
     gather_rows,
     gather_to_mxfp8_dual,
     gather_to_mxfp8_dim0,
     route_plan,
+    route_topk,
 )
 from .torchao_compat import (
     apply,
@@ -70,7 +72,7 @@ __all__ = [
     "triton_mxfp8_grouped_mm", "triton_mxfp8_wgrad", "triton_mxfp8_wgrad_v2", "apply",
     "WeightCastCache",
     "MXFP8GroupedMM", "mxfp8_grouped_mm", "MXFP8ExpertFFN", "moe_ffn", "moe_ffn_unfused",
-    "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
+    "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
     "combine_score_grad", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
 ]

@@ -35,16 +35,28 @@ OUT_F32 = 1
 SCALES_ROW_MAJOR = 0
 SCALES_BLOCK_MAJOR = 1
 
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
+
 OFFS_ENDS = 0
 OFFS_SIZES = 1
 OFFS_AUTO = 2
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 MAX_GROUPS = 1024  # groups of one call
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+
+
+class RouteOptions(ctypes.Structure):
+    """mxgg_route_options."""
+
+    _fields_ = [(n, _I64) for n in ("experts", "topk", "groups", "top_groups")] + \
+               [(n, ctypes.c_int32) for n in ("score", "dtype", "group_best", "renormalize")] + \
+               [("scale", ctypes.c_float)]
+
 
 # name -> (restype, argtypes); must list every function of include/mxgg.h
 SIGNATURES = {
@@ -132,6 +144,8 @@ SIGNATURES = {
     "mxgg_combine_score_grad": (
         _I, [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P],
     ),
+    "mxgg_route_topk": (_I, [_P, _I64, _P, _P, _P, _P, _P, _P]),
+    "mxgg_route_topk_grad": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P]),
 }
 
 

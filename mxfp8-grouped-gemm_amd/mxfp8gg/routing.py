@@ -10,7 +10,8 @@ three small kernels (no host sync), the gather is fused into the MXFP8 casts of 
 input (the bf16 routed copy is never written), and the combine sums the top-k
 terms in fp32 and rounds once.
 
-    plan = route_plan(expert_idx, num_experts)          # [T, topk] int
+    idx, scores = route_topk(logits, topk)              # [T, E] -> [T, topk]
+    plan = route_plan(idx, num_experts)                 # [T, topk] int
     q, s, qt, st, pad = gather_to_mxfp8_dual(x, plan)   # routed MXFP8 input
     ...                                                  # grouped GEMMs over plan.offs
     out = combine(y_routed, plan, scores)                # [T, H] bf16
@@ -20,6 +21,7 @@ one GPU every expert is local and dispatch is this gather.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -28,8 +30,104 @@ from . import _lib, ops
 from .ops import (_FP8, _MODES, _block_major_buffer, _mode, _native, _need_gpu, _stream_ptr,
                   _tensors, _took, padded_token_capacity)
 
-__all__ = ["RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual",
+__all__ = ["route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual",
            "gather_to_mxfp8_dim0", "combine", "combine_score_grad"]
+
+
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+_LOGIT_TYPES = {torch.float32: _lib.OUT_F32, torch.bfloat16: _lib.OUT_BF16}
+
+
+def _route_forward(logits, bias, opt, keep):
+    """(expert_idx, scores, selected or None) of contiguous logits."""
+    T, dev = logits.shape[0], logits.device
+    idx = torch.empty((T, opt.topk), dtype=torch.int32, device=dev)
+    scores = torch.empty((T, opt.topk), dtype=torch.float32, device=dev)
+    selected = torch.empty_like(scores) if keep else None
+    _lib.check(
+        _lib.load().mxgg_route_topk(
+            logits.data_ptr(), T, bias.data_ptr() if bias is not None else None,
+            ctypes.byref(opt), idx.data_ptr(), scores.data_ptr(),
+            selected.data_ptr() if keep else None, _stream_ptr(logits)),
+        "route_topk",
+    )
+    return idx, scores, selected
+
+
+class RouteTopK(torch.autograd.Function):
+    """route_topk with the gradient of the scores with respect to the logits.
+
+    What the forward keeps is [tokens, topk]: the ids and the selected scores.
+    The logits are kept for softmax scores without renormalisation only, whose
+    gradient reaches every expert."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, opt):
+        x = logits.contiguous()
+        idx, scores, selected = _route_forward(x, bias, opt, True)
+        whole = opt.score == _lib.SCORE_SOFTMAX and not opt.renormalize
+        ctx.save_for_backward(idx, selected, *([x] if whole else []))
+        ctx.opt = opt
+        ctx.like = (logits.shape, logits.dtype)
+        ctx.mark_non_differentiable(idx)
+        return idx, scores
+
+    @staticmethod
+    def backward(ctx, _, dscores):
+        idx, selected, *x = ctx.saved_tensors
+        shape, dtype = ctx.like
+        d = dscores.to(torch.float32).contiguous()
+        out = torch.empty(shape, dtype=dtype, device=d.device)
+        _lib.check(
+            _lib.load().mxgg_route_topk_grad(
+                d.data_ptr(), idx.data_ptr(), selected.data_ptr(), x[0].data_ptr() if x else None,
+                shape[0], ctypes.byref(ctx.opt), out.data_ptr(), _stream_ptr(d)),
+            "route_topk_grad",
+        )
+        return out, None, None
+
+
+def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax",
+               bias: torch.Tensor | None = None, num_groups: int = 1,
+               top_groups: int | None = None, group_best: int = 1, renormalize: bool = True,
+               scale: float = 1.0):
+    """The routing decision that route_plan, combine and moe_routed_ffn take:
+    (expert_idx int32 [tokens, topk], scores float32 [tokens, topk]) from the
+    router's logits [tokens, E] (fp32 or bf16 on the GPU).
+
+    score        "softmax" over the experts, or "sigmoid" of every logit, in fp32
+    bias         fp32 [E], added to the scores for the choice alone (a balance
+                 bias: it has no gradient and is not part of the weights)
+    num_groups   experts come in groups of E / num_groups; only those of the
+                 top_groups best groups can be chosen.  A group is worth its best
+                 expert (group_best=1), or the sum of its two best scores, with
+                 the bias (group_best=2)
+    renormalize  divide a token's scores by their sum; scale multiplies them last
+
+    Experts come in the order of their rank; equal ones lowest index first.  An
+    expert whose logit (or biased score) is -inf is never chosen, and a slot
+    that none is left for holds id -1 (route_plan drops it) and score 0: a token
+    with every logit -inf goes nowhere.  A NaN logit is chosen first and its
+    score is NaN.  E <= 1024, topk <= 32, num_groups <= 64.  Differentiable in
+    the logits."""
+    _need_gpu(logits, "logits")
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES:
+        raise TypeError("logits must be a 2-D float32 or bfloat16 tensor [tokens, experts]")
+    if score not in _SCORES:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+    E = logits.shape[1]
+    if bias is not None:
+        _need_gpu(bias, "bias")
+        if bias.shape != (E,):
+            raise ValueError(f"bias must have one value per expert ({E}), got {tuple(bias.shape)}")
+        bias = bias.detach().to(device=logits.device, dtype=torch.float32).contiguous()
+    opt = _lib.RouteOptions(E, topk, num_groups, num_groups if top_groups is None else top_groups,
+                            _SCORES[score], _LOGIT_TYPES[logits.dtype], group_best,
+                            bool(renormalize), scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return RouteTopK.apply(logits, bias, opt)
+    idx, scores, _ = _route_forward(logits.detach().contiguous(), bias, opt, False)
+    return idx, scores
 
 
 class RoutePlan(NamedTuple):

@@ -1,0 +1,83 @@
+"""Plain 64-bit implementations of the operators around the expert FFN, written
+from their definitions (loops over rows where that is clearest)."""
+import numpy as np
+
+NEG = -np.inf
+
+
+def route_topk(logits, topk, score="softmax", bias=None, num_groups=1, top_groups=None,
+               group_best=1, renormalize=True, scale=1.0):
+    """(idx int32 [T, K], weights float64 [T, K]) of float64 logits [T, E]."""
+    T, E = logits.shape
+    per = E // num_groups
+    top_groups = num_groups if top_groups is None else top_groups
+    idx = np.full((T, topk), -1, np.int32)
+    weights = np.zeros((T, topk))
+    for t in range(T):
+        x = logits[t]
+        with np.errstate(all="ignore"):
+            if score == "sigmoid":
+                s = 1.0 / (1.0 + np.exp(-x))
+            else:
+                m = np.max(x) if not np.isnan(x).any() else np.nan
+                e = np.exp(x - m) if m != NEG else np.zeros(E)
+                s = e / e.sum() if m != NEG else e
+        c = x.copy() if bias is None else np.where(x == NEG, NEG, s + bias)
+        live = c != NEG
+        key = lambda v: (1, 0.0) if np.isnan(v) else (0, v)  # noqa: E731  NaN first
+        if num_groups > 1:
+            worth = []
+            for g in range(num_groups):
+                own = [e for e in range(g * per, (g + 1) * per) if live[e]]
+                own.sort(key=lambda e: key(c[e]), reverse=True)
+                if not own:
+                    continue
+                if group_best == 1:
+                    w = c[own[0]]
+                else:
+                    w = sum((c[e] if bias is not None else s[e]) for e in own[:2])
+                worth.append((g, w))
+            worth.sort(key=lambda gw: key(gw[1]), reverse=True)  # stable: lowest group first
+            kept = {g for g, _ in worth[:top_groups]}
+            live = live & np.array([e // per in kept for e in range(E)])
+        order = sorted((e for e in range(E) if live[e]), key=lambda e: key(c[e]), reverse=True)
+        order = order[:topk]
+        if not order:
+            continue
+        idx[t, :len(order)] = order
+        if renormalize and score == "softmax":
+            z = x[order]
+            with np.errstate(all="ignore"):
+                p = np.exp(z - (np.max(z) if not np.isnan(z).any() else np.nan))
+            w = p / p.sum()
+        else:
+            w = s[order]
+            if renormalize:
+                w = w / w.sum() if w.sum() != 0 else w
+        weights[t, :len(order)] = scale * w
+    return idx, weights
+
+
+def route_grad(logits, idx, dw, score="softmax", renormalize=True, scale=1.0):
+    """d logits of the weights, the choice held fixed: J^T dw from the full
+    Jacobian of every token."""
+    T, E = logits.shape
+    out = np.zeros((T, E))
+    for t in range(T):
+        sel = [int(e) for e in idx[t] if e >= 0]
+        if not sel:
+            continue
+        x = logits[t]
+        if score == "sigmoid":
+            s = 1.0 / (1.0 + np.exp(-x))
+            js = np.diag(s * (1.0 / (1.0 + np.exp(x))))
+        else:
+            e = np.exp(x - x.max())
+            s = e / e.sum()
+            js = np.diag(s) - np.outer(s, s)
+        v, j = s[sel], js[sel]
+        if renormalize:
+            total = v.sum()
+            j = j / total - np.outer(v, j.sum(axis=0)) / total ** 2
+        out[t] = scale * (dw[t, :len(sel)] @ j)
+    return out
