@@ -596,6 +596,39 @@ int mxgg_route_topk_grad(const float* grad_weights, const int32_t* expert_idx,
                          const float* selected, const void* logits, int64_t tokens,
                          const mxgg_route_options* options, void* grad_logits, void* stream);
 
+/*
+ * Layer norm (center != 0) or root-mean-square norm over the rows of x:
+ *   xhat = (x - mean) * rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ *   y = xhat * weight + bias        (center == 0: mean = 0, bias ignored)
+ * x, y: [rows, cols] of `dtype` (an mxgg_out_dtype), row strides ldx, ldy, any
+ * alignment of the element; weight, bias: [cols] of their own types, or NULL.
+ * stats: fp32 [2][rows] (means, then rstd; the means are not written without
+ * `center`) for mxgg_norm_grad, or NULL.  1 <= cols <= 32768.  `options` is host
+ * memory, read during the call.
+ */
+typedef struct mxgg_norm_options {
+  int64_t rows, cols;
+  int32_t dtype, weight_dtype, bias_dtype, center;
+  float eps;
+} mxgg_norm_options;
+
+int mxgg_norm(const void* x, int64_t ldx, const void* weight, const void* bias,
+              const mxgg_norm_options* options, void* y, int64_t ldy, float* stats, void* stream);
+
+/*
+ * Gradients of mxgg_norm from grad_y [rows, cols] (row stride ldg) and the
+ * forward's x and stats: grad_x (row stride ldgx), grad_weight and grad_bias
+ * [cols] of the parameters' types; each may be NULL.  grad_weight and grad_bias
+ * are sums over the rows in fp32, in an order that depends on the shape alone,
+ * and need a workspace of mxgg_norm_grad_workspace_bytes(options) bytes (4-byte
+ * aligned, no initialisation).
+ */
+int64_t mxgg_norm_grad_workspace_bytes(const mxgg_norm_options* options);
+int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
+                   const void* weight, const float* stats, const mxgg_norm_options* options,
+                   void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1089,4 +1089,78 @@ int mxgg_route_topk_grad(const float* grad_weights, const int32_t* expert_idx,
                       "route_topk_grad");
 }
 
+static int check_norm(const char* what, const mxgg_norm_options* o) {
+  if (!o) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null options", what);
+  if (o->rows < 0 || o->cols < 1)
+    return set_error(MXGG_ERR_SHAPE, "%s: rows=%lld, cols=%lld", what, (long long)o->rows,
+                     (long long)o->cols);
+  if (o->cols > 32768)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: cols=%lld above 32768", what, (long long)o->cols);
+  for (const int t : {o->dtype, o->weight_dtype, o->bias_dtype})
+    if (t != MXGG_OUT_BF16 && t != MXGG_OUT_F32)
+      return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", what, t);
+  return MXGG_OK;
+}
+
+int mxgg_norm(const void* x, int64_t ldx, const void* weight, const void* bias,
+              const mxgg_norm_options* options, void* y, int64_t ldy, float* stats, void* stream) {
+  const int rc = check_norm("norm", options);
+  if (rc != MXGG_OK) return rc;
+  const mxgg_norm_options& o = *options;
+  if (o.rows == 0) return MXGG_OK;
+  if (!x || !y) return set_error(MXGG_ERR_INVALID_ARGUMENT, "norm: null pointer");
+  if (ldx < o.cols || ldy < o.cols)
+    return set_error(MXGG_ERR_SHAPE, "norm: leading dimension smaller than the row");
+  const NormArgs a{x,      weight, o.center ? bias : nullptr, y, stats, o.rows, ldx, ldy,
+                   (int32_t)o.cols, o.dtype == MXGG_OUT_BF16, o.weight_dtype == MXGG_OUT_BF16,
+                   o.bias_dtype == MXGG_OUT_BF16, o.center != 0, o.eps};
+  return check_launch(launch_norm_fwd(a, static_cast<hipStream_t>(stream)), "norm");
+}
+
+int64_t mxgg_norm_grad_workspace_bytes(const mxgg_norm_options* options) {
+  if (check_norm("norm_grad_workspace_bytes", options) != MXGG_OK) return -1;
+  return 8 * options->cols * norm_grad_parts(options->rows, (int)options->cols,
+                                             options->dtype == MXGG_OUT_BF16);
+}
+
+int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
+                   const void* weight, const float* stats, const mxgg_norm_options* options,
+                   void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_norm("norm_grad", options);
+  if (rc != MXGG_OK) return rc;
+  const mxgg_norm_options& o = *options;
+  const bool sums = grad_weight || grad_bias;
+  if (o.rows > 0 && (!grad_y || !x || !stats))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "norm_grad: null pointer");
+  if (o.rows > 0 && (ldx < o.cols || ldg < o.cols || (grad_x && ldgx < o.cols)))
+    return set_error(MXGG_ERR_SHAPE, "norm_grad: leading dimension smaller than the row");
+  const int64_t need = mxgg_norm_grad_workspace_bytes(options);
+  if (sums && workspace_bytes < need)
+    return set_error(MXGG_ERR_SHAPE, "norm_grad: workspace of %lld bytes, %lld needed",
+                     (long long)workspace_bytes, (long long)need);
+  if (sums && need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
+    return set_error(workspace ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
+                     "norm_grad: the workspace must be a 4-byte aligned device buffer");
+  NormGradArgs a{};
+  a.dy = grad_y;
+  a.x = x;
+  a.w = weight;
+  a.stats = stats;
+  a.dx = grad_x;
+  a.dw = grad_weight;
+  a.db = grad_bias;
+  a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  a.rows = o.rows;
+  a.lddy = ldg;
+  a.ldx = ldx;
+  a.lddx = ldgx;
+  a.cols = (int32_t)o.cols;
+  a.bf16 = o.dtype == MXGG_OUT_BF16;
+  a.w_bf16 = o.weight_dtype == MXGG_OUT_BF16;
+  a.b_bf16 = o.bias_dtype == MXGG_OUT_BF16;
+  a.center = o.center != 0;
+  return check_launch(launch_norm_bwd(a, static_cast<hipStream_t>(stream)), "norm_grad");
+}
+
 }  // extern "C"

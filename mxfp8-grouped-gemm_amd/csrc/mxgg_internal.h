@@ -141,6 +141,34 @@ struct RouteTopkGradArgs {
 };
 hipError_t launch_route_topk_grad(RouteTopkGradArgs args, hipStream_t stream);
 
+// Layer norm and root-mean-square norm (norm.hip); stats: fp32 [2][rows], the
+// row's mean (layer norm) and its reciprocal deviation.
+struct NormArgs {
+  const void* x;  // [rows], row stride ldx, fp32 or bf16
+  const void* w;  // [cols] or nullptr
+  const void* b;
+  void* y;
+  float* stats;   // or nullptr
+  int64_t rows, ldx, ldy;
+  int32_t cols, bf16, w_bf16, b_bf16, center;
+  float eps;
+};
+hipError_t launch_norm_fwd(const NormArgs& args, hipStream_t stream);
+struct NormGradArgs {
+  const void* dy;
+  const void* x;
+  const void* w;
+  const float* stats;
+  void* dx;        // or nullptr
+  void* dw;        // [cols] or nullptr, of the weight's type
+  void* db;
+  float* partial;  // [2][norm_grad_parts()][cols], needed for dw or db
+  int64_t rows, lddy, ldx, lddx;
+  int32_t cols, bf16, w_bf16, b_bf16, center;
+};
+hipError_t launch_norm_bwd(const NormGradArgs& args, hipStream_t stream);
+int norm_grad_parts(int64_t rows, int cols, int bf16);
+
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,
                                int32_t* ends, hipStream_t stream);

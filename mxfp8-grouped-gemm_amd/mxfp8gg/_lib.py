@@ -58,6 +58,14 @@ class RouteOptions(ctypes.Structure):
                [("scale", ctypes.c_float)]
 
 
+class NormOptions(ctypes.Structure):
+    """mxgg_norm_options."""
+
+    _fields_ = [(n, _I64) for n in ("rows", "cols")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "bias_dtype", "center")] + \
+               [("eps", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); must list every function of include/mxgg.h
 SIGNATURES = {
     "mxgg_abi_version": (_I, []),
@@ -146,6 +154,11 @@ SIGNATURES = {
     ),
     "mxgg_route_topk": (_I, [_P, _I64, _P, _P, _P, _P, _P, _P]),
     "mxgg_route_topk_grad": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P]),
+    "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
+    "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
+    "mxgg_norm_grad": (
+        _I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P],
+    ),
 }
 
 

@@ -81,3 +81,25 @@ def route_grad(logits, idx, dw, score="softmax", renormalize=True, scale=1.0):
             j = j / total - np.outer(v, j.sum(axis=0)) / total ** 2
         out[t] = scale * (dw[t, :len(sel)] @ j)
     return out
+
+
+def norm(x, weight=None, bias=None, eps=1e-5, center=True):
+    """(y, xhat, r) over the last axis."""
+    mu = x.mean(axis=-1, keepdims=True) if center else 0.0
+    r = 1.0 / np.sqrt(((x - mu) ** 2).mean(axis=-1, keepdims=True) + eps)
+    xhat = (x - mu) * r
+    y = xhat * (1.0 if weight is None else weight)
+    return (y if bias is None else y + bias), xhat, r
+
+
+def norm_grad(dy, x, weight=None, eps=1e-5, center=True):
+    """(dx, dweight, dbias): dx from the Jacobian of xhat, row by row."""
+    _, xhat, r = norm(x, eps=eps, center=center)
+    n = x.shape[-1]
+    u = dy * (1.0 if weight is None else weight)
+    dx = np.zeros_like(x)
+    for i in range(x.shape[0]):
+        h = xhat[i]
+        # d xhat_a / d x_b = r (delta_ab - [1/n] - h_a h_b / n)
+        dx[i] = r[i] * (u[i] - (u[i].mean() if center else 0.0) - h * (u[i] @ h) / n)
+    return dx, (dy * xhat).sum(axis=0), dy.sum(axis=0)
