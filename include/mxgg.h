@@ -629,6 +629,43 @@ int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
                    void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
                    void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * One AdamW step (decoupled weight decay) over `count` tensors, in place:
+ *   p <- p (1 - lr weight_decay);  m <- beta1 m + (1 - beta1) g
+ *   v <- beta2 v + (1 - beta2) g^2
+ *   p <- p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32.  param, grad: n contiguous elements, fp32 or bf16 each (mxgg_out_dtype).
+ * master: fp32 copy of the weight, or NULL; with it the step is taken there and
+ * param is written as its rounding.
+ *   state_bits 32 : exp_avg = m, exp_avg_sq = v, fp32 [n]; scales unused
+ *   state_bits 8  : exp_avg = m, exp_avg_sq = sqrt(v), e4m3 [n] with E8M0 scales
+ *                   uint8 [ceil(n / 32)], one for every 32 consecutive elements:
+ *                   b = max(ceil(log2(amax / 448)), -126) + 127, rounded to
+ *                   nearest even; a block with an infinity or a NaN is all NaN
+ * Any element alignment; tensors must not overlap.  `tensors` and `options` are
+ * host memory, read during the call.  One kernel launch for every 48 tensors.
+ */
+typedef struct mxgg_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* exp_avg_scales;
+  void* exp_avg_sq_scales;
+  float* master;
+  int64_t n;
+  int32_t param_dtype, grad_dtype;
+} mxgg_adamw_tensor;
+
+typedef struct mxgg_adamw_options {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step; /* of this update, from 1 */
+  int32_t state_bits;
+} mxgg_adamw_options;
+
+int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
+                    const mxgg_adamw_options* options, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

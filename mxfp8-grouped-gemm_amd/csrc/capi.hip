@@ -5,6 +5,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <cmath>
 #include <mutex>
 #include <vector>
 
@@ -1161,6 +1162,74 @@ int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
   a.b_bf16 = o.bias_dtype == MXGG_OUT_BF16;
   a.center = o.center != 0;
   return check_launch(launch_norm_bwd(a, static_cast<hipStream_t>(stream)), "norm_grad");
+}
+
+int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
+                    const mxgg_adamw_options* options, void* stream) {
+  if (!options || (count > 0 && !tensors))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "adamw_step: null pointer");
+  const mxgg_adamw_options& o = *options;
+  if (count < 0 || o.step < 1)
+    return set_error(MXGG_ERR_SHAPE, "adamw_step: count=%lld, step=%lld", (long long)count,
+                     (long long)o.step);
+  if (o.state_bits != 8 && o.state_bits != 32)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "adamw_step: state_bits=%d", o.state_bits);
+  if (!(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0 && o.lr >= 0 &&
+        o.weight_decay >= 0))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT,
+                     "adamw_step: lr=%g, betas=(%g, %g), eps=%g, weight_decay=%g", o.lr, o.beta1,
+                     o.beta2, o.eps, o.weight_decay);
+  AdamScalars s;
+  s.beta1 = (float)o.beta1;
+  s.one_beta1 = (float)(1 - o.beta1);
+  s.beta2 = (float)o.beta2;
+  s.one_beta2 = (float)(1 - o.beta2);
+  s.decay = (float)(1 - o.lr * o.weight_decay);
+  s.step_size = (float)(o.lr / (1 - std::pow(o.beta1, (double)o.step)));
+  s.inv_root_bias2 = (float)(1 / std::sqrt(1 - std::pow(o.beta2, (double)o.step)));
+  s.eps = (float)o.eps;
+  // checked and launched in runs of a fixed size: nothing is allocated
+  constexpr int64_t kRun = 48;
+  AdamTensor run[kRun];
+  for (int pass = 0; pass < 2; ++pass)  // every tensor is checked before the first launch
+    for (int64_t i = 0; i < count; i += kRun) {
+      const int64_t n = count - i < kRun ? count - i : kRun;
+      for (int64_t j = 0; j < n; ++j) {
+        const mxgg_adamw_tensor& t = tensors[i + j];
+        const long long at = (long long)(i + j);
+        if (pass == 0) {
+          for (const int d : {t.param_dtype, t.grad_dtype})
+            if (d != MXGG_OUT_BF16 && d != MXGG_OUT_F32)
+              return set_error(MXGG_ERR_INVALID_ARGUMENT, "adamw_step: tensor %lld: type %d", at, d);
+          if (t.n < 0) return set_error(MXGG_ERR_SHAPE, "adamw_step: tensor %lld: n=%lld", at,
+                                        (long long)t.n);
+          if (t.n > adamw_max_elements())
+            return set_error(MXGG_ERR_UNSUPPORTED, "adamw_step: tensor %lld has %lld elements", at,
+                             (long long)t.n);
+          if (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
+                          (o.state_bits == 8 && (!t.exp_avg_scales || !t.exp_avg_sq_scales))))
+            return set_error(MXGG_ERR_INVALID_ARGUMENT, "adamw_step: tensor %lld: null pointer", at);
+          continue;
+        }
+        AdamTensor& d = run[j];
+        d.param = t.param;
+        d.grad = t.grad;
+        d.m = t.exp_avg;
+        d.v = t.exp_avg_sq;
+        d.m_scales = static_cast<uint8_t*>(t.exp_avg_scales);
+        d.v_scales = static_cast<uint8_t*>(t.exp_avg_sq_scales);
+        d.master = t.master;
+        d.n = t.n;
+        d.param_bf16 = t.param_dtype == MXGG_OUT_BF16;
+        d.grad_bf16 = t.grad_dtype == MXGG_OUT_BF16;
+      }
+      if (pass == 1) {
+        const int rc = check_launch(
+            launch_adamw(run, n, o.state_bits, s, static_cast<hipStream_t>(stream)), "adamw_step");
+        if (rc != MXGG_OK) return rc;
+      }
+    }
+  return MXGG_OK;
 }
 
 }  // extern "C"

@@ -169,6 +169,25 @@ struct NormGradArgs {
 hipError_t launch_norm_bwd(const NormGradArgs& args, hipStream_t stream);
 int norm_grad_parts(int64_t rows, int cols, int bf16);
 
+// AdamW over many tensors (adamw.hip).  The scales are used with 8-bit states.
+struct AdamTensor {
+  void* param;
+  const void* grad;
+  void* m;
+  void* v;
+  uint8_t* m_scales;
+  uint8_t* v_scales;
+  float* master;  // or nullptr
+  int64_t n : 62;
+  uint64_t param_bf16 : 1, grad_bf16 : 1;
+};
+struct AdamScalars {
+  float beta1, one_beta1, beta2, one_beta2, decay, step_size, inv_root_bias2, eps;
+};
+hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int state_bits,
+                        const AdamScalars& scalars, hipStream_t stream);
+int64_t adamw_max_elements();
+
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,
                                int32_t* ends, hipStream_t stream);

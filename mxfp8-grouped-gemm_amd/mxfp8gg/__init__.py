@@ -52,6 +52,7 @@ from .routing import (
     route_plan,
     route_topk,
 )
+from .optim import AdamW, adamw_state, adamw_step
 from .norm import Norm, layer_norm, rms_norm
 from .torchao_compat import (
     apply,
@@ -75,5 +76,6 @@ __all__ = [
     "MXFP8GroupedMM", "mxfp8_grouped_mm", "MXFP8ExpertFFN", "moe_ffn", "moe_ffn_unfused",
     "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
-    "combine_score_grad", "Norm", "layer_norm", "rms_norm", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
+    "combine_score_grad", "Norm", "layer_norm", "rms_norm",
+    "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
 ]

@@ -58,6 +58,21 @@ class RouteOptions(ctypes.Structure):
                [("scale", ctypes.c_float)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """mxgg_adamw_tensor."""
+
+    _fields_ = [(n, _P) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scales",
+                                  "exp_avg_sq_scales", "master")] + \
+               [("n", _I64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
+
+
+class AdamwOptions(ctypes.Structure):
+    """mxgg_adamw_options."""
+
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + \
+               [("step", _I64), ("state_bits", ctypes.c_int32)]
+
+
 class NormOptions(ctypes.Structure):
     """mxgg_norm_options."""
 
@@ -154,6 +169,7 @@ SIGNATURES = {
     ),
     "mxgg_route_topk": (_I, [_P, _I64, _P, _P, _P, _P, _P, _P]),
     "mxgg_route_topk_grad": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P]),
+    "mxgg_adamw_step": (_I, [_P, _I64, _P, _P]),
     "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
     "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
     "mxgg_norm_grad": (

@@ -103,3 +103,23 @@ def norm_grad(dy, x, weight=None, eps=1e-5, center=True):
         # d xhat_a / d x_b = r (delta_ab - [1/n] - h_a h_b / n)
         dx[i] = r[i] * (u[i] - (u[i].mean() if center else 0.0) - h * (u[i] @ h) / n)
     return dx, (dy * xhat).sum(axis=0), dy.sum(axis=0)
+
+
+def adamw(p, g, m, v, step, lr, betas, eps, weight_decay):
+    """(p, m, v) after one step, v the second moment itself."""
+    b1, b2 = betas
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    p = p * (1 - lr * weight_decay)
+    return p - lr * (m / (1 - b1 ** step)) / (np.sqrt(v / (1 - b2 ** step)) + eps), m, v
+
+
+def mx8_values(q, s):
+    """float64 values of an 8-bit state: e4m3 payload bytes, E8M0 scale bytes."""
+    q = np.asarray(q, np.uint8).reshape(-1)
+    sign = np.where(q & 0x80, -1.0, 1.0)
+    e, f = ((q >> 3) & 15).astype(int), (q & 7).astype(float)
+    val = np.where(e == 0, f * 2.0 ** -9, (1 + f / 8) * 2.0 ** (e - 7))
+    val = np.where((q & 0x7F) == 0x7F, np.nan, val)
+    up = np.repeat(2.0 ** (np.asarray(s, np.uint8).reshape(-1).astype(int) - 127), 32)[:q.size]
+    return sign * val * up
