@@ -666,6 +666,51 @@ typedef struct mxgg_adamw_options {
 int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
                     const mxgg_adamw_options* options, void* stream);
 
+/*
+ * Softmax cross entropy of a linear layer, z = x W^T, without keeping z:
+ *   token_loss[t] = log(sum over v of exp(z[t][v])) - z[t][target[t]]
+ * x: bf16 [tokens, hidden], W: bf16 [vocab, hidden] (row strides ldx, ldw: 16-byte
+ * aligned rows, hidden % 8 == 0); target: int32, or int64 with target_int64.
+ * A token whose target is ignore_index has loss 0 and no gradient; one whose
+ * target is otherwise outside [0, vocab) has loss NaN.  z is summed in fp32.
+ *   reduction : NONE (loss = the token losses, fp32 [tokens]), SUM, or MEAN over
+ *               the tokens that are not ignored (loss: fp32 [1])
+ *   stats     : fp32 [tokens + 1], written for the gradient
+ *   workspace : mxgg_linear_cross_entropy_workspace_bytes(options), 16-byte
+ *               aligned, no initialisation
+ */
+typedef enum mxgg_reduction {
+  MXGG_REDUCE_NONE = 0,
+  MXGG_REDUCE_SUM = 1,
+  MXGG_REDUCE_MEAN = 2
+} mxgg_reduction;
+
+typedef struct mxgg_loss_options {
+  int64_t tokens, vocab, hidden, ldx, ldw, ignore_index;
+  int32_t target_int64, reduction;
+} mxgg_loss_options;
+
+int64_t mxgg_linear_cross_entropy_workspace_bytes(const mxgg_loss_options* options);
+int mxgg_linear_cross_entropy(const void* x, const void* weight, const void* target,
+                              const mxgg_loss_options* options, float* loss, float* stats,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients, from grad_loss (fp32 [1], or [tokens] for NONE) and the
+ * forward's stats: grad_x bf16 [tokens, hidden] and grad_weight bf16 [vocab,
+ * hidden], contiguous, each NULL if not wanted.  z is computed again in pieces of
+ * the vocabulary; d loss / d z is rounded to bf16 between the products, which sum
+ * in fp32 in a fixed order.  need_x, need_weight: which gradients the workspace
+ * is for.
+ */
+int64_t mxgg_linear_cross_entropy_grad_workspace_bytes(const mxgg_loss_options* options, int need_x,
+                                                       int need_weight);
+int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const void* weight,
+                                   const void* target, const float* stats,
+                                   const mxgg_loss_options* options, void* grad_x,
+                                   void* grad_weight, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1232,4 +1232,117 @@ int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
   return MXGG_OK;
 }
 
+static int check_loss(const char* what, const mxgg_loss_options* o) {
+  if (!o) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null options", what);
+  if (o->tokens < 0 || o->vocab < 1 || o->hidden < 8 || o->hidden % 8 != 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld, vocab=%lld, hidden=%lld (a multiple of 8)",
+                     what, (long long)o->tokens, (long long)o->vocab, (long long)o->hidden);
+  if (o->ldx < o->hidden || o->ldw < o->hidden)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (o->ldx % 8 != 0 || o->ldw % 8 != 0)
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: leading dimensions multiples of 8", what);
+  // a tile of 256 rows stays within a 2 GiB buffer range: also the rows of d, its
+  // transpose and the transposed operands (at most tokens or a piece long)
+  if (2 * o->ldx > kMaxRowStride || 2 * o->ldw > kMaxRowStride ||
+      o->tokens > kMaxRowStride / 4 || o->vocab > INT64_C(1) << 24 ||
+      (o->vocab + 255) / 256 * ((o->tokens + 255) / 256) >= INT64_C(1) << 24)
+    return set_error(MXGG_ERR_UNSUPPORTED,
+                     "%s: rows longer than 2^22, tokens above 2^21, vocab above 2^24 or 2^24 "
+                     "tiles of 256 x 256", what);
+  if (o->reduction != MXGG_REDUCE_NONE && o->reduction != MXGG_REDUCE_SUM &&
+      o->reduction != MXGG_REDUCE_MEAN)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: reduction=%d", what, o->reduction);
+  return MXGG_OK;
+}
+
+static LossArgs loss_args(const void* x, const void* w, const void* target,
+                          const mxgg_loss_options& o) {
+  LossArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.w = static_cast<const uint16_t*>(w);
+  a.target = target;
+  a.T = o.tokens;
+  a.V = o.vocab;
+  a.H = o.hidden;
+  a.ldx = o.ldx;
+  a.ldw = o.ldw;
+  a.ignore_index = o.ignore_index;
+  a.target64 = o.target_int64 != 0;
+  a.mean = o.reduction == MXGG_REDUCE_MEAN;
+  a.per_token = o.reduction == MXGG_REDUCE_NONE;
+  return a;
+}
+
+static int check_loss_workspace(const char* what, const void* ws, int64_t bytes, int64_t need) {
+  if (bytes < need)
+    return set_error(MXGG_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", what,
+                     (long long)bytes, (long long)need);
+  if (need > 0 && (!ws || !aligned16(ws)))
+    return set_error(ws ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
+                     "%s: the workspace must be a 16-byte aligned device buffer", what);
+  return MXGG_OK;
+}
+
+int64_t mxgg_linear_cross_entropy_workspace_bytes(const mxgg_loss_options* options) {
+  if (check_loss("linear_cross_entropy_workspace_bytes", options) != MXGG_OK) return -1;
+  return loss_workspace_bytes(loss_args(nullptr, nullptr, nullptr, *options));
+}
+
+int mxgg_linear_cross_entropy(const void* x, const void* weight, const void* target,
+                              const mxgg_loss_options* options, float* loss, float* stats,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "linear_cross_entropy";
+  int rc = check_loss(what, options);
+  if (rc != MXGG_OK) return rc;
+  const mxgg_loss_options& o = *options;
+  if (!stats || (!loss && (o.tokens > 0 || o.reduction != MXGG_REDUCE_NONE)) || !weight ||
+      (o.tokens > 0 && (!x || !target)))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!aligned16(x) || !aligned16(weight))
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: x and weight 16-byte aligned", what);
+  LossArgs a = loss_args(x, weight, target, o);
+  rc = check_loss_workspace(what, workspace, workspace_bytes, loss_workspace_bytes(a));
+  if (rc != MXGG_OK) return rc;
+  a.stats = stats;
+  (o.reduction == MXGG_REDUCE_NONE ? a.token_loss : a.loss) = loss;
+  return check_launch(launch_loss(a, static_cast<uint8_t*>(workspace),
+                                  static_cast<hipStream_t>(stream)), what);
+}
+
+int64_t mxgg_linear_cross_entropy_grad_workspace_bytes(const mxgg_loss_options* options, int need_x,
+                                                       int need_weight) {
+  if (check_loss("linear_cross_entropy_grad_workspace_bytes", options) != MXGG_OK) return -1;
+  return loss_grad_workspace_bytes(loss_args(nullptr, nullptr, nullptr, *options), need_x != 0,
+                                   need_weight != 0);
+}
+
+int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const void* weight,
+                                   const void* target, const float* stats,
+                                   const mxgg_loss_options* options, void* grad_x,
+                                   void* grad_weight, void* workspace, int64_t workspace_bytes,
+                                   void* stream) {
+  const char* what = "linear_cross_entropy_grad";
+  int rc = check_loss(what, options);
+  if (rc != MXGG_OK) return rc;
+  const mxgg_loss_options& o = *options;
+  if (o.tokens == 0)
+    return grad_weight ? set_error(MXGG_ERR_SHAPE, "%s: no tokens: grad_weight is zero", what)
+                       : MXGG_OK;
+  if (!grad_x && !grad_weight) return MXGG_OK;
+  if (!grad_loss || !x || !weight || !target || !stats)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(grad_x) || !aligned16(grad_weight))
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: matrices 16-byte aligned", what);
+  LossArgs a = loss_args(x, weight, target, o);
+  rc = check_loss_workspace(what, workspace, workspace_bytes,
+                            loss_grad_workspace_bytes(a, grad_x != nullptr, grad_weight != nullptr));
+  if (rc != MXGG_OK) return rc;
+  a.grad_loss = grad_loss;
+  a.stats = const_cast<float*>(stats);
+  return check_launch(launch_loss_grad(a, static_cast<uint16_t*>(grad_x),
+                                       static_cast<uint16_t*>(grad_weight),
+                                       static_cast<uint8_t*>(workspace),
+                                       static_cast<hipStream_t>(stream)), what);
+}
+
 }  // extern "C"

@@ -188,6 +188,29 @@ hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int state_bits
                         const AdamScalars& scalars, hipStream_t stream);
 int64_t adamw_max_elements();
 
+// Cross entropy of a linear layer (loss.hip).  The launchers fill in what lies in
+// their workspace (part, target_logit, d, dt, ldt, token_loss where it is null).
+struct LossArgs {
+  const uint16_t* x;   // bf16 [T][H], row stride ldx
+  const uint16_t* w;   // bf16 [V][H], row stride ldw
+  const void* target;  // [T] int32 or int64
+  float* stats;        // [T + 1]: log of the sum of exponentials, then the factor of the mean
+  float* token_loss;   // [T]
+  float* loss;         // [1], or nullptr: no reduction
+  const float* grad_loss;  // [1], or [T] with per_token
+  float2* part;
+  float* target_logit;
+  uint16_t* d;
+  uint16_t* dt;
+  int64_t T, V, H, ldx, ldw, ldt, ignore_index;
+  int32_t target64, mean, per_token;
+};
+int64_t loss_workspace_bytes(const LossArgs& args);
+hipError_t launch_loss(LossArgs args, uint8_t* ws, hipStream_t stream);
+int64_t loss_grad_workspace_bytes(const LossArgs& args, bool need_x, bool need_w);
+hipError_t launch_loss_grad(LossArgs args, uint16_t* dx, uint16_t* dw, uint8_t* ws,
+                            hipStream_t stream);
+
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,
                                int32_t* ends, hipStream_t stream);

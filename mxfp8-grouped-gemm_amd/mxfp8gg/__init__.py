@@ -52,6 +52,7 @@ from .routing import (
     route_plan,
     route_topk,
 )
+from .loss import LinearCrossEntropy, linear_cross_entropy
 from .optim import AdamW, adamw_state, adamw_step
 from .norm import Norm, layer_norm, rms_norm
 from .torchao_compat import (
@@ -77,5 +78,5 @@ __all__ = [
     "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
     "combine_score_grad", "Norm", "layer_norm", "rms_norm",
-    "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
+    "LinearCrossEntropy", "linear_cross_entropy", "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
 ]

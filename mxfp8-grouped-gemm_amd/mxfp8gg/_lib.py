@@ -35,6 +35,10 @@ OUT_F32 = 1
 SCALES_ROW_MAJOR = 0
 SCALES_BLOCK_MAJOR = 1
 
+REDUCE_NONE = 0
+REDUCE_SUM = 1
+REDUCE_MEAN = 2
+
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
 
@@ -71,6 +75,13 @@ class AdamwOptions(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + \
                [("step", _I64), ("state_bits", ctypes.c_int32)]
+
+
+class LossOptions(ctypes.Structure):
+    """mxgg_loss_options."""
+
+    _fields_ = [(n, _I64) for n in ("tokens", "vocab", "hidden", "ldx", "ldw", "ignore_index")] + \
+               [(n, ctypes.c_int32) for n in ("target_int64", "reduction")]
 
 
 class NormOptions(ctypes.Structure):
@@ -170,6 +181,12 @@ SIGNATURES = {
     "mxgg_route_topk": (_I, [_P, _I64, _P, _P, _P, _P, _P, _P]),
     "mxgg_route_topk_grad": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P]),
     "mxgg_adamw_step": (_I, [_P, _I64, _P, _P]),
+    "mxgg_linear_cross_entropy_workspace_bytes": (_I64, [_P]),
+    "mxgg_linear_cross_entropy": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "mxgg_linear_cross_entropy_grad_workspace_bytes": (_I64, [_P, _I, _I]),
+    "mxgg_linear_cross_entropy_grad": (
+        _I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P],
+    ),
     "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
     "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
     "mxgg_norm_grad": (

@@ -1,0 +1,119 @@
+"""Softmax cross entropy of a linear layer over a large vocabulary.
+
+    loss = linear_cross_entropy(x, weight, target)   # x [T, H], weight [V, H], target [T]
+    loss.backward()
+
+is cross_entropy(x @ weight.T, target) without the logits [T, V]: the forward
+pass keeps one fp32 value a token, the backward pass computes the logits again
+in pieces of the vocabulary and holds about 1 GiB for one piece.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _need_gpu, _stream_ptr
+
+__all__ = ["linear_cross_entropy", "LinearCrossEntropy"]
+
+_REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
+
+
+def _operand(t: torch.Tensor):
+    """(t, row stride) with the 16-byte aligned rows that the kernels read: a copy
+    where t has none."""
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.stride(1) == 1 and ld >= t.shape[1] and ld % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, ld
+    return t.clone(memory_format=torch.contiguous_format), t.shape[1]
+
+
+def _forward(x, w, target, opt):
+    lib, dev = _lib.load(), x.device
+    loss = torch.empty(opt.tokens if opt.reduction == _lib.REDUCE_NONE else (),
+                       dtype=torch.float32, device=dev)
+    stats = torch.empty(opt.tokens + 1, dtype=torch.float32, device=dev)
+    nbytes = lib.mxgg_linear_cross_entropy_workspace_bytes(ctypes.byref(opt))
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
+    _lib.check(
+        lib.mxgg_linear_cross_entropy(x.data_ptr(), w.data_ptr(), target.data_ptr(),
+                                      ctypes.byref(opt), loss.data_ptr(), stats.data_ptr(),
+                                      ws.data_ptr(), nbytes, _stream_ptr(x)),
+        "linear_cross_entropy",
+    )
+    return loss, stats
+
+
+class LinearCrossEntropy(torch.autograd.Function):
+    """linear_cross_entropy with the gradients of x and the weight."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, opt):
+        (x2, opt.ldx), (w2, opt.ldw) = _operand(x), _operand(weight)
+        loss, stats = _forward(x2, w2, target, opt)
+        ctx.save_for_backward(x2, w2, target, stats)
+        ctx.opt = opt
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        x, w, target, stats = ctx.saved_tensors
+        opt, dev = ctx.opt, x.device
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        if opt.tokens == 0:
+            return dx, torch.zeros(w.shape, dtype=w.dtype, device=dev) if need_w else None, None, None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
+        d = dloss.to(torch.float32).contiguous()
+        lib = _lib.load()
+        nbytes = lib.mxgg_linear_cross_entropy_grad_workspace_bytes(ctypes.byref(opt), need_x,
+                                                                    need_w)
+        ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.mxgg_linear_cross_entropy_grad(
+                d.data_ptr(), x.data_ptr(), w.data_ptr(), target.data_ptr(), stats.data_ptr(),
+                ctypes.byref(opt), dx.data_ptr() if need_x else None,
+                dw.data_ptr() if need_w else None, ws.data_ptr(), nbytes, _stream_ptr(x)),
+            "linear_cross_entropy_grad",
+        )
+        return dx, dw, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """cross_entropy(x @ weight.T, target), in fp32, without the logits.
+
+    x: bf16 [..., H]; weight: bf16 [V, H] (H a multiple of 8); target: int32 or
+    int64 of x's leading dimensions.  Tokens whose target is ignore_index have
+    loss 0 and no gradient, and the mean is over the others (NaN if there are
+    none, as torch's); any other target outside [0, V) gives a NaN loss.
+    reduction: "mean", "sum" or "none" (target's shape).  Differentiable in x and
+    weight; the same bits on every run."""
+    _need_gpu(x, "x")
+    for name, t in (("weight", weight), ("target", target)):
+        _need_gpu(t, name)
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"x and weight must be bfloat16, got {x.dtype} and {weight.dtype}")
+    if target.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"target must be int32 or int64, got {target.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] \
+            or target.shape != x.shape[:-1]:
+        raise ValueError(f"shapes must be x [..., H], weight [V, H], target [...], got "
+                         f"{tuple(x.shape)}, {tuple(weight.shape)}, {tuple(target.shape)}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    H = x.shape[-1]
+    x2 = x.reshape(-1, H) if H else x.new_empty((0, 0))
+    t = target.reshape(-1).contiguous()
+    opt = _lib.LossOptions(x2.shape[0], weight.shape[0], H, H, H, ignore_index,
+                           target.dtype == torch.int64, _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = LinearCrossEntropy.apply(x2, weight, t, opt)
+    else:
+        (a, opt.ldx), (w, opt.ldw) = _operand(x2.detach()), _operand(weight.detach())
+        loss, _ = _forward(a, w, t, opt)
+    return loss.view(target.shape) if reduction == "none" else loss

@@ -123,3 +123,19 @@ def mx8_values(q, s):
     val = np.where((q & 0x7F) == 0x7F, np.nan, val)
     up = np.repeat(2.0 ** (np.asarray(s, np.uint8).reshape(-1).astype(int) - 127), 32)[:q.size]
     return sign * val * up
+
+
+def linear_cross_entropy(x, w, target, ignore=-100):
+    """(token losses, d token loss / d z [T, V]) in float64; ignored tokens 0."""
+    z = x @ w.T
+    m = z.max(axis=1, keepdims=True)
+    p = np.exp(z - m)
+    total = p.sum(axis=1, keepdims=True)
+    live = target != ignore
+    loss = np.zeros(len(target))
+    rows = np.arange(len(target))[live]
+    loss[live] = (np.log(total) + m)[live, 0] - z[rows, target[live]]
+    d = p / total
+    d[rows, target[live]] -= 1
+    d[~live] = 0
+    return loss, d
