@@ -115,6 +115,30 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));
 }
 
+// Sum over each row of 16 lanes, in every lane of it (DPP quad permutations and
+// mirrors: VALU only, no LDS round trip).  Every lane must be active.
+template <int CTRL>
+__device__ __forceinline__ float dpp_mov(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row16_sum(float x) {
+  x += dpp_mov<0xB1>(x);   // quad_perm [1,0,3,2]
+  x += dpp_mov<0x4E>(x);   // quad_perm [2,3,0,1]
+  x += dpp_mov<0x141>(x);  // row_half_mirror
+  return x + dpp_mov<0x140>(x);  // row_mirror
+}
+
+// Sum over the wave, in every lane: rows of 16 joined by the gfx950 lane swaps
+// (v_permlane16_swap, v_permlane32_swap with both operands x give the values of
+// the other row, or half, without an LDS round trip).
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row16_sum(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
 // Streaming (nontemporal) 8-byte store of payload bytes that this kernel does
 // not read back.
 __device__ __forceinline__ void store_stream(uint8_t* p, uint2 v) {

@@ -8,11 +8,12 @@
 //
 // Memory-bound: a row is read once and kept in registers (16-byte chunks, CH a
 // thread), so mean and variance are two exact passes over registers; statistics
-// and sums are fp32.  Workgroups are persistent and take rows blockIdx, blockIdx
-// + grid, ...: w and b stay in registers, the next row's loads go out before the
-// current row's reductions, and in the backward pass every workgroup keeps its
-// own dw and db, written once at its end and added over workgroups in a fixed
-// order by a second kernel (no atomics: the sums are the same on every run).
+// and sums are fp32.  A short row belongs to one wave (no barriers, the waves of a
+// workgroup run apart), a longer one to a workgroup.  Workgroups are persistent:
+// w and b stay in registers, the next row's loads go out before the current row's
+// reductions, and in the backward pass every workgroup keeps its own dw and db,
+// written once at its end and added over workgroups in a fixed order by a second
+// kernel (no atomics: the sums are the same on every run).
 #include <algorithm>
 
 #include "mx_device.h"
@@ -21,11 +22,10 @@
 namespace mxgg {
 namespace {
 
-// 512 threads leave 256 registers each: rows of up to 16384 stay in them in both
-// passes; the backward pass of longer ones spills.
-constexpr int kNormMaxThreads = 512;
+constexpr int kNormMaxThreads = 512;  // leaves a thread 256 registers
+constexpr int kWaveRows = 4;          // waves, and rows at a time, of a workgroup of one-wave rows
 
-// EPC elements of a 16-byte chunk, read and written at any element alignment.
+// The elements of a 16-byte chunk, read and written at any element alignment.
 template <typename T>
 struct Elems;
 template <>
@@ -56,12 +56,20 @@ struct Elems<uint16_t> {
   __device__ static void put(uint16_t* p, float f) { *p = (uint16_t)pack_bf16x2(f, 0.0f); }
 };
 
-// n of a chunk's elements (0 past the end of the row).
-template <typename T>
+// n of a chunk's elements (0 past the end of the row).  Outputs are written past
+// the caches, and the backward pass reads past them too (16384 x 7168 bf16: its
+// 169 us become 152); the forward pass is faster with ordinary loads (81 us, 95
+// past the caches).
+template <bool STREAM, typename T>
 __device__ __forceinline__ uint4 load_chunk(const T* p, int n) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (n >= Elems<T>::kCount) {
-    __builtin_memcpy(&v, p, 16);
+    if (STREAM && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+      const u32x4 u = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+      v = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      __builtin_memcpy(&v, p, 16);
+    }
   } else if (n > 0) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -78,7 +86,10 @@ template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, const float* f, int n) {
   if (n >= Elems<T>::kCount) {
     const uint4 v = Elems<T>::pack(f);
-    __builtin_memcpy(p, &v, 16);
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0)
+      __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(p));
+    else
+      __builtin_memcpy(p, &v, 16);
   } else {
 #pragma unroll
     for (int j = 0; j < Elems<T>::kCount; ++j)
@@ -86,81 +97,113 @@ __device__ __forceinline__ void store_chunk(T* p, const float* f, int n) {
   }
 }
 
-// Weight or bias element c (fp32 or bf16), 0 past the end.
-__device__ __forceinline__ float param_at(const void* p, int bf16, int c, int cols) {
-  if (c >= cols) return 0.0f;
-  return bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[c])
-              : static_cast<const float*>(p)[c];
+// E elements of the weight or bias from c on (fp32 or bf16), 0 past the end.
+template <int E>
+__device__ __forceinline__ void load_params(const void* p, int bf16, int c, int cols, float* v) {
+  const float* f = static_cast<const float*>(p) + c;
+  const uint16_t* h = static_cast<const uint16_t*>(p) + c;
+  if (c + E <= cols) {
+    if (bf16) {
+      uint16_t u[E];
+      __builtin_memcpy(u, h, sizeof(u));
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = bf16_bits_to_f32(u[j]);
+    } else {
+      __builtin_memcpy(v, f, 4 * E);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < E; ++j)
+    v[j] = c + j >= cols ? 0.0f : bf16 ? bf16_bits_to_f32(h[j]) : f[j];
 }
 
-// Sum over the workgroup; every thread gets it.  `slots` holds one value per wave
-// and is free again after the next barrier.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-  return v;
-}
-template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float (*slots)[kNormMaxThreads / 64]) {
-  const int waves = (int)(blockDim.x >> 6);
+// Sums over the row's threads, in every one of them.  `slots` holds one value per
+// wave and is free again after the next barrier; 16 lanes read them together.
+template <bool WAVE, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*slots)[kNormMaxThreads / 64]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
-  if (waves == 1) return;
+  const int waves = (int)(blockDim.x >> 6);
+  if (WAVE || waves == 1) return;
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) slots[i][threadIdx.x >> 6] = v[i];
   }
   __syncthreads();
+  const int w = threadIdx.x & 15;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = 0.0f;
-    for (int w = 0; w < waves; ++w) v[i] += slots[i][w];
-  }
+  for (int i = 0; i < N; ++i) v[i] = row16_sum(w < waves ? slots[i][w] : 0.0f);
 }
 
-template <typename T, int CH, bool CENTER>
-__global__ __launch_bounds__(kNormMaxThreads) void k_norm_fwd(NormArgs a) {
+// A thread's place: first row, rows to the next one, and its number among the
+// `threads` of its row.
+template <bool WAVE>
+struct RowPlace {
+  int64_t first, step;
+  int thread, threads;
+  __device__ __forceinline__ RowPlace() {
+    if (WAVE) {
+      const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+      first = (int64_t)blockIdx.x * kWaveRows + wave;
+      step = (int64_t)gridDim.x * kWaveRows;
+      thread = threadIdx.x & 63;
+      threads = 64;
+    } else {
+      first = blockIdx.x;
+      step = gridDim.x;
+      thread = threadIdx.x;
+      threads = blockDim.x;
+    }
+  }
+};
+
+template <typename T, int CH, bool CENTER, bool WAVE>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_norm_fwd(NormArgs a) {
   constexpr int E = Elems<T>::kCount;
   __shared__ float slots[2][2][1][kNormMaxThreads / 64];  // [row parity][sum]
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
-  const int threads = (int)blockDim.x;
+  const RowPlace<WAVE> at_row;
   int n[CH];
   float w[CH * E], b[CH * E];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int at = (threadIdx.x + c * threads) * E;
+    const int at = (at_row.thread + c * at_row.threads) * E;
     n[c] = min(max(a.cols - at, 0), E);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      w[c * E + j] = a.w ? param_at(a.w, a.w_bf16, at + j, a.cols) : 1.0f;
-      b[c * E + j] = CENTER && a.b ? param_at(a.b, a.b_bf16, at + j, a.cols) : 0.0f;
+      w[c * E + j] = 1.0f;
+      b[c * E + j] = 0.0f;
     }
+    if (a.w) load_params<E>(a.w, a.w_bf16, at, a.cols, w + c * E);
+    if (CENTER && a.b) load_params<E>(a.b, a.b_bf16, at, a.cols, b + c * E);
   }
   const float cols = (float)a.cols;  // sums are divided: a constant row's mean is its value
   uint4 next[CH];
-  int64_t row = blockIdx.x;
+  int64_t row = at_row.first;
+  if (row < a.rows)
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-    next[c] = load_chunk<T>(x + row * a.ldx + (int64_t)(threadIdx.x + c * threads) * E, n[c]);
-  for (int parity = 0; row < a.rows; row += gridDim.x, parity ^= 1) {
+    for (int c = 0; c < CH; ++c)
+      next[c] = load_chunk<false>(x + row * a.ldx + (int64_t)(at_row.thread + c * at_row.threads) * E, n[c]);
+  for (int parity = 0; row < a.rows; row += at_row.step, parity ^= 1) {
     float v[CH * E];
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < E; ++j) v[c * E + j] = Elems<T>::get(next[c], j);
-    const int64_t after = row + gridDim.x;
+    const int64_t after = row + at_row.step;
     if (after < a.rows) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        next[c] = load_chunk<T>(x + after * a.ldx + (int64_t)(threadIdx.x + c * threads) * E, n[c]);
+        next[c] = load_chunk<false>(x + after * a.ldx + (int64_t)(at_row.thread + c * at_row.threads) * E, n[c]);
     }
     float mu = 0.0f;
     if (CENTER) {
       float s[1] = {0.0f};
 #pragma unroll
       for (int i = 0; i < CH * E; ++i) s[0] += v[i];
-      block_sum<1>(s, slots[parity][0]);
+      row_sum<WAVE, 1>(s, slots[parity][0]);
       mu = s[0] / cols;
     }
     float s[1] = {0.0f};
@@ -172,7 +215,7 @@ __global__ __launch_bounds__(kNormMaxThreads) void k_norm_fwd(NormArgs a) {
         if (CENTER) d = j < n[c] ? d - mu : 0.0f;
         s[0] = __builtin_fmaf(d, d, s[0]);
       }
-    block_sum<1>(s, slots[parity][1]);
+    row_sum<WAVE, 1>(s, slots[parity][1]);
     const float r = 1.0f / sqrtf(s[0] / cols + a.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -181,92 +224,117 @@ __global__ __launch_bounds__(kNormMaxThreads) void k_norm_fwd(NormArgs a) {
       for (int j = 0; j < E; ++j)
         o[j] = CENTER ? __builtin_fmaf(v[c * E + j] * r, w[c * E + j], b[c * E + j])
                       : v[c * E + j] * r * w[c * E + j];
-      store_chunk<T>(y + row * a.ldy + (int64_t)(threadIdx.x + c * threads) * E, o, n[c]);
+      store_chunk<T>(y + row * a.ldy + (int64_t)(at_row.thread + c * at_row.threads) * E, o, n[c]);
     }
-    if (a.stats && threadIdx.x == 0) {
+    if (a.stats && at_row.thread == 0) {
       if (CENTER) a.stats[row] = mu;
       a.stats[a.rows + row] = r;
     }
   }
 }
 
-template <typename T, int CH, bool CENTER>
-__global__ __launch_bounds__(kNormMaxThreads) void k_norm_bwd(NormGradArgs a) {
+template <typename T, int CH, bool CENTER, bool WAVE>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_norm_bwd(NormGradArgs a) {
   constexpr int E = Elems<T>::kCount;
   __shared__ float slots[2][2][kNormMaxThreads / 64];
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   T* dx = static_cast<T*>(a.dx);
-  const int threads = (int)blockDim.x;
+  const RowPlace<WAVE> at_row;
   int n[CH];
   float w[CH * E], dw[CH * E], db[CH * E];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int at = (threadIdx.x + c * threads) * E;
+    const int at = (at_row.thread + c * at_row.threads) * E;
     n[c] = min(max(a.cols - at, 0), E);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      w[c * E + j] = a.w ? param_at(a.w, a.w_bf16, at + j, a.cols) : 1.0f;
+      w[c * E + j] = 1.0f;
       dw[c * E + j] = db[c * E + j] = 0.0f;
     }
+    if (a.w) load_params<E>(a.w, a.w_bf16, at, a.cols, w + c * E);
   }
-  const float inv = 1.0f / (float)a.cols;
+  const float cols = (float)a.cols;
   uint4 nx[CH], ng[CH];
-  int64_t row = blockIdx.x;
+  int64_t row = at_row.first;
+  if (row < a.rows)
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int64_t at = (int64_t)(threadIdx.x + c * threads) * E;
-    nx[c] = load_chunk<T>(x + row * a.ldx + at, n[c]);
-    ng[c] = load_chunk<T>(dy + row * a.lddy + at, n[c]);
-  }
-  for (int parity = 0; row < a.rows; row += gridDim.x, parity ^= 1) {
+    for (int c = 0; c < CH; ++c) {
+      const int64_t at = (int64_t)(at_row.thread + c * at_row.threads) * E;
+      nx[c] = load_chunk<true>(x + row * a.ldx + at, n[c]);
+      ng[c] = load_chunk<true>(dy + row * a.lddy + at, n[c]);
+    }
+  for (int parity = 0; row < a.rows; row += at_row.step, parity ^= 1) {
     const float mu = CENTER ? a.stats[row] : 0.0f, r = a.stats[a.rows + row];
-    float h[CH * E], g[CH * E];
+    // the chunks stay packed; xhat and dy w are formed again after the sums
+    uint4 cx[CH], cg[CH];
     float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      cx[c] = nx[c];
+      cg[c] = ng[c];
+    }
+    const int64_t after = row + at_row.step;
+    if (after < a.rows) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int64_t at = (int64_t)(at_row.thread + c * at_row.threads) * E;
+        nx[c] = load_chunk<true>(x + after * a.ldx + at, n[c]);
+        ng[c] = load_chunk<true>(dy + after * a.lddy + at, n[c]);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int i = c * E + j;
         // past the end of the row dy is 0, so xhat's value there does not matter
-        h[i] = (Elems<T>::get(nx[c], j) - mu) * r;
-        g[i] = Elems<T>::get(ng[c], j);
-        dw[i] = __builtin_fmaf(g[i], h[i], dw[i]);
-        db[i] += g[i];
-        g[i] *= w[i];
-        s[0] = __builtin_fmaf(g[i], h[i], s[0]);
-        s[1] += g[i];
+        const float h = (Elems<T>::get(cx[c], j) - mu) * r, g = Elems<T>::get(cg[c], j);
+        dw[i] = __builtin_fmaf(g, h, dw[i]);
+        db[i] += g;
+        const float u = g * w[i];
+        s[0] = __builtin_fmaf(u, h, s[0]);
+        s[1] += u;
       }
-    const int64_t after = row + gridDim.x;
-    if (after < a.rows) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int64_t at = (int64_t)(threadIdx.x + c * threads) * E;
-        nx[c] = load_chunk<T>(x + after * a.ldx + at, n[c]);
-        ng[c] = load_chunk<T>(dy + after * a.lddy + at, n[c]);
-      }
-    }
     if (!dx) continue;
-    block_sum<2>(s, slots[parity]);
-    const float mh = s[0] * inv, mg = CENTER ? s[1] * inv : 0.0f;
+    row_sum<WAVE, 2>(s, slots[parity]);
+    const float mh = s[0] / cols, mg = CENTER ? s[1] / cols : 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float o[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const int i = c * E + j;
-        o[j] = r * (g[i] - mg - h[i] * mh);
+        const float h = (Elems<T>::get(cx[c], j) - mu) * r;
+        o[j] = r * (Elems<T>::get(cg[c], j) * w[c * E + j] - mg - h * mh);
       }
-      store_chunk<T>(dx + row * a.lddx + (int64_t)(threadIdx.x + c * threads) * E, o, n[c]);
+      store_chunk<T>(dx + row * a.lddx + (int64_t)(at_row.thread + c * at_row.threads) * E, o, n[c]);
     }
   }
   // this workgroup's part of dw and db: fp32 [2][grid][cols]
   if (!a.partial) return;
   float* pw = a.partial + (int64_t)blockIdx.x * a.cols;
   float* pb = pw + (int64_t)gridDim.x * a.cols;
+  if constexpr (WAVE) {  // the waves' sums first, in wave order
+    __shared__ float part[kWaveRows][64 * CH * E];
+    for (int k = 0; k < 2; ++k) {
+      if (k ? !a.db : !a.dw) continue;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < CH * E; ++i)
+        part[threadIdx.x >> 6][i * 64 + at_row.thread] = k ? db[i] : dw[i];
+      __syncthreads();
+      for (int e = threadIdx.x; e < 64 * CH * E; e += 64 * kWaveRows) {
+        const int i = e >> 6, col = ((e & 63) + i / E * 64) * E + i % E;
+        float v = 0.0f;
+        for (int u = 0; u < kWaveRows; ++u) v += part[u][e];
+        if (col < a.cols) (k ? pb : pw)[col] = v;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int at = (threadIdx.x + c * threads) * E;
+    const int at = (at_row.thread + c * at_row.threads) * E;
 #pragma unroll
     for (int j = 0; j < E; ++j)
       if (j < n[c]) {
@@ -277,8 +345,8 @@ __global__ __launch_bounds__(kNormMaxThreads) void k_norm_bwd(NormGradArgs a) {
 }
 
 // dw[c] and db[c] (blockIdx.y) from the partials of `parts` workgroups: 64
-// columns a workgroup, 4 runs of workgroups side by side, added in order.
-constexpr int kNormReduceCols = 64, kNormReduceRuns = 4;
+// columns a workgroup, 16 runs of partials side by side, joined in order.
+constexpr int kNormReduceCols = 64, kNormReduceRuns = 16;
 __global__ __launch_bounds__(kNormReduceCols* kNormReduceRuns) void k_norm_reduce(
     const float* __restrict__ partial, int parts, int cols, void* dw, int dw_bf16, void* db,
     int db_bf16) {
@@ -289,10 +357,20 @@ __global__ __launch_bounds__(kNormReduceCols* kNormReduceRuns) void k_norm_reduc
   if (!out) return;
   const int bf16 = blockIdx.y ? db_bf16 : dw_bf16;
   const float* p = partial + (int64_t)blockIdx.y * parts * cols;
-  const int per = (parts + kNormReduceRuns - 1) / kNormReduceRuns;
   float s = 0.0f;
-  if (c < cols)
-    for (int i = run * per; i < min(parts, (run + 1) * per); ++i) s += p[(int64_t)i * cols + c];
+  if (c < cols) {
+    constexpr int kAhead = 8;  // loads in flight
+    for (int i0 = run; i0 < parts; i0 += kNormReduceRuns * kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kNormReduceRuns;
+        v[u] = i < parts ? p[(int64_t)i * cols + c] : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) s += v[u];
+    }
+  }
   sums[run][lane] = s;
   __syncthreads();
   if (run != 0 || c >= cols) return;
@@ -303,47 +381,68 @@ __global__ __launch_bounds__(kNormReduceCols* kNormReduceRuns) void k_norm_reduc
     static_cast<float*>(out)[c] = s;
 }
 
-// Threads, and chunks a thread, for a row: as few chunks as kNormMaxThreads allow.
+// How a row of `cols` is shared out: rows of at most 1024 elements go to one wave,
+// longer ones to a workgroup with four chunks a thread, or more where 512 threads
+// ask for it.  Four chunks against one a thread (7168 bf16: 256 threads against
+// 896), forward 81 us against 88, with the backward pass 250 against 263: fewer
+// waves share a row's reductions.
 struct NormShape {
   int ch, threads;
+  bool wave;
 };
 NormShape norm_shape(int cols, int per_chunk) {
   const int chunks = (cols + per_chunk - 1) / per_chunk;
-  int ch = 2;
-  while (ch * kNormMaxThreads < chunks) ch *= 2;
-  const int threads = (chunks + ch - 1) / ch;
-  return {ch, (threads + 63) / 64 * 64};
+  if (cols <= 1024) {
+    int ch = 1;
+    while (64 * ch < chunks) ch *= 2;
+    return {ch, 64 * kWaveRows, true};
+  }
+  int ch = 4;
+  while (kNormMaxThreads * ch < chunks) ch *= 2;
+  return {ch, ((chunks + ch - 1) / ch + 63) / 64 * 64, false};
 }
 
-template <typename T, bool CENTER>
-hipError_t run_fwd(const NormArgs& a, int grid, const NormShape& s, hipStream_t stream) {
-  if (s.ch == 2)
-    hipLaunchKernelGGL((k_norm_fwd<T, 2, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if (s.ch == 4)
-    hipLaunchKernelGGL((k_norm_fwd<T, 4, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if (sizeof(T) == 2 || s.ch == 8)  // 32768 is the longest row: 8 chunks of bf16
-    hipLaunchKernelGGL((k_norm_fwd<T, 8, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((k_norm_fwd<T, 16, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
+template <typename T, bool CENTER, int CH, bool WAVE>
+void run_norm(const NormArgs& a, int grid, int threads, hipStream_t stream) {
+  hipLaunchKernelGGL((k_norm_fwd<T, CH, CENTER, WAVE>), dim3(grid), dim3(threads), 0, stream, a);
+}
+template <typename T, bool CENTER, int CH, bool WAVE>
+void run_norm(const NormGradArgs& a, int grid, int threads, hipStream_t stream) {
+  hipLaunchKernelGGL((k_norm_bwd<T, CH, CENTER, WAVE>), dim3(grid), dim3(threads), 0, stream, a);
+}
+// Chunks reached: one wave 1, 2 (bf16: 1024 = 2 * 64 * 8) and 4 (fp32); workgroups
+// 4, 8 (bf16: 32768 = 8 * 512 * 8) and 16 (fp32).
+template <typename T, bool CENTER, typename Args>
+hipError_t run_shape(const Args& a, int grid, const NormShape& s, hipStream_t stream) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  if (s.wave) {
+    if (s.ch == 1) run_norm<T, CENTER, 1, true>(a, grid, s.threads, stream);
+    else if (!kF32 || s.ch == 2) run_norm<T, CENTER, 2, true>(a, grid, s.threads, stream);
+    else if constexpr (kF32) run_norm<T, CENTER, 4, true>(a, grid, s.threads, stream);
+  } else {
+    if (s.ch == 4) run_norm<T, CENTER, 4, false>(a, grid, s.threads, stream);
+    else if (!kF32 || s.ch == 8) run_norm<T, CENTER, 8, false>(a, grid, s.threads, stream);
+    else if constexpr (kF32) run_norm<T, CENTER, 16, false>(a, grid, s.threads, stream);
+  }
   return hipGetLastError();
 }
-template <typename T, bool CENTER>
-hipError_t run_bwd(const NormGradArgs& a, int grid, const NormShape& s, hipStream_t stream) {
-  if (s.ch == 2)
-    hipLaunchKernelGGL((k_norm_bwd<T, 2, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if (s.ch == 4)
-    hipLaunchKernelGGL((k_norm_bwd<T, 4, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if (sizeof(T) == 2 || s.ch == 8)  // 32768 is the longest row: 8 chunks of bf16
-    hipLaunchKernelGGL((k_norm_bwd<T, 8, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  else if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((k_norm_bwd<T, 16, CENTER>), dim3(grid), dim3(s.threads), 0, stream, a);
-  return hipGetLastError();
+template <typename Args>
+hipError_t run_types(const Args& a, int grid, const NormShape& s, hipStream_t stream) {
+  if (a.bf16)
+    return a.center ? run_shape<uint16_t, true>(a, grid, s, stream)
+                    : run_shape<uint16_t, false>(a, grid, s, stream);
+  return a.center ? run_shape<float, true>(a, grid, s, stream)
+                  : run_shape<float, false>(a, grid, s, stream);
 }
 
-// Waves that a CU holds of these kernels, and the grid that fills the chip.
-int norm_grid(int64_t rows, int threads, int waves_cu) {
-  const int64_t per_cu = std::max(1, waves_cu / (threads / 64));
-  return (int)std::min<int64_t>(rows, std::max(1, device_cu_count()) * per_cu);
+// Workgroups: 32 chunks a lane on every compute unit (32 KB of a row's loads in
+// flight each).  7168 bf16, waves a unit, forward us: 4 112, 8 81, 12 89, 16 93;
+// with the backward pass 4 294, 8 250, 12 310 (its registers hold 8).
+int norm_grid(int64_t rows, const NormShape& s) {
+  const int waves = std::max(1, 32 / s.ch);
+  const int64_t per_cu = std::max(1, waves / (s.threads / 64));
+  const int64_t own = s.wave ? (rows + kWaveRows - 1) / kWaveRows : rows;
+  return (int)std::min<int64_t>(own, std::max(1, device_cu_count()) * per_cu);
 }
 
 }  // namespace
@@ -351,30 +450,18 @@ int norm_grid(int64_t rows, int threads, int waves_cu) {
 hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;
   const NormShape s = norm_shape(a.cols, a.bf16 ? 8 : 4);
-  const int grid = norm_grid(a.rows, s.threads, 16);
-  if (a.bf16)
-    return a.center ? run_fwd<uint16_t, true>(a, grid, s, stream)
-                    : run_fwd<uint16_t, false>(a, grid, s, stream);
-  return a.center ? run_fwd<float, true>(a, grid, s, stream)
-                  : run_fwd<float, false>(a, grid, s, stream);
+  return run_types(a, norm_grid(a.rows, s), s, stream);
 }
 
 int norm_grad_parts(int64_t rows, int cols, int bf16) {
-  return rows == 0 ? 0 : norm_grid(rows, norm_shape(cols, bf16 ? 8 : 4).threads, 14);
+  const NormShape s = norm_shape(cols, bf16 ? 8 : 4);
+  return rows == 0 ? 0 : norm_grid(rows, s);
 }
 
 hipError_t launch_norm_bwd(const NormGradArgs& a, hipStream_t stream) {
   const int parts = norm_grad_parts(a.rows, a.cols, a.bf16);
   hipError_t err = hipSuccess;
-  if (parts > 0) {
-    const NormShape s = norm_shape(a.cols, a.bf16 ? 8 : 4);
-    if (a.bf16)
-      err = a.center ? run_bwd<uint16_t, true>(a, parts, s, stream)
-                     : run_bwd<uint16_t, false>(a, parts, s, stream);
-    else
-      err = a.center ? run_bwd<float, true>(a, parts, s, stream)
-                     : run_bwd<float, false>(a, parts, s, stream);
-  }
+  if (parts > 0) err = run_types(a, parts, norm_shape(a.cols, a.bf16 ? 8 : 4), stream);
   if (err != hipSuccess || (!a.dw && !a.db)) return err;
   const dim3 grid((unsigned)((a.cols + kNormReduceCols - 1) / kNormReduceCols), 2);
   hipLaunchKernelGGL(k_norm_reduce, grid, dim3(kNormReduceCols * kNormReduceRuns), 0, stream,

@@ -29,6 +29,7 @@ namespace {
 constexpr int kTopkThreads = 256;
 constexpr int kTopkWaves = kTopkThreads / 64;
 constexpr int kGradTile = 2048;  // gradients of a wave's tile, at most
+constexpr int kGradSlots = 128;  // and slots
 
 // LDS index with one word of padding every 32: lanes that walk rows of 32 words
 // in step fall on different banks.
@@ -52,20 +53,29 @@ __device__ __forceinline__ float unsortable(uint32_t k) {
   return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
 }
 
-// Key and index as a double in [1, 2); 0.0 = absent.
+__device__ __forceinline__ double join_f64(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ uint32_t low_word(double v) {
+  return (uint32_t)__builtin_bit_cast(uint64_t, v);
+}
+__device__ __forceinline__ uint32_t high_word(double v) {
+  return (uint32_t)(__builtin_bit_cast(uint64_t, v) >> 32);
+}
+// Key and index as a double in [1, 2); absent: a high word of 0, which is below
+// every key whatever the low word holds.
 constexpr uint32_t kIndexMask = 1023u;
 static_assert(kMaxGroups <= (int)kIndexMask + 1, "an expert index takes ten bits");
 __device__ __forceinline__ double pack_key(uint32_t key, uint32_t idx) {
-  const uint64_t b =
-      ((uint64_t)(0x3FF00000u | (key >> 12)) << 32) | (key << 20) | (kIndexMask - idx);
-  return __builtin_bit_cast(double, b);
+  return join_f64((key << 20) | (kIndexMask - idx), __builtin_amdgcn_alignbit(0x3FFu, key, 12));
 }
 __device__ __forceinline__ uint32_t key_of(double d) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, d);
-  return (uint32_t)(b >> 32) << 12 | (uint32_t)b >> 20;
+  return __builtin_amdgcn_alignbit(high_word(d), low_word(d), 20);
 }
-__device__ __forceinline__ int index_of(double d) {
-  return (int)(kIndexMask - ((uint32_t)__builtin_bit_cast(uint64_t, d) & kIndexMask));
+__device__ __forceinline__ int index_of(double d) { return (int)(kIndexMask - (low_word(d) & kIndexMask)); }
+__device__ __forceinline__ bool absent(double d) { return high_word(d) == 0u; }
+__device__ __forceinline__ double absent_if(bool out, double d) {
+  return join_f64(low_word(d), out ? 0u : high_word(d));
 }
 
 // Plain v_max_f64 / v_min_f64: the keys are ordinary numbers, so the
@@ -120,22 +130,50 @@ __device__ __forceinline__ void merge_top(double (&a)[L], const double (&b)[L]) 
 }
 
 __device__ __forceinline__ double shfl_xor_f64(double v, int off) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, off);
-  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(b >> 32), off);
-  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+  return join_f64((uint32_t)__shfl_xor((int)low_word(v), off),
+                  (uint32_t)__shfl_xor((int)high_word(v), off));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  return join_f64((uint32_t)__builtin_amdgcn_mov_dpp((int)low_word(v), CTRL, 0xF, 0xF, false),
+                  (uint32_t)__builtin_amdgcn_mov_dpp((int)high_word(v), CTRL, 0xF, 0xF, false));
 }
 
-// The list of the L largest over this lane and lane ^ off.
+// The list of the L largest over this lane's run of `off` lanes, which all hold the
+// run's list, and the run beside it.  Any lane of the other run will do as the
+// partner: within 16 lanes a DPP mirror (VALU only) reaches one.
 template <int L>
 __device__ __forceinline__ void merge_lanes(double (&a)[L], int off) {
   double b[L];
+  if (off == 1) {
 #pragma unroll
-  for (int i = 0; i < L; ++i) b[i] = shfl_xor_f64(a[i], off);
+    for (int i = 0; i < L; ++i) b[i] = dpp_f64<0xB1>(a[i]);   // quad_perm [1,0,3,2]
+  } else if (off == 2) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) b[i] = dpp_f64<0x4E>(a[i]);   // quad_perm [2,3,0,1]
+  } else if (off == 4) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) b[i] = dpp_f64<0x141>(a[i]);  // row_half_mirror
+  } else if (off == 8) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) b[i] = dpp_f64<0x140>(a[i]);  // row_mirror
+  } else {
+#pragma unroll
+    for (int i = 0; i < L; ++i) b[i] = shfl_xor_f64(a[i], off);
+  }
   merge_top<L>(a, b);
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// The same bits for |x| <= 87: no range tests in the exponential, and one Newton
+// step on v_rcp_f32 for the quotient, which returns the correctly rounded 1 / d for
+// every mantissa of d (checked over all 2^23 of them, and at other exponents).
+constexpr float kModerate = 87.0f;
+__device__ __forceinline__ float sigmoid_moderate(float x) {
+  const float d = 1.0f + exp_moderate(-x), r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-r, d, 1.0f), r, r);
+}
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ float load_one(const uint16_t* p) { return bf16_bits_to_f32(*p); }
@@ -193,20 +231,34 @@ __device__ __forceinline__ int div_k(int p, uint32_t recip) {
   return (int)(((uint32_t)p * recip) >> 20);
 }
 
+// A wave's share of the workgroup's LDS, in words.
+struct TopkLds {
+  int ids, values, stats, words;
+  __host__ __device__ TopkLds(int E, int K, int tokens) {
+    ids = pad32(tokens * E);
+    values = ids + tokens * K;
+    stats = (values + tokens * K + 1) & ~1;
+    words = stats + 2 * tokens;
+  }
+};
+
 template <int VPL, int L, typename T>
 __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
   static_assert(VPL >= L, "a lane's list is cut from its own experts");
-  __shared__ float tiles[kTopkWaves][pad32(64 * VPL)];
-  __shared__ float bias_s[pad32(kMaxGroups)];
-  __shared__ float2 stats[kTopkWaves][64];       // softmax maximum and sum of a token
-  __shared__ int32_t picked[kTopkWaves][64 * L];
-  __shared__ float value[kTopkWaves][64 * L];
+  extern __shared__ float lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int per_wave = 64 / a.lanes;
   const int64_t t0 = ((int64_t)blockIdx.x * kTopkWaves + wave) * per_wave;
   const int nt = (int)std::min<int64_t>(per_wave, std::max<int64_t>(0, a.tokens - t0));
-  float* tile = tiles[wave];
+  // of every wave: its logits, then the slots' ids and values and (max, sum) of a
+  // token's softmax; the bias behind the waves
+  const TopkLds at(a.E, a.K, per_wave);
+  float* tile = lds + wave * at.words;
+  int32_t* pk = reinterpret_cast<int32_t*>(tile + at.ids);
+  float* val = tile + at.values;
+  float2* stats = reinterpret_cast<float2*>(tile + at.stats);
+  float* bias_s = lds + kTopkWaves * at.words;
   load_tile<64 * VPL, T>(static_cast<const T*>(a.logits) + t0 * a.E, nt * a.E, tile);
   if (a.bias != nullptr)
     for (int e = tid; e < a.E; e += kTopkThreads) bias_s[pad32(e)] = a.bias[e];
@@ -237,22 +289,39 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
     for (int v = 0; v < VPL; ++v) total += expf(x[v] - top);
     for (int off = 1; off < a.lanes; off <<= 1) total += __shfl_xor(total, off);
     if (total == 0.0f) total = 1.0f;  // every expert is out
-    if (sub == 0) stats[wave][tok] = make_float2(top, total);
+    if (sub == 0 && tok < nt) stats[tok] = make_float2(top, total);
   }
 
   // choice keys, and the L largest of the lane
   double list[L];
   {
+    float c[VPL];
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) c[v] = x[v];
+    if (a.bias != nullptr) {
+      if (a.softmax) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) c[v] = expf(x[v] - top) / total;
+      } else {
+        bool moderate = true;  // also where the expert is out or absent
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) moderate &= !(__builtin_fabsf(x[v]) > kModerate) || x[v] == kNegInf;
+        if (__all(moderate)) {
+#pragma unroll
+          for (int v = 0; v < VPL; ++v) c[v] = sigmoid_moderate(x[v]);
+        } else {
+#pragma unroll
+          for (int v = 0; v < VPL; ++v) c[v] = sigmoid(x[v]);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < VPL; ++v)
+        c[v] = x[v] == kNegInf ? kNegInf : c[v] + bias_s[pad32(min(e0 + v, a.E - 1))];
+    }
     double key[VPL];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      float c = x[v];
-      if (a.bias != nullptr && v < count) {
-        const float s = a.softmax ? expf(c - top) / total : sigmoid(c);
-        c = c == kNegInf ? c : s + bias_s[pad32(e0 + v)];
-      }
-      key[v] = c == kNegInf ? 0.0 : pack_key(sortable(c), (uint32_t)(e0 + v));
-    }
+    for (int v = 0; v < VPL; ++v)
+      key[v] = absent_if(c[v] == kNegInf, pack_key(sortable(c[v]), (uint32_t)(e0 + v)));
 #pragma unroll
     for (int i = 0; i < L; ++i) list[i] = key[i];
     sort_net<0, L>(list);
@@ -276,28 +345,26 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
       for (int i = 0; i < 2; ++i) {
         w[i] = unsortable(key_of(list[i]));
         if (a.bias == nullptr) w[i] = a.softmax ? expf(w[i] - top) / total : sigmoid(w[i]);
-        if (list[i] == 0.0) w[i] = 0.0f;
+        if (absent(list[i])) w[i] = 0.0f;
       }
       worth = sortable(w[0] + w[1]);
     }
-    const double mine = list[0] == 0.0 ? 0.0 : pack_key(worth, (uint32_t)g);
+    const double mine = absent_if(absent(list[0]), pack_key(worth, (uint32_t)g));
     int above = 0;
     for (int off = a.lanes_group; off < a.lanes; off += a.lanes_group)
       above += shfl_xor_f64(mine, off) > mine ? 1 : 0;
     if (above >= a.top_groups) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) list[i] = 0.0;
+      for (int i = 0; i < L; ++i) list[i] = absent_if(true, list[i]);
     }
     for (int off = a.lanes_group; off < a.lanes; off <<= 1) merge_lanes<L>(list, off);
   }
 
   // weights: one (token, slot) a lane, sums over a token's slots in slot order
-  int32_t* pk = picked[wave];
-  float* val = value[wave];
   if (sub == 0 && tok < nt) {
 #pragma unroll
     for (int i = 0; i < L; ++i)
-      if (i < a.K) pk[tok * a.K + i] = list[i] == 0.0 ? -1 : index_of(list[i]);
+      if (i < a.K) pk[tok * a.K + i] = absent(list[i]) ? -1 : index_of(list[i]);
   }
   wave_sync();
   const int slots = nt * a.K;
@@ -310,7 +377,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
       if (!a.softmax) {
         s = sigmoid(xe);
       } else if (!a.renorm) {
-        s = expf(xe - stats[wave][t].x) / stats[wave][t].y;
+        s = expf(xe - stats[t].x) / stats[t].y;
       } else {
         // relative to the largest selected logit: the first slot's without a bias
         float m = row_x[pad32(t * a.E + pk[t * a.K])];
@@ -351,40 +418,43 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradArgs a) {
   __shared__ float grad_s[kTopkWaves][kGradTile];
+  __shared__ float2 slot_s[kTopkWaves][kGradSlots];  // (s, s dw) of a slot
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t0 = ((int64_t)blockIdx.x * kTopkWaves + wave) * a.tokens_wave;
   const int nt = (int)std::min<int64_t>(a.tokens_wave, std::max<int64_t>(0, a.tokens - t0));
   if (nt == 0) return;
   float* grad = grad_s[wave];
+  float2* slot = slot_s[wave];
   const int n = nt * a.E, slots = nt * a.K;
-  for (int i = 4 * lane; i < n; i += 256)
-    *reinterpret_cast<float4*>(grad + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  wave_sync();
   const int32_t* idx = a.idx + t0 * a.K;
   const float* sel = a.sel + t0 * a.K;
   const float* dw = a.dweights + t0 * a.K;
+  for (int p = lane; p < slots; p += 64) {  // slots without an expert add nothing
+    const bool live = (uint32_t)idx[p] < (uint32_t)a.E;
+    const float s = live ? sel[p] : 0.0f;
+    slot[p] = make_float2(s, live ? s * dw[p] : 0.0f);
+  }
+  for (int i = 4 * lane; i < n; i += 256)
+    *reinterpret_cast<float4*>(grad + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  wave_sync();
   for (int p = lane; p < slots; p += 64) {
     const int t = div_k(p, a.k_recip), e = idx[p];
     if ((uint32_t)e >= (uint32_t)a.E) continue;
-    const float s = sel[p];
-    float d = dw[p], g;
-    if (a.renorm || a.softmax) {
-      float dot = 0.0f, sum = 0.0f;
+    float dot = 0.0f, sum = 0.0f;
+    if (a.renorm)
       for (int j = 0; j < a.K; ++j) {
-        const int q = t * a.K + j;
-        if ((uint32_t)idx[q] < (uint32_t)a.E) {
-          dot += sel[q] * dw[q];
-          sum += sel[q];
-        }
+        sum += slot[t * a.K + j].x;
+        dot += slot[t * a.K + j].y;
       }
-      if (a.softmax)
-        g = a.scale * (a.renorm ? s * (d - dot) : d);
-      else
-        g = sum == 0.0f ? 0.0f : a.scale * (d - dot / sum) / sum * s * (1.0f - s);
-    } else {
+    const float s = slot[p].x, d = dw[p];
+    float g;
+    if (a.softmax)
+      g = a.scale * (a.renorm ? s * (d - dot) : d);
+    else if (a.renorm)
+      g = sum == 0.0f ? 0.0f : a.scale * (d - dot / sum) / sum * s * (1.0f - s);
+    else
       g = a.scale * d * s * (1.0f - s);
-    }
     grad[t * a.E + e] = g;
   }
   wave_sync();
@@ -399,10 +469,7 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradA
       for (int e = sub; e < a.E; e += lanes) total += expf(load_one(x + e) - top);
       for (int off = 1; off < lanes; off <<= 1) total += __shfl_xor(total, off);
       if (total == 0.0f) total = 1.0f;
-      for (int j = 0; j < a.K; ++j) {
-        const int q = t * a.K + j;
-        if ((uint32_t)idx[q] < (uint32_t)a.E) dot += sel[q] * a.scale * dw[q];
-      }
+      for (int j = 0; j < a.K; ++j) dot += a.scale * slot[t * a.K + j].y;
       for (int e = sub; e < a.E; e += lanes) {
         const float p = expf(load_one(x + e) - top) / total;
         grad[t * a.E + e] = p * (grad[t * a.E + e] - dot);
@@ -419,26 +486,43 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradA
   }
 }
 
+constexpr int64_t kSmallExperts = INT64_C(1) << 21;
+
 int next_pow2(int v) {
   int p = 1;
   while (p < v) p <<= 1;
   return p;
 }
 
+// Lanes of a group and of a token.  Longer lists take more lanes, so fewer tokens
+// and slots a wave: the LDS of a workgroup stays below 64 KB.
+template <int VPL, int L>
+void set_lanes(RouteTopkArgs& a) {
+  const int per = a.E / a.groups, groups = next_pow2(a.groups);
+  a.lanes_group = std::max(next_pow2((per + VPL - 1) / VPL), L / 8 / groups);
+  a.lanes = a.lanes_group * groups;
+}
+
 template <int VPL, int L, typename T>
 hipError_t run_topk(RouteTopkArgs a, hipStream_t stream) {
-  const int per = a.E / a.groups;
-  a.lanes_group = next_pow2((per + VPL - 1) / VPL);
-  a.lanes = a.lanes_group * next_pow2(a.groups);
+  set_lanes<VPL, L>(a);
   const int64_t tokens = (int64_t)kTopkWaves * (64 / a.lanes);
+  const int words = kTopkWaves * TopkLds(a.E, a.K, 64 / a.lanes).words + (a.bias ? pad32(a.E) : 0);
   hipLaunchKernelGGL((k_route_topk<VPL, L, T>), dim3((unsigned)((a.tokens + tokens - 1) / tokens)),
-                     dim3(kTopkThreads), 0, stream, a);
+                     dim3(kTopkThreads), 4 * words, stream, a);
   return hipGetLastError();
 }
 
+// Lists of the smallest length that holds topk, cut from 32 experts a lane (32
+// lanes hold 1024).  Few tokens take 8 experts a lane where 64 lanes hold them, so
+// that the chip has more waves of less work.
 template <typename T>
-hipError_t run_topk_list(const RouteTopkArgs& a, hipStream_t stream) {
-  if (a.K <= 8) return run_topk<32, 8, T>(a, stream);
+hipError_t run_topk_list(RouteTopkArgs a, hipStream_t stream) {
+  if (a.K <= 8) {
+    set_lanes<8, 8>(a);
+    if (a.lanes <= 64 && a.tokens * a.E <= kSmallExperts) return run_topk<8, 8, T>(a, stream);
+    return run_topk<32, 8, T>(a, stream);
+  }
   if (a.K <= 16) return run_topk<32, 16, T>(a, stream);
   return run_topk<32, 32, T>(a, stream);
 }
@@ -454,8 +538,9 @@ hipError_t launch_route_topk(RouteTopkArgs a, hipStream_t stream) {
 hipError_t launch_route_topk_grad(RouteTopkGradArgs a, hipStream_t stream) {
   if (a.tokens == 0) return hipSuccess;
   a.k_recip = (uint32_t)(((1u << 20) + a.K - 1) / a.K);
-  // whole tokens a wave: as many as its LDS tile holds, a power of two
-  a.tokens_wave = 64;
+  // whole tokens a wave, a power of two: as many as its LDS tile holds, and about a
+  // slot for every lane (16384 x 32, top-8: 64 tokens a wave 17.0 us, 8 tokens 3.7)
+  a.tokens_wave = next_pow2((64 + a.K - 1) / a.K);
   while (a.tokens_wave * a.E > kGradTile) a.tokens_wave >>= 1;
   const int64_t tokens = (int64_t)kTopkWaves * a.tokens_wave;
   const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens));

@@ -75,6 +75,22 @@ def test_groups_by_two_best_scores(gpu, score):
     _check(x, 6, dict(score=score, num_groups=6, top_groups=2, group_best=2, renormalize=True))
 
 
+@pytest.mark.parametrize("score,biased,best", [("softmax", False, 1), ("sigmoid", True, 2)])
+@pytest.mark.parametrize("E,G,K", [(256, 8, 8), (32, 1, 8), (320, 8, 6), (1024, 1, 3)])
+def test_large_and_small_calls_agree(gpu, E, G, K, score, biased, best):
+    """The same bits whether a token comes in a call of millions of logits or in
+    one of few (other shares of a token to a lane)."""
+    T = 2_500_000 // E
+    x = _logits(gpu, T, E, torch.float32, E)
+    bias = (torch.randn(E, generator=torch.Generator().manual_seed(E)) * 0.1).to(gpu)
+    f = lambda z: mxfp8gg.route_topk(z, K, score=score, num_groups=G, top_groups=(G + 1) // 2,  # noqa: E731
+                                     group_best=best, bias=bias if biased else None)
+    idx, w = f(x)
+    for a in (0, 777, T - 100):
+        i, v = f(x[a:a + 100])
+        assert torch.equal(i, idx[a:a + 100]) and torch.equal(v, w[a:a + 100])
+
+
 def test_all_experts_equal_take_the_lowest_ids(gpu):
     for E, K, G in ((64, 8, 1), (256, 8, 8), (1024, 32, 4)):
         idx, w = mxfp8gg.route_topk(torch.zeros((5, E), device=gpu), K, num_groups=G, top_groups=1)
