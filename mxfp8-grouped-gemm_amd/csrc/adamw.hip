@@ -27,7 +27,9 @@ namespace {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamVec = 8;
-constexpr int64_t kAdamChunk = 4096;  // elements of a workgroup
+// Elements of a workgroup, 8 a thread.  Twice as many in a loop of two trips:
+// 235 M bf16 weights with fp32 states 1257 us against 1228, 8-bit 437 against 430.
+constexpr int64_t kAdamChunk = kAdamThreads * kAdamVec;
 constexpr int kAdamTensors = 48;      // of a launch: 3.3 of the 4 KB of kernel arguments
 
 struct AdamTable {
@@ -161,51 +163,46 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw(AdamTable a) {
   const int64_t base = (int64_t)((int)blockIdx.x - a.first[lo]) * kAdamChunk;
   void* weights = t.master ? static_cast<void*>(t.master) : t.param;
   const bool w_bf16 = !t.master && t.param_bf16;
-#pragma unroll 1
-  for (int k = 0; k < (int)(kAdamChunk / (kAdamThreads * kAdamVec)); ++k) {
-    const int64_t i = base + (int64_t)(k * kAdamThreads + (int)threadIdx.x) * kAdamVec;
-    const int64_t left = t.n - i;
-    const int n = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-    if (!__any(n > 0)) break;
-    float p[8], g[8], m[8], v[8];
-    if (n > 0) {
-      load8(weights, w_bf16, i, n, p);
-      load8(t.grad, t.grad_bf16, i, n, g);
-    } else {
+  const int64_t i = base + (int64_t)threadIdx.x * kAdamVec, left = t.n - i;
+  const int n = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+  float p[8], g[8], m[8], v[8];
+  if (n > 0) {
+    load8(weights, w_bf16, i, n, p);
+    load8(t.grad, t.grad_bf16, i, n, g);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = g[j] = 0.0f;
-    }
-    if (SMALL) {
-      unpack8(static_cast<const uint8_t*>(t.m), t.m_scales, i, n, m);
-      unpack8(static_cast<const uint8_t*>(t.v), t.v_scales, i, n, v);
-    } else if (n > 0) {
-      load8(t.m, false, i, n, m);
-      load8(t.v, false, i, n, v);
-    } else {
+    for (int j = 0; j < 8; ++j) p[j] = g[j] = 0.0f;
+  }
+  if (SMALL) {
+    unpack8(static_cast<const uint8_t*>(t.m), t.m_scales, i, n, m);
+    unpack8(static_cast<const uint8_t*>(t.v), t.v_scales, i, n, v);
+  } else if (n > 0) {
+    load8(t.m, false, i, n, m);
+    load8(t.v, false, i, n, v);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m[j] = v[j] = 0.0f;
-    }
+    for (int j = 0; j < 8; ++j) m[j] = v[j] = 0.0f;
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = m[j] * s.beta1 + g[j] * s.one_beta1;
-      const float old = SMALL ? v[j] * v[j] : v[j];
-      const float now = old * s.beta2 + (g[j] * g[j]) * s.one_beta2;
-      const float root = sqrtf(now);
-      v[j] = SMALL ? root : now;
-      p[j] = p[j] * s.decay - s.step_size * (m[j] / (root * s.inv_root_bias2 + s.eps));
+  for (int j = 0; j < 8; ++j) {
+    m[j] = m[j] * s.beta1 + g[j] * s.one_beta1;
+    const float old = SMALL ? v[j] * v[j] : v[j];
+    const float now = old * s.beta2 + (g[j] * g[j]) * s.one_beta2;
+    const float root = sqrtf(now);
+    v[j] = SMALL ? root : now;
+    p[j] = p[j] * s.decay - s.step_size * (m[j] / (root * s.inv_root_bias2 + s.eps));
+  }
+  if (SMALL) {
+    pack8(static_cast<uint8_t*>(t.m), t.m_scales, i, n, m);
+    pack8(static_cast<uint8_t*>(t.v), t.v_scales, i, n, v);
+  }
+  if (n > 0) {
+    if (!SMALL) {
+      store8(t.m, false, i, n, m);
+      store8(t.v, false, i, n, v);
     }
-    if (SMALL) {
-      pack8(static_cast<uint8_t*>(t.m), t.m_scales, i, n, m);
-      pack8(static_cast<uint8_t*>(t.v), t.v_scales, i, n, v);
-    }
-    if (n > 0) {
-      if (!SMALL) {
-        store8(t.m, false, i, n, m);
-        store8(t.v, false, i, n, v);
-      }
-      store8(weights, w_bf16, i, n, p);
-      if (t.master) store8(t.param, t.param_bf16, i, n, p);
-    }
+    store8(weights, w_bf16, i, n, p);
+    if (t.master) store8(t.param, t.param_bf16, i, n, p);
   }
 }
 

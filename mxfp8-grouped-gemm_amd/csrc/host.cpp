@@ -17,6 +17,7 @@
 // another ABI version than the header this module was compiled with.
 #include <torch/extension.h>
 
+#include <cstring>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -38,7 +39,9 @@ struct Lib {
   MXGG_FN(quant_dim0) MXGG_FN(quant_dim1) MXGG_FN(quant_dual) MXGG_FN(zero_rows_past_groups) \
   MXGG_FN(grouped_fwd) MXGG_FN(grouped_fwd_split) MXGG_FN(grouped_fwd_swiglu_quant)          \
   MXGG_FN(grouped_fwd_swiglu_quant_keep_h) MXGG_FN(grouped_wgrad) MXGG_FN(swiglu_bwd_quant)  \
-  MXGG_FN(gather_quant_dual) MXGG_FN(gather_quant_dim0) MXGG_FN(combine)
+  MXGG_FN(gather_quant_dual) MXGG_FN(gather_quant_dim0) MXGG_FN(combine)                     \
+  MXGG_FN(route_topk) MXGG_FN(route_topk_grad) MXGG_FN(norm) MXGG_FN(norm_grad)              \
+  MXGG_FN(norm_grad_workspace_bytes) MXGG_FN(adamw_step) MXGG_FN(last_error)
   MXGG_FNS
 #undef MXGG_FN
 };
@@ -382,6 +385,224 @@ Result combine(const Tensor& y, const Tensor& perm, int64_t tokens, int topk,
   return out;
 }
 
+// The operators below are differentiable here as well: an autograd function in
+// Python costs more host time than their kernels take on small inputs.  Their
+// backward passes launch on the stream of the forward pass, where autograd runs
+// them.  Arguments that the library would refuse are left to the Python form.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check(int rc, const char* what) {
+  TORCH_CHECK(rc == MXGG_OK, what, ": status ", rc, ": ", lib.last_error());
+}
+// A plain struct kept for the backward pass.
+template <class T>
+void keep(AutogradContext* ctx, const char* name, const T& v) {
+  ctx->saved_data[name] = std::string(reinterpret_cast<const char*>(&v), sizeof(T));
+}
+template <class T>
+T kept(AutogradContext* ctx, const char* name) {
+  T v;
+  const std::string s = ctx->saved_data[name].toStringRef();
+  std::memcpy(&v, s.data(), sizeof(T));
+  return v;
+}
+bool grad_needed(const OptTensor& a) { return a && a->requires_grad(); }
+bool f32_or_bf16(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+int32_t type_of(const Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 ? MXGG_OUT_BF16 : MXGG_OUT_F32;
+}
+void* vp_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const void* cp_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// (expert_idx, weights) and, for the gradient, the selected scores.
+variable_list route_forward(const Tensor& logits, const float* bias,
+                            const mxgg_route_options& o, bool keep_selected, int64_t stream) {
+  const int64_t tokens = logits.size(0);
+  Tensor idx = empty({tokens, o.topk}, logits, at::kInt);
+  Tensor weights = empty({tokens, o.topk}, logits, at::kFloat);
+  Tensor selected;
+  if (keep_selected) selected = empty({tokens, o.topk}, logits, at::kFloat);
+  check(lib.route_topk(cp(logits), tokens, bias, &o,
+                       idx.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                       static_cast<float*>(vp_or_null(selected)), st(stream)),
+        "route_topk");
+  return {idx, weights, selected};
+}
+
+struct RouteTopK : torch::autograd::Function<RouteTopK> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const float* bias,
+                               const mxgg_route_options& o, int64_t stream) {
+    variable_list r = route_forward(logits, bias, o, true, stream);
+    const bool whole = o.score == MXGG_SCORE_SOFTMAX && !o.renormalize;
+    ctx->save_for_backward({r[0], r[2], whole ? logits : Tensor()});
+    keep(ctx, "options", o);
+    ctx->saved_data["stream"] = stream;
+    ctx->mark_non_differentiable({r[0]});
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const auto o = kept<mxgg_route_options>(ctx, "options");
+    const Tensor d = grads[1].to(at::kFloat).contiguous();
+    Tensor out = empty({d.size(0), o.experts}, d,
+                       o.dtype == MXGG_OUT_BF16 ? at::kBFloat16 : at::kFloat);
+    check(lib.route_topk_grad(d.const_data_ptr<float>(), saved[0].const_data_ptr<int32_t>(),
+                              saved[1].const_data_ptr<float>(), cp_or_null(saved[2]), d.size(0),
+                              &o, vp(out), st(ctx->saved_data["stream"].toInt())),
+          "route_topk_grad");
+    return {out, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Result route_topk(const Tensor& logits, const OptTensor& bias, int64_t topk, int64_t groups,
+                  int64_t top_groups, int score, int group_best, bool renormalize, double scale,
+                  int64_t stream) {
+  if (!plain(logits) || logits.dim() != 2 || !f32_or_bf16(logits) || !logits.is_contiguous() ||
+      (bias && (!plain(*bias) || bias->scalar_type() != at::kFloat || bias->dim() != 1 ||
+                bias->size(0) != logits.size(1) || !bias->is_contiguous() ||
+                bias->device() != logits.device())))
+    return none();
+  const int64_t E = logits.size(1);
+  if (E > 1024 || topk < 1 || topk > std::min<int64_t>(E, 32) || groups < 1 || groups > 64 ||
+      E % groups != 0 || top_groups < 1 || top_groups > groups ||
+      (group_best != 1 && group_best != 2) || logits.size(0) >= INT64_C(1) << 24)
+    return none();
+  const mxgg_route_options o{E,          topk,           groups,     top_groups,
+                             score,      type_of(logits), group_best, renormalize,
+                             (float)scale};
+  const float* b = bias ? bias->const_data_ptr<float>() : nullptr;
+  variable_list r = at::GradMode::is_enabled() && logits.requires_grad()
+                        ? RouteTopK::apply(logits, b, o, stream)
+                        : route_forward(logits, b, o, false, stream);
+  return std::make_tuple(r[0], r[1]);
+}
+
+// Rows that the norm kernels read in place: the row stride, or -1.
+int64_t row_stride(const Tensor& t) {
+  const int64_t cols = t.size(-1);
+  if (t.is_contiguous()) return cols;
+  return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= cols ? t.stride(0) : -1;
+}
+variable_list norm_forward(const Tensor& x, const OptTensor& w, const OptTensor& b,
+                           const mxgg_norm_options& o, bool keep_stats, int64_t stream) {
+  Tensor y = empty(x.sizes(), x, x.scalar_type()), stats;
+  if (keep_stats) stats = empty({2, o.rows}, x, at::kFloat);
+  check(lib.norm(cp(x), row_stride(x), w ? cp(*w) : nullptr, b ? cp(*b) : nullptr, &o, vp(y), o.cols,
+                 static_cast<float*>(vp_or_null(stats)), st(stream)),
+        "norm");
+  return {y, stats};
+}
+
+struct Norm : torch::autograd::Function<Norm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w,
+                        const OptTensor& b, const mxgg_norm_options& o, int64_t stream) {
+    const variable_list r = norm_forward(x, w, b, o, true, stream);
+    ctx->save_for_backward({x, w.value_or(Tensor()), r[1]});
+    keep(ctx, "options", o);
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["need"] =
+        (int64_t)(x.requires_grad() | grad_needed(w) << 1 | grad_needed(b) << 2);
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    const auto o = kept<mxgg_norm_options>(ctx, "options");
+    const int64_t need = ctx->saved_data["need"].toInt();
+    Tensor dy = grads[0].to(x.scalar_type());
+    if (row_stride(dy) < 0) dy = dy.contiguous();
+    const auto param = [&](int bit, int32_t type) {
+      return need & bit ? empty({o.cols}, x, type == MXGG_OUT_BF16 ? at::kBFloat16 : at::kFloat)
+                        : Tensor();
+    };
+    Tensor dx = need & 1 ? empty(x.sizes(), x, x.scalar_type()) : Tensor();
+    Tensor dw = param(2, o.weight_dtype), db = param(4, o.bias_dtype), ws;
+    if (need & 6) ws = empty({lib.norm_grad_workspace_bytes(&o)}, x, at::kByte);
+    check(lib.norm_grad(cp(dy), row_stride(dy), cp(x), row_stride(x), cp_or_null(w),
+                        stats.const_data_ptr<float>(), &o, vp_or_null(dx), o.cols, vp_or_null(dw),
+                        vp_or_null(db), vp_or_null(ws), ws.defined() ? ws.numel() : 0,
+                        st(ctx->saved_data["stream"].toInt())),
+          "norm_grad");
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Result norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
+            bool center, int64_t stream) {
+  if (!plain(x) || !f32_or_bf16(x) || x.dim() < 1 || x.size(-1) > 32768 || row_stride(x) < 0)
+    return none();
+  const int64_t cols = x.size(-1);
+  for (const OptTensor* p : {&weight, &bias})
+    if (*p && (!plain(**p) || !f32_or_bf16(**p) || (*p)->dim() != 1 || (*p)->size(0) != cols ||
+               !(*p)->is_contiguous() || (*p)->device() != x.device()))
+      return none();
+  const mxgg_norm_options o{x.numel() / cols,
+                            cols,
+                            type_of(x),
+                            weight ? type_of(*weight) : MXGG_OUT_F32,
+                            bias ? type_of(*bias) : MXGG_OUT_F32,
+                            center,
+                            (float)eps};
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || grad_needed(weight) || grad_needed(bias)))
+    return Norm::apply(x, weight, bias, o, stream);
+  return norm_forward(x, weight, bias, o, false, stream)[0];
+}
+
+// One AdamW step of lists of tensors; m_scales and v_scales are empty for 32-bit
+// states, masters without master copies.
+Result adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
+             const std::vector<Tensor>& m, const std::vector<Tensor>& v,
+             const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales,
+             const std::vector<Tensor>& masters, int64_t step, double lr, double beta1,
+             double beta2, double eps, double weight_decay, int64_t stream) {
+  const size_t n = params.size();
+  const bool small = !m_scales.empty();
+  if (n == 0 || grads.size() != n || m.size() != n || v.size() != n ||
+      (small && (m_scales.size() != n || v_scales.size() != n)) ||
+      (!masters.empty() && masters.size() != n))
+    return none();
+  const auto device = params[0].device();
+  const auto ok = [&](const Tensor& t, int64_t numel) {
+    return plain(t) && t.is_contiguous() && t.numel() == numel && t.device() == device;
+  };
+  const auto state_type = [&](const Tensor& t) {
+    return small ? bytes(t) : t.scalar_type() == at::kFloat;
+  };
+  std::vector<mxgg_adamw_tensor> table(n);
+  for (size_t i = 0; i < n; ++i) {
+    const int64_t size = params[i].numel(), blocks = (size + 31) / 32;
+    if (!ok(params[i], size) || !f32_or_bf16(params[i]) || !ok(grads[i], size) ||
+        !f32_or_bf16(grads[i]) || !ok(m[i], size) || !state_type(m[i]) || !ok(v[i], size) ||
+        !state_type(v[i]))
+      return none();
+    if (small && (!ok(m_scales[i], blocks) || m_scales[i].scalar_type() != at::kByte ||
+                  !ok(v_scales[i], blocks) || v_scales[i].scalar_type() != at::kByte))
+      return none();
+    if (!masters.empty() && (!ok(masters[i], size) || masters[i].scalar_type() != at::kFloat))
+      return none();
+    table[i] = {vp(params[i]),
+                cp(grads[i]),
+                vp(m[i]),
+                vp(v[i]),
+                small ? vp(m_scales[i]) : nullptr,
+                small ? vp(v_scales[i]) : nullptr,
+                masters.empty() ? nullptr : masters[i].data_ptr<float>(),
+                size,
+                type_of(params[i]),
+                type_of(grads[i])};
+  }
+  const mxgg_adamw_options o{lr, beta1, beta2, eps, weight_decay, step, small ? 8 : 32};
+  const int rc = lib.adamw_step(table.data(), (int64_t)n, &o, st(stream));
+  if (rc == MXGG_OK)  // modified in place, as far as torch and weight caches are concerned
+    for (const auto* list : {&params, &m, &v, &m_scales, &v_scales, &masters})
+      for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
+  return rc;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -397,4 +618,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_dual", torch::wrap_pybind_function_no_gil(&gather_dual));
   m.def("gather_dim0", torch::wrap_pybind_function_no_gil(&gather_dim0));
   m.def("combine", torch::wrap_pybind_function_no_gil(&combine));
+  m.def("route_topk", torch::wrap_pybind_function_no_gil(&route_topk));
+  m.def("norm", torch::wrap_pybind_function_no_gil(&norm));
+  m.def("adamw", torch::wrap_pybind_function_no_gil(&adamw));
 }

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _need_gpu, _stream_ptr
+from .ops import _native, _need_gpu, _stream_ptr, _tensors, _took
 
 __all__ = ["layer_norm", "rms_norm", "Norm"]
 
@@ -87,6 +87,11 @@ class Norm(torch.autograd.Function):
 
 
 def _norm(x, weight, bias, eps, center):
+    host = _native(x)
+    if host is not None and _tensors(weight, bias):
+        r = host.norm(x, weight, bias, eps, center, _stream_ptr(x))
+        if _took(r, "norm"):
+            return r
     _need_gpu(x, "x")
     if x.dtype not in _TYPES or x.dim() < 1:
         raise TypeError("x must be a float32 or bfloat16 tensor [..., cols]")

@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _FP8, _need_gpu, _stream_ptr
+from .ops import _FP8, _native, _need_gpu, _stream_ptr, _tensors, _took
 
 __all__ = ["AdamW", "adamw_step", "adamw_state"]
 
@@ -77,6 +77,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: int, lr: float = 1e-3,
     if small:
         ms, vs = [s[1] for s in exp_avg], [s[1] for s in exp_avg_sq]
         exp_avg, exp_avg_sq = [s[0] for s in exp_avg], [s[0] for s in exp_avg_sq]
+    else:
+        ms = vs = []
+    host = _native(params[0])
+    if host is not None and _tensors(*params, *grads, *exp_avg, *exp_avg_sq, *ms, *vs, *masters):
+        r = host.adamw(params, grads, exp_avg, exp_avg_sq, ms, vs, masters, step, lr, betas[0],
+                       betas[1], eps, weight_decay, _stream_ptr(params[0]))
+        if _took(r, "adamw_step"):
+            return
     opt = _lib.AdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, 8 if small else 32)
     first = params[0]
     table = (_lib.AdamwTensor * n)()
@@ -99,7 +107,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: int, lr: float = 1e-3,
         e.grad_dtype = _TYPES[grads[i].dtype]
     _lib.check(_lib.load().mxgg_adamw_step(table, n, ctypes.byref(opt), _stream_ptr(first)),
                "adamw_step")
-    torch.autograd.graph.increment_version([*params, *exp_avg, *exp_avg_sq, *masters])
+    torch.autograd.graph.increment_version([*params, *exp_avg, *exp_avg_sq, *ms, *vs, *masters])
 
 
 class AdamW(torch.optim.Optimizer):

@@ -110,6 +110,13 @@ def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax",
     with every logit -inf goes nowhere.  A NaN logit is chosen first and its
     score is NaN.  E <= 1024, topk <= 32, num_groups <= 64.  Differentiable in
     the logits."""
+    host = _native(logits)
+    if host is not None and score in _SCORES and _tensors(bias):
+        r = host.route_topk(logits, bias, topk, num_groups,
+                            num_groups if top_groups is None else top_groups, _SCORES[score],
+                            group_best, renormalize, scale, _stream_ptr(logits))
+        if _took(r, "route_topk"):
+            return r
     _need_gpu(logits, "logits")
     if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES:
         raise TypeError("logits must be a 2-D float32 or bfloat16 tensor [tokens, experts]")

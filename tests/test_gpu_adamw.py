@@ -86,7 +86,7 @@ def _check_state(state, want):
         return
     pad = np.pad(want, (0, -want.size % 32)).reshape(-1, 32)
     amax = np.abs(pad).max(axis=1)
-    with np.errstate(divide="ignore"):
+    with np.errstate(divide="ignore", invalid="ignore"):
         j = np.ceil(np.log2(amax / 448))
         edge = np.abs(np.log2(amax / 448) - np.rint(np.log2(amax / 448))) < 1e-6
     b = np.clip(j, -126, 127) + 127
