@@ -27,8 +27,9 @@ namespace {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamVec = 8;
-// Elements of a workgroup, 8 a thread.  Twice as many in a loop of two trips:
-// 235 M bf16 weights with fp32 states 1257 us against 1228, 8-bit 437 against 430.
+// Elements of a workgroup, 8 a thread.  235 M bf16 weights with fp32 states and
+// master copy: 1231 us (5.3 TB/s); twice as many elements in two trips 1249, runs
+// of 4 whose lanes follow each other without gaps 1253.  8-bit states: 435 us.
 constexpr int64_t kAdamChunk = kAdamThreads * kAdamVec;
 constexpr int kAdamTensors = 48;      // of a launch: 3.3 of the 4 KB of kernel arguments
 
@@ -40,51 +41,66 @@ struct AdamTable {
 };
 static_assert(sizeof(AdamTable) <= 4096, "kernel arguments");
 
-// Eight consecutive fp32 or bf16 values at p + i, `n` of them inside the tensor.
+// Words at any element alignment, as one access each.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+// Eight consecutive fp32 or bf16 values at p + i; FULL: all of them lie inside the
+// tensor, else `n` of them do and the rest read as 0.
+template <bool FULL>
 __device__ __forceinline__ void load8(const void* p, bool bf16, int64_t i, int n, float (&v)[8]) {
   if (bf16) {
     const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (n >= 8) {
-      __builtin_memcpy(w, q, 16);
+    u32x4 w;
+    if constexpr (FULL) {
+      w = *reinterpret_cast<const u32x4_any*>(q);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n) w[j >> 1] |= (uint32_t)q[j] << (16 * (j & 1));
+      for (int j = 0; j < 8; j += 2)
+        w[j / 2] = (j < n ? q[j] : 0u) | (j + 1 < n ? (uint32_t)q[j + 1] : 0u) << 16;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
-  } else {
-    const float* q = static_cast<const float*>(p) + i;
-    if (n >= 8) {
-      __builtin_memcpy(v, q, 16);
-      __builtin_memcpy(v + 4, q + 4, 16);
+    return;
+  }
+  const float* q = static_cast<const float*>(p) + i;
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    if constexpr (FULL) {
+      const u32x4 w = *reinterpret_cast<const u32x4_any*>(q + k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[k + j] = __uint_as_float(w[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? q[j] : 0.0f;
+      for (int j = k; j < k + 4; ++j) v[j] = j < n ? q[j] : 0.0f;
     }
   }
 }
+template <bool FULL>
 __device__ __forceinline__ void store8(void* p, bool bf16, int64_t i, int n, const float (&v)[8]) {
   if (bf16) {
     uint16_t* q = static_cast<uint16_t*>(p) + i;
-    const uint32_t w[4] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                           pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    if (n >= 8) {
-      __builtin_memcpy(q, w, 16);
+    const u32x4 w{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                  pack_bf16x2(v[6], v[7])};
+    if constexpr (FULL) {
+      *reinterpret_cast<u32x4_any*>(q) = w;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (j < n) q[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
     }
-  } else {
-    float* q = static_cast<float*>(p) + i;
-    if (n >= 8) {
-      __builtin_memcpy(q, v, 16);
-      __builtin_memcpy(q + 4, v + 4, 16);
+    return;
+  }
+  float* q = static_cast<float*>(p) + i;
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    if constexpr (FULL) {
+      *reinterpret_cast<u32x4_any*>(q + k) =
+          u32x4{__float_as_uint(v[k]), __float_as_uint(v[k + 1]), __float_as_uint(v[k + 2]),
+                __float_as_uint(v[k + 3])};
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = k; j < k + 4; ++j)
         if (j < n) q[j] = v[j];
     }
   }
@@ -92,11 +108,14 @@ __device__ __forceinline__ void store8(void* p, bool bf16, int64_t i, int n, con
 
 // Eight values of an 8-bit state: payload bytes at q + i, block byte b.  Byte
 // 255 stands for a block of NaN (its payload bytes are NaN codes).
+template <bool FULL>
 __device__ __forceinline__ void unpack8(const uint8_t* q, const uint8_t* s, int64_t i, int n,
                                         float (&v)[8]) {
   uint32_t w[2] = {0, 0};
-  if (n >= 8) {
-    __builtin_memcpy(w, q + i, 8);
+  if constexpr (FULL) {
+    const u32x2 u = *reinterpret_cast<const u32x2_any*>(q + i);
+    w[0] = u[0];
+    w[1] = u[1];
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -119,6 +138,7 @@ __device__ __forceinline__ void unpack8(const uint8_t* q, const uint8_t* s, int6
 // which the four lanes of a quad hold together: every lane of the wave calls it.
 // b = ceil(log2(amax / 448)) + 127, at least 1 (normal scales); 255 if the block
 // holds an infinity or a NaN.
+template <bool FULL>
 __device__ __forceinline__ void pack8(uint8_t* q, uint8_t* s, int64_t i, int n,
                                       const float (&v)[8]) {
   uint32_t amax = 0;
@@ -138,8 +158,8 @@ __device__ __forceinline__ void pack8(uint8_t* q, uint8_t* s, int64_t i, int n,
     w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)u, true);
     if (b == 255) w[k] = 0x7F7F7F7Fu;
   }
-  if (n >= 8) {
-    __builtin_memcpy(q + i, w, 8);
+  if constexpr (FULL) {
+    *reinterpret_cast<u32x2_any*>(q + i) = u32x2{w[0], w[1]};
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -148,40 +168,25 @@ __device__ __forceinline__ void pack8(uint8_t* q, uint8_t* s, int64_t i, int n,
   if (n > 0 && (i & 31) == 0) s[i >> 5] = (uint8_t)b;
 }
 
-template <bool SMALL>
-__global__ __launch_bounds__(kAdamThreads) void k_adamw(AdamTable a) {
+// Eight consecutive elements from i on; every lane of the wave calls it.
+template <bool SMALL, bool FULL>
+__device__ __forceinline__ void step(const AdamTensor& t, const AdamScalars& s, int64_t i) {
   // every product and sum rounds by itself: a fused multiply-add would make the
   // states depend on how the compiler pairs them
 #pragma clang fp contract(off)
-  int lo = 0, hi = a.count;  // last tensor that starts at or before this workgroup
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid;
-  }
-  const AdamTensor t = a.t[lo];
-  const AdamScalars s = a.s;
-  const int64_t base = (int64_t)((int)blockIdx.x - a.first[lo]) * kAdamChunk;
+  const int64_t left = t.n - i;
+  const int n = FULL || left >= 8 ? 8 : left > 0 ? (int)left : 0;
   void* weights = t.master ? static_cast<void*>(t.master) : t.param;
   const bool w_bf16 = !t.master && t.param_bf16;
-  const int64_t i = base + (int64_t)threadIdx.x * kAdamVec, left = t.n - i;
-  const int n = left >= 8 ? 8 : left > 0 ? (int)left : 0;
   float p[8], g[8], m[8], v[8];
-  if (n > 0) {
-    load8(weights, w_bf16, i, n, p);
-    load8(t.grad, t.grad_bf16, i, n, g);
+  load8<FULL>(weights, w_bf16, i, n, p);
+  load8<FULL>(t.grad, t.grad_bf16, i, n, g);
+  if constexpr (SMALL) {
+    unpack8<FULL>(static_cast<const uint8_t*>(t.m), t.m_scales, i, n, m);
+    unpack8<FULL>(static_cast<const uint8_t*>(t.v), t.v_scales, i, n, v);
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = g[j] = 0.0f;
-  }
-  if (SMALL) {
-    unpack8(static_cast<const uint8_t*>(t.m), t.m_scales, i, n, m);
-    unpack8(static_cast<const uint8_t*>(t.v), t.v_scales, i, n, v);
-  } else if (n > 0) {
-    load8(t.m, false, i, n, m);
-    load8(t.v, false, i, n, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = v[j] = 0.0f;
+    load8<FULL>(t.m, false, i, n, m);
+    load8<FULL>(t.v, false, i, n, v);
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -192,18 +197,32 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw(AdamTable a) {
     v[j] = SMALL ? root : now;
     p[j] = p[j] * s.decay - s.step_size * (m[j] / (root * s.inv_root_bias2 + s.eps));
   }
-  if (SMALL) {
-    pack8(static_cast<uint8_t*>(t.m), t.m_scales, i, n, m);
-    pack8(static_cast<uint8_t*>(t.v), t.v_scales, i, n, v);
+  if constexpr (SMALL) {
+    pack8<FULL>(static_cast<uint8_t*>(t.m), t.m_scales, i, n, m);
+    pack8<FULL>(static_cast<uint8_t*>(t.v), t.v_scales, i, n, v);
+  } else {
+    store8<FULL>(t.m, false, i, n, m);
+    store8<FULL>(t.v, false, i, n, v);
   }
-  if (n > 0) {
-    if (!SMALL) {
-      store8(t.m, false, i, n, m);
-      store8(t.v, false, i, n, v);
-    }
-    store8(weights, w_bf16, i, n, p);
-    if (t.master) store8(t.param, t.param_bf16, i, n, p);
+  store8<FULL>(weights, w_bf16, i, n, p);
+  if (t.master) store8<FULL>(t.param, t.param_bf16, i, n, p);
+}
+
+template <bool SMALL>
+__global__ __launch_bounds__(kAdamThreads) void k_adamw(AdamTable a) {
+  int lo = 0, hi = a.count;  // last tensor that starts at or before this workgroup
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid;
   }
+  const AdamTensor t = a.t[lo];
+  const int64_t base = (int64_t)((int)blockIdx.x - a.first[lo]) * kAdamChunk;
+  const bool full = base + kAdamChunk <= t.n;  // the tensor's last workgroup may not be
+  const int64_t i = base + (int64_t)threadIdx.x * kAdamVec;
+  if (full)
+    step<SMALL, true>(t, a.s, i);
+  else
+    step<SMALL, false>(t, a.s, i);
 }
 
 }  // namespace
