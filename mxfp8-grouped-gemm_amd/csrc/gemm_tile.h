@@ -7,6 +7,9 @@
 //          chunks (g and g + 4) that lane m + 16g holds of row m are its operands
 //          of the first and of the second one
 // Both instructions return D[4g + r][c] in register r of lane c + 16g.
+// A bf16 operand may also be K-MAJOR: rows of the contraction, contiguous along p
+// (or q).  A stage is then 64 rows of 256 columns, 512 bytes each, and the
+// fragments are read with the transposing ds_read_b64_tr_b16.
 #pragma once
 
 #include <type_traits>
@@ -73,6 +76,11 @@ struct Operand {
   // consecutive rows; F for the gate+up tile of the fused SwiGLU forward
   // (tile rows 0..127 = gate rows, 128..255 = the matching up rows F later).
   uint32_t hi;
+  // K-major: first row of the contraction, at the tile's first column; ld as above.
+  // Offsets stay within a stage (the stage's rows are the base), so `bytes`, from
+  // base to the end of the last row, may pass 32 bits; rows past it read as zero.
+  const uint8_t* base;
+  int64_t bytes;
 };
 
 // Cache-policy operand of the buffer store builtins: the nontemporal bit.
@@ -153,9 +161,17 @@ __device__ __forceinline__ void dma_x1(const desc_t& d, uint32_t lds_addr, uint3
 //  Scales: wave w copies block k0/32 + w of both operands: 256 rows = 64 lanes
 //  x 4 bytes in row order.  A block outside [klo, kend) lands as zeros (scale
 //  2^-127 on zero payload).
-template <bool SCALED, bool MASK = false>
+//  K-major data (PK, QK): the LDS bytes are the same, row k = 8i + 2w + l/32 of the
+//  stage at byte 512 k, and the lane fetches logical chunk (l%32) ^ 2 kswz(k) of that
+//  row.  kswz(k) = (k mod 4) + 4 ((k/8) mod 2) changes with i by its last bit only:
+//  one base offset for even and one for odd loads.
+__device__ __forceinline__ uint32_t kswz(uint32_t k) { return (k & 3u) | ((k >> 3) & 1u) << 2; }
+
+template <bool SCALED, bool MASK = false, bool PK = false, bool QK = false>
 struct Stream {
   uint32_t vp, vq;   // lane offset of load 0 without k0
+  uint32_t op, oq;   // K-major: lane offset of load 1, less its rows' step
+  desc_t dp, dq;     // K-major: the stage's rows
   uint32_t kcol;     // lane's chunk column within a stage (bytes)
   uint32_t sp, sq;   // lane offset of its scale dword within a block-row
   uint32_t klo, kend;
@@ -170,6 +186,18 @@ struct Stream {
     const uint32_t r = 4u * (8u * wave + (lane >> 3));
     vp = (P.row0 + r) * P.ld + kcol;
     vq = (Q.row0 + r) * Q.ld + kcol;
+    if constexpr (PK || QK) {
+      const uint32_t k = 2u * wave + (lane >> 5);
+      const uint32_t even = 16u * ((lane & 31u) ^ (kswz(k) << 1));
+      if (PK) {
+        vp = k * P.ld + even;
+        op = k * P.ld + (even ^ 128u);
+      }
+      if (QK) {
+        vq = k * Q.ld + even;
+        oq = k * Q.ld + (even ^ 128u);
+      }
+    }
     if (SCALED) {
       sp = P.row0 + 4u * lane + (lane >= 32u ? P.hi - 128u : 0u);
       sq = Q.row0 + 4u * lane + (lane >= 32u ? Q.hi - 128u : 0u);
@@ -180,11 +208,18 @@ struct Stream {
   // [klo, kend); adding a step to it stays out of range).
   // MASK: a chunk that overlaps [klo, kend) at all is loaded (the bytes outside
   // are zeroed in registers after the fragment reads, mask_frags()).
-  __device__ __forceinline__ void stage_base(uint32_t k0, uint32_t& bp, uint32_t& bq) const {
+  __device__ __forceinline__ void stage_base(const Operand& P, const Operand& Q, uint32_t k0,
+                                             uint32_t& bp, uint32_t& bq) {
     const uint32_t k = k0 + kcol;
     const bool ok = (MASK ? k + 16u > klo : k >= klo) && k < kend;
     bp = ok ? vp + k0 : kOobOffset;
     bq = ok ? vq + k0 : kOobOffset;
+    if (PK) dp = stage_rows(P, k0);
+    if (QK) dq = stage_rows(Q, k0);
+  }
+  __device__ __forceinline__ static desc_t stage_rows(const Operand& X, uint32_t k0) {
+    const int64_t off = (int64_t)(k0 >> 1) * X.ld, left = X.bytes - off;
+    return make_desc(X.base + off, (uint32_t)(left < 0 ? 0 : left > 0x7FFFFFF0 ? 0x7FFFFFF0 : left));
   }
 
   __device__ __forceinline__ static uint32_t step(uint32_t i, const Operand& X) {
@@ -193,12 +228,19 @@ struct Stream {
 
   __device__ __forceinline__ void load_p(uint8_t* stage, const Operand& P, uint32_t bp,
                                          uint32_t i) const {
-    dma_x4(P.data, lds_offset(stage) + 4096u * i + 1024u * wave_id(), bp, step(i, P));
+    const uint32_t dst = lds_offset(stage) + 4096u * i + 1024u * wave_id();
+    if constexpr (PK)
+      dma_x4(dp, dst, (i & 1u) ? op : vp, 8u * i * P.ld);
+    else
+      dma_x4(P.data, dst, bp, step(i, P));
   }
   __device__ __forceinline__ void load_q(uint8_t* stage, const Operand& Q, uint32_t bq,
                                          uint32_t i) const {
-    dma_x4(Q.data, lds_offset(stage) + kOpBytes + 4096u * i + 1024u * wave_id(),
-           bq, step(i, Q));
+    const uint32_t dst = lds_offset(stage) + kOpBytes + 4096u * i + 1024u * wave_id();
+    if constexpr (QK)
+      dma_x4(dq, dst, (i & 1u) ? oq : vq, 8u * i * Q.ld);
+    else
+      dma_x4(Q.data, dst, bq, step(i, Q));
   }
   // Scale rows of k-block k0/32 + wave; operand X = P (OP 0) or Q (OP 1).
   template <int OP>
@@ -215,7 +257,7 @@ struct Stream {
 
   // The loads of a tile's first two stages (18 each with scales), stage 0 first.
   __device__ __forceinline__ void prologue(uint8_t* s0, uint8_t* s1, const Operand& P,
-                                           const Operand& Q, uint32_t kbeg, uint32_t nst) const {
+                                           const Operand& Q, uint32_t kbeg, uint32_t nst) {
     load_scale<0>(s0, P, kbeg);
     load_scale<1>(s0, Q, kbeg);
     issue_data(s0, P, Q, kbeg);
@@ -228,9 +270,9 @@ struct Stream {
 
   // The 16 data loads of one stage, back to back (prologue only).
   __device__ __forceinline__ void issue_data(uint8_t* stage, const Operand& P, const Operand& Q,
-                                             uint32_t k0) const {
+                                             uint32_t k0) {
     uint32_t bp, bq;
-    stage_base(k0, bp, bq);
+    stage_base(P, Q, k0, bp, bq);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) load_p(stage, P, bp, i);
 #pragma unroll
@@ -256,8 +298,15 @@ struct Frags {
 //   128w + 64G + 4m + i (m = 0..15): LDS slots 128w + 32i + 16G + m of the
 //   DMA's slot layout.  Its scale byte is byte i of the dword of rows
 //   128w + 64G + 4m .. +3 of the lane's block.
+// K-major operands: fragment f of a wave half w is its columns 128w + 16f .. + 15.
+// ds_read_b64_tr_b16 takes a 4 x 16 block from 16 lanes, lane i the four elements
+// 4 (i%4) .. + 3 of row i/4, and returns column i: so lane i of group g reads row
+// k = 8g + i/4 (+ 4 for the upper half of its eight, + 32 for the second k step), and
+// its 16-byte chunk 2f + (i/2)%2 is XORed with 2 kswz(k), which is the same for
+// those rows.  A read's 64 lanes then touch every bank twice.
 struct FragAddr {
   uint32_t plo, phi, qlo, qhi, ps, qs;
+  uint32_t kp, kq;  // K-major: fragment 0; fragment f at kp ^ 32 f
 
   __device__ __forceinline__ void init() {
     const uint32_t lane = threadIdx.x & 63u;
@@ -273,6 +322,17 @@ struct FragAddr {
     qhi = rq + (((g + 4u) ^ sw) << 4);
     ps = kScaleOff + g * kScaleBlk + wp * 128u + 4u * m;
     qs = kScaleOff + 256u + g * kScaleBlk + wq * 128u + 4u * m;
+  }
+
+  __device__ __forceinline__ void init_k_major() {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = threadIdx.x >> 6;
+    const uint32_t wp = wave & 1u, wq = wave >> 1;
+    const uint32_t m = lane & 15u, g = lane >> 4;
+    const uint32_t k = 8u * g + (m >> 2);
+    const uint32_t kb = 512u * k + (kswz(k) << 5) + 16u * ((m >> 1) & 1u) + 8u * (m & 1u);
+    kp = kb + 256u * wp;
+    kq = kOpBytes + kb + 256u * wq;
   }
 };
 
@@ -290,13 +350,35 @@ __device__ __forceinline__ v8i lds_v8i(const uint8_t* lo, const uint8_t* hi) {
   return f;
 }
 
-template <int F>
-__device__ __forceinline__ void read_a(const uint8_t* stage, const FragAddr& fa, Frags& f) {
-  f.a[F] = lds_v8i(stage + fa.plo + frag_off(F), stage + fa.phi + frag_off(F));
+// A K-major fragment from its lane address: eight contraction elements of each k step.
+__device__ __forceinline__ v8i lds_k_major(const uint8_t* p) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  v8i f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const u32x2 w = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (lds_v4s*)(p + 2048 * (k & 1) + 16384 * (k >> 1))));
+    f[2 * k] = (int)w[0];
+    f[2 * k + 1] = (int)w[1];
+  }
+  return f;
 }
-template <int F>
+
+template <bool KM, int F>
+__device__ __forceinline__ void read_a(const uint8_t* stage, const FragAddr& fa, Frags& f) {
+  if constexpr (KM)
+    f.a[F] = lds_k_major(stage + (fa.kp ^ (32u * F)));
+  else
+    f.a[F] = lds_v8i(stage + fa.plo + frag_off(F), stage + fa.phi + frag_off(F));
+}
+template <bool KM, int F>
 __device__ __forceinline__ void read_b(const uint8_t* stage, const FragAddr& fa, Frags& f) {
-  f.b[F] = lds_v8i(stage + fa.qlo + frag_off(F), stage + fa.qhi + frag_off(F));
+  if constexpr (KM)
+    f.b[F] = lds_k_major(stage + (fa.kq ^ (32u * F)));
+  else
+    f.b[F] = lds_v8i(stage + fa.qlo + frag_off(F), stage + fa.qhi + frag_off(F));
 }
 // Unscaled kernels use scale byte 127 (2^0) in every position.
 template <bool SCALED, int G>
@@ -404,10 +486,12 @@ __device__ __forceinline__ void release_barrier() {
 // leave those stores in flight: they drain behind this tile's first two stages.
 // With fewer stores the counts would reach into the loads; more vector-memory
 // instructions (a spill) only make them stricter.
-template <bool SCALED, bool MASK = false, bool AHEAD = false, bool BF16 = false, class SM>
+template <bool SCALED, bool MASK = false, bool AHEAD = false, bool BF16 = false, bool PK = false,
+          bool QK = false, class SM>
 __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand& Q,
                                          uint32_t klo, uint32_t kend, v4f (&acc)[64]) {
   static_assert(!(SCALED && MASK), "a scale block cannot be split by a token mask");
+  static_assert(BF16 || !(PK || QK), "K-major operands are bf16");
   static_assert(!BF16 || !(SCALED || MASK), "bf16 operands have neither scales nor a byte mask");
   static_assert(SCALED || !AHEAD, "the wait counts of AHEAD include the scale loads");
 #pragma unroll
@@ -415,10 +499,11 @@ __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand
   if (kend <= klo) return;
   const uint32_t kbeg = klo & ~(uint32_t)(kStageK - 1);
   const uint32_t nst = (kend - kbeg + kStageK - 1) / kStageK;
-  Stream<SCALED, MASK> st;
+  Stream<SCALED, MASK, PK, QK> st;
   st.init(P, Q, klo, kend);
   FragAddr fa;
   fa.init();
+  if constexpr (PK || QK) fa.init_k_major();
   // Prologue: all of stage 0 and, if there is one, of stage 1 (issued here or by
   // the caller), then publish stage 0 and read the part of it that the loop
   // reads one stage ahead.
@@ -438,14 +523,14 @@ __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand
   if constexpr (MASK) apply_mask(f.b[F], km)
   {
     const uint8_t* r0 = sm.ring[0];
-    read_b<0>(r0, fa, f); MASKB(0);
-    read_b<1>(r0, fa, f); MASKB(1);
-    read_b<2>(r0, fa, f); MASKB(2);
-    read_b<3>(r0, fa, f); MASKB(3);
-    read_a<0>(r0, fa, f); MASKA(0);
-    read_a<1>(r0, fa, f); MASKA(1);
-    read_a<2>(r0, fa, f); MASKA(2);
-    read_a<3>(r0, fa, f); MASKA(3);
+    read_b<QK, 0>(r0, fa, f); MASKB(0);
+    read_b<QK, 1>(r0, fa, f); MASKB(1);
+    read_b<QK, 2>(r0, fa, f); MASKB(2);
+    read_b<QK, 3>(r0, fa, f); MASKB(3);
+    read_a<PK, 0>(r0, fa, f); MASKA(0);
+    read_a<PK, 1>(r0, fa, f); MASKA(1);
+    read_a<PK, 2>(r0, fa, f); MASKA(2);
+    read_a<PK, 3>(r0, fa, f); MASKA(3);
     read_sa<SCALED, 0>(r0, fa, f);
     read_sb<SCALED, 0>(r0, fa, f);
   }
@@ -462,16 +547,16 @@ __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand
     uint8_t* cur = sm.ring[s & 1u];
     uint8_t* nxt = sm.ring[(s & 1u) ^ 1u];
     uint32_t bp = 0, bq = 0;
-    if constexpr (LOADS) st.stage_base(kbeg + (s + 2) * kStageK, bp, bq);
-      mma<BF16, 0, 0>(f, acc); read_a<4>(cur, fa, f); MASKA(4); MXGG_FENCE();
+    if constexpr (LOADS) st.stage_base(P, Q, kbeg + (s + 2) * kStageK, bp, bq);
+      mma<BF16, 0, 0>(f, acc); read_a<PK, 4>(cur, fa, f); MASKA(4); MXGG_FENCE();
       mma<BF16, 0, 1>(f, acc); read_sa<SCALED, 1>(cur, fa, f); MXGG_FENCE();
-      mma<BF16, 0, 2>(f, acc); read_a<5>(cur, fa, f); MASKA(5); MXGG_FENCE();
-      mma<BF16, 0, 3>(f, acc); read_b<4>(cur, fa, f); MASKB(4); MXGG_FENCE();
-      mma<BF16, 1, 0>(f, acc); read_a<6>(cur, fa, f); MASKA(6); MXGG_FENCE();
-      mma<BF16, 1, 1>(f, acc); read_b<5>(cur, fa, f); MASKB(5); MXGG_FENCE();
-      mma<BF16, 1, 2>(f, acc); read_a<7>(cur, fa, f); MASKA(7); MXGG_FENCE();
-      mma<BF16, 1, 3>(f, acc); read_b<6>(cur, fa, f); MASKB(6); MXGG_FENCE();
-      mma<BF16, 2, 0>(f, acc); read_sb<SCALED, 1>(cur, fa, f); read_b<7>(cur, fa, f); MASKB(7); MXGG_FENCE();
+      mma<BF16, 0, 2>(f, acc); read_a<PK, 5>(cur, fa, f); MASKA(5); MXGG_FENCE();
+      mma<BF16, 0, 3>(f, acc); read_b<QK, 4>(cur, fa, f); MASKB(4); MXGG_FENCE();
+      mma<BF16, 1, 0>(f, acc); read_a<PK, 6>(cur, fa, f); MASKA(6); MXGG_FENCE();
+      mma<BF16, 1, 1>(f, acc); read_b<QK, 5>(cur, fa, f); MASKB(5); MXGG_FENCE();
+      mma<BF16, 1, 2>(f, acc); read_a<PK, 7>(cur, fa, f); MASKA(7); MXGG_FENCE();
+      mma<BF16, 1, 3>(f, acc); read_b<QK, 6>(cur, fa, f); MASKB(6); MXGG_FENCE();
+      mma<BF16, 2, 0>(f, acc); read_sb<SCALED, 1>(cur, fa, f); read_b<QK, 7>(cur, fa, f); MASKB(7); MXGG_FENCE();
       mma<BF16, 2, 1>(f, acc); MXGG_FENCE();
       mma<BF16, 2, 2>(f, acc); MXGG_FENCE();
       mma<BF16, 2, 3>(f, acc); MXGG_FENCE();
@@ -504,26 +589,26 @@ __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand
       MXGG_FENCE();
       if constexpr (MASK) k_mask(km, kbeg + (s + 1) * kStageK, klo, kend);
       mma<BF16, 0, 4>(f, acc); MXGG_FENCE();
-      mma<BF16, 0, 5>(f, acc); read_b<0>(nxt, fa, f); MASKB(0); MXGG_FENCE();
+      mma<BF16, 0, 5>(f, acc); read_b<QK, 0>(nxt, fa, f); MASKB(0); MXGG_FENCE();
       mma<BF16, 0, 6>(f, acc); if constexpr (LOADS) st.load_p(cur, P, bp, 7); MXGG_FENCE();
       mma<BF16, 0, 7>(f, acc); MXGG_FENCE();
-      mma<BF16, 1, 4>(f, acc); read_a<0>(nxt, fa, f); MASKA(0); MXGG_FENCE();
+      mma<BF16, 1, 4>(f, acc); read_a<PK, 0>(nxt, fa, f); MASKA(0); MXGG_FENCE();
       mma<BF16, 1, 5>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 0); MXGG_FENCE();
       mma<BF16, 1, 6>(f, acc); MXGG_FENCE();
-      mma<BF16, 1, 7>(f, acc); read_b<1>(nxt, fa, f); MASKB(1); MXGG_FENCE();
+      mma<BF16, 1, 7>(f, acc); read_b<QK, 1>(nxt, fa, f); MASKB(1); MXGG_FENCE();
       mma<BF16, 2, 4>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 1); MXGG_FENCE();
-      mma<BF16, 2, 5>(f, acc); read_a<1>(nxt, fa, f); MASKA(1); MXGG_FENCE();
+      mma<BF16, 2, 5>(f, acc); read_a<PK, 1>(nxt, fa, f); MASKA(1); MXGG_FENCE();
       mma<BF16, 2, 6>(f, acc); MXGG_FENCE();
       mma<BF16, 2, 7>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 2); MXGG_FENCE();
       mma<BF16, 3, 4>(f, acc); MXGG_FENCE();
-      mma<BF16, 3, 5>(f, acc); read_b<2>(nxt, fa, f); MASKB(2); if constexpr (LOADS) st.load_q(cur, Q, bq, 3); MXGG_FENCE();
-      mma<BF16, 3, 6>(f, acc); read_a<2>(nxt, fa, f); MASKA(2); MXGG_FENCE();
+      mma<BF16, 3, 5>(f, acc); read_b<QK, 2>(nxt, fa, f); MASKB(2); if constexpr (LOADS) st.load_q(cur, Q, bq, 3); MXGG_FENCE();
+      mma<BF16, 3, 6>(f, acc); read_a<PK, 2>(nxt, fa, f); MASKA(2); MXGG_FENCE();
       mma<BF16, 3, 7>(f, acc); MXGG_FENCE();
       mma<BF16, 4, 4>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 4); MXGG_FENCE();
       mma<BF16, 4, 5>(f, acc); MXGG_FENCE();
-      mma<BF16, 4, 6>(f, acc); read_a<3>(nxt, fa, f); MASKA(3); MXGG_FENCE();
+      mma<BF16, 4, 6>(f, acc); read_a<PK, 3>(nxt, fa, f); MASKA(3); MXGG_FENCE();
       mma<BF16, 4, 7>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 5); MXGG_FENCE();
-      mma<BF16, 5, 4>(f, acc); read_b<3>(nxt, fa, f); MASKB(3); MXGG_FENCE();
+      mma<BF16, 5, 4>(f, acc); read_b<QK, 3>(nxt, fa, f); MASKB(3); MXGG_FENCE();
       mma<BF16, 5, 5>(f, acc); MXGG_FENCE();
       mma<BF16, 5, 6>(f, acc); if constexpr (LOADS) st.load_q(cur, Q, bq, 6); MXGG_FENCE();
       mma<BF16, 5, 7>(f, acc); read_sb<SCALED, 0>(nxt, fa, f); MXGG_FENCE();

@@ -9,13 +9,14 @@
 // tile leaves one maximum and one sum of exponentials a token, joined over the
 // tiles by a second kernel.
 // Backward: pieces of the vocabulary.  The tiles of a piece are computed again
-// (8 T H V operations in all, 6 with kept logits) and leave d rounded to bf16,
-// as d [T][piece] and as d^T [piece][T]; with W^T of the piece and x^T (plain
-// transposes) both products then run with operands that are contiguous along
-// their contraction.  Rounding d is one bf16 rounding per term of sums whose
+// (8 T H V operations in all, 6 with kept logits) and leave d / g rounded to bf16,
+// [T][piece].  Both products read it, W and x as they lie: an operand that is not
+// contiguous along its contraction is transposed on the way from LDS to registers.
+// Where g is one number for all tokens it multiplies the products' sums in fp32,
+// so what is rounded is p - 1 or p itself: one bf16 rounding per term of sums whose
 // result is rounded to bf16 anyway.  dx is carried over pieces in fp32.
-// Few output tiles are split along the contraction, and the fp32 partials added
-// in order.
+// A product with few tiles is split along the contraction, and the fp32 partials
+// added in order.
 #include <algorithm>
 
 #include "gemm_tile.h"
@@ -45,12 +46,26 @@ __device__ __forceinline__ Operand tile_rows(const uint16_t* p, int64_t ld, int6
   return o;
 }
 
-// Tile of a workgroup.  Workgroups go round-robin to the 8 XCDs: each XCD takes a
+// Columns col0 .. of a bf16 matrix of k rows as a K-major tile operand.
+__device__ __forceinline__ Operand tile_columns(const uint16_t* p, int64_t ld, int64_t k,
+                                                int64_t col0, int64_t cols) {
+  Operand o;
+  o.data = o.scale = desc_t{0, 0, 0, 0};  // not read
+  o.base = reinterpret_cast<const uint8_t*>(p + col0);
+  o.bytes = ((k - 1) * ld + cols - col0) * 2;
+  o.ld = (uint32_t)(ld * 2);
+  o.lds = 0;
+  o.row0 = 0;
+  o.hi = 128;
+  return o;
+}
+
+// Tile `block` of np x nq.  Workgroups go round-robin to the 8 XCDs: each XCD takes a
 // contiguous run of tiles in an order of bands of 8 token tiles, so the 32 tiles
 // it works on at a time share 8 + 4 operand panels in its L2.
-__device__ __forceinline__ void tile_of(int np, int nq, int& p, int& q) {
+__device__ __forceinline__ void tile_of(int block, int np, int nq, int& p, int& q) {
   const int total = np * nq, per = total / 8, rest = total % 8;
-  const int xcd = (int)blockIdx.x % 8, slot = (int)blockIdx.x / 8;
+  const int xcd = block % 8, slot = block / 8;
   const int n = xcd * per + min(xcd, rest) + slot;
   const int band = n / (8 * np), in = n - band * 8 * np;
   const int width = min(8, nq - band * 8);
@@ -89,7 +104,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a) {
   __shared__ LossSmem sm;
   const int np = (int)((a.V + kTile - 1) / kTile), nq = (int)((a.T + kTile - 1) / kTile);
   int pt, qt;
-  tile_of(np, nq, pt, qt);
+  tile_of((int)blockIdx.x, np, nq, pt, qt);
   const int64_t p0 = (int64_t)pt * kTile, q0 = (int64_t)qt * kTile;
   const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H);
   const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
@@ -211,7 +226,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
   __shared__ LossSmem sm;
   const int np = width / kTile, nq = (int)((a.T + kTile - 1) / kTile);
   int pt, qt;
-  tile_of(np, nq, pt, qt);
+  tile_of((int)blockIdx.x, np, nq, pt, qt);
   const int64_t p0 = v0 + (int64_t)pt * kTile, q0 = (int64_t)qt * kTile;
   const Place at;
   v4f acc[64];
@@ -224,17 +239,18 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t t = q0 + at.q(H, j);
-      float shift = 0.0f, g = 0.0f;
+      float shift = 0.0f, g = 1.0f;
       int64_t word = -1;
+      bool none = true;
       if (t < a.T) {
         word = target_of(a, t);
         if (word != -1) {
+          none = false;
           shift = -a.stats[t] * kLog2e;
-          g = a.per_token ? a.grad_loss[t] : a.grad_loss[0] * a.stats[a.T];
+          if (a.per_token) g = a.grad_loss[t];
         }
         word -= p0;
       }
-      const bool none = g == 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -246,126 +262,109 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
               none || p >= words ? 0.0f : (e - (word == p ? 1.0f : 0.0f)) * g;
         }
     }
-  if (a.d != nullptr) {  // rows of tokens: 16 consecutive words a lane
-    const int64_t ldd = width;
+  // rows of tokens: 16 consecutive words a lane
 #pragma unroll
-    for (int H = 0; H < 2; ++H)
+  for (int H = 0; H < 2; ++H)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t t = q0 + at.q(H, j);
-        if (t >= a.T) continue;
+    for (int j = 0; j < 4; ++j) {
+      const int64_t t = q0 + at.q(H, j);
+      if (t >= a.T) continue;
 #pragma unroll
-        for (int G = 0; G < 2; ++G) {
-          uint32_t w[8];
+      for (int G = 0; G < 2; ++G) {
+        uint32_t w[8];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              w[2 * r + u] = pack_bf16x2(acc[8 * (4 * G + 2 * u) + 4 * H + j][r],
-                                         acc[8 * (4 * G + 2 * u + 1) + 4 * H + j][r]);
-          uint4* o = reinterpret_cast<uint4*>(a.d + t * ldd + (int64_t)pt * kTile + at.p(G, 0, 0));
-          o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          o[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
+          for (int u = 0; u < 2; ++u)
+            w[2 * r + u] = pack_bf16x2(acc[8 * (4 * G + 2 * u) + 4 * H + j][r],
+                                       acc[8 * (4 * G + 2 * u + 1) + 4 * H + j][r]);
+        uint4* o = reinterpret_cast<uint4*>(a.d + t * width + (int64_t)pt * kTile + at.p(G, 0, 0));
+        o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        o[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
-  }
-  if (a.dt != nullptr) {  // rows of words: 4 consecutive tokens a lane, 64 a row
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int H = 0; H < 2; ++H) {
-          const int64_t row = (int64_t)pt * kTile + at.p(k >> 2, r, k & 3);
-          *reinterpret_cast<uint2*>(a.dt + row * a.ldt + q0 + at.q(H, 0)) =
-              make_uint2(pack_bf16x2(acc[8 * k + 4 * H][r], acc[8 * k + 4 * H + 1][r]),
-                         pack_bf16x2(acc[8 * k + 4 * H + 2][r], acc[8 * k + 4 * H + 3][r]));
-        }
-  }
+    }
 }
 
-// out[c][r] = in[r][c], rows of `out` filled with zeros from r = rows to ldo.
-__global__ __launch_bounds__(256) void k_transpose(const uint16_t* __restrict__ in, int64_t ldi,
-                                                   int64_t rows, int64_t cols,
-                                                   uint16_t* __restrict__ out, int64_t ldo) {
-  __shared__ uint16_t tile[64][66];
-  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int r = i >> 3, c = 8 * (i & 7);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r0 + r < rows && c0 + c < cols)
-      v = *reinterpret_cast<const uint4*>(in + (r0 + r) * ldi + c0 + c);
-    uint32_t* d = reinterpret_cast<uint32_t*>(&tile[r][c]);
-    d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int c = i >> 3, r = 8 * (i & 7);
-    if (c0 + c >= cols || r0 + r >= ldo) continue;
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      w[k] = tile[r + 2 * k][c] | (uint32_t)tile[r + 2 * k + 1][c] << 16;
-    *reinterpret_cast<uint4*>(out + (c0 + c) * ldo + r0 + r) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-// out[q][p] = sum_k Q[q][k] P[p][k] (+ out's fp32 value so far), written as bf16,
-// or as fp32 (partials of the ranges of k along blockIdx.y, nq * np apart).
-struct ProductArgs {
+// out[q][p] = scale * sum_k Q[q][k] P[k][p] (+ out's fp32 value so far), written as
+// bf16, or as fp32 (a partial of every range of k, nq * np apart).  P is K-major; Q
+// is [nq][k], or K-major ([k][nq]) with QK.  Q's rows go on to a multiple of 8, with
+// zeros: a 16-byte load is cut at the end of its buffer by whole dwords.
+struct Product {
   const uint16_t* P;
   const uint16_t* Q;
   const float* before;  // fp32 [nq][np] to add, or nullptr
   uint16_t* out;        // bf16 [nq][np], or nullptr
   float* out32;         // fp32 [ranges][nq][np]
+  const float* scale;   // two factors, at scale[0] and scale2[0], or nullptr
+  const float* scale2;
   int64_t ldp, ldq, np, nq, k;  // elements
   int64_t range;                // k of a range, a multiple of 64
+  int32_t blocks;               // workgroups: tiles times ranges
 };
-__global__ __launch_bounds__(kThreads, 1) void k_product(ProductArgs a) {
-  __shared__ LossSmem sm;
+
+template <bool QK>
+__device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int block) {
   const int pts = (int)((a.np + kTile - 1) / kTile), qts = (int)((a.nq + kTile - 1) / kTile);
+  const int range = block / (pts * qts);
   int pt, qt;
-  tile_of(pts, qts, pt, qt);
+  tile_of(block - range * pts * qts, pts, qts, pt, qt);
   const int64_t p0 = (int64_t)pt * kTile, q0 = (int64_t)qt * kTile;
-  const int64_t k0 = (int64_t)blockIdx.y * a.range, k1 = std::min<int64_t>(a.k, k0 + a.range);
-  const Operand P = tile_rows(a.P + k0, a.ldp, p0, a.np, k1 - k0);
-  const Operand Q = tile_rows(a.Q + k0, a.ldq, q0, a.nq, k1 - k0);
+  const int64_t k0 = (int64_t)range * a.range, k = std::min<int64_t>(a.k - k0, a.range);
+  const Operand P = tile_columns(a.P + k0 * a.ldp, a.ldp, k, p0, a.np);
+  const Operand Q = QK ? tile_columns(a.Q + k0 * a.ldq, a.ldq, k, q0, (a.nq + 7) / 8 * 8)
+                       : tile_rows(a.Q + k0, a.ldq, q0, a.nq, (k + 7) / 8 * 8);
   v4f acc[64];
-  mainloop<false, false, false, true>(sm, P, Q, 0u, (uint32_t)(2 * (k1 - k0)), acc);
+  mainloop<false, false, false, true, true, QK>(sm, P, Q, 0u, (uint32_t)(2 * k), acc);
   const Place at;
-  float* out32 = a.out32 + (int64_t)blockIdx.y * a.nq * a.np;
+  const float scale = a.scale ? a.scale[0] * a.scale2[0] : 1.0f;
+  float* out32 = a.out32 + (int64_t)range * a.nq * a.np;
+  // Accumulator 8F + J, register r: P index 128 wp + 16 F + 4 g + r, and Q index
+  // 128 wq + 16 J + c (K-major), or that of Place::q.
 #pragma unroll
-  for (int H = 0; H < 2; ++H)
+  for (int J = 0; J < 8; ++J) {
+    const int64_t q = q0 + (QK ? 128 * at.wq + 16 * J + at.c : at.q(J >> 2, J & 3));
+    const bool row = q < a.nq;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t q = q0 + at.q(H, j);
-      if (q >= a.nq) continue;
+    for (int F = 0; F < 8; F += 2) {
+      float v[2][4];
 #pragma unroll
-      for (int G = 0; G < 2; ++G)
+      for (int u = 0; u < 2; ++u) {
+        const int64_t p = p0 + 128 * at.wp + 16 * (F + u) + 4 * at.g, o = q * a.np + p;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 8 consecutive columns
-          const int64_t p = p0 + at.p(G, 2 * h, 0);
-          if (p >= a.np) continue;
-          float v[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) v[u] = acc[8 * (4 * G + (u & 3)) + 4 * H + j][2 * h + (u >> 2)];
-          const int64_t o = q * a.np + p;
-          if (a.before != nullptr) {
-            const float4 b0 = *reinterpret_cast<const float4*>(a.before + o);
-            const float4 b1 = *reinterpret_cast<const float4*>(a.before + o + 4);
-            v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
-            v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
-          }
-          if (a.out != nullptr) {
-            *reinterpret_cast<uint4*>(a.out + o) =
-                make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                           pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-          } else {
-            *reinterpret_cast<float4*>(out32 + o) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(out32 + o + 4) = make_float4(v[4], v[5], v[6], v[7]);
-          }
+        for (int r = 0; r < 4; ++r) v[u][r] = acc[8 * (F + u) + J][r] * scale;
+        if (!row || p >= a.np) continue;
+        if (a.before != nullptr) {
+          const float4 b = *reinterpret_cast<const float4*>(a.before + o);
+          v[u][0] += b.x; v[u][1] += b.y; v[u][2] += b.z; v[u][3] += b.w;
         }
+        if (a.out == nullptr)
+          *reinterpret_cast<float4*>(out32 + o) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+      }
+      if (a.out == nullptr) continue;
+      // Lanes of rows g and g + 1 (g even) change quads, so that one holds 8
+      // consecutive columns of fragment F and the other of fragment F + 1.
+      u32x2 w[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        w[u] = u32x2{pack_bf16x2(v[u][0], v[u][1]), pack_bf16x2(v[u][2], v[u][3])};
+      const auto lo = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+      const auto hi = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+      const int64_t p = p0 + 128 * at.wp + 16 * (F + (at.g & 1)) + 8 * (at.g >> 1);
+      if (row && p < a.np)
+        *reinterpret_cast<uint4*>(a.out + q * a.np + p) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
     }
+  }
+}
+
+// Both products of a piece in one launch, the one with the longer tiles first: the
+// short tiles of the other fill the compute units that its last round leaves idle.
+__global__ __launch_bounds__(kThreads, 1) void k_products(Product dx, Product dw, int dx_first) {
+  __shared__ LossSmem sm;
+  const int first = dx_first ? dx.blocks : dw.blocks, block = (int)blockIdx.x;
+  if ((block < first) == (dx_first != 0))
+    product_tile<false>(sm, dx, dx_first ? block : block - first);
+  else
+    product_tile<true>(sm, dw, dx_first ? block - first : block);
 }
 
 // Sum of the partials of the ranges in order (after `before`), as bf16 or fp32.
@@ -388,87 +387,91 @@ __global__ __launch_bounds__(256) void k_product_join(const float* __restrict__ 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
 
-// Ranges of k that a product is cut into: as many as give every compute unit a
-// tile, of at least 512 elements each.
-int product_ranges(int64_t np, int64_t nq, int64_t k) {
+// Ranges of k for a product: none takes more stages than about half of what a
+// compute unit gets of the launch's work (so that the longest tiles do not outlast
+// the rest), none less than 512 of k; the partials stay below two tiles a unit.
+// A tile's start and end cost about as much as kTileStages stages.
+constexpr int64_t kTileStages = 8;
+int64_t stages(int64_t k) { return (k + 63) / 64; }
+int product_ranges(int64_t np, int64_t nq, int64_t k, int64_t work) {
   const int64_t n = tiles(np) * tiles(nq), cus = std::max(1, device_cu_count());
-  return (int)std::max<int64_t>(1, std::min<int64_t>(cus / n, k / 512));
+  const int64_t share = std::max<int64_t>(1, work / cus / 2);
+  return (int)std::max<int64_t>(
+      1, std::min({(stages(k) + share - 1) / share, k / 512, 2 * cus / n}));
+}
+int64_t product_work(int64_t np, int64_t nq, int64_t k) {
+  return tiles(np) * tiles(nq) * (stages(k) + kTileStages);
 }
 
-hipError_t run_product(ProductArgs a, float* partials, float* acc, hipStream_t stream) {
-  const int ranges = product_ranges(a.np, a.nq, a.k);
-  a.range = up((a.k + ranges - 1) / ranges, 64);
-  const int used = (int)((a.k + a.range - 1) / a.range);
-  const dim3 grid((unsigned)(tiles(a.np) * tiles(a.nq)), (unsigned)used);
-  if (used == 1) {
-    a.out32 = acc;
-    hipLaunchKernelGGL(k_product, grid, dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
-  }
-  const float* before = a.before;
-  uint16_t* out = a.out;
-  a.before = nullptr;
-  a.out = nullptr;
-  a.out32 = partials;
-  hipLaunchKernelGGL(k_product, grid, dim3(kThreads), 0, stream, a);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  const int64_t n = a.np * a.nq;
-  hipLaunchKernelGGL(k_product_join, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream,
-                     partials, used, n, before, out, acc);
-  return hipGetLastError();
-}
-
-hipError_t transpose(const uint16_t* in, int64_t ldi, int64_t rows, int64_t cols, uint16_t* out,
-                     int64_t ldo, hipStream_t stream) {
-  const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)((ldo + 63) / 64));
-  hipLaunchKernelGGL(k_transpose, grid, dim3(256), 0, stream, in, ldi, rows, cols, out, ldo);
-  return hipGetLastError();
-}
-
-// Words of a piece: d, d^T and W^T of it stay within kPieceBytes, the pieces of
-// one vocabulary are alike.
-constexpr int64_t kPieceBytes = INT64_C(1) << 30;
+// Words of a piece: its d stays within kPieceBytes, and the pieces of one vocabulary
+// are alike.
+constexpr int64_t kPieceBytes = INT64_C(1) << 28;
 int64_t piece_words(const LossArgs& a) {
-  const int64_t most = std::max<int64_t>(kTile, kPieceBytes / (4 * up(a.T, kTile) + 2 * a.H) / kTile * kTile);
+  const int64_t most = std::min<int64_t>(
+      std::max<int64_t>(kTile, kPieceBytes / (2 * a.T) / kTile * kTile), INT64_C(1) << 21);
   const int64_t pieces = (a.V + most - 1) / most;
   return up((a.V + pieces - 1) / pieces, kTile);
 }
 
+// Ranges of the two products of a piece of `words` words; the same where only one
+// gradient is wanted, which then has the same bits.
+struct PieceRanges {
+  int dx, dw;
+};
+PieceRanges piece_ranges(const LossArgs& a, int64_t words) {
+  const int64_t work = product_work(a.H, a.T, words) + product_work(a.H, words, a.T);
+  return {product_ranges(a.H, a.T, words, work), product_ranges(a.H, words, a.T, work)};
+}
+
 // Offsets of the gradient's workspace.
 struct GradSpace {
-  int64_t piece, d, dt, wt, xt, acc, part, bytes;
+  int64_t piece, d, acc, part_x, part_w, bytes;
 };
 GradSpace grad_space(const LossArgs& a, bool need_x, bool need_w) {
   GradSpace s{};
   s.piece = piece_words(a);
-  const int64_t ldt = up(a.T, kTile);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t o = at;
     at += up(bytes, 256);
     return o;
   };
-  int64_t part = 0;
-  if (need_x) {
-    s.d = take(a.T * s.piece * 2);
-    s.wt = take(a.H * s.piece * 2);
-    if (s.piece < a.V) s.acc = take(a.T * a.H * 4);
-    const int ranges = product_ranges(a.H, a.T, s.piece);
-    if (ranges > 1) part = ranges * a.T * a.H * 4;
+  s.d = take(a.T * s.piece * 2);
+  if (need_x && s.piece < a.V) s.acc = take(a.T * a.H * 4);
+  int64_t part_x = 0, part_w = 0;
+  const int64_t last = a.V - (a.V - 1) / s.piece * s.piece;
+  for (const int64_t words : {std::min(s.piece, a.V), last}) {
+    const PieceRanges r = piece_ranges(a, words);
+    if (need_x && r.dx > 1) part_x = std::max(part_x, r.dx * a.T * a.H * 4);
+    if (need_w && r.dw > 1) part_w = std::max(part_w, r.dw * words * a.H * 4);
   }
-  if (need_w) {
-    s.dt = take(s.piece * ldt * 2);
-    s.xt = take(a.H * ldt * 2);
-    const int64_t rows = std::min(s.piece, a.V);
-    for (int64_t n : {rows, a.V - (a.V - 1) / s.piece * s.piece}) {  // a piece, and the last one
-      const int ranges = product_ranges(a.H, n, ldt);
-      if (ranges > 1) part = std::max<int64_t>(part, ranges * n * a.H * 4);
-    }
-  }
-  s.part = take(part);
+  s.part_x = take(part_x);
+  s.part_w = take(part_w);
   s.bytes = at;
   return s;
+}
+
+// Cuts a product into `ranges` of k (fewer where they come out empty) and gives its
+// number of workgroups; with more than one they write partials.
+Product cut(Product p, int ranges, float* partials, float* acc) {
+  p.range = up((p.k + ranges - 1) / ranges, 64);
+  const int used = (int)((p.k + p.range - 1) / p.range);
+  p.blocks = (int32_t)(tiles(p.np) * tiles(p.nq) * used);
+  p.out32 = acc;
+  if (used > 1) {
+    p.out = nullptr;
+    p.before = nullptr;
+    p.out32 = partials;
+  }
+  return p;
+}
+hipError_t join(const Product& p, int ranges, float* partials, float* acc, hipStream_t stream) {
+  const int64_t range = up((p.k + ranges - 1) / ranges, 64), n = p.np * p.nq;
+  const int used = (int)((p.k + range - 1) / range);
+  if (used <= 1) return hipSuccess;
+  hipLaunchKernelGGL(k_product_join, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream,
+                     partials, used, n, p.before, p.out, acc);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -503,48 +506,50 @@ int64_t loss_grad_workspace_bytes(const LossArgs& a, bool need_x, bool need_w) {
 hipError_t launch_loss_grad(LossArgs a, uint16_t* dx, uint16_t* dw, uint8_t* ws,
                             hipStream_t stream) {
   const GradSpace s = grad_space(a, dx != nullptr, dw != nullptr);
-  a.ldt = up(a.T, kTile);
-  a.d = dx ? reinterpret_cast<uint16_t*>(ws + s.d) : nullptr;
-  a.dt = dw ? reinterpret_cast<uint16_t*>(ws + s.dt) : nullptr;
-  uint16_t* wt = reinterpret_cast<uint16_t*>(ws + s.wt);
-  uint16_t* xt = reinterpret_cast<uint16_t*>(ws + s.xt);
+  a.d = reinterpret_cast<uint16_t*>(ws + s.d);
   float* acc = reinterpret_cast<float*>(ws + s.acc);
-  float* part = reinterpret_cast<float*>(ws + s.part);
-  hipError_t err;
-  if (dw && (err = transpose(a.x, a.ldx, a.T, a.H, xt, a.ldt, stream)) != hipSuccess) return err;
+  float* part_x = reinterpret_cast<float*>(ws + s.part_x);
+  float* part_w = reinterpret_cast<float*>(ws + s.part_w);
   for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) {
-    const int64_t words = std::min<int64_t>(s.piece, a.V - v0);
-    const int64_t width = up(words, kTile);
+    const int64_t words = std::min<int64_t>(s.piece, a.V - v0), width = up(words, kTile);
     hipLaunchKernelGGL(k_loss_grad_tile, dim3((unsigned)(width / kTile * tiles(a.T))),
                        dim3(kThreads), 0, stream, a, v0, (int)width);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    const PieceRanges r = piece_ranges(a, words);
+    Product px{}, pw{};
+    if (!a.per_token) {
+      px.scale = pw.scale = a.grad_loss;
+      px.scale2 = pw.scale2 = a.stats + a.T;
+    }
+    px.np = pw.np = a.H;
+    if (dx) {  // dx[t][h] = sum over words of d[t][v] W[v][h]
+      px.P = a.w + v0 * a.ldw;
+      px.ldp = a.ldw;
+      px.Q = a.d;
+      px.ldq = width;
+      px.nq = a.T;
+      px.k = words;
+      px.before = v0 > 0 ? acc : nullptr;
+      px.out = v0 + words == a.V ? dx : nullptr;
+    }
+    if (dw) {  // dW[v][h] = sum over tokens of d[t][v] x[t][h]
+      pw.P = a.x;
+      pw.ldp = a.ldx;
+      pw.Q = a.d;
+      pw.ldq = width;
+      pw.nq = words;
+      pw.k = a.T;
+      pw.out = dw + v0 * a.H;
+    }
+    const Product cx = dx ? cut(px, r.dx, part_x, acc) : px;
+    const Product cw = dw ? cut(pw, r.dw, part_w, nullptr) : pw;
+    const bool dx_first = dx && (!dw || cx.range >= cw.range);
+    hipLaunchKernelGGL(k_products, dim3((unsigned)(cx.blocks + cw.blocks)), dim3(kThreads), 0,
+                       stream, cx, cw, (int)dx_first);
     if ((err = hipGetLastError()) != hipSuccess) return err;
-    if (dx) {
-      err = transpose(a.w + v0 * a.ldw, a.ldw, words, a.H, wt, width, stream);
-      if (err != hipSuccess) return err;
-      ProductArgs p{};
-      p.P = wt;
-      p.ldp = width;
-      p.np = a.H;
-      p.Q = a.d;
-      p.ldq = width;
-      p.nq = a.T;
-      p.k = width;
-      p.before = v0 > 0 ? acc : nullptr;
-      p.out = v0 + words == a.V ? dx : nullptr;
-      if ((err = run_product(p, part, acc, stream)) != hipSuccess) return err;
-    }
-    if (dw) {
-      ProductArgs p{};
-      p.P = xt;
-      p.ldp = a.ldt;
-      p.np = a.H;
-      p.Q = a.dt;
-      p.ldq = a.ldt;
-      p.nq = words;
-      p.k = up(a.T, 8);
-      p.out = dw + v0 * a.H;
-      if ((err = run_product(p, part, nullptr, stream)) != hipSuccess) return err;
-    }
+    if (dx && (err = join(px, r.dx, part_x, acc, stream)) != hipSuccess) return err;
+    if (dw && (err = join(pw, r.dw, part_w, nullptr, stream)) != hipSuccess) return err;
   }
   return hipSuccess;
 }

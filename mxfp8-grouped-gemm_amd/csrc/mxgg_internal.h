@@ -189,7 +189,7 @@ hipError_t launch_adamw(const AdamTensor* tensors, int64_t count, int state_bits
 int64_t adamw_max_elements();
 
 // Cross entropy of a linear layer (loss.hip).  The launchers fill in what lies in
-// their workspace (part, target_logit, d, dt, ldt, token_loss where it is null).
+// their workspace (part, target_logit, d, token_loss where it is null).
 struct LossArgs {
   const uint16_t* x;   // bf16 [T][H], row stride ldx
   const uint16_t* w;   // bf16 [V][H], row stride ldw
@@ -201,8 +201,7 @@ struct LossArgs {
   float2* part;
   float* target_logit;
   uint16_t* d;
-  uint16_t* dt;
-  int64_t T, V, H, ldx, ldw, ldt, ignore_index;
+  int64_t T, V, H, ldx, ldw, ignore_index;
   int32_t target64, mean, per_token;
 };
 int64_t loss_workspace_bytes(const LossArgs& args);

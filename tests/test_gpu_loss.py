@@ -89,9 +89,13 @@ def test_matches_oracle(gpu, T, V, H, reduction):
 
 
 def test_many_pieces(gpu):
-    """A vocabulary of several pieces (4 * 1024 + 2 * 32768 bytes a word: 15360
-    words for 1 GiB), the last one shorter, and tokens and words past a tile."""
-    T, V, H = 1000, 33000, 32768
+    """Long rows, and a vocabulary of several pieces (of 256 MiB of 2 T bytes a
+    word), the last one shorter; tokens and words past a tile."""
+    for T, V, H in ((1000, 33000, 32768), (4100, 70001, 72)):
+        _large(gpu, T, V, H)
+
+
+def _large(gpu, T, V, H):
     g = torch.Generator(device=gpu).manual_seed(2)
     x = torch.randn((T, H), generator=g, device=gpu).to(torch.bfloat16)
     w = (torch.randn((V, H), generator=g, device=gpu) / H ** 0.5).to(torch.bfloat16)
