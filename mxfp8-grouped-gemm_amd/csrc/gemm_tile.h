@@ -390,22 +390,24 @@ __device__ __forceinline__ void read_sb(const uint8_t* stage, const FragAddr& fa
   f.sb[H] = SCALED ? *reinterpret_cast<const uint32_t*>(stage + fa.qs + 64u * H) : 0x7F7F7F7Fu;
 }
 
+// Both k steps of a bf16 stage: the low halves of two fragments, then the high ones.
+__device__ __forceinline__ v4f mfma_bf16_stage(const v8i& a, const v8i& b, v4f c) {
+  typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  const auto lo = [](const v8i& x) { return __builtin_bit_cast(v8bf, (v4i){x[0], x[1], x[2], x[3]}); };
+  const auto hi = [](const v8i& x) { return __builtin_bit_cast(v8bf, (v4i){x[4], x[5], x[6], x[7]}); };
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo(a), lo(b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi(a), hi(b), c, 0, 0, 0);
+}
+
 // One MFMA: P fragment PI against Q fragment QJ into accumulator 8 PI + QJ;
 // op_sel picks byte PI % 4 of the P scale dword of half PI / 4 and byte
 // QJ % 4 of the Q dword of half QJ / 4.
-// BF16: both k steps of the stage.
+// BF16: both k steps of the stage, no scales.
 template <bool BF16, int PI, int QJ>
 __device__ __forceinline__ void mma(const Frags& f, v4f (&acc)[64]) {
   if constexpr (BF16) {
-    typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-    typedef int v4i __attribute__((ext_vector_type(4)));
-    const v8i a = f.a[PI], b = f.b[QJ];
-    const auto lo = [](const v8i& x) { return __builtin_bit_cast(v8bf, (v4i){x[0], x[1], x[2], x[3]}); };
-    const auto hi = [](const v8i& x) { return __builtin_bit_cast(v8bf, (v4i){x[4], x[5], x[6], x[7]}); };
-    acc[8 * PI + QJ] =
-        __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo(a), lo(b), acc[8 * PI + QJ], 0, 0, 0);
-    acc[8 * PI + QJ] =
-        __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi(a), hi(b), acc[8 * PI + QJ], 0, 0, 0);
+    acc[8 * PI + QJ] = mfma_bf16_stage(f.a[PI], f.b[QJ], acc[8 * PI + QJ]);
     return;
   }
   acc[8 * PI + QJ] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(

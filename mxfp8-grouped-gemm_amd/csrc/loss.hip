@@ -27,15 +27,26 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 256;
+constexpr int kSmallTile = 128;
 
 struct __align__(16) LossSmem {
   uint8_t ring[2][kStageBytes];
 };
 
-// Rows row0 .. of a bf16 matrix as a tile operand, `cols` of them contiguous.
+// Tiles of 128 x 128 for calls that large ones would leave most of the chip idle:
+// four waves of 64 x 64, four ring stages of 64 contraction elements (three in
+// flight), one barrier a stage.  A row is 128 bytes, its 16-byte chunk c at
+// c ^ swz(row), so a half-wave's fragment read touches every bank twice.
+constexpr uint32_t kSmallOp = 128u * kStageK;  // one operand of a stage: 16 KB
+constexpr int kSmallLoads = 8;                 // of a wave for a stage
+struct __align__(16) SmallSmem {
+  uint8_t ring[4][2 * kSmallOp];
+};
+
+// Rows row0 .. of a bf16 matrix as a tile operand, `cols` elements of each.
 __device__ __forceinline__ Operand tile_rows(const uint16_t* p, int64_t ld, int64_t row0,
-                                             int64_t rows, int64_t cols) {
-  const int64_t n = std::min<int64_t>(kTile, rows - row0);
+                                             int64_t rows, int64_t cols, int tile = kTile) {
+  const int64_t n = std::min<int64_t>(tile, rows - row0);
   Operand o;
   o.data = make_desc(p + row0 * ld, (uint32_t)(((n - 1) * ld + cols) * 2));
   o.scale = o.data;  // not read
@@ -91,11 +102,69 @@ struct Place {
   __device__ __forceinline__ int q(int H, int j) const { return 128 * wq + 64 * H + 4 * c + j; }
 };
 
+// Accumulators of a wave's 64 x 64 part of a small tile: acc[4F + J], register r of
+// lane c + 16g, is P index 64 wp + 16 F + 4 g + r and Q index 64 wq + 16 J + c.
+__device__ __forceinline__ void small_loop(SmallSmem& sm, const Operand& P, const Operand& Q,
+                                           uint32_t kend, v4f (&acc)[16]) {
+  const uint32_t lane = threadIdx.x & 63u, wave = wave_id();
+  const uint32_t wp = wave & 1u, wq = wave >> 1, m = lane & 15u, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t nst = (kend + kStageK - 1) / kStageK;
+  // Load i of wave w fills rows 32i + 8w .. + 7 of an operand, eight lanes a row.
+  const uint32_t row = 8u * wave + (lane >> 3);
+  const uint32_t kcol = 16u * ((lane & 7u) ^ swz(row));
+  const uint32_t vp = row * P.ld + kcol, vq = row * Q.ld + kcol;
+  const auto load = [&](uint32_t s) __attribute__((always_inline)) {
+    const uint32_t k0 = s * kStageK, dst = lds_offset(sm.ring[s & 3u]) + 1024u * wave;
+    const bool ok = k0 + kcol < kend;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      dma_x4(P.data, dst + 4096u * i, ok ? vp + k0 : kOobOffset, 32u * i * P.ld);
+      dma_x4(Q.data, dst + kSmallOp + 4096u * i, ok ? vq + k0 : kOobOffset, 32u * i * Q.ld);
+    }
+  };
+  const uint32_t lo = ((g ^ swz(m)) << 4), hi = (((g + 4u) ^ swz(m)) << 4);
+  const uint32_t rp = (64u * wp + m) * kStageK, rq = kSmallOp + (64u * wq + m) * kStageK;
+  load(0);
+  if (nst > 1) load(1);
+  if (nst > 2) load(2);
+  for (uint32_t s = 0; s < nst; ++s) {
+    // stage s has landed for every wave, and every wave has read stage s - 1, whose
+    // slot the next load takes
+    if (s + 2 < nst) wait_barrier<2 * kSmallLoads>();
+    else if (s + 1 < nst) wait_barrier<kSmallLoads>();
+    else wait_barrier<0>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 3 < nst) load(s + 3);
+    const uint8_t* st = sm.ring[s & 3u];
+    Frags f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f.a[i] = lds_v8i(st + rp + lo + 2048 * i, st + rp + hi + 2048 * i);
+      f.b[i] = lds_v8i(st + rq + lo + 2048 * i, st + rq + hi + 2048 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[4 * i + j] = mfma_bf16_stage(f.a[i], f.b[j], acc[4 * i + j]);
+  }
+  release_barrier();
+}
+
 // Target of token t: its word, -1 = ignored, -2 = outside the vocabulary.
 __device__ __forceinline__ int64_t target_of(const LossArgs& a, int64_t t) {
   const int64_t v = a.target64 ? static_cast<const int64_t*>(a.target)[t]
                                : (int64_t) static_cast<const int32_t*>(a.target)[t];
   return v == a.ignore_index ? -1 : v >= 0 && v < a.V ? v : -2;
+}
+
+// (max, sum of exp(z - max)) of two sets of words.
+__device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
+  const float m = __builtin_fmaxf(u.x, v.x);
+  const float base = m == -__builtin_inff() ? 0.0f : m;
+  return make_float2(m, u.y * __builtin_amdgcn_exp2f((u.x - base) * kLog2e) +
+                            v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e));
 }
 
 // Statistics of a tile: part[p tile][t] = (max, sum of exp(z - max)) over the
@@ -157,12 +226,55 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a) {
   __syncthreads();
   const int64_t t = q0 + threadIdx.x;
   if (t >= a.T) return;
-  const float2 u = joined[threadIdx.x], v = joined[256 + threadIdx.x];
-  const float m = __builtin_fmaxf(u.x, v.x);
-  const float base = m == -__builtin_inff() ? 0.0f : m;
-  a.part[(int64_t)pt * a.T + t] =
-      make_float2(m, u.y * __builtin_amdgcn_exp2f((u.x - base) * kLog2e) +
-                         v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e));
+  a.part[(int64_t)pt * a.T + t] = join_halves(joined[threadIdx.x], joined[256 + threadIdx.x]);
+}
+
+// The same for small tiles.
+__global__ __launch_bounds__(kThreads) void k_loss_fwd_small(LossArgs a) {
+  __shared__ SmallSmem sm;
+  const int np = (int)((a.V + kSmallTile - 1) / kSmallTile);
+  const int nq = (int)((a.T + kSmallTile - 1) / kSmallTile);
+  int pt, qt;
+  tile_of((int)blockIdx.x, np, nq, pt, qt);
+  const int64_t p0 = (int64_t)pt * kSmallTile, q0 = (int64_t)qt * kSmallTile;
+  const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H, kSmallTile);
+  const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H, kSmallTile);
+  v4f acc[16];
+  small_loop(sm, P, Q, (uint32_t)(2 * a.H), acc);
+
+  const Place at;
+  const int words = (int)std::min<int64_t>(kSmallTile, a.V - p0);
+  const int first = 64 * at.wp + 4 * at.g;  // + 16 F + r
+  float2* joined = reinterpret_cast<float2*>(&sm.ring[0][0]);  // [wp][token]
+#pragma unroll
+  for (int J = 0; J < 4; ++J) {
+    const int q = 64 * at.wq + 16 * J + at.c;
+    float z[16], m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      z[i] = first + 16 * (i >> 2) + (i & 3) < words ? acc[4 * (i >> 2) + J][i & 3]
+                                                     : -__builtin_inff();
+      m = __builtin_fmaxf(m, z[i]);
+    }
+    m = __builtin_fmaxf(m, __shfl_xor(m, 16));
+    m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+    const float shift = m == -__builtin_inff() ? 0.0f : -m * kLog2e;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], kLog2e, shift));
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (at.g == 0) joined[kSmallTile * at.wp + q] = make_float2(m, s);
+    const int64_t t = q0 + q, word = t < a.T ? target_of(a, t) - p0 - first : -1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (word == 16 * (i >> 2) + (i & 3)) a.target_logit[t] = z[i];
+  }
+  __syncthreads();
+  const int64_t t = q0 + threadIdx.x;
+  if (threadIdx.x >= kSmallTile || t >= a.T) return;
+  a.part[(int64_t)pt * a.T + t] = join_halves(joined[threadIdx.x], joined[kSmallTile + threadIdx.x]);
 }
 
 // lse and loss of every token from its tiles' statistics: 16 tokens a workgroup,
@@ -172,21 +284,24 @@ __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a
   __shared__ float2 run_s[kJoinRuns][kJoinTokens];
   const int k = threadIdx.x % kJoinTokens, run = threadIdx.x / kJoinTokens;
   const int64_t t = (int64_t)blockIdx.x * kJoinTokens + k;
-  float m = -__builtin_inff(), s = 0.0f;
-  const auto join = [&](float2 v) {
-    const float top = __builtin_fmaxf(m, v.x);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f((m - base) * kLog2e) +
-        v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e);
-    m = top;
-  };
+  float2 sum = make_float2(-__builtin_inff(), 0.0f);
+  constexpr int kAhead = 8;  // loads in flight
   if (t < a.T)
-    for (int i = run; i < tiles; i += kJoinRuns) join(a.part[(int64_t)i * a.T + t]);
-  run_s[run][k] = make_float2(m, s);
+    for (int i0 = run; i0 < tiles; i0 += kJoinRuns * kAhead) {
+      float2 v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kJoinRuns;
+        v[u] = i < tiles ? a.part[(int64_t)i * a.T + t] : make_float2(-__builtin_inff(), 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) sum = join_halves(sum, v[u]);
+    }
+  run_s[run][k] = sum;
   __syncthreads();
   if (run != 0 || t >= a.T) return;
-  for (int i = 1; i < kJoinRuns; ++i) join(run_s[i][k]);
-  const float lse = m + __builtin_amdgcn_logf(s) * kLn2;
+  for (int i = 1; i < kJoinRuns; ++i) sum = join_halves(sum, run_s[i][k]);
+  const float lse = sum.x + __builtin_amdgcn_logf(sum.y) * kLn2;
   const int64_t target = target_of(a, t);
   const float nan = __builtin_nanf("");
   a.stats[t] = target == -2 ? nan : lse;
@@ -283,6 +398,49 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
         o[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
     }
+}
+
+// The same for small tiles (width: the words rounded up to 256 as well).
+__global__ __launch_bounds__(kThreads) void k_loss_grad_small(LossArgs a, int64_t v0, int width) {
+  __shared__ SmallSmem sm;
+  const int np = width / kSmallTile, nq = (int)((a.T + kSmallTile - 1) / kSmallTile);
+  int pt, qt;
+  tile_of((int)blockIdx.x, np, nq, pt, qt);
+  const int64_t p0 = v0 + (int64_t)pt * kSmallTile, q0 = (int64_t)qt * kSmallTile;
+  v4f acc[16];
+  if (p0 < a.V) {  // a width rounded up to 256 can end in a tile without words
+    const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H, kSmallTile);
+    const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H, kSmallTile);
+    small_loop(sm, P, Q, (uint32_t)(2 * a.H), acc);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const Place at;
+  const int words = (int)std::min<int64_t>(kSmallTile, a.V - p0);
+  const int first = 64 * at.wp + 4 * at.g;
+#pragma unroll
+  for (int J = 0; J < 4; ++J) {
+    const int64_t t = q0 + 64 * at.wq + 16 * J + at.c;
+    if (t >= a.T) continue;
+    const int64_t target = target_of(a, t);
+    const float shift = target == -1 ? 0.0f : -a.stats[t] * kLog2e;
+    const float g = target != -1 && a.per_token ? a.grad_loss[t] : 1.0f;
+    const int64_t word = target - p0 - first;
+#pragma unroll
+    for (int F = 0; F < 4; ++F) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * F + J][r], kLog2e, shift));
+        v[r] = target == -1 || first + 16 * F + r >= words
+                   ? 0.0f
+                   : (e - (word == 16 * F + r ? 1.0f : 0.0f)) * g;
+      }
+      *reinterpret_cast<uint2*>(a.d + t * width + (int64_t)pt * kSmallTile + first + 16 * F) =
+          make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+  }
 }
 
 // out[q][p] = scale * sum_k Q[q][k] P[k][p] (+ out's fp32 value so far), written as
@@ -386,6 +544,14 @@ __global__ __launch_bounds__(256) void k_product_join(const float* __restrict__ 
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
+int64_t small_tiles(int64_t n) { return (n + kSmallTile - 1) / kSmallTile; }
+
+// Whether `words` words of logits go by small tiles: where those are one round of
+// the chip.  Small / large, hidden size 1024, us: 128 tokens, 32000 words (250 small
+// tiles) 25.8 / 33.8; 128 x 64000 (500) 46.2 / 38.9; 256 x 32000 (500) 40.9 / 33.6.
+bool use_small(const LossArgs& a, int64_t words) {
+  return small_tiles(words) * small_tiles(a.T) <= std::max(1, device_cu_count());
+}
 
 // Ranges of k for a product: none takes more stages than about half of what a
 // compute unit gets of the launch's work (so that the longest tiles do not outlast
@@ -477,20 +643,27 @@ hipError_t join(const Product& p, int ranges, float* partials, float* acc, hipSt
 }  // namespace
 
 int64_t loss_workspace_bytes(const LossArgs& a) {
-  return up(tiles(a.V) * a.T * 8, 256) + up(a.T * 4, 256) * 2;
+  const int64_t n = use_small(a, a.V) ? small_tiles(a.V) : tiles(a.V);
+  return up(n * a.T * 8, 256) + up(a.T * 4, 256) * 2;
 }
 
 hipError_t launch_loss(LossArgs a, uint8_t* ws, hipStream_t stream) {
   if (a.T > 0) {
+    const bool small = use_small(a, a.V);
+    const int64_t np = small ? small_tiles(a.V) : tiles(a.V);
     a.part = reinterpret_cast<float2*>(ws);
-    a.target_logit = reinterpret_cast<float*>(ws + up(tiles(a.V) * a.T * 8, 256));
+    a.target_logit = reinterpret_cast<float*>(ws + up(np * a.T * 8, 256));
     if (!a.token_loss) a.token_loss = a.target_logit + up(a.T * 4, 256) / 4;
-    hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)(tiles(a.V) * tiles(a.T))), dim3(kThreads), 0,
-                       stream, a);
+    if (small)
+      hipLaunchKernelGGL(k_loss_fwd_small, dim3((unsigned)(np * small_tiles(a.T))), dim3(kThreads),
+                         0, stream, a);
+    else
+      hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)(np * tiles(a.T))), dim3(kThreads), 0, stream,
+                         a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     hipLaunchKernelGGL(k_loss_join, dim3((unsigned)((a.T + kJoinTokens - 1) / kJoinTokens)),
-                       dim3(kJoinTokens * kJoinRuns), 0, stream, a, (int)tiles(a.V));
+                       dim3(kJoinTokens * kJoinRuns), 0, stream, a, (int)np);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
@@ -512,8 +685,13 @@ hipError_t launch_loss_grad(LossArgs a, uint16_t* dx, uint16_t* dw, uint8_t* ws,
   float* part_w = reinterpret_cast<float*>(ws + s.part_w);
   for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) {
     const int64_t words = std::min<int64_t>(s.piece, a.V - v0), width = up(words, kTile);
-    hipLaunchKernelGGL(k_loss_grad_tile, dim3((unsigned)(width / kTile * tiles(a.T))),
-                       dim3(kThreads), 0, stream, a, v0, (int)width);
+    if (use_small(a, words))
+      hipLaunchKernelGGL(k_loss_grad_small,
+                         dim3((unsigned)(width / kSmallTile * small_tiles(a.T))), dim3(kThreads), 0,
+                         stream, a, v0, (int)width);
+    else
+      hipLaunchKernelGGL(k_loss_grad_tile, dim3((unsigned)(width / kTile * tiles(a.T))),
+                         dim3(kThreads), 0, stream, a, v0, (int)width);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     const PieceRanges r = piece_ranges(a, words);
