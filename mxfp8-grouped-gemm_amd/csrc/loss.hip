@@ -42,6 +42,10 @@ constexpr int kSmallLoads = 8;                 // of a wave for a stage
 struct __align__(16) SmallSmem {
   uint8_t ring[4][2 * kSmallOp];
 };
+union TileSmem {
+  LossSmem large;
+  SmallSmem small;
+};
 
 // Rows row0 .. of a bf16 matrix as a tile operand, `cols` elements of each.
 __device__ __forceinline__ Operand tile_rows(const uint16_t* p, int64_t ld, int64_t row0,
@@ -167,14 +171,10 @@ __device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
                             v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e));
 }
 
-// Statistics of a tile: part[p tile][t] = (max, sum of exp(z - max)) over the
+// Statistics of a tile: part[part row][t] = (max, sum of exp(z - max)) over the
 // tile's words, and the target's logit.
-__global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a) {
-  __shared__ LossSmem sm;
-  const int np = (int)((a.V + kTile - 1) / kTile), nq = (int)((a.T + kTile - 1) / kTile);
-  int pt, qt;
-  tile_of((int)blockIdx.x, np, nq, pt, qt);
-  const int64_t p0 = (int64_t)pt * kTile, q0 = (int64_t)qt * kTile;
+__device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_t p0, int64_t q0,
+                                         int64_t part_row) {
   const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H);
   const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
   v4f acc[64];
@@ -226,17 +226,12 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a) {
   __syncthreads();
   const int64_t t = q0 + threadIdx.x;
   if (t >= a.T) return;
-  a.part[(int64_t)pt * a.T + t] = join_halves(joined[threadIdx.x], joined[256 + threadIdx.x]);
+  a.part[part_row * a.T + t] = join_halves(joined[threadIdx.x], joined[256 + threadIdx.x]);
 }
 
-// The same for small tiles.
-__global__ __launch_bounds__(kThreads) void k_loss_fwd_small(LossArgs a) {
-  __shared__ SmallSmem sm;
-  const int np = (int)((a.V + kSmallTile - 1) / kSmallTile);
-  const int nq = (int)((a.T + kSmallTile - 1) / kSmallTile);
-  int pt, qt;
-  tile_of((int)blockIdx.x, np, nq, pt, qt);
-  const int64_t p0 = (int64_t)pt * kSmallTile, q0 = (int64_t)qt * kSmallTile;
+// The same for a small tile.
+__device__ __forceinline__ void fwd_tile_small(SmallSmem& sm, const LossArgs& a, int64_t p0,
+                                               int64_t q0, int64_t part_row) {
   const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H, kSmallTile);
   const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H, kSmallTile);
   v4f acc[16];
@@ -274,7 +269,24 @@ __global__ __launch_bounds__(kThreads) void k_loss_fwd_small(LossArgs a) {
   __syncthreads();
   const int64_t t = q0 + threadIdx.x;
   if (threadIdx.x >= kSmallTile || t >= a.T) return;
-  a.part[(int64_t)pt * a.T + t] = join_halves(joined[threadIdx.x], joined[kSmallTile + threadIdx.x]);
+  a.part[part_row * a.T + t] = join_halves(joined[threadIdx.x], joined[kSmallTile + threadIdx.x]);
+}
+
+// Large tiles for the first large_words words, small ones for the rest.
+__global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a, int64_t large_words) {
+  __shared__ TileSmem sm;
+  const int np = (int)((large_words + kTile - 1) / kTile), nq = (int)((a.T + kTile - 1) / kTile);
+  const int large = np * nq, block = (int)blockIdx.x;
+  int pt, qt;
+  if (block < large) {
+    tile_of(block, np, nq, pt, qt);
+    fwd_tile(sm.large, a, (int64_t)pt * kTile, (int64_t)qt * kTile, pt);
+  } else {
+    const int ns = (int)((a.V - large_words + kSmallTile - 1) / kSmallTile);
+    tile_of(block - large, ns, (int)((a.T + kSmallTile - 1) / kSmallTile), pt, qt);
+    fwd_tile_small(sm.small, a, large_words + (int64_t)pt * kSmallTile, (int64_t)qt * kSmallTile,
+                   np + pt);
+  }
 }
 
 // lse and loss of every token from its tiles' statistics: 16 tokens a workgroup,
@@ -335,20 +347,16 @@ __global__ __launch_bounds__(kReduceThreads) void k_loss_reduce(LossArgs a) {
   }
 }
 
-// d of words v0 .. v0 + width of the vocabulary (width: the piece's words rounded
-// up to 256; words past the vocabulary, and tokens past the last, get zeros).
-__global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int64_t v0, int width) {
-  __shared__ LossSmem sm;
-  const int np = width / kTile, nq = (int)((a.T + kTile - 1) / kTile);
-  int pt, qt;
-  tile_of((int)blockIdx.x, np, nq, pt, qt);
-  const int64_t p0 = v0 + (int64_t)pt * kTile, q0 = (int64_t)qt * kTile;
+// d of the tile of words v0 + p0 .. and tokens q0 ..; row t of d at a.d + t * width.
+// Words past the vocabulary get zeros.
+__device__ __forceinline__ void grad_tile(LossSmem& sm, const LossArgs& a, int64_t v0, int64_t p0,
+                                          int64_t q0, int64_t width) {
   const Place at;
   v4f acc[64];
-  const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H);
+  const Operand P = tile_rows(a.w, a.ldw, v0 + p0, a.V, a.H);
   const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
   mainloop<false, false, false, true>(sm, P, Q, 0u, (uint32_t)(2 * a.H), acc);
-  const int words = (int)std::min<int64_t>(kTile, a.V - p0);
+  const int words = (int)std::min<int64_t>(kTile, a.V - v0 - p0);
 #pragma unroll
   for (int H = 0; H < 2; ++H)
 #pragma unroll
@@ -364,7 +372,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
           shift = -a.stats[t] * kLog2e;
           if (a.per_token) g = a.grad_loss[t];
         }
-        word -= p0;
+        word -= v0 + p0;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -393,23 +401,19 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int6
           for (int u = 0; u < 2; ++u)
             w[2 * r + u] = pack_bf16x2(acc[8 * (4 * G + 2 * u) + 4 * H + j][r],
                                        acc[8 * (4 * G + 2 * u + 1) + 4 * H + j][r]);
-        uint4* o = reinterpret_cast<uint4*>(a.d + t * width + (int64_t)pt * kTile + at.p(G, 0, 0));
+        uint4* o = reinterpret_cast<uint4*>(a.d + t * width + p0 + at.p(G, 0, 0));
         o[0] = make_uint4(w[0], w[1], w[2], w[3]);
         o[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
     }
 }
 
-// The same for small tiles (width: the words rounded up to 256 as well).
-__global__ __launch_bounds__(kThreads) void k_loss_grad_small(LossArgs a, int64_t v0, int width) {
-  __shared__ SmallSmem sm;
-  const int np = width / kSmallTile, nq = (int)((a.T + kSmallTile - 1) / kSmallTile);
-  int pt, qt;
-  tile_of((int)blockIdx.x, np, nq, pt, qt);
-  const int64_t p0 = v0 + (int64_t)pt * kSmallTile, q0 = (int64_t)qt * kSmallTile;
+// The same for a small tile (without words where the width ends in one).
+__device__ __forceinline__ void grad_tile_small(SmallSmem& sm, const LossArgs& a, int64_t v0,
+                                                int64_t p0, int64_t q0, int64_t width) {
   v4f acc[16];
-  if (p0 < a.V) {  // a width rounded up to 256 can end in a tile without words
-    const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H, kSmallTile);
+  if (v0 + p0 < a.V) {
+    const Operand P = tile_rows(a.w, a.ldw, v0 + p0, a.V, a.H, kSmallTile);
     const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H, kSmallTile);
     small_loop(sm, P, Q, (uint32_t)(2 * a.H), acc);
   } else {
@@ -417,7 +421,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_grad_small(LossArgs a, int64_
     for (int i = 0; i < 16; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const Place at;
-  const int words = (int)std::min<int64_t>(kSmallTile, a.V - p0);
+  const int words = (int)std::min<int64_t>(kSmallTile, a.V - v0 - p0);
   const int first = 64 * at.wp + 4 * at.g;
 #pragma unroll
   for (int J = 0; J < 4; ++J) {
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_grad_small(LossArgs a, int64_
     const int64_t target = target_of(a, t);
     const float shift = target == -1 ? 0.0f : -a.stats[t] * kLog2e;
     const float g = target != -1 && a.per_token ? a.grad_loss[t] : 1.0f;
-    const int64_t word = target - p0 - first;
+    const int64_t word = target - v0 - p0 - first;
 #pragma unroll
     for (int F = 0; F < 4; ++F) {
       float v[4];
@@ -437,9 +441,28 @@ __global__ __launch_bounds__(kThreads) void k_loss_grad_small(LossArgs a, int64_
                    ? 0.0f
                    : (e - (word == 16 * F + r ? 1.0f : 0.0f)) * g;
       }
-      *reinterpret_cast<uint2*>(a.d + t * width + (int64_t)pt * kSmallTile + first + 16 * F) =
+      *reinterpret_cast<uint2*>(a.d + t * width + p0 + first + 16 * F) =
           make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     }
+  }
+}
+
+// d of words v0 .. v0 + width (width: the piece's words rounded up to 256): large
+// tiles for the first large_words of them, small ones for the rest.
+__global__ __launch_bounds__(kThreads, 1) void k_loss_grad_tile(LossArgs a, int64_t v0, int width,
+                                                                int large_words) {
+  __shared__ TileSmem sm;
+  const int np = (large_words + kTile - 1) / kTile, nq = (int)((a.T + kTile - 1) / kTile);
+  const int large = np * nq, block = (int)blockIdx.x;
+  int pt, qt;
+  if (block < large) {
+    tile_of(block, np, nq, pt, qt);
+    grad_tile(sm.large, a, v0, (int64_t)pt * kTile, (int64_t)qt * kTile, width);
+  } else {
+    tile_of(block - large, (width - np * kTile) / kSmallTile,
+            (int)((a.T + kSmallTile - 1) / kSmallTile), pt, qt);
+    grad_tile_small(sm.small, a, v0, np * kTile + (int64_t)pt * kSmallTile,
+                    (int64_t)qt * kSmallTile, width);
   }
 }
 
@@ -546,11 +569,25 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t tiles(int64_t n) { return (n + kTile - 1) / kTile; }
 int64_t small_tiles(int64_t n) { return (n + kSmallTile - 1) / kSmallTile; }
 
-// Whether `words` words of logits go by small tiles: where those are one round of
-// the chip.  Small / large, hidden size 1024, us: 128 tokens, 32000 words (250 small
-// tiles) 25.8 / 33.8; 128 x 64000 (500) 46.2 / 38.9; 256 x 32000 (500) 40.9 / 33.6.
-bool use_small(const LossArgs& a, int64_t words) {
-  return small_tiles(words) * small_tiles(a.T) <= std::max(1, device_cu_count());
+// How many of `words` words of logits go by large tiles: all of them, or whole
+// rounds of the chip where the rest is one round of small tiles (none of them, where
+// everything is).  A round of small tiles takes about half as long as one of large
+// ones.  Hidden size 1024, all small / all large, us: 128 tokens, 32000 words (250
+// small tiles) 25.8 / 33.8; 128 x 64000 (500) 46.2 / 38.9; 256 x 32000 (500) 40.9 /
+// 33.6.  1000 x 50021 x 2048, three rounds and 56 small tiles / four: 175 / 197.
+int64_t large_words(const LossArgs& a, int64_t words) {
+  const int64_t cus = std::max(1, device_cu_count()), nq = std::max<int64_t>(1, tiles(a.T));
+  const int64_t whole = tiles(words) * nq / cus * cus / nq * kTile;
+  const int64_t left = words - whole;
+  return left > 0 && small_tiles(left) * small_tiles(a.T) <= cus ? whole : words;
+}
+// Rows of statistics, and workgroups, of such a launch.
+int64_t part_rows(int64_t words, int64_t large) {
+  return tiles(large) + (words > large ? small_tiles(words - large) : 0);
+}
+int64_t tile_blocks(const LossArgs& a, int64_t words, int64_t large) {
+  return tiles(large) * tiles(a.T) +
+         (words > large ? small_tiles(words - large) * small_tiles(a.T) : 0);
 }
 
 // Ranges of k for a product: none takes more stages than about half of what a
@@ -643,27 +680,21 @@ hipError_t join(const Product& p, int ranges, float* partials, float* acc, hipSt
 }  // namespace
 
 int64_t loss_workspace_bytes(const LossArgs& a) {
-  const int64_t n = use_small(a, a.V) ? small_tiles(a.V) : tiles(a.V);
-  return up(n * a.T * 8, 256) + up(a.T * 4, 256) * 2;
+  return up(part_rows(a.V, large_words(a, a.V)) * a.T * 8, 256) + up(a.T * 4, 256) * 2;
 }
 
 hipError_t launch_loss(LossArgs a, uint8_t* ws, hipStream_t stream) {
   if (a.T > 0) {
-    const bool small = use_small(a, a.V);
-    const int64_t np = small ? small_tiles(a.V) : tiles(a.V);
+    const int64_t large = large_words(a, a.V), rows = part_rows(a.V, large);
     a.part = reinterpret_cast<float2*>(ws);
-    a.target_logit = reinterpret_cast<float*>(ws + up(np * a.T * 8, 256));
+    a.target_logit = reinterpret_cast<float*>(ws + up(rows * a.T * 8, 256));
     if (!a.token_loss) a.token_loss = a.target_logit + up(a.T * 4, 256) / 4;
-    if (small)
-      hipLaunchKernelGGL(k_loss_fwd_small, dim3((unsigned)(np * small_tiles(a.T))), dim3(kThreads),
-                         0, stream, a);
-    else
-      hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)(np * tiles(a.T))), dim3(kThreads), 0, stream,
-                         a);
+    hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)tile_blocks(a, a.V, large)), dim3(kThreads), 0,
+                       stream, a, large);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     hipLaunchKernelGGL(k_loss_join, dim3((unsigned)((a.T + kJoinTokens - 1) / kJoinTokens)),
-                       dim3(kJoinTokens * kJoinRuns), 0, stream, a, (int)np);
+                       dim3(kJoinTokens * kJoinRuns), 0, stream, a, (int)rows);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
@@ -685,13 +716,10 @@ hipError_t launch_loss_grad(LossArgs a, uint16_t* dx, uint16_t* dw, uint8_t* ws,
   float* part_w = reinterpret_cast<float*>(ws + s.part_w);
   for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) {
     const int64_t words = std::min<int64_t>(s.piece, a.V - v0), width = up(words, kTile);
-    if (use_small(a, words))
-      hipLaunchKernelGGL(k_loss_grad_small,
-                         dim3((unsigned)(width / kSmallTile * small_tiles(a.T))), dim3(kThreads), 0,
-                         stream, a, v0, (int)width);
-    else
-      hipLaunchKernelGGL(k_loss_grad_tile, dim3((unsigned)(width / kTile * tiles(a.T))),
-                         dim3(kThreads), 0, stream, a, v0, (int)width);
+    int64_t large = large_words(a, words);
+    if (large == words) large = width;
+    hipLaunchKernelGGL(k_loss_grad_tile, dim3((unsigned)tile_blocks(a, width, large)),
+                       dim3(kThreads), 0, stream, a, v0, (int)width, (int)large);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     const PieceRanges r = piece_ranges(a, words);
