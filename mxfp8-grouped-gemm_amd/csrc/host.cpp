@@ -41,7 +41,9 @@ struct Lib {
   MXGG_FN(grouped_fwd_swiglu_quant_keep_h) MXGG_FN(grouped_wgrad) MXGG_FN(swiglu_bwd_quant)  \
   MXGG_FN(gather_quant_dual) MXGG_FN(gather_quant_dim0) MXGG_FN(combine)                     \
   MXGG_FN(route_topk) MXGG_FN(route_topk_grad) MXGG_FN(norm) MXGG_FN(norm_grad)              \
-  MXGG_FN(norm_grad_workspace_bytes) MXGG_FN(adamw_step) MXGG_FN(last_error)
+  MXGG_FN(norm_grad_workspace_bytes) MXGG_FN(adamw_step) MXGG_FN(last_error)                 \
+  MXGG_FN(linear_cross_entropy) MXGG_FN(linear_cross_entropy_workspace_bytes)                \
+  MXGG_FN(linear_cross_entropy_grad) MXGG_FN(linear_cross_entropy_grad_workspace_bytes)
   MXGG_FNS
 #undef MXGG_FN
 };
@@ -552,6 +554,73 @@ Result norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, dou
   return norm_forward(x, weight, bias, o, false, stream)[0];
 }
 
+// bf16 rows the loss kernels read in place.
+bool loss_rows(const Tensor& t) {
+  return plain(t) && t.scalar_type() == at::kBFloat16 && t.dim() >= 1 && row_stride(t) > 0 &&
+         row_stride(t) % 8 == 0 && aligned(t.const_data_ptr(), 16);
+}
+// (loss, stats)
+variable_list loss_forward(const Tensor& x, const Tensor& w, const Tensor& target,
+                           const mxgg_loss_options& o, int64_t stream) {
+  const bool each = o.reduction == MXGG_REDUCE_NONE;
+  Tensor loss = each ? empty(target.sizes(), x, at::kFloat) : empty({}, x, at::kFloat);
+  Tensor stats = empty({o.tokens + 1}, x, at::kFloat);
+  const int64_t bytes = lib.linear_cross_entropy_workspace_bytes(&o);
+  Tensor ws = empty({std::max<int64_t>(bytes, 0)}, x, at::kByte);
+  check(lib.linear_cross_entropy(cp(x), cp(w), cp(target), &o, loss.data_ptr<float>(),
+                                 stats.data_ptr<float>(), vp(ws), bytes, st(stream)),
+        "linear_cross_entropy");
+  return {loss, stats};
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const Tensor& target, const mxgg_loss_options& o, int64_t stream) {
+    const variable_list r = loss_forward(x, w, target, o, stream);
+    ctx->save_for_backward({x, w, target, r[1]});
+    keep(ctx, "options", o);
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["need"] = (int64_t)(x.requires_grad() | (int)w.requires_grad() << 1);
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &target = saved[2], &stats = saved[3];
+    const auto o = kept<mxgg_loss_options>(ctx, "options");
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const Tensor d = grads[0].to(at::kFloat).contiguous();
+    Tensor dx, dw;
+    if (need & 1) dx = empty(x.sizes(), x, x.scalar_type());
+    if (need & 2) dw = empty(w.sizes(), w, w.scalar_type());
+    const int64_t bytes =
+        lib.linear_cross_entropy_grad_workspace_bytes(&o, (int)(need & 1), (int)(need & 2));
+    Tensor ws = empty({std::max<int64_t>(bytes, 0)}, x, at::kByte);
+    check(lib.linear_cross_entropy_grad(d.const_data_ptr<float>(), cp(x), cp(w), cp(target),
+                                        stats.const_data_ptr<float>(), &o, vp_or_null(dx),
+                                        vp_or_null(dw), vp(ws), bytes,
+                                        st(ctx->saved_data["stream"].toInt())),
+          "linear_cross_entropy_grad");
+    return {dx, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Result linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& target,
+                            int64_t ignore_index, int reduction, int64_t stream) {
+  if (!loss_rows(x) || !loss_rows(w) || w.dim() != 2 || x.size(-1) != w.size(1) ||
+      w.device() != x.device() || !plain(target) || !target.is_contiguous() ||
+      (target.scalar_type() != at::kInt && target.scalar_type() != at::kLong) ||
+      target.device() != x.device() || target.dim() != x.dim() - 1 ||
+      target.sizes() != x.sizes().slice(0, x.dim() - 1))
+    return none();
+  const mxgg_loss_options o{target.numel(), w.size(0),    x.size(-1),
+                            row_stride(x),  row_stride(w), ignore_index,
+                            target.scalar_type() == at::kLong, reduction};
+  if (lib.linear_cross_entropy_workspace_bytes(&o) < 0) return none();
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
+    return LinearCrossEntropy::apply(x, w, target, o, stream);
+  return loss_forward(x, w, target, o, stream)[0];
+}
+
 // One AdamW step of lists of tensors; m_scales and v_scales are empty for 32-bit
 // states, masters without master copies.
 Result adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
@@ -620,5 +689,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("combine", torch::wrap_pybind_function_no_gil(&combine));
   m.def("route_topk", torch::wrap_pybind_function_no_gil(&route_topk));
   m.def("norm", torch::wrap_pybind_function_no_gil(&norm));
+  m.def("linear_cross_entropy", torch::wrap_pybind_function_no_gil(&linear_cross_entropy));
   m.def("adamw", torch::wrap_pybind_function_no_gil(&adamw));
 }

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _need_gpu, _stream_ptr
+from .ops import _native, _need_gpu, _stream_ptr, _tensors, _took
 
 __all__ = ["linear_cross_entropy", "LinearCrossEntropy"]
 
@@ -91,6 +91,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     none, as torch's); any other target outside [0, V) gives a NaN loss.
     reduction: "mean", "sum" or "none" (target's shape).  Differentiable in x and
     weight; the same bits on every run."""
+    host = _native(x)
+    if host is not None and reduction in _REDUCTIONS and _tensors(weight, target) \
+            and weight is not None and target is not None:
+        r = host.linear_cross_entropy(x, weight, target, ignore_index, _REDUCTIONS[reduction],
+                                      _stream_ptr(x))
+        if _took(r, "linear_cross_entropy"):
+            return r
     _need_gpu(x, "x")
     for name, t in (("weight", weight), ("target", target)):
         _need_gpu(t, name)

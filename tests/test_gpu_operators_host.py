@@ -1,4 +1,4 @@
-"""The native host path of route_topk, layer_norm / rms_norm and adamw_step
+"""The native host path of route_topk, the norms, the loss and adamw_step
 (csrc/host.cpp) and their Python form call the same kernels with the same
 arguments: equal bits, types, shapes and gradients, also on another stream and
 through autograd's own accumulation."""
@@ -28,7 +28,7 @@ def _same(a, b):
     assert len(a) == len(b)
     for x, y in zip(a, b):
         assert x.dtype == y.dtype and x.shape == y.shape and x.device == y.device
-        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+        assert torch.equal(x.reshape(-1).view(torch.uint8), y.reshape(-1).view(torch.uint8))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -90,6 +90,28 @@ def test_adamw(gpu, monkeypatch, bits, master):
             mxfp8gg.adamw_step(params, g0, *states, step=step, masters=masters)
             assert all(t._version > v for t, v in zip(params + flat + (masters or []), old))
         return params + flat + (masters or [])
+    _same(*_both(monkeypatch, f))
+
+
+@pytest.mark.parametrize("shape,itype", [((70,), torch.int64), ((2, 35), torch.int32)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_linear_cross_entropy(gpu, monkeypatch, shape, itype, reduction):
+    g = torch.Generator().manual_seed(3)
+    x0 = torch.randn((*shape, 64), generator=g).to(torch.bfloat16).to(gpu)
+    w0 = (torch.randn((300, 64), generator=g) / 8).to(torch.bfloat16).to(gpu)
+    t = torch.randint(0, 300, shape, generator=g).to(itype).to(gpu)
+    t.view(-1)[::5] = -100
+    d = torch.randn(shape if reduction == "none" else (), generator=g).to(gpu)
+
+    def f():
+        x, w = (p.clone().requires_grad_(True) for p in (x0, w0))
+        loss = mxfp8gg.linear_cross_entropy(x, w, t, reduction=reduction)
+        loss.backward(d)
+        only = w0.clone().requires_grad_(True)
+        mxfp8gg.linear_cross_entropy(x0, only, t, reduction=reduction).backward(d)
+        with torch.no_grad():
+            again = mxfp8gg.linear_cross_entropy(x, w, t, reduction=reduction)
+        return loss.detach(), x.grad, w.grad, only.grad, again
     _same(*_both(monkeypatch, f))
 
 
