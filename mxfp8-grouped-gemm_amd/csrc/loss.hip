@@ -171,13 +171,6 @@ __device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
                             v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e));
 }
 
-// A token's target as its place among the 128 words from `first` on, -1 if it is not
-// among them.
-__device__ __forceinline__ int place_of(int64_t target, int64_t first) {
-  const int64_t p = target - first;
-  return p >= 0 && p < 128 ? (int)p : -1;
-}
-
 // Statistics of a tile: part[part row][t] = (max, sum of exp(z - max)) over the
 // tile's words, and the target's logit.
 __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_t p0, int64_t q0,
@@ -195,13 +188,6 @@ __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (at.p(k >> 5, r, (k >> 3) & 3) >= words) acc[k][r] = -__builtin_inff();
-  }
-  // the tokens' targets, all loads before the first use
-  int word[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t t = q0 + at.q(k >> 2, k & 3);
-    word[k] = place_of(t < a.T ? target_of(a, t) : -1, p0 + 128 * at.wp);
   }
   float2* joined = reinterpret_cast<float2*>(&sm.ring[0][0]);  // [wp][token]
 #pragma unroll
@@ -225,21 +211,16 @@ __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if (at.g == 0) joined[256 * at.wp + at.q(H, j)] = make_float2(m, s);
-      // the target's logit, where it is one of this wave's words: picked from the lane's
-      // 32, stored by the lane that holds it
-      const int mine = word[4 * H + j];
-      if (__any(mine >= 0)) {
-        float z = 0.0f;
-        bool here = false;
+      // the target's logit, where it is one of this wave's words
+      const int64_t t = q0 + at.q(H, j);
+      const int64_t word = t < a.T ? target_of(a, t) - p0 - 128 * at.wp : -1;
+      if (__any(word >= 0 && word < 128)) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool hit = mine == at.p(k >> 2, r, k & 3) - 128 * at.wp;
-            z = hit ? acc[8 * k + 4 * H + j][r] : z;
-            here |= hit;
-          }
-        if (here) a.target_logit[q0 + at.q(H, j)] = z;
+          for (int r = 0; r < 4; ++r)
+            if (word == at.p(k >> 2, r, k & 3) - 128 * at.wp)
+              a.target_logit[t] = acc[8 * k + 4 * H + j][r];
       }
     }
   __syncthreads();
@@ -259,12 +240,6 @@ __device__ __forceinline__ void fwd_tile_small(SmallSmem& sm, const LossArgs& a,
   const Place at;
   const int words = (int)std::min<int64_t>(kSmallTile, a.V - p0);
   const int first = 64 * at.wp + 4 * at.g;  // + 16 F + r
-  int64_t word[4];
-#pragma unroll
-  for (int J = 0; J < 4; ++J) {
-    const int64_t t = q0 + 64 * at.wq + 16 * J + at.c;
-    word[J] = (t < a.T ? target_of(a, t) : -1) - p0 - first;
-  }
   float2* joined = reinterpret_cast<float2*>(&sm.ring[0][0]);  // [wp][token]
 #pragma unroll
   for (int J = 0; J < 4; ++J) {
@@ -286,9 +261,10 @@ __device__ __forceinline__ void fwd_tile_small(SmallSmem& sm, const LossArgs& a,
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
     if (at.g == 0) joined[kSmallTile * at.wp + q] = make_float2(m, s);
+    const int64_t t = q0 + q, word = t < a.T ? target_of(a, t) - p0 - first : -1;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (word[J] == 16 * (i >> 2) + (i & 3)) a.target_logit[q0 + q] = z[i];
+      if (word == 16 * (i >> 2) + (i & 3)) a.target_logit[t] = z[i];
   }
   __syncthreads();
   const int64_t t = q0 + threadIdx.x;
@@ -381,51 +357,33 @@ __device__ __forceinline__ void grad_tile(LossSmem& sm, const LossArgs& a, int64
   const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
   mainloop<false, false, false, true>(sm, P, Q, 0u, (uint32_t)(2 * a.H), acc);
   const int words = (int)std::min<int64_t>(kTile, a.V - v0 - p0);
-  // what the tokens bring, all loads before the first use
-  int word[8];
-  bool none[8];
-  float shift[8], g[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t t = q0 + at.q(k >> 2, k & 3), target = t < a.T ? target_of(a, t) : -1;
-    none[k] = target == -1;
-    word[k] = place_of(target, v0 + p0 + 128 * at.wp);
-    shift[k] = t < a.T ? -a.stats[t] * kLog2e : 0.0f;
-    g[k] = t < a.T && a.per_token ? a.grad_loss[t] : 1.0f;
-  }
-  // the probabilities, and what few tiles or calls ask for beside them
 #pragma unroll
   for (int H = 0; H < 2; ++H)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int mine = word[4 * H + j];
+      const int64_t t = q0 + at.q(H, j);
+      float shift = 0.0f, g = 1.0f;
+      int64_t word = -1;
+      bool none = true;
+      if (t < a.T) {
+        word = target_of(a, t);
+        if (word != -1) {
+          none = false;
+          shift = -a.stats[t] * kLog2e;
+          if (a.per_token) g = a.grad_loss[t];
+        }
+        word -= v0 + p0;
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          acc[8 * k + 4 * H + j][r] = __builtin_amdgcn_exp2f(
-              __builtin_fmaf(acc[8 * k + 4 * H + j][r], kLog2e, shift[4 * H + j]));
-      if (__any(mine >= 0)) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[8 * k + 4 * H + j][r] -=
-                mine == at.p(k >> 2, r, k & 3) - 128 * at.wp ? 1.0f : 0.0f;
-      }
-      if (a.per_token) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[8 * k + 4 * H + j][r] *= g[4 * H + j];
-      }
-      if (words < kTile || __any(none[4 * H + j])) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (none[4 * H + j] || at.p(k >> 2, r, k & 3) >= words) acc[8 * k + 4 * H + j][r] = 0.0f;
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int p = at.p(k >> 2, r, k & 3);
+          const float z = acc[8 * k + 4 * H + j][r];
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, shift));
+          acc[8 * k + 4 * H + j][r] =
+              none || p >= words ? 0.0f : (e - (word == p ? 1.0f : 0.0f)) * g;
+        }
     }
   // rows of tokens: 16 consecutive words a lane
 #pragma unroll
