@@ -482,20 +482,20 @@ __device__ __forceinline__ void release_barrier() {
 // them are loaded whole and the bytes outside are zeroed in registers right
 // after each fragment read.  Only experts whose token range is not a multiple
 // of 16 take this path.
-// AHEAD (scaled only): the caller issued the loads of the first two stages
-// itself (Stream::prologue), then exactly kAheadStores stores of the tile before,
+// AHEAD (scaled, bf16): the caller issued the loads of the first two stages
+// itself (Stream::prologue), then exactly LEFT stores of the tile before,
 // or waited for all of it.  vmcnt retires in issue order, so the first waits
 // leave those stores in flight: they drain behind this tile's first two stages.
 // With fewer stores the counts would reach into the loads; more vector-memory
 // instructions (a spill) only make them stricter.
 template <bool SCALED, bool MASK = false, bool AHEAD = false, bool BF16 = false, bool PK = false,
-          bool QK = false, class SM>
+          bool QK = false, int LEFT = kAheadStores, class SM>
 __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand& Q,
                                          uint32_t klo, uint32_t kend, v4f (&acc)[64]) {
   static_assert(!(SCALED && MASK), "a scale block cannot be split by a token mask");
   static_assert(BF16 || !(PK || QK), "K-major operands are bf16");
   static_assert(!BF16 || !(SCALED || MASK), "bf16 operands have neither scales nor a byte mask");
-  static_assert(SCALED || !AHEAD, "the wait counts of AHEAD include the scale loads");
+  static_assert(SCALED || BF16 || !AHEAD, "the wait counts of AHEAD include the scale loads");
 #pragma unroll
   for (int i = 0; i < 64; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   if (kend <= klo) return;
@@ -510,7 +510,7 @@ __device__ __forceinline__ void mainloop(SM& sm, const Operand& P, const Operand
   // the caller), then publish stage 0 and read the part of it that the loop
   // reads one stage ahead.
   if constexpr (!AHEAD) st.prologue(sm.ring[0], sm.ring[1], P, Q, kbeg, nst);
-  constexpr int kLeft = AHEAD ? kAheadStores : 0;
+  constexpr int kLeft = AHEAD ? LEFT : 0;
   if (nst > 1)
     wait_barrier<kStageLoads + (SCALED ? kScaleLoads : 0) + kLeft>();
   else

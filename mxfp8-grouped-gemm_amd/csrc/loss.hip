@@ -29,8 +29,16 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 256;
 constexpr int kSmallTile = 128;
 
+// What a tile's tokens bring to its epilogue, loaded by one thread each with the first
+// stages of the main loop.
+struct TokenInfo {
+  int32_t word;  // target's place among the tile's words, kNoWord or kIgnored
+  float shift, g;
+};
+constexpr int32_t kNoWord = -1, kIgnored = -2;
 struct __align__(16) LossSmem {
   uint8_t ring[2][kStageBytes];
+  TokenInfo token[kTile];
 };
 
 // Tiles of 128 x 128 for calls that large ones would leave most of the chip idle:
@@ -163,6 +171,33 @@ __device__ __forceinline__ int64_t target_of(const LossArgs& a, int64_t t) {
   return v == a.ignore_index ? -1 : v >= 0 && v < a.V ? v : -2;
 }
 
+// The logits of a large tile, and what its tokens (from q0) bring in sm.token; `first` is
+// the tile's first word.
+template <bool GRAD>
+__device__ __forceinline__ void logits(LossSmem& sm, const LossArgs& a, int64_t first, int64_t q0,
+                                       v4f (&acc)[64]) {
+  const Operand P = tile_rows(a.w, a.ldw, first, a.V, a.H);
+  const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
+  const uint32_t kend = (uint32_t)(2 * a.H);
+  const int64_t t = q0 + threadIdx.x;
+  int64_t target = -1;
+  float lse = 0.0f, g = 1.0f;
+  if (t < a.T) {
+    target = target_of(a, t);
+    if (GRAD) lse = a.stats[t];
+    if (GRAD && a.per_token) g = a.grad_loss[t];
+  }
+  Stream<false> st;
+  st.init(P, Q, 0u, kend);
+  st.prologue(sm.ring[0], sm.ring[1], P, Q, 0u, (kend + kStageK - 1) / kStageK);
+  const int64_t word = target - first;
+  sm.token[threadIdx.x] = {target == -1                 ? kIgnored
+                           : word >= 0 && word < kTile ? (int32_t)word
+                                                        : kNoWord,
+                           -lse * kLog2e, g};
+  mainloop<false, false, true, true, false, false, 0>(sm, P, Q, 0u, kend, acc);
+}
+
 // (max, sum of exp(z - max)) of two sets of words.
 __device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
   const float m = __builtin_fmaxf(u.x, v.x);
@@ -175,10 +210,8 @@ __device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
 // tile's words, and the target's logit.
 __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_t p0, int64_t q0,
                                          int64_t part_row) {
-  const Operand P = tile_rows(a.w, a.ldw, p0, a.V, a.H);
-  const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
   v4f acc[64];
-  mainloop<false, false, false, true>(sm, P, Q, 0u, (uint32_t)(2 * a.H), acc);
+  logits<false>(sm, a, p0, q0, acc);
 
   const Place at;
   const int words = (int)std::min<int64_t>(kTile, a.V - p0);
@@ -213,7 +246,7 @@ __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_
       if (at.g == 0) joined[256 * at.wp + at.q(H, j)] = make_float2(m, s);
       // the target's logit, where it is one of this wave's words
       const int64_t t = q0 + at.q(H, j);
-      const int64_t word = t < a.T ? target_of(a, t) - p0 - 128 * at.wp : -1;
+      const int word = sm.token[at.q(H, j)].word - 128 * at.wp;
       if (__any(word >= 0 && word < 128)) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -353,36 +386,23 @@ __device__ __forceinline__ void grad_tile(LossSmem& sm, const LossArgs& a, int64
                                           int64_t q0, int64_t width) {
   const Place at;
   v4f acc[64];
-  const Operand P = tile_rows(a.w, a.ldw, v0 + p0, a.V, a.H);
-  const Operand Q = tile_rows(a.x, a.ldx, q0, a.T, a.H);
-  mainloop<false, false, false, true>(sm, P, Q, 0u, (uint32_t)(2 * a.H), acc);
+  logits<true>(sm, a, v0 + p0, q0, acc);
   const int words = (int)std::min<int64_t>(kTile, a.V - v0 - p0);
 #pragma unroll
   for (int H = 0; H < 2; ++H)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t t = q0 + at.q(H, j);
-      float shift = 0.0f, g = 1.0f;
-      int64_t word = -1;
-      bool none = true;
-      if (t < a.T) {
-        word = target_of(a, t);
-        if (word != -1) {
-          none = false;
-          shift = -a.stats[t] * kLog2e;
-          if (a.per_token) g = a.grad_loss[t];
-        }
-        word -= v0 + p0;
-      }
+      const TokenInfo own = sm.token[at.q(H, j)];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int p = at.p(k >> 2, r, k & 3);
           const float z = acc[8 * k + 4 * H + j][r];
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, shift));
-          acc[8 * k + 4 * H + j][r] =
-              none || p >= words ? 0.0f : (e - (word == p ? 1.0f : 0.0f)) * g;
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, own.shift));
+          acc[8 * k + 4 * H + j][r] = own.word == kIgnored || p >= words
+                                          ? 0.0f
+                                          : (e - (own.word == p ? 1.0f : 0.0f)) * own.g;
         }
     }
   // rows of tokens: 16 consecutive words a lane
