@@ -506,8 +506,6 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradA
   }
 }
 
-constexpr int64_t kSmallExperts = INT64_C(1) << 21;
-
 int next_pow2(int v) {
   int p = 1;
   while (p < v) p <<= 1;
@@ -534,13 +532,19 @@ hipError_t run_topk(RouteTopkArgs a, hipStream_t stream) {
 }
 
 // Lists of the smallest length that holds topk, cut from 32 experts a lane (32
-// lanes hold 1024).  Few tokens take 8 experts a lane where 64 lanes hold them, so
-// that the chip has more waves of less work.
+// lanes hold 1024).  Few tokens take 8 experts a lane where 64 lanes hold them: more
+// waves of less work, as long as 32 a lane leave a SIMD without a wave.  256 experts
+// in 8 groups, 32 / 8 a lane, us: 1 token 7.5 / 5.2, 4096 8.2 / 7.3, 8192 (a wave a
+// SIMD) 8.4 / 9.8, 131072 54 / 88; 32 experts: 32768 tokens 8.6 / 5.6, 65536 (a wave a
+// SIMD) 9.0 / 7.3, 131072 11.1 / 11.2.
 template <typename T>
 hipError_t run_topk_list(RouteTopkArgs a, hipStream_t stream) {
   if (a.K <= 8) {
+    set_lanes<32, 8>(a);
+    const int64_t waves = (a.tokens * a.lanes + 63) / 64;
     set_lanes<8, 8>(a);
-    if (a.lanes <= 64 && a.tokens * a.E <= kSmallExperts) return run_topk<8, 8, T>(a, stream);
+    if (a.lanes <= 64 && waves < 4 * std::max(1, device_cu_count()))
+      return run_topk<8, 8, T>(a, stream);
     return run_topk<32, 8, T>(a, stream);
   }
   if (a.K <= 16) return run_topk<32, 16, T>(a, stream);
