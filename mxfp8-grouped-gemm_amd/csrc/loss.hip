@@ -559,6 +559,12 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
 
 // Both products of a piece in one launch, the one with the longer tiles first: the
 // short tiles of the other fill the compute units that its last round leaves idle.
+// Bound by the matrix cores at the clock that the power limit leaves: 4096 tokens,
+// 131072 words, hidden 7168 1.37 PFLOP/s, and with 1024 tokens (short tiles of dW) the
+// main loop runs at 1.6 GHz, with 64 tokens at 2.3.  Loading the next tile's stages
+// before the stores, fewer instructions in the epilogue, streaming stores and half the
+// workgroups in reverse order each left the launch as long as it was: a shorter
+// epilogue lowers the main loop's clock.
 __global__ __launch_bounds__(kThreads, 1) void k_products(Product dx, Product dw, int dx_first) {
   __shared__ LossSmem sm;
   const int first = dx_first ? dx.blocks : dw.blocks, block = (int)blockIdx.x;
@@ -610,15 +616,17 @@ int64_t tile_blocks(const LossArgs& a, int64_t words, int64_t large) {
          (words > large ? small_tiles(words - large) * small_tiles(a.T) : 0);
 }
 
-// Ranges of k for a product: none takes more stages than about half of what a
+// Ranges of k for a product: none takes more stages than about two thirds of what a
 // compute unit gets of the launch's work (so that the longest tiles do not outlast
 // the rest), none less than 512 of k; the partials stay below two tiles a unit.
-// A tile's start and end cost about as much as kTileStages stages.
+// A tile's start and end cost about as much as kTileStages stages.  A share of a
+// quarter / half / two thirds / all of it, us: 1000 tokens, 50021 words, hidden 2048
+// 779 / 762 / 752 / 748; 64 x 131072 x 7168 1656 / 1687 / 1685 / 1740.
 constexpr int64_t kTileStages = 8;
 int64_t stages(int64_t k) { return (k + 63) / 64; }
 int product_ranges(int64_t np, int64_t nq, int64_t k, int64_t work) {
   const int64_t n = tiles(np) * tiles(nq), cus = std::max(1, device_cu_count());
-  const int64_t share = std::max<int64_t>(1, work / cus / 2);
+  const int64_t share = std::max<int64_t>(1, work * 2 / (3 * cus));
   return (int)std::max<int64_t>(
       1, std::min({(stages(k) + share - 1) / share, k / 512, 2 * cus / n}));
 }
@@ -627,8 +635,10 @@ int64_t product_work(int64_t np, int64_t nq, int64_t k) {
 }
 
 // Words of a piece: its d stays within kPieceBytes, and the pieces of one vocabulary
-// are alike.
-constexpr int64_t kPieceBytes = INT64_C(1) << 28;
+// are alike.  64 MiB / 256 MiB / 1 GiB / 4 GiB of d, ms: 4096 tokens, 131072 words,
+// hidden 7168 22.3 / 22.0 / 21.6 / 21.7; 16384 x 32000 x 1024 4.35 / 3.76 / 3.60 / 3.60:
+// what a piece costs beside its products (dx in fp32, the ends of its launches).
+constexpr int64_t kPieceBytes = INT64_C(1) << 30;
 int64_t piece_words(const LossArgs& a) {
   const int64_t most = std::min<int64_t>(
       std::max<int64_t>(kTile, kPieceBytes / (2 * a.T) / kTile * kTile), INT64_C(1) << 21);

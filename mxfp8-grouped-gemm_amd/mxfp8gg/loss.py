@@ -5,7 +5,8 @@
 
 is cross_entropy(x @ weight.T, target) without the logits [T, V]: the forward
 pass keeps one fp32 value a token, the backward pass computes the logits again
-in pieces of the vocabulary and holds about 1 GiB for one piece.
+in pieces of the vocabulary and holds at most 1 GiB of bf16 [T, piece] (and dx in
+fp32 where there are several).
 """
 from __future__ import annotations
 

@@ -89,9 +89,9 @@ def test_matches_oracle(gpu, T, V, H, reduction):
 
 
 def test_many_pieces(gpu):
-    """Long rows, and a vocabulary of several pieces (of 256 MiB of 2 T bytes a
-    word), the last one shorter; tokens and words past a tile."""
-    for T, V, H in ((1000, 33000, 32768), (4100, 70001, 72)):
+    """Long rows, and a vocabulary of several pieces (of 1 GiB of 2 T bytes a
+    word: three), the last one shorter; tokens and words past a tile."""
+    for T, V, H in ((1000, 33000, 32768), (4100, 70001, 72), (16400, 70001, 72)):
         _large(gpu, T, V, H)
 
 
