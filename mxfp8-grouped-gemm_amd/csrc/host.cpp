@@ -419,6 +419,12 @@ int32_t type_of(const Tensor& t) {
 void* vp_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 const void* cp_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
+// Refuses a backward pass under create_graph: the gradients would be constants in its
+// graph, and second derivatives would leave their part out unnoticed.
+void first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice (create_graph)");
+}
+
 // (expert_idx, weights) and, for the gradient, the selected scores.
 variable_list route_forward(const Tensor& logits, const float* bias,
                             const mxgg_route_options& o, bool keep_selected, int64_t stream) {
@@ -446,6 +452,7 @@ struct RouteTopK : torch::autograd::Function<RouteTopK> {
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_order("route_topk");
     const variable_list saved = ctx->get_saved_variables();
     const auto o = kept<mxgg_route_options>(ctx, "options");
     const Tensor d = grads[1].to(at::kFloat).contiguous();
@@ -510,6 +517,7 @@ struct Norm : torch::autograd::Function<Norm> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_order("norm");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const auto o = kept<mxgg_norm_options>(ctx, "options");
@@ -584,6 +592,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_order("linear_cross_entropy");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &target = saved[2], &stats = saved[3];
     const auto o = kept<mxgg_loss_options>(ctx, "options");

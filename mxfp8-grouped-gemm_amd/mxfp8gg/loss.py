@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _native, _need_gpu, _stream_ptr, _tensors, _took
+from .ops import _first_order, _native, _need_gpu, _stream_ptr, _tensors, _took
 
 __all__ = ["linear_cross_entropy", "LinearCrossEntropy"]
 
@@ -60,6 +60,7 @@ class LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
+        _first_order("linear_cross_entropy")
         x, w, target, stats = ctx.saved_tensors
         opt, dev = ctx.opt, x.device
         need_x, need_w = ctx.needs_input_grad[:2]

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _native, _need_gpu, _stream_ptr, _tensors, _took
+from .ops import _first_order, _native, _need_gpu, _stream_ptr, _tensors, _took
 
 __all__ = ["layer_norm", "rms_norm", "Norm"]
 
@@ -63,6 +63,7 @@ class Norm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _first_order("norm")
         x2, w, stats = ctx.saved_tensors
         opt, dev = ctx.opt, x2.device
         dy2 = _rows(dy.to(x2.dtype), opt.cols)

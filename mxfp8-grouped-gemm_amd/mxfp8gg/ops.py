@@ -73,6 +73,13 @@ def _need_gpu(t: torch.Tensor, name: str) -> None:
         )
 
 
+def _first_order(what: str) -> None:
+    """Refuses a backward pass under create_graph: the gradients would be constants in
+    its graph, and second derivatives would leave their part out unnoticed."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} cannot be differentiated twice (create_graph)")
+
+
 def _mode(scaling_mode) -> int:
     if isinstance(scaling_mode, int):
         return scaling_mode

@@ -27,8 +27,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
-from .ops import (_FP8, _MODES, _block_major_buffer, _mode, _native, _need_gpu, _stream_ptr,
-                  _tensors, _took, padded_token_capacity)
+from .ops import (_FP8, _MODES, _block_major_buffer, _first_order, _mode, _native, _need_gpu,
+                  _stream_ptr, _tensors, _took, padded_token_capacity)
 
 __all__ = ["route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual",
            "gather_to_mxfp8_dim0", "combine", "combine_score_grad"]
@@ -74,6 +74,7 @@ class RouteTopK(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, _, dscores):
+        _first_order("route_topk")
         idx, selected, *x = ctx.saved_tensors
         shape, dtype = ctx.like
         d = dscores.to(torch.float32).contiguous()

@@ -135,3 +135,27 @@ def test_backward_on_the_forward_stream(gpu, monkeypatch):
     a, b = _both(monkeypatch, lambda: [f(torch.cuda.Stream())])
     _same(a, [want])
     _same(b, [want])
+
+
+@pytest.mark.parametrize("op", ["route_topk", "norm", "linear_cross_entropy"])
+def test_second_derivatives_are_refused(gpu, monkeypatch, op):
+    """create_graph would leave these operators' part of a second derivative out: it is
+    refused, and the same graph still gives its first derivative."""
+    g = torch.Generator().manual_seed(3)
+    x0 = torch.randn((12, 64), generator=g).bfloat16().to(gpu)
+    w0 = torch.randn((40, 64), generator=g).bfloat16().to(gpu)
+    t = torch.randint(0, 40, (12,), generator=g).to(gpu)
+
+    def f():
+        x = x0.clone().requires_grad_(True)
+        if op == "route_topk":
+            y = mxfp8gg.route_topk(x, 4)[1]
+        elif op == "norm":
+            y = mxfp8gg.rms_norm(x)
+        else:
+            y = mxfp8gg.linear_cross_entropy(x, w0, t)
+        total = y.float().sum() + x.float().pow(2).sum()
+        with pytest.raises(RuntimeError, match=f"{op} cannot be differentiated twice"):
+            torch.autograd.grad(total, x, create_graph=True, retain_graph=True)
+        return torch.autograd.grad(total, x)
+    _same(*_both(monkeypatch, f))
