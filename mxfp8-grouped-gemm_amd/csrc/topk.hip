@@ -12,15 +12,15 @@
 // An expert with c = -inf (or x = -inf) is out of the choice; a slot that no
 // expert is left for gets id -1 and weight 0.
 //
-// Selection: c becomes a sortable 32-bit integer, packed with the inverted
-// expert index into the mantissa of a double in [1, 2): one v_max_f64 then
-// compares key and index together, at the full rate of the vector unit, and no
-// two keys are equal.  A token is held by 2^k lanes of VPL experts each; every
+// Selection: c becomes a double with the expert's index in the mantissa bits that an
+// fp32 value leaves zero: one v_max_f64 then compares value and index together, at
+// the full rate of the vector unit, and no two keys are equal.  A token is held by 2^k lanes of VPL experts each; every
 // lane sorts its keys in registers down to the L largest and log2(lanes)
 // butterfly steps merge the sorted lists (L max and a bitonic clean each).
 //
-// 131072 tokens, 256 fp32 experts in 8 groups, sigmoid and bias: 54 us, 134 MB read at
-// 2.5 TB/s; bound by the vector unit, the sorting networks and their merges.  One
+// 131072 tokens, 256 fp32 experts in 8 groups, sigmoid and bias: 52 us, 134 MB read at
+// 2.6 TB/s; bound by the vector unit, busy for 45 of them: sigmoids, keys and sorting
+// networks take about as much each.  One
 // token: 5.2 us, a launch and its chain of dependent steps.  The gradient writes every
 // logit's and reads the chosen ones: 27 us, 5 TB/s.
 #include <algorithm>
@@ -48,16 +48,6 @@ __device__ __forceinline__ void wave_sync() {
 
 constexpr float kNegInf = -__builtin_inff();
 
-// Order of fp32 values as unsigned integers; NaN above all, -0 with +0.
-__device__ __forceinline__ uint32_t sortable(float x) {
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-  return x != x ? 0xFFFFFFFFu : k;
-}
-__device__ __forceinline__ float unsortable(uint32_t k) {
-  return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
-}
-
 __device__ __forceinline__ double join_f64(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
@@ -67,20 +57,41 @@ __device__ __forceinline__ uint32_t low_word(double v) {
 __device__ __forceinline__ uint32_t high_word(double v) {
   return (uint32_t)(__builtin_bit_cast(uint64_t, v) >> 32);
 }
-// Key and index as a double in [1, 2); absent: a high word of 0, which is below
-// every key whatever the low word holds.
+// A key: an fp32 value as a double, with the index in the ten lowest mantissa bits,
+// which are zero in every such double; turned over so that the lower index is the
+// larger of two equal values, above and below zero.  Infinities and NaN become the
+// numbers +-2^1022 and 2^1023, so that keys are ordered and none is a NaN; an absent
+// one is -2^1023, below every key whatever its low word holds.
 constexpr uint32_t kIndexMask = 1023u;
 static_assert(kMaxGroups <= (int)kIndexMask + 1, "an expert index takes ten bits");
-__device__ __forceinline__ double pack_key(uint32_t key, uint32_t idx) {
-  return join_f64((key << 20) | (kIndexMask - idx), __builtin_amdgcn_alignbit(0x3FFu, key, 12));
+constexpr uint32_t kNanHigh = 0x7FE00000u, kAbsentHigh = 0xFFE00000u;
+__device__ __forceinline__ uint32_t turned(uint32_t idx, uint32_t high) {
+  return ((kIndexMask - idx) ^ (uint32_t)((int32_t)high >> 31)) & kIndexMask;
 }
-__device__ __forceinline__ uint32_t key_of(double d) {
-  return __builtin_amdgcn_alignbit(high_word(d), low_word(d), 20);
+__device__ __forceinline__ double finite_key(float v, uint32_t idx) {
+  const double d = v;
+  return join_f64(low_word(d) | turned(idx, high_word(d)), high_word(d));
 }
-__device__ __forceinline__ int index_of(double d) { return (int)(kIndexMask - (low_word(d) & kIndexMask)); }
-__device__ __forceinline__ bool absent(double d) { return high_word(d) == 0u; }
-__device__ __forceinline__ double absent_if(bool out, double d) {
-  return join_f64(low_word(d), out ? 0u : high_word(d));
+__device__ __forceinline__ double any_key(float v, uint32_t idx) {
+  const double d = v;
+  uint32_t high = high_word(d);
+  high = __builtin_fabsf(v) == __builtin_inff() ? high - 0x00200000u : high;
+  high = v != v ? kNanHigh : high;
+  return join_f64((v != v ? 0u : low_word(d)) | turned(idx, high), high);
+}
+__device__ __forceinline__ double with_index(double key, uint32_t idx) {
+  return join_f64((low_word(key) & ~kIndexMask) | turned(idx, high_word(key)), high_word(key));
+}
+__device__ __forceinline__ float value_of(double key) {
+  const float v = (float)join_f64(low_word(key) & ~kIndexMask, high_word(key));
+  return high_word(key) == kNanHigh ? __builtin_nanf("") : v;
+}
+__device__ __forceinline__ int index_of(double key) {
+  return (int)turned(low_word(key) & kIndexMask, high_word(key));
+}
+__device__ __forceinline__ bool absent(double key) { return high_word(key) == kAbsentHigh; }
+__device__ __forceinline__ double absent_if(bool out, double key) {
+  return join_f64(low_word(key), out ? kAbsentHigh : high_word(key));
 }
 
 // Plain v_max_f64 / v_min_f64: the keys are ordinary numbers, so the
@@ -265,8 +276,17 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
   float2* stats = reinterpret_cast<float2*>(tile + at.stats);
   float* bias_s = lds + kTopkWaves * at.words;
   load_tile<64 * VPL, T>(static_cast<const T*>(a.logits) + t0 * a.E, nt * a.E, tile);
-  if (a.bias != nullptr)
-    for (int e = tid; e < a.E; e += kTopkThreads) bias_s[pad32(e)] = a.bias[e];
+  __shared__ uint32_t odd_s[kTopkWaves];  // whether a wave's part of the bias is infinite or NaN
+  if (a.bias != nullptr) {
+    uint32_t most = 0;
+    for (int e = tid; e < a.E; e += kTopkThreads) {
+      const float b = a.bias[e];
+      most = max(most, __float_as_uint(b) & 0x7FFFFFFFu);
+      bias_s[pad32(e)] = b;
+    }
+    const bool odd = __any(most >= 0x7F800000u);
+    if (lane == 0) odd_s[wave] = odd;
+  }
   __syncthreads();
   if (nt == 0) return;
 
@@ -313,6 +333,23 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
   // choice keys, and the L largest of the lane
   double list[L];
   {
+    // Most waves hold no infinity or NaN (nor, where a sigmoid is taken, a logit past
+    // 87): the largest bit patterns, signed and not, say so for 32 experts in 32
+    // operations, and such keys take 5 operations instead of 12 (131072 x 256: 55 -> 52
+    // us).  A lane without experts is put right after the sort.
+    int32_t high = 0;
+    uint32_t low = 0;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      high = max(high, (int32_t)__float_as_uint(x[v]));
+      low = max(low, __float_as_uint(x[v]));
+    }
+    const bool sigmoids = a.bias != nullptr && !a.softmax;
+    const uint32_t bound = sigmoids ? __float_as_uint(kModerate) : 0x7F7FFFFFu;
+    bool usual = __all(count == 0 || ((uint32_t)high <= bound && low <= (bound | 0x80000000u)));
+    if (a.bias != nullptr)
+#pragma unroll
+      for (int w = 0; w < kTopkWaves; ++w) usual &= odd_s[w] == 0u;
     float c[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) c[v] = x[v];
@@ -320,33 +357,32 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
       if (a.softmax) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) c[v] = expf(x[v] - top) / total;
+      } else if (usual) {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) c[v] = sigmoid_moderate(x[v]);
       } else {
-        bool moderate = true;  // also where the expert is out or absent
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) moderate &= !(__builtin_fabsf(x[v]) > kModerate) || x[v] == kNegInf;
-        if (__all(moderate)) {
-#pragma unroll
-          for (int v = 0; v < VPL; ++v) c[v] = sigmoid_moderate(x[v]);
-        } else {
-#pragma unroll
-          for (int v = 0; v < VPL; ++v) c[v] = sigmoid(x[v]);
-        }
+        for (int v = 0; v < VPL; ++v) c[v] = sigmoid(x[v]);
       }
-      const float* bias = bias_s + (count > 0 ? pad32(e0) : 0);
       if (whole) {
+        const float* bias = bias_s + (count > 0 ? pad32(e0) : 0);
 #pragma unroll
         for (int v = 0; v < VPL; ++v) c[v] += bias[v];
       } else {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) c[v] += bias_s[pad32(min(e0 + v, a.E - 1))];
       }
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) c[v] = x[v] == kNegInf ? kNegInf : c[v];
     }
     double key[VPL];
+    if (usual) {
 #pragma unroll
-    for (int v = 0; v < VPL; ++v)
-      key[v] = absent_if(c[v] == kNegInf, pack_key(sortable(c[v]), (uint32_t)(e0 + v)));
+      for (int v = 0; v < VPL; ++v) key[v] = finite_key(c[v] + 0.0f, (uint32_t)(e0 + v));
+    } else {
+#pragma unroll
+      for (int v = 0; v < VPL; ++v)
+        key[v] = absent_if(x[v] == kNegInf || c[v] == kNegInf,
+                           any_key(c[v] + 0.0f, (uint32_t)(e0 + v)));
+    }
 #pragma unroll
     for (int i = 0; i < L; ++i) list[i] = key[i];
     sort_net<0, L>(list);
@@ -358,23 +394,25 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
       sort_net<0, L>(more);
       merge_top<L>(list, more);
     }
+#pragma unroll
+    for (int i = 0; i < L; ++i) list[i] = absent_if(count == 0, list[i]);
   }
   for (int off = 1; off < a.lanes_group; off <<= 1) merge_lanes<L>(list, off);
 
   // groups: the list now holds the group's best; rank its worth among the token's
   if (a.groups > 1) {
-    uint32_t worth = key_of(list[0]);
+    double mine = with_index(list[0], (uint32_t)g);
     if (sums) {
       float w[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        w[i] = unsortable(key_of(list[i]));
+        w[i] = value_of(list[i]);
         if (a.bias == nullptr) w[i] = a.softmax ? expf(w[i] - top) / total : sigmoid(w[i]);
         if (absent(list[i])) w[i] = 0.0f;
       }
-      worth = sortable(w[0] + w[1]);
+      mine = any_key(w[0] + w[1] + 0.0f, (uint32_t)g);
     }
-    const double mine = absent_if(absent(list[0]), pack_key(worth, (uint32_t)g));
+    mine = absent_if(absent(list[0]), mine);
     int above = 0;
     for (int off = a.lanes_group; off < a.lanes; off += a.lanes_group)
       above += shfl_xor_f64(mine, off) > mine ? 1 : 0;
@@ -539,9 +577,9 @@ hipError_t run_topk(RouteTopkArgs a, hipStream_t stream) {
 // Lists of the smallest length that holds topk, cut from 32 experts a lane (32
 // lanes hold 1024).  Few tokens take 8 experts a lane where 64 lanes hold them: more
 // waves of less work, as long as 32 a lane leave a SIMD without a wave.  256 experts
-// in 8 groups, 32 / 8 a lane, us: 1 token 7.5 / 5.2, 4096 8.2 / 7.3, 8192 (a wave a
-// SIMD) 8.4 / 9.8, 131072 54 / 88; 32 experts: 32768 tokens 8.6 / 5.6, 65536 (a wave a
-// SIMD) 9.0 / 7.3, 131072 11.1 / 11.2.
+// in 8 groups, 32 / 8 a lane, us: 1 token 6.8 / 5.2, 4096 7.7 / 7.3, 8192 (a wave a
+// SIMD) 7.9 / 9.6, 131072 52 / 86; 32 experts: 32768 tokens 8.5 / 5.7, 65536 (a wave a
+// SIMD) 8.8 / 7.4, 131072 10.8 / 11.4.
 template <typename T>
 hipError_t run_topk_list(RouteTopkArgs a, hipStream_t stream) {
   if (a.K <= 8) {
