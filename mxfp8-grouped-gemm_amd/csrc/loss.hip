@@ -327,6 +327,125 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a, int64_t la
   }
 }
 
+// The forward pass of few tokens, which reads W once and has little else to do: 64
+// words a tile, the four waves of a workgroup a quarter of the contraction each (stages
+// of 64 in turn), operands straight from memory to registers.  A workgroup keeps the
+// statistics of its tiles and leaves one a token.
+constexpr int kFewFrags = 4, kFewWords = 16 * kFewFrags;
+template <int NB>  // tokens / 16
+struct FewStage {
+  v8i w[kFewFrags], x[NB];
+};
+template <int NB>
+__global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int tiles) {
+  // partial sums of the waves: [tile parity][wave][word block][token block][lane]
+  __shared__ v4f part_s[2][4][kFewFrags][NB][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = wave_id(), m = lane & 15u, g = lane >> 4;
+  const uint32_t kend = (uint32_t)(2 * a.H), nst = (kend + kStageK - 1) / kStageK;
+  const auto rows_of = [](const uint16_t* p, int64_t ld, int64_t rows, int64_t cols)
+                           __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), (short)0,
+                                             (int)(((rows - 1) * ld + cols) * 2), 0x00020000);
+  };
+  const auto xs = rows_of(a.x, a.ldx, a.T, a.H);
+  const uint32_t ldw = (uint32_t)(2 * a.ldw), ldx = (uint32_t)(2 * a.ldx);
+  // the statistics of tokens 16 j + m, j % 4 = this wave, and their targets
+  float most[(NB + 3) / 4], sum[(NB + 3) / 4];
+  int64_t target[(NB + 3) / 4];
+#pragma unroll
+  for (int i = 0; i < (NB + 3) / 4; ++i) {
+    const int64_t t = 16 * (4 * i + (int64_t)wave) + m;
+    most[i] = -__builtin_inff();
+    sum[i] = 0.0f;
+    target[i] = t < a.T ? target_of(a, t) : -1;
+  }
+  int parity = 0;
+  for (int tile = (int)blockIdx.x; tile < tiles; tile += (int)gridDim.x, parity ^= 1) {
+    const int64_t p0 = (int64_t)tile * kFewWords;
+    const int64_t words = std::min<int64_t>(kFewWords, a.V - p0);
+    const auto ws = rows_of(a.w + p0 * a.ldw, a.ldw, words, a.H);
+    v4f acc[kFewFrags][NB];
+#pragma unroll
+    for (int F = 0; F < kFewFrags; ++F)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[F][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto load = [&](FewStage<NB>& st, uint32_t s) __attribute__((always_inline)) {
+      const uint32_t k = s * kStageK + 16u * g;  // chunk g, and g + 4
+      const auto chunk = [&](auto rsrc, uint32_t row, uint32_t ld) __attribute__((always_inline)) {
+        const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, k < kend ? row * ld + k : kOobOffset, 0, 0);
+        const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, k + 64u < kend ? row * ld + k + 64u : kOobOffset, 0, 0);
+        return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3],
+                   (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+      };
+#pragma unroll
+      for (uint32_t F = 0; F < kFewFrags; ++F) st.w[F] = chunk(ws, 16u * F + m, ldw);
+#pragma unroll
+      for (uint32_t j = 0; j < NB; ++j) st.x[j] = chunk(xs, 16u * j + m, ldx);
+    };
+    const auto multiply = [&](const FewStage<NB>& st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int F = 0; F < kFewFrags; ++F)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[F][j] = mfma_bf16_stage(st.w[F], st.x[j], acc[F][j]);
+    };
+    // two stages in flight (loads past the last one are zeros)
+    FewStage<NB> st[2];
+    load(st[0], wave);
+    load(st[1], wave + 4u);
+    for (uint32_t s = wave; s < nst; s += 8u) {
+      multiply(st[0]);
+      load(st[0], s + 8u);
+      multiply(st[1]);
+      load(st[1], s + 12u);
+    }
+#pragma unroll
+    for (int F = 0; F < kFewFrags; ++F)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) part_s[parity][wave][F][j][lane] = acc[F][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < (NB + 3) / 4; ++i) {
+      const int j = 4 * i + (int)wave;
+      if (j >= NB) break;
+      // words 16 F + 4 g + r of token 16 j + m
+      float z[4 * kFewFrags], best = most[i];
+#pragma unroll
+      for (int F = 0; F < kFewFrags; ++F) {
+        v4f v = part_s[parity][0][F][j][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += part_s[parity][w][F][j][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          z[4 * F + r] = 16 * F + 4 * (int)g + r < words ? v[r] : -__builtin_inff();
+          best = __builtin_fmaxf(best, z[4 * F + r]);
+        }
+      }
+      best = __builtin_fmaxf(best, __shfl_xor(best, 16));
+      best = __builtin_fmaxf(best, __shfl_xor(best, 32));
+      const float base = best == -__builtin_inff() ? 0.0f : best;
+      sum[i] *= __builtin_amdgcn_exp2f((most[i] - base) * kLog2e);  // this lane's words
+      most[i] = best;
+#pragma unroll
+      for (int u = 0; u < 4 * kFewFrags; ++u)
+        sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[u], kLog2e, -base * kLog2e));
+      const int64_t word = target[i] - p0 - 4 * (int64_t)g;
+#pragma unroll
+      for (int u = 0; u < 4 * kFewFrags; ++u)
+        if (word == 16 * (u >> 2) + (u & 3)) a.target_logit[16 * j + m] = z[u];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < (NB + 3) / 4; ++i) {
+    const int64_t t = 16 * (4 * i + (int64_t)wave) + m;
+    float s = sum[i];
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (g == 0 && t < a.T) a.part[(int64_t)blockIdx.x * a.T + t] = make_float2(most[i], s);
+  }
+}
+
 // lse and loss of every token from its tiles' statistics: 16 tokens a workgroup,
 // 16 runs of tiles each.
 constexpr int kJoinTokens = 16, kJoinRuns = 16;
@@ -612,6 +731,21 @@ int64_t large_words(const LossArgs& a, int64_t words) {
   const int64_t left = words - whole;
   return left > 0 && small_tiles(left) * small_tiles(a.T) <= cus ? whole : words;
 }
+// Forward passes of at most 64 tokens that k_loss_few takes: those whose small tiles
+// would leave so much of the chip's last round empty that rereading x for every 64
+// words, which grows with the tokens, costs less.  Words x hidden (small tiles), 16 /
+// 32 / 64 tokens, us, against the tiles: 16384 x 4096 (128) 27 / 31 / 38 and 42 / 43 /
+// 44; 35328 x 2136 (276) 41 / 43 / 59 and 50 / 50 / 50; 70016 x 2048 (547) 69 / 79 / 109
+// and 72 / 73 / 74; 131072 x 4096 (1024) 234 / 251 / 333 and 209 / 211 / 216.
+bool few_tokens(const LossArgs& a) {
+  const int64_t n = small_tiles(a.V), cus = std::max(1, device_cu_count());
+  const int64_t room = (n + cus - 1) / cus * cus;  // small tiles in as many rounds
+  return a.T > 0 && a.T <= 64 && 5 * room >= (6 + (a.T + 15) / 16) * n;
+}
+int64_t few_blocks(const LossArgs& a) {
+  return std::min<int64_t>((a.V + kFewWords - 1) / kFewWords,
+                           4 * std::max(1, device_cu_count()));
+}
 // Rows of statistics, and workgroups, of such a launch.
 int64_t part_rows(int64_t words, int64_t large) {
   return tiles(large) + (words > large ? small_tiles(words - large) : 0);
@@ -714,18 +848,35 @@ hipError_t join(const Product& p, int ranges, float* partials, float* acc, hipSt
 
 }  // namespace
 
+// Rows of statistics of the forward pass.
+static int64_t forward_rows(const LossArgs& a) {
+  return few_tokens(a) ? few_blocks(a) : part_rows(a.V, large_words(a, a.V));
+}
+
 int64_t loss_workspace_bytes(const LossArgs& a) {
-  return up(part_rows(a.V, large_words(a, a.V)) * a.T * 8, 256) + up(a.T * 4, 256) * 2;
+  return up(forward_rows(a) * a.T * 8, 256) + up(a.T * 4, 256) * 2;
 }
 
 hipError_t launch_loss(LossArgs a, uint8_t* ws, hipStream_t stream) {
   if (a.T > 0) {
-    const int64_t large = large_words(a, a.V), rows = part_rows(a.V, large);
+    const int64_t rows = forward_rows(a);
     a.part = reinterpret_cast<float2*>(ws);
     a.target_logit = reinterpret_cast<float*>(ws + up(rows * a.T * 8, 256));
     if (!a.token_loss) a.token_loss = a.target_logit + up(a.T * 4, 256) / 4;
-    hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)tile_blocks(a, a.V, large)), dim3(kThreads), 0,
-                       stream, a, large);
+    if (few_tokens(a)) {
+      const int n = (int)((a.V + kFewWords - 1) / kFewWords);
+      const dim3 grid((unsigned)rows);
+      if (a.T <= 16)
+        hipLaunchKernelGGL((k_loss_few<1>), grid, dim3(kThreads), 0, stream, a, n);
+      else if (a.T <= 32)
+        hipLaunchKernelGGL((k_loss_few<2>), grid, dim3(kThreads), 0, stream, a, n);
+      else
+        hipLaunchKernelGGL((k_loss_few<4>), grid, dim3(kThreads), 0, stream, a, n);
+    } else {
+      const int64_t large = large_words(a, a.V);
+      hipLaunchKernelGGL(k_loss_fwd, dim3((unsigned)tile_blocks(a, a.V, large)), dim3(kThreads), 0,
+                         stream, a, large);
+    }
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     hipLaunchKernelGGL(k_loss_join, dim3((unsigned)((a.T + kJoinTokens - 1) / kJoinTokens)),

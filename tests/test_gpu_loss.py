@@ -88,6 +88,21 @@ def test_matches_oracle(gpu, T, V, H, reduction):
     _check(x, w, t, reduction, dl)
 
 
+@pytest.mark.parametrize("T,V,H", [
+    (1, 64, 8), (2, 70100, 40), (16, 8191, 520), (17, 30000, 72), (32, 65, 1000), (33, 129, 2056),
+    (48, 5000, 136), (64, 16384, 24), (64, 4097, 264)])
+def test_few_tokens(gpu, T, V, H):
+    """Workgroups with one tile of words and with several, vocabularies that end
+    inside one, contractions that end inside a stage and that some waves have no part
+    of, one to four blocks of tokens; strided rows give the same bits."""
+    x, w, t = _inputs(gpu, T, V, H, 7 * T + V)
+    _check(x, w, t, "none", torch.randn(T, generator=torch.Generator().manual_seed(2)).to(gpu))
+    ref = mxfp8gg.linear_cross_entropy(x, w, t)
+    xs, ws = (torch.full((len(m), H + 24), float("nan"), dtype=m.dtype, device=gpu) for m in (x, w))
+    xs[:, :H], ws[:, :H] = x, w
+    assert torch.equal(mxfp8gg.linear_cross_entropy(xs[:, :H], ws[:, :H], t), ref)
+
+
 def test_many_pieces(gpu):
     """Long rows, and a vocabulary of several pieces (of 1 GiB of 2 T bytes a
     word: three), the last one shorter; tokens and words past a tile."""
