@@ -7,7 +7,7 @@
 //
 // Forward: 256 (vocabulary) x 256 (token) tiles of z on the matrix cores; every
 // tile leaves one maximum and one sum of exponentials a token, joined over the
-// tiles by a second kernel.
+// tiles by a second kernel.  Few tokens stream W past the tiles.
 // Backward: pieces of the vocabulary.  The tiles of a piece are computed again
 // (8 T H V operations in all, 6 with kept logits) and leave d / g rounded to bf16,
 // [T][piece].  Both products read it, W and x as they lie: an operand that is not
@@ -328,7 +328,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a, int64_t la
 }
 
 // The forward pass of few tokens, which reads W once and has little else to do: 64
-// words a tile, the four waves of a workgroup a quarter of the contraction each (stages
+// words a tile (16 / 32 / 64 of them, 32 tokens, 70016 x 2048: 117 / 91 / 79 us: x is
+// read for every tile), the four waves of a workgroup a quarter of the contraction each (stages
 // of 64 in turn), operands straight from memory to registers.  A workgroup keeps the
 // statistics of its tiles and leaves one a token.
 constexpr int kFewFrags = 4, kFewWords = 16 * kFewFrags;
@@ -731,16 +732,19 @@ int64_t large_words(const LossArgs& a, int64_t words) {
   const int64_t left = words - whole;
   return left > 0 && small_tiles(left) * small_tiles(a.T) <= cus ? whole : words;
 }
-// Forward passes of at most 64 tokens that k_loss_few takes: those whose small tiles
-// would leave so much of the chip's last round empty that rereading x for every 64
-// words, which grows with the tokens, costs less.  Words x hidden (small tiles), 16 /
-// 32 / 64 tokens, us, against the tiles: 16384 x 4096 (128) 27 / 31 / 38 and 42 / 43 /
-// 44; 35328 x 2136 (276) 41 / 43 / 59 and 50 / 50 / 50; 70016 x 2048 (547) 69 / 79 / 109
-// and 72 / 73 / 74; 131072 x 4096 (1024) 234 / 251 / 333 and 209 / 211 / 216.
+// Forward passes of at most 64 tokens that k_loss_few takes.  Up to 8 tokens: all of
+// more than one round of small tiles.  Else those whose tiles would leave so much of
+// the chip's last round empty that rereading x for every 64 words, which grows with the
+// tokens, costs less.  Words x hidden (small tiles), us, against the tiles: 8 tokens,
+// 65536 x 4096 (512) 121 and 136, 131072 x 4096 (1024) 223 and 211, 32000 x 4096 (250)
+// 62 and 47; 16 / 32 / 64 tokens, 16384 x 4096 (128) 27 / 31 / 38 and 42 / 43 / 44,
+// 35328 x 2136 (276) 41 / 43 / 59 and 50 / 50 / 50, 70016 x 2048 (547) 69 / 79 / 109 and
+// 72 / 73 / 74, 131072 x 4096 234 / 251 / 333 and 209 / 211 / 216.
 bool few_tokens(const LossArgs& a) {
   const int64_t n = small_tiles(a.V), cus = std::max(1, device_cu_count());
   const int64_t room = (n + cus - 1) / cus * cus;  // small tiles in as many rounds
-  return a.T > 0 && a.T <= 64 && 5 * room >= (6 + (a.T + 15) / 16) * n;
+  if (a.T < 1 || a.T > 64) return false;
+  return (a.T <= 8 && n > cus) || 5 * room >= (6 + (a.T + 15) / 16) * n;
 }
 int64_t few_blocks(const LossArgs& a) {
   return std::min<int64_t>((a.V + kFewWords - 1) / kFewWords,
