@@ -328,10 +328,10 @@ __global__ __launch_bounds__(kThreads, 1) void k_loss_fwd(LossArgs a, int64_t la
 }
 
 // The forward pass of few tokens, which reads W once and has little else to do: 64
-// words a tile (16 / 32 / 64 of them, 32 tokens, 70016 x 2048: 117 / 91 / 79 us: x is
-// read for every tile), the four waves of a workgroup a quarter of the contraction each (stages
-// of 64 in turn), operands straight from memory to registers.  A workgroup keeps the
-// statistics of its tiles and leaves one a token.
+// words a tile (16 / 32 / 64 of them, 32 tokens, 70016 x 2048: 117 / 91 / 79 us, since x
+// is read for every tile), the four waves of a workgroup a quarter of the contraction
+// each (stages of 64 in turn), operands straight from memory to registers.  A workgroup
+// keeps the statistics of its tiles and leaves one a token.
 constexpr int kFewFrags = 4, kFewWords = 16 * kFewFrags;
 template <int NB>  // tokens / 16
 struct FewStage {
