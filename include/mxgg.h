@@ -674,7 +674,8 @@ int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
  * A token whose target is ignore_index has loss 0 and no gradient; one whose
  * target is otherwise outside [0, vocab) has loss NaN.  z is summed in fp32.
  *   reduction : NONE (loss = the token losses, fp32 [tokens]), SUM, or MEAN over
- *               the tokens that are not ignored (loss: fp32 [1])
+ *               the tokens that are not ignored (loss: fp32 [1]; NaN where there
+ *               are none, with gradients of 0)
  *   stats     : fp32 [tokens + 1], written for the gradient
  *   workspace : mxgg_linear_cross_entropy_workspace_bytes(options), 16-byte
  *               aligned, no initialisation

@@ -479,7 +479,9 @@ __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a
 }
 
 // Sum (or mean over the tokens that count) of the token losses, in a fixed
-// order, and the reciprocal count behind the tokens' lse.
+// order, and the factor of their gradients behind the tokens' lse: the reciprocal
+// count of the mean, 0 where no token counts (its mean is 0 / 0, but nothing has a
+// gradient).
 constexpr int kReduceThreads = 1024;
 __global__ __launch_bounds__(kReduceThreads) void k_loss_reduce(LossArgs a) {
   __shared__ float sums[kReduceThreads];
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(kReduceThreads) void k_loss_reduce(LossArgs a) {
   }
   if (threadIdx.x == 0) {
     a.loss[0] = a.mean ? sums[0] / (float)counts[0] : sums[0];
-    a.stats[a.T] = a.mean ? 1.0f / (float)counts[0] : 1.0f;
+    a.stats[a.T] = counts[0] == 0 ? 0.0f : a.mean ? 1.0f / (float)counts[0] : 1.0f;
   }
 }
 
@@ -621,8 +623,8 @@ struct Product {
   const float* before;  // fp32 [nq][np] to add, or nullptr
   uint16_t* out;        // bf16 [nq][np], or nullptr
   float* out32;         // fp32 [ranges][nq][np]
-  const float* scale;   // two factors, at scale[0] and scale2[0], or nullptr
-  const float* scale2;
+  const float* scale;   // two factors, at scale[0] and scale2[0], or nullptr; a zero at
+  const float* scale2;  // scale2 makes the output 0 whatever is at scale
   int64_t ldp, ldq, np, nq, k;  // elements
   int64_t range;                // k of a range, a multiple of 64
   int32_t blocks;               // workgroups: tiles times ranges
@@ -642,7 +644,8 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
   v4f acc[64];
   mainloop<false, false, false, true, true, QK>(sm, P, Q, 0u, (uint32_t)(2 * k), acc);
   const Place at;
-  const float scale = a.scale ? a.scale[0] * a.scale2[0] : 1.0f;
+  float scale = 1.0f;
+  if (a.scale) scale = a.scale2[0] == 0.0f ? 0.0f : a.scale[0] * a.scale2[0];
   float* out32 = a.out32 + (int64_t)range * a.nq * a.np;
   // Accumulator 8F + J, register r: P index 128 wp + 16 F + 4 g + r, and Q index
   // 128 wq + 16 J + c (K-major), or that of Place::q.

@@ -89,8 +89,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     x: bf16 [..., H]; weight: bf16 [V, H] (H a multiple of 8); target: int32 or
     int64 of x's leading dimensions.  Tokens whose target is ignore_index have
-    loss 0 and no gradient, and the mean is over the others (NaN if there are
-    none, as torch's); any other target outside [0, V) gives a NaN loss.
+    loss 0 and no gradient, and the mean is over the others (as torch's, NaN with
+    gradients of 0 if there are none); any other target outside [0, V) gives a NaN
+    loss.
     reduction: "mean", "sum" or "none" (target's shape).  Differentiable in x and
     weight; the same bits on every run."""
     host = _native(x)
