@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define MXGG_ABI_VERSION 14
+#define MXGG_ABI_VERSION 15
 
 typedef enum mxgg_status {
   MXGG_OK = 0,
@@ -676,7 +676,7 @@ int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,
  *   reduction : NONE (loss = the token losses, fp32 [tokens]), SUM, or MEAN over
  *               the tokens that are not ignored (loss: fp32 [1]; NaN where there
  *               are none, with gradients of 0)
- *   stats     : fp32 [tokens + 1], written for the gradient
+ *   stats     : fp32 [2 tokens + 1], written for the gradient
  *   workspace : mxgg_linear_cross_entropy_workspace_bytes(options), 16-byte
  *               aligned, no initialisation
  */

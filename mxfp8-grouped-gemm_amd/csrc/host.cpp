@@ -572,7 +572,7 @@ variable_list loss_forward(const Tensor& x, const Tensor& w, const Tensor& targe
                            const mxgg_loss_options& o, int64_t stream) {
   const bool each = o.reduction == MXGG_REDUCE_NONE;
   Tensor loss = each ? empty(target.sizes(), x, at::kFloat) : empty({}, x, at::kFloat);
-  Tensor stats = empty({o.tokens + 1}, x, at::kFloat);
+  Tensor stats = empty({2 * o.tokens + 1}, x, at::kFloat);
   const int64_t bytes = lib.linear_cross_entropy_workspace_bytes(&o);
   Tensor ws = empty({std::max<int64_t>(bytes, 0)}, x, at::kByte);
   check(lib.linear_cross_entropy(cp(x), cp(w), cp(target), &o, loss.data_ptr<float>(),

@@ -6,8 +6,11 @@
 //   dx = d W,   dW = d^T x        (g: the loss's gradient per token, 0 where ignored)
 //
 // Forward: 256 (vocabulary) x 256 (token) tiles of z on the matrix cores; every
-// tile leaves one maximum and one sum of exponentials a token, joined over the
-// tiles by a second kernel.  Few tokens stream W past the tiles.
+// tile leaves one maximum m and one sum s of exp(z - m) a token, joined over the tiles
+// by a second kernel.  Few tokens stream W past the tiles.
+// lse = m + log(s) is never formed: a token that is sure of its target has a loss and
+// a p - 1 far below the spacing of fp32 numbers at lse.  The loss is (m - z) + log(s),
+// and m and 1 / s are kept for p = exp(z - m) / s.
 // Backward: pieces of the vocabulary.  The tiles of a piece are computed again
 // (8 T H V operations in all, 6 with kept logits) and leave d / g rounded to bf16,
 // [T][piece].  Both products read it, W and x as they lie: an operand that is not
@@ -30,7 +33,7 @@ namespace mxgg {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_inff();
 constexpr int kTile = 256;
 constexpr int kSmallTile = 128;
 
@@ -38,7 +41,7 @@ constexpr int kSmallTile = 128;
 // stages of the main loop.
 struct TokenInfo {
   int32_t word;  // target's place among the tile's words, kNoWord or kIgnored
-  float shift, g;
+  float most, scale, g;  // scale = g / s
 };
 constexpr int32_t kNoWord = -1, kIgnored = -2;
 struct __align__(16) LossSmem {
@@ -186,10 +189,13 @@ __device__ __forceinline__ void logits(LossSmem& sm, const LossArgs& a, int64_t 
   const uint32_t kend = (uint32_t)(2 * a.H);
   const int64_t t = q0 + threadIdx.x;
   int64_t target = -1;
-  float lse = 0.0f, g = 1.0f;
+  float most = 0.0f, over_sum = 0.0f, g = 1.0f;
   if (t < a.T) {
     target = target_of(a, t);
-    if (GRAD) lse = a.stats[t];
+    if (GRAD) {
+      most = a.stats[t];
+      over_sum = a.stats[a.T + t];
+    }
     if (GRAD && a.per_token) g = a.grad_loss[t];
   }
   Stream<false> st;
@@ -199,16 +205,21 @@ __device__ __forceinline__ void logits(LossSmem& sm, const LossArgs& a, int64_t 
   sm.token[threadIdx.x] = {target == -1                 ? kIgnored
                            : word >= 0 && word < kTile ? (int32_t)word
                                                         : kNoWord,
-                           -lse * kLog2e, g};
+                           most, over_sum * g, g};
   mainloop<false, false, true, true, false, false, 0>(sm, P, Q, 0u, kend, acc);
 }
 
+// exp(z - m).
+__device__ __forceinline__ float exp_over(float z, float m) {
+  return __builtin_amdgcn_exp2f((z - m) * kLog2e);
+}
+// What to subtract where m is the largest of some words, or of none (-infinity).
+__device__ __forceinline__ float or_zero(float m) { return m == kNegInf ? 0.0f : m; }
+
 // (max, sum of exp(z - max)) of two sets of words.
 __device__ __forceinline__ float2 join_halves(float2 u, float2 v) {
-  const float m = __builtin_fmaxf(u.x, v.x);
-  const float base = m == -__builtin_inff() ? 0.0f : m;
-  return make_float2(m, u.y * __builtin_amdgcn_exp2f((u.x - base) * kLog2e) +
-                            v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e));
+  const float m = __builtin_fmaxf(u.x, v.x), sub = or_zero(m);
+  return make_float2(m, u.y * exp_over(u.x, sub) + v.y * exp_over(v.x, sub));
 }
 
 // Statistics of a tile: part[part row][t] = (max, sum of exp(z - max)) over the
@@ -225,27 +236,26 @@ __device__ __forceinline__ void fwd_tile(LossSmem& sm, const LossArgs& a, int64_
     for (int k = 0; k < 64; ++k)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (at.p(k >> 5, r, (k >> 3) & 3) >= words) acc[k][r] = -__builtin_inff();
+        if (at.p(k >> 5, r, (k >> 3) & 3) >= words) acc[k][r] = kNegInf;
   }
   float2* joined = reinterpret_cast<float2*>(&sm.ring[0][0]);  // [wp][token]
 #pragma unroll
   for (int H = 0; H < 2; ++H)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float m = -__builtin_inff();
+      float m = kNegInf;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
         for (int r = 0; r < 4; ++r) m = __builtin_fmaxf(m, acc[8 * k + 4 * H + j][r]);
       m = __builtin_fmaxf(m, __shfl_xor(m, 16));
       m = __builtin_fmaxf(m, __shfl_xor(m, 32));
-      const float shift = m == -__builtin_inff() ? 0.0f : -m * kLog2e;
+      const float sub = or_zero(m);
       float s = 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[8 * k + 4 * H + j][r], kLog2e, shift));
+        for (int r = 0; r < 4; ++r) s += exp_over(acc[8 * k + 4 * H + j][r], sub);
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if (at.g == 0) joined[256 * at.wp + at.q(H, j)] = make_float2(m, s);
@@ -282,20 +292,19 @@ __device__ __forceinline__ void fwd_tile_small(SmallSmem& sm, const LossArgs& a,
 #pragma unroll
   for (int J = 0; J < 4; ++J) {
     const int q = 64 * at.wq + 16 * J + at.c;
-    float z[16], m = -__builtin_inff();
+    float z[16], m = kNegInf;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       z[i] = first + 16 * (i >> 2) + (i & 3) < words ? acc[4 * (i >> 2) + J][i & 3]
-                                                     : -__builtin_inff();
+                                                     : kNegInf;
       m = __builtin_fmaxf(m, z[i]);
     }
     m = __builtin_fmaxf(m, __shfl_xor(m, 16));
     m = __builtin_fmaxf(m, __shfl_xor(m, 32));
-    const float shift = m == -__builtin_inff() ? 0.0f : -m * kLog2e;
+    const float sub = or_zero(m);
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], kLog2e, shift));
+    for (int i = 0; i < 16; ++i) s += exp_over(z[i], sub);
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
     if (at.g == 0) joined[kSmallTile * at.wp + q] = make_float2(m, s);
@@ -356,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int tiles) {
 #pragma unroll
   for (int i = 0; i < (NB + 3) / 4; ++i) {
     const int64_t t = 16 * (4 * i + (int64_t)wave) + m;
-    most[i] = -__builtin_inff();
+    most[i] = kNegInf;
     sum[i] = 0.0f;
     target[i] = t < a.T ? target_of(a, t) : -1;
   }
@@ -419,18 +428,17 @@ __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int tiles) {
         for (int w = 1; w < 4; ++w) v += part_s[parity][w][F][j][lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          z[4 * F + r] = 16 * F + 4 * (int)g + r < words ? v[r] : -__builtin_inff();
+          z[4 * F + r] = 16 * F + 4 * (int)g + r < words ? v[r] : kNegInf;
           best = __builtin_fmaxf(best, z[4 * F + r]);
         }
       }
       best = __builtin_fmaxf(best, __shfl_xor(best, 16));
       best = __builtin_fmaxf(best, __shfl_xor(best, 32));
-      const float base = best == -__builtin_inff() ? 0.0f : best;
-      sum[i] *= __builtin_amdgcn_exp2f((most[i] - base) * kLog2e);  // this lane's words
+      const float sub = or_zero(best);
+      sum[i] *= exp_over(most[i], sub);  // this lane's words
       most[i] = best;
 #pragma unroll
-      for (int u = 0; u < 4 * kFewFrags; ++u)
-        sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[u], kLog2e, -base * kLog2e));
+      for (int u = 0; u < 4 * kFewFrags; ++u) sum[i] += exp_over(z[u], sub);
       const int64_t word = target[i] - p0 - 4 * (int64_t)g;
 #pragma unroll
       for (int u = 0; u < 4 * kFewFrags; ++u)
@@ -447,14 +455,14 @@ __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int tiles) {
   }
 }
 
-// lse and loss of every token from its tiles' statistics: 16 tokens a workgroup,
+// Statistics and loss of every token from its tiles': 16 tokens a workgroup,
 // 16 runs of tiles each.
 constexpr int kJoinTokens = 16, kJoinRuns = 16;
 __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a, int tiles) {
   __shared__ float2 run_s[kJoinRuns][kJoinTokens];
   const int k = threadIdx.x % kJoinTokens, run = threadIdx.x / kJoinTokens;
   const int64_t t = (int64_t)blockIdx.x * kJoinTokens + k;
-  float2 sum = make_float2(-__builtin_inff(), 0.0f);
+  float2 sum = make_float2(kNegInf, 0.0f);
   constexpr int kAhead = 8;  // loads in flight
   if (t < a.T)
     for (int i0 = run; i0 < tiles; i0 += kJoinRuns * kAhead) {
@@ -462,7 +470,7 @@ __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int i = i0 + u * kJoinRuns;
-        v[u] = i < tiles ? a.part[(int64_t)i * a.T + t] : make_float2(-__builtin_inff(), 0.0f);
+        v[u] = i < tiles ? a.part[(int64_t)i * a.T + t] : make_float2(kNegInf, 0.0f);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) sum = join_halves(sum, v[u]);
@@ -471,15 +479,19 @@ __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a
   __syncthreads();
   if (run != 0 || t >= a.T) return;
   for (int i = 1; i < kJoinRuns; ++i) sum = join_halves(sum, run_s[i][k]);
-  const float lse = sum.x + __builtin_amdgcn_logf(sum.y) * kLn2;
   const int64_t target = target_of(a, t);
   const float nan = __builtin_nanf("");
-  a.stats[t] = target == -2 ? nan : lse;
-  a.token_loss[t] = target == -1 ? 0.0f : target == -2 ? nan : lse - a.target_logit[t];
+  a.stats[t] = sum.x;
+  a.stats[a.T + t] = target == -2 ? nan : 1.0f / sum.y;
+  if (target < 0) {
+    a.token_loss[t] = target == -1 ? 0.0f : nan;
+    return;
+  }
+  a.token_loss[t] = (sum.x - a.target_logit[t]) + logf(sum.y);
 }
 
 // Sum (or mean over the tokens that count) of the token losses, in a fixed
-// order, and the factor of their gradients behind the tokens' lse: the reciprocal
+// order, and the factor of their gradients behind the tokens' statistics: the reciprocal
 // count of the mean, 0 where no token counts (its mean is 0 / 0, but nothing has a
 // gradient).
 constexpr int kReduceThreads = 1024;
@@ -503,7 +515,7 @@ __global__ __launch_bounds__(kReduceThreads) void k_loss_reduce(LossArgs a) {
   }
   if (threadIdx.x == 0) {
     a.loss[0] = a.mean ? sums[0] / (float)counts[0] : sums[0];
-    a.stats[a.T] = counts[0] == 0 ? 0.0f : a.mean ? 1.0f / (float)counts[0] : 1.0f;
+    a.stats[2 * a.T] = counts[0] == 0 ? 0.0f : a.mean ? 1.0f / (float)counts[0] : 1.0f;
   }
 }
 
@@ -525,11 +537,11 @@ __device__ __forceinline__ void grad_tile(LossSmem& sm, const LossArgs& a, int64
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int p = at.p(k >> 2, r, k & 3);
-          const float z = acc[8 * k + 4 * H + j][r];
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, own.shift));
-          acc[8 * k + 4 * H + j][r] = own.word == kIgnored || p >= words
-                                          ? 0.0f
-                                          : (e - (own.word == p ? 1.0f : 0.0f)) * own.g;
+          const float e = exp_over(acc[8 * k + 4 * H + j][r], own.most);
+          acc[8 * k + 4 * H + j][r] =
+              own.word == kIgnored || p >= words
+                  ? 0.0f
+                  : __builtin_fmaf(e, own.scale, own.word == p ? -own.g : 0.0f);
         }
     }
   // rows of tokens: 16 consecutive words a lane
@@ -575,18 +587,18 @@ __device__ __forceinline__ void grad_tile_small(SmallSmem& sm, const LossArgs& a
     const int64_t t = q0 + 64 * at.wq + 16 * J + at.c;
     if (t >= a.T) continue;
     const int64_t target = target_of(a, t);
-    const float shift = target == -1 ? 0.0f : -a.stats[t] * kLog2e;
     const float g = target != -1 && a.per_token ? a.grad_loss[t] : 1.0f;
+    const float most = a.stats[t], scale = a.stats[a.T + t] * g;
     const int64_t word = target - v0 - p0 - first;
 #pragma unroll
     for (int F = 0; F < 4; ++F) {
       float v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * F + J][r], kLog2e, shift));
+        const float e = exp_over(acc[4 * F + J][r], most);
         v[r] = target == -1 || first + 16 * F + r >= words
                    ? 0.0f
-                   : (e - (word == 16 * F + r ? 1.0f : 0.0f)) * g;
+                   : __builtin_fmaf(e, scale, word == 16 * F + r ? -g : 0.0f);
       }
       *reinterpret_cast<uint2*>(a.d + t * width + p0 + first + 16 * F) =
           make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -920,7 +932,7 @@ hipError_t launch_loss_grad(LossArgs a, uint16_t* dx, uint16_t* dw, uint8_t* ws,
     Product px{}, pw{};
     if (!a.per_token) {
       px.scale = pw.scale = a.grad_loss;
-      px.scale2 = pw.scale2 = a.stats + a.T;
+      px.scale2 = pw.scale2 = a.stats + 2 * a.T;
     }
     px.np = pw.np = a.H;
     if (dx) {  // dx[t][h] = sum over words of d[t][v] W[v][h]

@@ -194,7 +194,7 @@ struct LossArgs {
   const uint16_t* x;   // bf16 [T][H], row stride ldx
   const uint16_t* w;   // bf16 [V][H], row stride ldw
   const void* target;  // [T] int32 or int64
-  float* stats;        // [T + 1]: log of the sum of exponentials, then the factor of the mean
+  float* stats;        // [2 T + 1]: maxima and 1 / sums of exponentials, then the gradients' factor
   float* token_loss;   // [T]
   float* loss;         // [1], or nullptr: no reduction
   const float* grad_loss;  // [1], or [T] with per_token

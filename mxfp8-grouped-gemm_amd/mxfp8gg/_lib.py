@@ -46,7 +46,7 @@ OFFS_ENDS = 0
 OFFS_SIZES = 1
 OFFS_AUTO = 2
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 MAX_GROUPS = 1024  # groups of one call
 
 _P = ctypes.c_void_p

@@ -4,7 +4,7 @@
     loss.backward()
 
 is cross_entropy(x @ weight.T, target) without the logits [T, V]: the forward
-pass keeps one fp32 value a token, the backward pass computes the logits again
+pass keeps two fp32 values a token, the backward pass computes the logits again
 in pieces of the vocabulary and holds at most 1 GiB of bf16 [T, piece] (and dx in
 fp32 where there are several).
 """
@@ -35,7 +35,7 @@ def _forward(x, w, target, opt):
     lib, dev = _lib.load(), x.device
     loss = torch.empty(opt.tokens if opt.reduction == _lib.REDUCE_NONE else (),
                        dtype=torch.float32, device=dev)
-    stats = torch.empty(opt.tokens + 1, dtype=torch.float32, device=dev)
+    stats = torch.empty(2 * opt.tokens + 1, dtype=torch.float32, device=dev)
     nbytes = lib.mxgg_linear_cross_entropy_workspace_bytes(ctypes.byref(opt))
     ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
     _lib.check(
