@@ -482,7 +482,7 @@ __global__ __launch_bounds__(kJoinTokens* kJoinRuns) void k_loss_join(LossArgs a
   const int64_t target = target_of(a, t);
   const float nan = __builtin_nanf("");
   a.stats[t] = sum.x;
-  a.stats[a.T + t] = target == -2 ? nan : 1.0f / sum.y;
+  a.stats[a.T + t] = target == -1 ? 0.0f : target == -2 ? nan : 1.0f / sum.y;
   if (target < 0) {
     a.token_loss[t] = target == -1 ? 0.0f : nan;
     return;
@@ -637,6 +637,7 @@ struct Product {
   float* out32;         // fp32 [ranges][nq][np]
   const float* scale;   // two factors, at scale[0] and scale2[0], or nullptr; a zero at
   const float* scale2;  // scale2 makes the output 0 whatever is at scale
+  const float* live;    // not QK: [nq], 0 for rows that are 0 whatever the scale
   int64_t ldp, ldq, np, nq, k;  // elements
   int64_t range;                // k of a range, a multiple of 64
   int32_t blocks;               // workgroups: tiles times ranges
@@ -656,6 +657,7 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
   // loaded ahead of the main loop: behind it they cost a tile 0.2 us
   const float grad = a.scale ? a.scale[0] : 1.0f, factor = a.scale ? a.scale2[0] : 1.0f;
   const float scale = factor == 0.0f ? 0.0f : grad * factor;
+  const bool odd_scale = !QK && !(__builtin_fabsf(scale) < __builtin_inff());
   v4f acc[64];
   mainloop<false, false, false, true, true, QK>(sm, P, Q, 0u, (uint32_t)(2 * k), acc);
   const Place at;
@@ -666,6 +668,8 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
   for (int J = 0; J < 8; ++J) {
     const int64_t q = q0 + (QK ? 128 * at.wq + 16 * J + at.c : at.q(J >> 2, J & 3));
     const bool row = q < a.nq;
+    // a row of zeros stays one under a factor that is not finite
+    const float times = odd_scale && row && a.live[q] == 0.0f ? 0.0f : scale;
 #pragma unroll
     for (int F = 0; F < 8; F += 2) {
       float v[2][4];
@@ -673,7 +677,7 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
       for (int u = 0; u < 2; ++u) {
         const int64_t p = p0 + 128 * at.wp + 16 * (F + u) + 4 * at.g, o = q * a.np + p;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[u][r] = acc[8 * (F + u) + J][r] * scale;
+        for (int r = 0; r < 4; ++r) v[u][r] = acc[8 * (F + u) + J][r] * times;
         if (!row || p >= a.np) continue;
         if (a.before != nullptr) {
           const float4 b = *reinterpret_cast<const float4*>(a.before + o);
@@ -943,6 +947,7 @@ hipError_t launch_loss_grad(LossArgs a, uint16_t* dx, uint16_t* dw, uint8_t* ws,
       px.nq = a.T;
       px.k = words;
       px.before = v0 > 0 ? acc : nullptr;
+      px.live = a.stats + a.T;
       px.out = v0 + words == a.V ? dx : nullptr;
     }
     if (dw) {  // dW[v][h] = sum over tokens of d[t][v] x[t][h]

@@ -42,3 +42,20 @@ def test_every_token_ignored(gpu, monkeypatch, T, V, H, native):
             only, = torch.autograd.grad(mxfp8gg.linear_cross_entropy(x.detach(), w, t,
                                                                      reduction=reduction), w, up)
             assert (only == 0).all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("T,V,H", SHAPES[1:] + [(16400, 70001, 72)])
+def test_ignored_rows_of_a_gradient_that_is_not_finite(gpu, monkeypatch, T, V, H, native):
+    """Also in vocabularies of several pieces; the rows that count are not finite."""
+    _path(monkeypatch, native)
+    x, w, t = _inputs(gpu, T, V, H)
+    out = torch.rand(T, device=gpu) < 0.5
+    out[0], out[-1] = True, False
+    t[out] = -100
+    for reduction in ("mean", "sum", "none"):
+        for scale in (float("inf"), float("nan")):
+            loss = mxfp8gg.linear_cross_entropy(x, w, t, reduction=reduction)
+            dx, = torch.autograd.grad(loss, x, torch.full_like(loss, scale))
+            assert (dx[out] == 0).all(), (reduction, scale)
+            assert not torch.isfinite(dx[~out]).any(dim=1).all()
