@@ -322,9 +322,21 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
     for (int v = 0; v < VPL; ++v) top = __builtin_fmaxf(top, x[v]);
     for (int off = 1; off < a.lanes; off <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, off));
     if (top == kNegInf) top = 0.0f;
-    total = 0.0f;
+    // in runs of 8 and then by pairs, as lanes of 8 experts each add them: a token's
+    // scores, and so a choice that goes by them, do not depend on the experts a lane
+    static_assert(VPL == 8 || VPL == 32, "a power of two of runs");
+    float run[VPL / 8];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) total += expf(x[v] - top);
+    for (int r = 0; r < VPL / 8; ++r) {
+      run[r] = 0.0f;
+#pragma unroll
+      for (int v = 8 * r; v < 8 * r + 8; ++v) run[r] += expf(x[v] - top);
+    }
+#pragma unroll
+    for (int w = 1; w < VPL / 8; w *= 2)
+#pragma unroll
+      for (int r = 0; r < VPL / 8; r += 2 * w) run[r] += run[r + w];
+    total = run[0];
     for (int off = 1; off < a.lanes; off <<= 1) total += __shfl_xor(total, off);
     if (total == 0.0f) total = 1.0f;  // every expert is out
     if (sub == 0 && tok < nt) stats[tok] = make_float2(top, total);
