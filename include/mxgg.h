@@ -569,7 +569,8 @@ int mxgg_combine_score_grad(const void* grad_out, int64_t ldg, const void* y, in
  *                      row's chosen s (0 where that sum is 0)
  * An expert with x = -inf or c = -inf cannot be chosen; a slot with no expert
  * left has id -1 (dropped by mxgg_route_plan) and weight 0.
- *   selected         : fp32 [tokens, topk] for mxgg_route_topk_grad, or NULL
+ *   selected         : fp32 [tokens, topk] for mxgg_route_topk_grad, or NULL: what it
+ *                      needs of the chosen (SIGMOID: their logits)
  * experts <= 1024, topk <= 32 and <= experts, groups <= 64 dividing experts.
  * `options` is host memory, read during the call.
  */

@@ -425,7 +425,7 @@ void first_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice (create_graph)");
 }
 
-// (expert_idx, weights) and, for the gradient, the selected scores.
+// (expert_idx, weights) and, for the gradient, what it needs of the chosen.
 variable_list route_forward(const Tensor& logits, const float* bias,
                             const mxgg_route_options& o, bool keep_selected, int64_t stream) {
   const int64_t tokens = logits.size(0);

@@ -181,14 +181,18 @@ __device__ __forceinline__ void merge_lanes(double (&a)[L], int off) {
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+constexpr float kSigmoidZero = -88.72284f;  // expf(-x) overflows below: the result is 0
 
 // The same bits for |x| <= 87: no range tests in the exponential, and one Newton
 // step on v_rcp_f32 for the quotient, which returns the correctly rounded 1 / d for
 // every mantissa of d (checked over all 2^23 of them, and at other exponents).
 constexpr float kModerate = 87.0f;
-__device__ __forceinline__ float sigmoid_moderate(float x) {
-  const float d = 1.0f + exp_moderate(-x), r = __builtin_amdgcn_rcpf(d);
+__device__ __forceinline__ float reciprocal(float d) {
+  const float r = __builtin_amdgcn_rcpf(d);
   return __builtin_fmaf(__builtin_fmaf(-r, d, 1.0f), r, r);
+}
+__device__ __forceinline__ float sigmoid_moderate(float x) {
+  return reciprocal(1.0f + exp_moderate(-x));
 }
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -446,9 +450,9 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
   for (int p = lane; p < slots; p += 64) {
     const int t = div_k(p, a.k_recip), e = pk[p];
     const float* row_x = tile;
-    float s = 0.0f;
+    float s = 0.0f, xe = 0.0f;
     if (e >= 0) {
-      const float xe = row_x[pad32(t * a.E + e)];
+      xe = row_x[pad32(t * a.E + e)];
       if (!a.softmax) {
         s = sigmoid(xe);
       } else if (!a.renorm) {
@@ -465,6 +469,8 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
       }
     }
     val[p] = s;
+    // for the gradient the logit: a score that is 1 to the last bit has lost its slope
+    if (a.sel != nullptr && !a.softmax) a.sel[t0 * a.K + p] = xe;
   }
   wave_sync();
   for (int p = lane; p < slots; p += 64) {
@@ -479,12 +485,12 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk(RouteTopkArgs a) {
     const int64_t at = t0 * a.K + p;
     a.idx[at] = pk[p];
     a.weights[at] = a.scale * w;
-    if (a.sel != nullptr) a.sel[at] = s;
+    if (a.sel != nullptr && a.softmax) a.sel[at] = s;
   }
 }
 
 // Gradient of the weights: dw [tokens][K] -> d logits [tokens][E].
-//   sigmoid        : dx = ds s (1 - s), zero for experts not selected
+//   sigmoid        : dx = ds sigma(x) sigma(-x), zero for experts not selected
 //   softmax, renorm: dx = p (dp - sum p dp) over the selected, zero elsewhere
 //   softmax alone  : dx = p (dp - sum p dp) over the whole row (p from the logits)
 // with ds = scale dw, or scale (dw - sum dw s / S) / S where s is divided by its
@@ -494,6 +500,7 @@ template <typename T>
 __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradArgs a) {
   __shared__ float grad_s[kTopkWaves][kGradTile];
   __shared__ float2 slot_s[kTopkWaves][kGradSlots];  // (s, s dw) of a slot
+  __shared__ float slope_s[kTopkWaves][kGradSlots];  // ds / dx of a sigmoid
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t0 = ((int64_t)blockIdx.x * kTopkWaves + wave) * a.tokens_wave;
@@ -501,13 +508,19 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradA
   if (nt == 0) return;
   float* grad = grad_s[wave];
   float2* slot = slot_s[wave];
+  float* slope = slope_s[wave];
   const int n = nt * a.E, slots = nt * a.K;
   const int32_t* idx = a.idx + t0 * a.K;
   const float* sel = a.sel + t0 * a.K;
   const float* dw = a.dweights + t0 * a.K;
   for (int p = lane; p < slots; p += 64) {  // slots without an expert add nothing
     const bool live = (uint32_t)idx[p] < (uint32_t)a.E;
-    const float s = live ? sel[p] : 0.0f;
+    float s = live ? sel[p] : 0.0f;
+    if (!a.softmax) {  // from the logit, without 1 - s
+      const float e = expf(-__builtin_fabsf(s)), r = reciprocal(1.0f + e);
+      slope[p] = e * r * r;
+      s = !live || s < kSigmoidZero ? 0.0f : s < 0.0f ? e * r : r;
+    }
     slot[p] = make_float2(s, live ? s * dw[p] : 0.0f);
   }
   for (int i = 4 * lane; i < n; i += 256)
@@ -527,9 +540,9 @@ __global__ __launch_bounds__(kTopkThreads) void k_route_topk_grad(RouteTopkGradA
     if (a.softmax)
       g = a.scale * (a.renorm ? s * (d - dot) : d);
     else if (a.renorm)
-      g = sum == 0.0f ? 0.0f : a.scale * (d - dot / sum) / sum * s * (1.0f - s);
+      g = sum == 0.0f ? 0.0f : a.scale * (d - dot / sum) / sum * slope[p];
     else
-      g = a.scale * d * s * (1.0f - s);
+      g = a.scale * d * slope[p];
     grad[t * a.E + e] = g;
   }
   wave_sync();

@@ -57,7 +57,8 @@ def _route_forward(logits, bias, opt, keep):
 class RouteTopK(torch.autograd.Function):
     """route_topk with the gradient of the scores with respect to the logits.
 
-    What the forward keeps is [tokens, topk]: the ids and the selected scores.
+    What the forward keeps is [tokens, topk]: the ids, and the chosen scores (softmax) or
+    logits (sigmoid).
     The logits are kept for softmax scores without renormalisation only, whose
     gradient reaches every expert."""
 

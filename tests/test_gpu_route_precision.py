@@ -1,4 +1,5 @@
 """route_topk where scores are close, saturated or taken on different paths."""
+import numpy as np
 import pytest
 import torch
 
@@ -23,3 +24,41 @@ def test_softmax_scores_do_not_depend_on_the_batch(gpu, E, G, K, biased):
     for a in (0, 777, T - 300):
         i, v = f(x[a:a + 300])
         assert torch.equal(i, idx[a:a + 300]) and torch.equal(v, w[a:a + 300])
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+def test_gradient_of_saturated_sigmoids(gpu, renorm):
+    """sigma(x) sigma(-x) keeps its digits where sigma(x) is 1 to the last bit.  A slot's
+    terms are a few fp32 operations each, 2^-20 relative; where scores are divided by
+    their sum the difference of two such terms, of their magnitudes."""
+    g = torch.Generator().manual_seed(1)
+    T, E, K = 500, 16, 5
+    x = ((torch.rand((T, E), generator=g) * 2 - 1) * 80).to(gpu).requires_grad_(True)
+    dw = torch.randn((T, K), generator=g).to(gpu)
+    idx, w = mxfp8gg.route_topk(x, K, score="sigmoid", renormalize=renorm)
+    dx, = torch.autograd.grad(w, x, dw)
+    at = idx.cpu().numpy().astype(np.int64)
+    z = np.take_along_axis(x.detach().cpu().double().numpy(), at, 1)
+    got = np.take_along_axis(dx.cpu().double().numpy(), at, 1)
+    d = dw.cpu().double().numpy()
+    s, slope = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(-z)) / (1 + np.exp(z))
+    if renorm:
+        total = s.sum(axis=1, keepdims=True)
+        want = (d - (d * s).sum(axis=1, keepdims=True) / total) / total * slope
+        size = (np.abs(d) + (np.abs(d) * s).sum(axis=1, keepdims=True) / total) / total * slope
+    else:
+        want, size = d * slope, np.abs(d) * slope
+    assert (z > 30).mean() > 0.3
+    bad = np.abs(got - want) > 2.0 ** -20 * size + 1e-37
+    assert not bad.any(), (z[bad][:5], got[bad][:5], want[bad][:5])
+
+
+def test_gradient_where_every_sigmoid_underflows(gpu):
+    """Weights that are 0 because the sum of the scores is have no gradient; slots beside
+    a score that is not 0 have that of their tiny slope."""
+    x = torch.tensor([[-90.0, -95.0, -100.0, -200.0], [-90.0, 0.0, -200.0, -300.0]], device=gpu)
+    x.requires_grad_(True)
+    idx, w = mxfp8gg.route_topk(x, 2, score="sigmoid")
+    assert idx.tolist() == [[0, 1], [1, 0]] and w.tolist() == [[0.0, 0.0], [1.0, 0.0]]
+    dx, = torch.autograd.grad(w, x, torch.tensor([[1.0, 2.0], [1.0, 3.0]], device=gpu))
+    assert (dx[0] == 0).all() and (dx[1, 1:] == 0).all() and 0 <= float(dx[1, 0]) < 1e-37
