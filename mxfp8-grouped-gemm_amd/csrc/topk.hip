@@ -185,7 +185,9 @@ constexpr float kSigmoidZero = -88.72284f;  // expf(-x) overflows below: the res
 
 // The same bits for |x| <= 87: no range tests in the exponential, and one Newton
 // step on v_rcp_f32 for the quotient, which returns the correctly rounded 1 / d for
-// every mantissa of d (checked over all 2^23 of them, and at other exponents).
+// every mantissa of d (compared with the division once for all 2^23 of them, and at other
+// exponents; tests/test_gpu_route_precision.py ranks four million logits, neighbours of
+// each other, by both sequences).
 constexpr float kModerate = 87.0f;
 __device__ __forceinline__ float reciprocal(float d) {
   const float r = __builtin_amdgcn_rcpf(d);

@@ -62,3 +62,25 @@ def test_gradient_where_every_sigmoid_underflows(gpu):
     assert idx.tolist() == [[0, 1], [1, 0]] and w.tolist() == [[0.0, 0.0], [1.0, 0.0]]
     dx, = torch.autograd.grad(w, x, torch.tensor([[1.0, 2.0], [1.0, 3.0]], device=gpu))
     assert (dx[0] == 0).all() and (dx[1, 1:] == 0).all() and 0 <= float(dx[1, 0]) < 1e-37
+
+
+def test_sigmoids_of_both_paths_are_the_same_bits(gpu):
+    """Waves whose logits and biases are moderate take sigmoids by a shorter sequence.
+    Runs of 32 neighbouring fp32 logits rank the same whether the expert that always
+    comes first has a large finite bias or an infinite one, which takes the general
+    sequence: a rounding apart would make a tie of two ranks or two ranks of a tie."""
+    g = torch.Generator(device=gpu).manual_seed(2)
+    T, E = 1 << 17, 33
+    base = torch.rand((T, 1), generator=g, device=gpu) * 37 - 20
+    base[: T // 8] *= 1e-3
+    step = torch.rand((T, 32), generator=g, device=gpu).argsort(dim=1).to(torch.int32)
+    near = (base.view(torch.int32) + step).view(torch.float32)
+    x = torch.cat([near, torch.zeros((T, 1), device=gpu)], dim=1)
+    assert torch.isfinite(x).all() and x.abs().max() < 87
+    out = []
+    for first in (1e30, float("inf")):
+        bias = torch.zeros(E, device=gpu)
+        bias[-1] = first
+        out.append(mxfp8gg.route_topk(x, 32, score="sigmoid", bias=bias)[0])
+    assert (out[0][:, 0] == E - 1).all()
+    assert torch.equal(*out)
