@@ -416,6 +416,9 @@ bool f32_or_bf16(const Tensor& t) {
 int32_t type_of(const Tensor& t) {
   return t.scalar_type() == at::kBFloat16 ? MXGG_OUT_BF16 : MXGG_OUT_F32;
 }
+// A tangent of forward-mode differentiation, which these operators do not propagate.
+bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool tangent(const OptTensor& t) { return t && tangent(*t); }
 void* vp_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 const void* cp_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
@@ -469,7 +472,7 @@ struct RouteTopK : torch::autograd::Function<RouteTopK> {
 Result route_topk(const Tensor& logits, const OptTensor& bias, int64_t topk, int64_t groups,
                   int64_t top_groups, int score, int group_best, bool renormalize, double scale,
                   int64_t stream) {
-  if (!plain(logits) || logits.dim() != 2 || !f32_or_bf16(logits) || !logits.is_contiguous() ||
+  if (!plain(logits) || tangent(logits) || logits.dim() != 2 || !f32_or_bf16(logits) || !logits.is_contiguous() ||
       (bias && (!plain(*bias) || bias->scalar_type() != at::kFloat || bias->dim() != 1 ||
                 bias->size(0) != logits.size(1) || !bias->is_contiguous() ||
                 bias->device() != logits.device())))
@@ -542,7 +545,8 @@ struct Norm : torch::autograd::Function<Norm> {
 
 Result norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
             bool center, int64_t stream) {
-  if (!plain(x) || !f32_or_bf16(x) || x.dim() < 1 || x.size(-1) > 32768 || row_stride(x) < 0)
+  if (!plain(x) || !f32_or_bf16(x) || x.dim() < 1 || x.size(-1) > 32768 || row_stride(x) < 0 ||
+      tangent(x) || tangent(weight) || tangent(bias))
     return none();
   const int64_t cols = x.size(-1);
   for (const OptTensor* p : {&weight, &bias})
@@ -619,7 +623,7 @@ Result linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& targ
       w.device() != x.device() || !plain(target) || !target.is_contiguous() ||
       (target.scalar_type() != at::kInt && target.scalar_type() != at::kLong) ||
       target.device() != x.device() || target.dim() != x.dim() - 1 ||
-      target.sizes() != x.sizes().slice(0, x.dim() - 1))
+      target.sizes() != x.sizes().slice(0, x.dim() - 1) || tangent(x) || tangent(w))
     return none();
   const mxgg_loss_options o{target.numel(), w.size(0),    x.size(-1),
                             row_stride(x),  row_stride(w), ignore_index,

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _first_order, _native, _need_gpu, _stream_ptr, _tensors, _took
+from .ops import _first_order, _native, _need_gpu, _no_tangent, _stream_ptr, _tensors, _took
 
 __all__ = ["linear_cross_entropy", "LinearCrossEntropy"]
 
@@ -116,6 +116,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
                          f"{tuple(x.shape)}, {tuple(weight.shape)}, {tuple(target.shape)}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    _no_tangent("linear_cross_entropy", x, weight)
     H = x.shape[-1]
     x2 = x.reshape(-1, H) if H else x.new_empty((0, 0))
     t = target.reshape(-1).contiguous()

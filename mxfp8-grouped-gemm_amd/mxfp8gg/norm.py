@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _first_order, _native, _need_gpu, _stream_ptr, _tensors, _took
+from .ops import _first_order, _native, _need_gpu, _no_tangent, _stream_ptr, _tensors, _took
 
 __all__ = ["layer_norm", "rms_norm", "Norm"]
 
@@ -109,6 +109,7 @@ def _norm(x, weight, bias, eps, center):
             raise ValueError(f"{name} must have shape ({cols},), got {tuple(p.shape)}")
         if p.device != x.device:
             raise ValueError(f"{name} is on {p.device}, x on {x.device}")
+    _no_tangent("layer_norm" if center else "rms_norm", x, weight, bias)
     kind = lambda p: _lib.OUT_F32 if p is None else _TYPES[p.dtype]  # noqa: E731
     opt = _lib.NormOptions(x.numel() // cols, cols, _TYPES[x.dtype], kind(weight),
                            kind(bias), center, eps)

@@ -80,6 +80,15 @@ def _first_order(what: str) -> None:
         raise RuntimeError(f"{what} cannot be differentiated twice (create_graph)")
 
 
+def _no_tangent(what: str, *ts) -> None:
+    """Refuses inputs that carry a tangent of forward-mode differentiation: the result
+    would come without one, which reads as a derivative of zero."""
+    if torch._C._is_fwd_grad_enabled() and any(
+            t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+            for t in ts):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _mode(scaling_mode) -> int:
     if isinstance(scaling_mode, int):
         return scaling_mode

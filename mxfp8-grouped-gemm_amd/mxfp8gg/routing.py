@@ -28,7 +28,7 @@ import torch
 
 from . import _lib, ops
 from .ops import (_FP8, _MODES, _block_major_buffer, _first_order, _mode, _native, _need_gpu,
-                  _stream_ptr, _tensors, _took, padded_token_capacity)
+                  _no_tangent, _stream_ptr, _tensors, _took, padded_token_capacity)
 
 __all__ = ["route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual",
            "gather_to_mxfp8_dim0", "combine", "combine_score_grad"]
@@ -122,6 +122,7 @@ def route_topk(logits: torch.Tensor, topk: int, *, score: str = "softmax",
     _need_gpu(logits, "logits")
     if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES:
         raise TypeError("logits must be a 2-D float32 or bfloat16 tensor [tokens, experts]")
+    _no_tangent("route_topk", logits)
     if score not in _SCORES:
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
     E = logits.shape[1]
