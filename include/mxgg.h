@@ -644,7 +644,8 @@ int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
  *                   b = max(ceil(log2(amax / 448)), -126) + 127, rounded to
  *                   nearest even; a block with an infinity or a NaN is all NaN
  * Any element alignment; tensors must not overlap.  `tensors` and `options` are
- * host memory, read during the call.  One kernel launch for every 48 tensors.
+ * host memory, read during the call; a graph that captures the call repeats the
+ * captured step, lr and bias corrections.  One kernel launch for every 48 tensors.
  */
 typedef struct mxgg_adamw_tensor {
   void* param;

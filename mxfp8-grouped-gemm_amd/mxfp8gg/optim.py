@@ -62,7 +62,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: int, lr: float = 1e-3,
     pairs as adamw_state makes them (8 bits; exp_avg_sq then holds the root).
     masters: fp32 copies of the weights, or None; with them the step is taken on
     the copies and `params` are written as their rounding.  step: the number of
-    this update, from 1."""
+    this update, from 1.  step, lr and the other numbers are arguments of the launch:
+    a captured graph repeats the captured ones at every replay."""
     params, grads, exp_avg, exp_avg_sq = map(list, (params, grads, exp_avg, exp_avg_sq))
     masters = list(masters) if masters is not None else []
     n = len(params)
@@ -118,7 +119,9 @@ class AdamW(torch.optim.Optimizer):
     master_weights  keep an fp32 copy of every bf16 weight and step on it
 
     Weights are fp32 or bf16 and contiguous; gradients fp32 or bf16 (a gradient
-    of another layout is copied).  Parameters without a gradient are skipped."""
+    of another layout is copied).  Parameters without a gradient are skipped.
+    step() raises while the stream is captured into a graph, whose replays would repeat
+    one step number and learning rate."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, state_bits: int = 32, master_weights: bool = False):
@@ -146,6 +149,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step in a graph capture: every replay would repeat this "
+                               "step's number and learning rate")
         loss = None
         if closure is not None:
             with torch.enable_grad():
