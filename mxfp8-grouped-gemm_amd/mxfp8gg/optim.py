@@ -162,8 +162,8 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 state = self._state_of(p, group)
-                state["step"] += 1
-                runs.setdefault((state["step"], "master" in state, p.device), []).append((p, state))
+                runs.setdefault((state["step"] + 1, "master" in state, p.device), []).append(
+                    (p, state))
             for (step, master, _), run in runs.items():
                 if group["state_bits"] == 8:
                     moments = [[(s[n], s[n + "_scales"]) for _, s in run]
@@ -174,6 +174,8 @@ class AdamW(torch.optim.Optimizer):
                            *moments, step=step, lr=float(group["lr"]), betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"],
                            masters=[s["master"] for _, s in run] if master else None)
+                for _, state in run:  # not of a step that was refused
+                    state["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):

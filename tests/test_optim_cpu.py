@@ -12,4 +12,4 @@ def test_step_without_a_gpu():
     p.grad = torch.ones(8)
     with pytest.raises(ValueError):
         opt.step()
-    assert (p == 1).all()
+    assert (p == 1).all() and opt.state[p]["step"] == 0  # a refused step is none
