@@ -29,7 +29,7 @@ constexpr int kAdamThreads = 256;
 constexpr int kAdamVec = 8;
 // Elements of a workgroup, 8 a thread.  235 M bf16 weights with fp32 states and
 // master copy: 1231 us (5.3 TB/s); twice as many elements in two trips 1249, runs
-// of 4 whose lanes follow each other without gaps 1253.  8-bit states: 435 us.
+// of 4 whose lanes follow each other without gaps 1253.  8-bit states: 420 to 435 us.
 constexpr int64_t kAdamChunk = kAdamThreads * kAdamVec;
 constexpr int kAdamTensors = 48;      // of a launch: 3.3 of the 4 KB of kernel arguments
 

@@ -1241,8 +1241,9 @@ static int check_loss(const char* what, const mxgg_loss_options* o) {
     return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
   if (o->ldx % 8 != 0 || o->ldw % 8 != 0)
     return set_error(MXGG_ERR_ALIGNMENT, "%s: leading dimensions multiples of 8", what);
-  // a tile of 256 rows stays within a 2 GiB buffer range: also the rows of d, its
-  // transpose and the transposed operands (at most tokens or a piece long)
+  // a tile's 256 rows of x, of W or of d (a piece is at most 2^21 words wide) stay
+  // within a 2 GiB buffer range; with 2^21 tokens the least piece, 256 words, holds all
+  // of d's 1 GiB; a launch has fewer than 2^24 tiles
   if (2 * o->ldx > kMaxRowStride || 2 * o->ldw > kMaxRowStride ||
       o->tokens > kMaxRowStride / 4 || o->vocab > INT64_C(1) << 24 ||
       (o->vocab + 255) / 256 * ((o->tokens + 255) / 256) >= INT64_C(1) << 24)

@@ -21,8 +21,9 @@
 // A product with few tiles is split along the contraction, and the fp32 partials
 // added in order.
 //
-// 4096 tokens, 131072 words, hidden 7168: forward 5.0 ms (1.54 PFLOP/s), tiles of d 5.2,
-// products 10.9 (1.41); a large product of the library runs 1.51 to 1.52 on this card.
+// 4096 tokens, 131072 words, hidden 7168, on two cards: forward 5.0 and 5.3 ms (1.54 and
+// 1.44 PFLOP/s), tiles of d 5.2 and 5.5, products 10.9 and 11.6 (1.41 and 1.32); a large
+// product of the library runs 1.51 to 1.52 on the first.
 // Bound by the matrix cores at the clock that the power limit leaves.  128 x 32000 x
 // 1024, forward: 16.4 us, the 66 MB of W at 4 TB/s in one round of small tiles.
 #include <algorithm>
@@ -705,7 +706,7 @@ __device__ __forceinline__ void product_tile(LossSmem& sm, const Product& a, int
 // Both products of a piece in one launch, the one with the longer tiles first: the
 // short tiles of the other fill the compute units that its last round leaves idle.
 // Bound by the matrix cores at the clock that the power limit leaves: 4096 tokens,
-// 131072 words, hidden 7168 1.37 PFLOP/s, and with 1024 tokens (short tiles of dW) the
+// 131072 words, hidden 7168 1.32 to 1.41 PFLOP/s, and with 1024 tokens (short tiles of dW) the
 // main loop runs at 1.6 GHz, with 64 tokens at 2.3.  Loading the next tile's stages
 // before the stores, fewer instructions in the epilogue, streaming stores and half the
 // workgroups in reverse order each left the launch as long as it was: a shorter

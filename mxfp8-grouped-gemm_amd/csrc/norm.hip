@@ -25,7 +25,9 @@
 namespace mxgg {
 namespace {
 
-constexpr int kNormMaxThreads = 512;  // leaves a thread 256 registers
+// Leaves a thread 256 registers: enough for 16 elements of every operand, not for 32 or
+// 64 in the backward pass (see norm_shape).
+constexpr int kNormMaxThreads = 512;
 constexpr int kWaveRows = 4;          // waves, and rows at a time, of a workgroup of one-wave rows
 
 // The elements of a 16-byte chunk, read and written at any element alignment.
@@ -391,6 +393,12 @@ __global__ __launch_bounds__(kNormReduceCols* kNormReduceRuns) void k_norm_reduc
 // waves share a row's reductions.  One wave against a workgroup, forward / backward us:
 // 65536 x 512 bf16 21 / 53 and 41 / 83, 65536 x 1024 bf16 41 / 75 and 45 / 99, fp32
 // 80 / 141 and 79 / 156.
+// Rows that take 8 or 16 chunks a thread (fp32 above 8192, bf16 above 16384) keep w, dw,
+// db and two streams of 32 or 64 elements, which do not fit 256 registers: the backward
+// kernel spills 164 of them (fp32 to 16384), 1474 (fp32 above) or 1006 (bf16 above
+// 16384), the forward one up to 548.  Layer norm, forward / backward TB/s of the bytes in
+// and out: fp32 4096 x 8192 (4 chunks) 5.8 / 5.2, 4096 x 16384 (8) 5.1 / 3.8, 2048 x 32768
+// (16) 2.8 / 0.7; bf16 4096 x 16384 (4) 5.5 / 3.9, 2048 x 32768 (8) 3.8 / 0.6.
 struct NormShape {
   int ch, threads;
   bool wave;

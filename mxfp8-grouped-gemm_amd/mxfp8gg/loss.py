@@ -5,8 +5,11 @@
 
 is cross_entropy(x @ weight.T, target) without the logits [T, V]: the forward
 pass keeps two fp32 values a token, the backward pass computes the logits again
-in pieces of the vocabulary and holds at most 1 GiB of bf16 [T, piece] (and dx in
-fp32 where there are several).
+in pieces of the vocabulary.  While it runs it holds at most 1 GiB of bf16 [T, piece],
+dx in fp32 where there are several pieces, and, where a product is split over the
+compute units, fp32 partial sums of at most two tiles of 256 KB a unit for each of the
+two gradients (128 MiB each on 256 units).  d loss / d logits is rounded to bf16 between
+the products, which sum in fp32.
 """
 from __future__ import annotations
 

@@ -6,7 +6,9 @@
 One kernel launch updates up to 48 tensors (weights and gradients bf16 or fp32).
 8-bit states are MXFP8 as the rest of this package uses it: e4m3 payloads with
 one E8M0 scale for every 32 consecutive elements; the second moment is kept as
-its root.  The update marks the weights as modified (torch's version counter),
+its root.  What is below about 2^-18 of its block's largest value is stored as 0, so a
+weight whose gradients are that small beside its neighbours' has no second moment from
+one step to the next.  The update marks the weights as modified (torch's version counter),
 so a WeightCastCache casts them again.
 """
 from __future__ import annotations
