@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define MXGG_ABI_VERSION 15
+#define MXGG_ABI_VERSION 16
 
 typedef enum mxgg_status {
   MXGG_OK = 0,
@@ -713,6 +713,60 @@ int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const 
                                    const mxgg_loss_options* options, void* grad_x,
                                    void* grad_weight, void* workspace, int64_t workspace_bytes,
                                    void* stream);
+
+/*
+ * e4m3 with one fp32 scale for each block of 128:
+ *   s = max(amax / 448, 2^-126),  q = e4m3(x * (1 / s)), nearest even
+ * (a block with a NaN has a NaN scale; one with an infinity an infinite one).
+ * Widths are multiples of 16; a last block may be narrower than 128.  x is bf16 with
+ * 16-byte aligned rows (ldx % 8 == 0), payload rows are 16-byte aligned.
+ *   dim0   : blocks of 1 x 128 along each row.  q [rows, cols]; scale of row m and
+ *            block b at scales[b * lds + m], lds >= rows.
+ *   dim1   : blocks of 128 x 1 along the tokens (rows), restarting at every group,
+ *            written transposed: qt [cols, rows_pad_cap] (contiguous), scale of
+ *            column c and token block b at st[b * ldst + c].  Every group is padded
+ *            with zeros to whole blocks; rows_pad_cap % 128 == 0, at least the padded
+ *            total; group_ends_pad receives the padded cumulative ends.  With q also
+ *            the dim0 cast of the rows inside groups (q and scales NULL: without).
+ *            group_ends NULL: one group of all rows.
+ *   weight : tiles of 128 x 128 of each [N, K] matrix of w [E, N, K] (contiguous):
+ *            q [E, N, K], scales [E, ceil(N / 128), ceil(K / 128)]; qt and st, if not
+ *            NULL, the same payload and scales transposed: qt [E, K, N].
+ */
+int mxgg_block_quant_dim0(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q,
+                          int64_t ldq, float* scales, int64_t lds, void* stream);
+int mxgg_block_quant_dim1(const void* x, int64_t rows, int64_t cols, int64_t ldx,
+                          const int32_t* group_ends, int64_t num_groups, int64_t rows_pad_cap,
+                          void* q, int64_t ldq, float* scales, int64_t lds, void* qt, float* st,
+                          int64_t ldst, int32_t* group_ends_pad, void* stream);
+int mxgg_block_quant_weight(const void* w, int64_t num_groups, int64_t N, int64_t K, void* q,
+                            float* scales, void* qt, float* st, void* stream);
+
+/*
+ * Product of block-scaled operands, grouped by rows:
+ *   out[m][n] = sum over blocks b of as[b][m] ws[g][n / 128][b]
+ *               * sum over k in b of a[m][k] w[g][n][k]        (m in group g)
+ * a [M, K] and w [num_groups, N, K] e4m3 (group stride w_gstride bytes), K % 16 == 0,
+ * 16-byte aligned rows; a_scales[b * ldas + m]; w_scales[g * ws_gstride + (n / 128) * ldws
+ * + b].  Sums are fp32.  out bf16 or fp32 [M, N], row stride ldo elements; rows outside
+ * every group are not written.  group_ends NULL: one group (num_groups = 1).
+ */
+int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t ldas, const void* w,
+                  int64_t w_gstride, int64_t ldw, const float* w_scales, int64_t ws_gstride,
+                  int64_t ldws, const int32_t* group_ends, int64_t num_groups, int64_t M,
+                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* stream);
+
+/*
+ * Weight gradient of block-scaled operands: dw[g][n][k] = sum over the tokens t of group g
+ * of dY[t][n] X[t][k], from the transposed payloads go_t [N, tokens] and ia_t [K, tokens]
+ * and their scales as mxgg_block_quant_dim1 writes them.  group_ends_pad: padded ends
+ * (multiples of 128; others are rounded down), NULL for one group; tokens % 128 == 0.
+ * dw bf16 or fp32 [num_groups, N, K], contiguous; empty groups are written as zeros.
+ */
+int mxgg_block_wgrad(const void* go_t, int64_t ldgo, const float* go_scales, int64_t ldgos,
+                     const void* ia_t, int64_t ldia, const float* ia_scales, int64_t ldias,
+                     const int32_t* group_ends_pad, int64_t num_groups, int64_t tokens, int64_t N,
+                     int64_t K, void* dw, int out_type, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,540 @@
+// Products of e4m3 operands with one fp32 scale for each block of 128.
+//
+//   forward : Y[m][n] = sum_b sa[b][m] sw[n / 128][b] sum_{k in b} A[m][k] W[n][k]
+//   wgrad   : dW[n][k] = sum_b sg[b][n] sx[b][k] sum_{t in b} dY^T[n][t] X^T[k][t]
+//
+// fp32 scales cannot ride in the matrix instruction (its E8M0 scales are powers of
+// two), so every 128-deep product starts from zero and is added to fp32 accumulators
+// with one multiply-add an element: acc += t * s.  That is 4 vector instructions (16
+// cycles) for each v_mfma_f32_16x16x128 (32 cycles), and the accumulators have to
+// live in vector registers, which the multiply-adds can address: 256 x 256 tiles take
+// eight waves of 128 x 64 (two a SIMD: one's multiply-adds run under the other's
+// matrix instructions) instead of the MX kernel's four of 128 x 128.  Where both
+// operands have a scale a row (wgrad) the multiply-add's factor is a product of its
+// own: 8 vector instructions a matrix instruction.
+//
+// Operands stream through two LDS stages of 128 bytes a row by DMA, laid out as in
+// gemm_tile.h; one barrier a stage, seven eighths through it: the next stage has
+// landed and every wave has read the current one, whose slot takes the stage after
+// next; the last matrix instructions of the stage run meanwhile.
+#include "gemm_tile.h"
+
+namespace mxgg {
+namespace {
+
+constexpr int kBlkK = 128;
+
+// One operand of a tile: rows from `data` on, `rows` of them (more read as zero),
+// `len` bytes along the contraction; scales of the tile's rows (one a row and block
+// row, ld floats apart) or of its 128-row blocks (ld floats from one to the next,
+// consecutive along the contraction).
+struct BlockOperand {
+  const uint8_t* data;
+  const float* scale;
+  int64_t ld, lds;
+  int64_t rows;
+};
+
+// Workgroup of WP x WQ waves, each 64 GP rows of P by 64 rows of Q.
+template <int WP, int GP, int WQ, bool ROWS>
+struct BlockTile {
+  static constexpr int kP = 64 * WP * GP, kQ = 64 * WQ;
+  static constexpr int kWavesT = WP * WQ, kThreadsT = 64 * kWavesT;
+  static constexpr uint32_t kData = (uint32_t)(kP + kQ) * kBlkK;
+  static constexpr uint32_t kStage = kData + 4u * (kP + kQ);
+  static constexpr int kLoads = (kP + kQ) / 8 / kWavesT;  // data loads of a wave and stage
+  static constexpr int kFrags = 4 * GP;                   // of P
+  static_assert((kP + kQ) / 64 == kWavesT, "one scale load a wave");
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)uniform((uint32_t)((uint64_t)x >> 32)) << 32 | uniform((uint32_t)x));
+}
+__device__ __forceinline__ desc_t uniform(desc_t d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_readfirstlane(d[i]);
+  return d;
+}
+
+// A wave's loads of one stage: load j fills LDS bytes [1024 (kWaves j + w), + 1024) of the
+// stage, P's slots then Q's.  Slot 128 a + 32 b + c of an operand holds its row
+// 128 a + 4 c + b, chunks XORed with swz(slot).  Scales: 64 floats a wave.
+template <class T, bool ROWS>
+struct BlockStream {
+  desc_t dp, dq, ds;
+  uint32_t vbase_p, vbase_q, ldp, ldq;
+  uint32_t kcol, len;
+  uint32_t vs, sstep;
+
+  __device__ __forceinline__ static uint32_t extent(const BlockOperand& X, uint32_t len) {
+    const int64_t n = X.rows <= 0 ? 0 : (X.rows - 1) * X.ld + len;
+    return (uint32_t)(n > 0x7FFFFFF0 ? 0x7FFFFFF0 : n);
+  }
+  __device__ __forceinline__ void init(const BlockOperand& P, const BlockOperand& Q, uint32_t klen) {
+    const uint32_t lane = threadIdx.x & 63u, wave = wave_id();
+    len = klen;
+    dp = uniform(make_desc(P.data, extent(P, klen)));
+    dq = uniform(make_desc(Q.data, extent(Q, klen)));
+    ldp = uniform((uint32_t)P.ld);
+    ldq = uniform((uint32_t)Q.ld);
+    // wave w of load j: slots 8 (kWaves j + w) + lane / 8; swz of them depends on w only
+    // (kWaves is a multiple of 4: 32-slot runs)
+    kcol = 16u * ((lane & 7u) ^ swz(8u * wave + (lane >> 3)));
+    const uint32_t r = 4u * (8u * (wave & 3u) + (lane >> 3));
+    vbase_p = r * ldp + kcol;
+    vbase_q = r * ldq + kcol;
+    // scales: the first T::kQ / 64 waves take Q's rows, the others P's
+    const bool of_q = wave < (uint32_t)T::kQ / 64u;
+    const uint32_t w = of_q ? wave : wave - (uint32_t)T::kQ / 64u;
+    if (of_q || ROWS) {
+      const BlockOperand& X = of_q ? Q : P;
+      // P's floats are kept in the order in which a lane's four rows follow each other
+      const uint32_t row = 64u * w + (of_q ? lane : (lane & 48u) + 4u * (lane & 3u) + ((lane >> 2) & 3u));
+      ds = uniform(make_desc(X.scale, 0x7FFFFFF0u));
+      vs = (int64_t)row < X.rows ? 4u * row : kOobOffset;
+      sstep = uniform(4u * (uint32_t)X.lds);
+    } else {  // one float for each 128 rows of P, twice
+      const uint32_t b = w >> 1;
+      ds = uniform(make_desc(P.scale, 0x7FFFFFF0u));
+      vs = 128 * (int64_t)b < P.rows ? 4u * b * (uint32_t)P.lds : kOobOffset;
+      sstep = 4u;
+    }
+  }
+  // Loads [FROM, TO) of stage s; the last one of a stage is the scales'.
+  template <int FROM, int TO>
+  __device__ __forceinline__ void load(uint8_t* stage, uint32_t s) const {
+    const uint32_t wave = wave_id(), k0 = s * kBlkK;
+    const bool ok = k0 + kcol < len;
+#pragma unroll
+    for (int j = FROM; j < TO; ++j) {
+      if (j == T::kLoads) {
+        dma_x1(ds, lds_offset(stage) + T::kData + 256u * wave, vs, s * sstep);
+        continue;
+      }
+      const uint32_t run = (uint32_t)T::kWavesT * j + wave;  // 1 KB runs of the stage
+      constexpr uint32_t kRunsP = T::kP / 8;
+      // every run of one load belongs to one operand: kP / 8 is a multiple of kWaves
+      const bool p = (uint32_t)T::kWavesT * j < kRunsP;
+      const uint32_t i = (p ? run : run - kRunsP) >> 2;  // 32-slot run of the operand
+      const uint32_t row = (i >> 2) * 128u + (i & 3u);
+      const uint32_t v = ok ? (p ? vbase_p : vbase_q) + k0 : kOobOffset;
+      dma_x4(p ? dp : dq, lds_offset(stage) + 1024u * run, v, row * (p ? ldp : ldq));
+    }
+  }
+};
+
+#define MXGG_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// acc[p][q] of the wave: P fragment p = 4 G + i holds rows 64 G + 4 m + i of the wave's
+// part (m = 0..15), Q fragment q rows 4 m + q; D[4g + r][c] is in register r of lane
+// c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i are 16 in a row for every G.
+template <int WP, int GP, int WQ, bool ROWS>
+__device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand& P,
+                                               const BlockOperand& Q, uint32_t len,
+                                               v4f (&acc)[4 * GP][4]) {
+  using T = BlockTile<WP, GP, WQ, ROWS>;
+#pragma unroll
+  for (int p = 0; p < 4 * GP; ++p)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[p][q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  len = uniform(len);
+  if (len == 0) return;
+  const uint32_t nst = (len + kBlkK - 1) / kBlkK;
+  BlockStream<T, ROWS> st;
+  st.init(P, Q, len);
+  uint8_t* slot[2] = {ring, ring + T::kStage};
+  st.template load<0, T::kLoads + 1>(slot[0], 0);
+  if (nst > 1) {
+    st.template load<0, T::kLoads + 1>(slot[1], 1);
+    wait_barrier<T::kLoads + 1>();
+  } else {
+    wait_barrier<0>();
+  }
+  MXGG_FENCE();
+
+  const uint32_t lane = threadIdx.x & 63u, wave = wave_id();
+  const uint32_t wp = wave % WP, wq = wave / WP;
+  const uint32_t m = lane & 15u, g = lane >> 4;
+  // 64-row part u of an operand: slots 128 (u / 2) + 16 (u % 2) + 32 i + m, i = 0..3
+  const auto part = [&](uint32_t u) { return (128u * (u >> 1) + 16u * (u & 1u) + m) * kBlkK; };
+  const uint32_t lo = (g ^ swz(m)) << 4, hi = ((g + 4u) ^ swz(m)) << 4;
+  uint32_t pa[GP];
+#pragma unroll
+  for (int G = 0; G < GP; ++G) pa[G] = part(wp * GP + G);
+  const uint32_t qa = T::kP * kBlkK + part(wq);
+  const uint32_t sq_at = T::kData + 4u * (64u * wq + 4u * m);  // Q rows 4 m .. + 3: fragments 0..3
+  const uint32_t sp_at = T::kData + 4u * T::kQ + 256u * wp * GP;
+  const auto read_p = [&](const uint8_t* s, int p) __attribute__((always_inline)) {
+    const uint8_t* at = s + pa[p >> 2] + 4096u * (p & 3);
+    return lds_v8i(at + lo, at + hi);
+  };
+  const auto read_q = [&](const uint8_t* s, int q) __attribute__((always_inline)) {
+    const uint8_t* at = s + qa + 4096u * q;
+    return lds_v8i(at + lo, at + hi);
+  };
+  // ROWS: the four scales of fragment p's rows; else the scale of the wave's 128 (or 64) rows
+  const auto read_sp = [&](const uint8_t* s, int p) __attribute__((always_inline)) {
+    if constexpr (ROWS)
+      return *reinterpret_cast<const float4*>(s + sp_at + 256u * (p >> 2) + 64u * g + 16u * (p & 3));
+    else
+      return make_float4(*reinterpret_cast<const float*>(s + sp_at), 0.0f, 0.0f, 0.0f);
+  };
+
+  v8i fa[2], fb[4];
+  float4 spn[2], sqn;   // scales of the fragments ahead, and of the stage ahead
+  float sc[4];          // of the stage: Q's scale (times P's)
+  v4f t[4];             // products in flight
+  float4 spt[4];
+  float sct[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) fb[q] = read_q(slot[0], q);
+  fa[0] = read_p(slot[0], 0);
+  spn[0] = read_sp(slot[0], 0);
+  sqn = *reinterpret_cast<const float4*>(slot[0] + sq_at);
+  const auto add = [&](v4f& a, const v4f& x, const float4& sp, float f) __attribute__((always_inline)) {
+    if constexpr (ROWS) {
+      a[0] = __builtin_fmaf(x[0], sp.x * f, a[0]);
+      a[1] = __builtin_fmaf(x[1], sp.y * f, a[1]);
+      a[2] = __builtin_fmaf(x[2], sp.z * f, a[2]);
+      a[3] = __builtin_fmaf(x[3], sp.w * f, a[3]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) a[r] = __builtin_fmaf(x[r], f, a[r]);
+    }
+  };
+  constexpr int kF = 4 * GP, kN = 4 * kF, kLag = 2;
+  for (uint32_t s = 0; s < nst; ++s) {
+    uint8_t* cur = slot[s & 1u];
+    uint8_t* nxt = slot[(s & 1u) ^ 1u];
+    sc[0] = sqn.x;
+    sc[1] = sqn.y;
+    sc[2] = sqn.z;
+    sc[3] = sqn.w;
+    if constexpr (!ROWS) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sc[q] *= spn[0].x;
+    }
+#pragma unroll
+    for (int n = 0; n < kN + kLag; ++n) {
+      const int p = n / 4, q = n % 4;
+      if (n < kN) {
+        if (q == 0) {
+          if (p == kF - 1) {
+            // the next stage has landed, every wave has read this one
+            wait_barrier<0>();
+            MXGG_FENCE();
+            if (s + 2 < nst) st.template load<0, T::kLoads + 1>(cur, s + 2);
+          }
+          const uint8_t* from = p == kF - 1 ? nxt : cur;
+          const int pn = p == kF - 1 ? 0 : p + 1;
+          fa[(p + 1) & 1] = read_p(from, pn);
+          if (ROWS || p == kF - 1) spn[(p + 1) & 1] = read_sp(from, pn);
+          if (p == kF - 1) sqn = *reinterpret_cast<const float4*>(nxt + sq_at);
+        }
+        t[n & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fa[p & 1], fb[q], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+        if (p == kF - 1) fb[q] = read_q(nxt, q);
+        sct[n & 3] = sc[q];
+        if (ROWS) spt[n & 3] = spn[p & 1];
+      }
+      if (n >= kLag) {
+        const int o = n - kLag;
+        add(acc[o / 4][o % 4], t[o & 3], spt[o & 3], sct[o & 3]);
+      }
+      MXGG_FENCE();
+    }
+  }
+  // the slots take the next tile's loads only after every wave's last reads
+  release_barrier();
+}
+
+// The wave's part of a tile to rows of `out` (row = Q row, contiguous along P).
+template <int GP, typename O>
+__device__ __forceinline__ void block_store(const v4f (&acc)[4 * GP][4], O* out, int64_t ldo,
+                                            int64_t p0, int64_t pn, int64_t q0, int64_t qn) {
+  const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t row = q0 + 4 * c + q;
+    if (row >= qn) continue;
+#pragma unroll
+    for (int G = 0; G < GP; ++G) {
+      const int64_t n = p0 + 64 * G + 16 * g;
+      O* o = out + row * ldo + n;
+      // element 4 r + i of the lane's 16
+      const auto at = [&](int e) { return acc[4 * G + (e & 3)][q][e >> 2]; };
+      if (n + 16 <= pn) {
+        if constexpr (sizeof(O) == 4) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float f[4] = {at(e), at(e + 1), at(e + 2), at(e + 3)};
+            __builtin_memcpy(o + e, f, 16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            const uint32_t w[4] = {pack_bf16x2(at(e), at(e + 1)), pack_bf16x2(at(e + 2), at(e + 3)),
+                                   pack_bf16x2(at(e + 4), at(e + 5)),
+                                   pack_bf16x2(at(e + 6), at(e + 7))};
+            __builtin_memcpy(o + e, w, 16);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (n + e < pn) {
+            if constexpr (sizeof(O) == 4) o[e] = at(e);
+            else o[e] = (uint16_t)pack_bf16x2(at(e), 0.0f);
+          }
+      }
+    }
+  }
+}
+
+// Tile of this workgroup: tiles of group g are ceil(size / q) * np, in group order;
+// consecutive workgroups go to the XCDs in turn, and each XCD takes a run of tiles.
+// g = E for a workgroup past the last tile.
+struct GroupTile {
+  int g;
+  int64_t begin, end, tile;
+};
+__device__ __forceinline__ GroupTile find_group(const int32_t* ends_s, int E, int q, int64_t np) {
+  const int lane = threadIdx.x & 63;
+  const auto tiles = [&](int g) {
+    return g < E ? (int64_t)((ends_s[g] - (g > 0 ? ends_s[g - 1] : 0) + q - 1) / q) * np : 0;
+  };
+  int64_t total = 0;
+  for (int g = lane; g < E; g += 64) total += tiles(g);
+  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+  const int64_t per = (total + 7) >> 3, t = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || t >= total) return {E, 0, 0, 0};
+  int64_t before = 0;
+  for (int g0 = 0; g0 < E; g0 += 64) {
+    const int64_t own = tiles(g0 + lane);
+    int64_t sum = own;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const uint64_t hit = __ballot(before + sum > t);
+    if (hit) {
+      const int at = __builtin_ctzll(hit), g = g0 + at;
+      const int64_t first = before + __shfl(sum - own, at);
+      return {(int)uniform((uint32_t)g), uniform((int64_t)(g > 0 ? ends_s[g - 1] : 0)),
+              uniform((int64_t)ends_s[g]), uniform(t - first)};
+    }
+    before += __shfl(sum, 63);
+  }
+  return {E, 0, 0, 0};
+}
+
+// Tiles of a group in bands of up to four along Q, the band's tiles of one P column
+// side by side, so that workgroups in flight on one XCD share operands in its L2.
+__device__ __forceinline__ void band(int64_t tile, int64_t nq, int64_t np, int64_t& tq, int64_t& tp) {
+  const int64_t per = 4 * np, b = tile / per, r = tile % per;
+  const int64_t h = min((int64_t)4, nq - 4 * b);
+  tq = 4 * b + r % h;
+  tp = r / h;
+}
+// The same order of tiles where their number is that of the grid.
+__device__ __forceinline__ int64_t xcd_tile() {
+  const int64_t per = gridDim.x >> 3;
+  return (int64_t)(blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+}
+
+template <int WP, int GP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
+  using T = BlockTile<WP, GP, WQ, false>;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * T::kStage];
+  __shared__ int32_t ends_s[1024];
+  const int64_t np = (a.N + T::kP - 1) / T::kP;
+  GroupTile at{0, 0, a.M, xcd_tile()};
+  if (a.ends) {
+    monotone_ends_to_lds(a.ends, a.E, a.M, ends_s);
+    at = find_group(ends_s, a.E, T::kQ, np);
+  }
+  const int64_t nq = (at.end - at.begin + T::kQ - 1) / T::kQ;
+  if (at.g >= a.E || at.tile >= nq * np) return;
+  int64_t tq, tp;
+  band(at.tile, nq, np, tq, tp);
+  const int64_t m0 = at.begin + tq * T::kQ, n0 = tp * T::kP;
+  const BlockOperand P{a.w + at.g * a.w_group + n0 * a.ldw, a.ws + at.g * a.ws_group + n0 / kBlkK * a.ldws,
+                       a.ldw, a.ldws, a.N - n0};
+  const BlockOperand Q{a.a + m0 * a.lda, a.as + m0, a.lda, a.ldas, a.M - m0};
+  v4f acc[4 * GP][4];
+  block_mainloop<WP, GP, WQ, false>(ring, P, Q, (uint32_t)a.K, acc);
+  const uint32_t wave = wave_id();
+  const int64_t p0 = n0 + 64 * GP * (wave % WP), q0 = m0 + 64 * (wave / WP);
+  if (a.out_f32)
+    block_store<GP>(acc, static_cast<float*>(a.out), a.ldo, p0, a.N, q0, at.end);
+  else
+    block_store<GP>(acc, static_cast<uint16_t*>(a.out), a.ldo, p0, a.N, q0, at.end);
+}
+
+template <int WP, int GP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ) void k_block_wgrad(BlockWgradArgs a) {
+  using T = BlockTile<WP, GP, WQ, true>;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * T::kStage];
+  __shared__ int32_t ends_s[1024];
+  const int64_t np = (a.K + T::kP - 1) / T::kP, nq = (a.N + T::kQ - 1) / T::kQ;
+  const int64_t tile = xcd_tile();
+  const int64_t g = tile / (np * nq);
+  if (g >= a.E) return;
+  int64_t t0 = 0, t1 = a.tokens;
+  if (a.ends) {
+    monotone_ends_to_lds(a.ends, a.E, a.tokens, ends_s);
+    // whole blocks: the casts' padded ends are multiples of 128, others are rounded down
+    t0 = (g > 0 ? ends_s[g - 1] : 0) & ~(kBlkK - 1);
+    t1 = ends_s[g] & ~(kBlkK - 1);
+  }
+  int64_t tq, tp;
+  band(tile % (np * nq), nq, np, tq, tp);
+  const int64_t k0 = tp * T::kP, n0 = tq * T::kQ;
+  const int64_t b0 = t0 / kBlkK;
+  const BlockOperand P{a.ia + k0 * a.ldia + t0, a.ias + b0 * a.ldias + k0, a.ldia, a.ldias, a.K - k0};
+  const BlockOperand Q{a.go + n0 * a.ldgo + t0, a.gos + b0 * a.ldgos + n0, a.ldgo, a.ldgos, a.N - n0};
+  v4f acc[4 * GP][4];
+  block_mainloop<WP, GP, WQ, true>(ring, P, Q, (uint32_t)(t1 > t0 ? t1 - t0 : 0), acc);
+  const uint32_t wave = wave_id();
+  const int64_t p0 = k0 + 64 * GP * (wave % WP), q0 = n0 + 64 * (wave / WP);
+  if (a.out_f32)
+    block_store<GP>(acc, static_cast<float*>(a.dw) + g * a.N * a.K, a.K, p0, a.K, q0, a.N);
+  else
+    block_store<GP>(acc, static_cast<uint16_t*>(a.dw) + g * a.N * a.K, a.K, p0, a.K, q0, a.N);
+}
+
+// Few rows: a workgroup takes 16 rows of W and all of its group's rows of A, 16 QF at
+// a time; its eight waves take blocks of the contraction in turn, straight from memory
+// into registers (W is read once and by nobody else), and their sums are added in wave
+// order.  Bound by W's bytes.
+constexpr int kFewWaves = 8;
+template <int QF>
+__global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
+  constexpr int kAhead = QF == 1 ? 8 : QF == 2 ? 4 : 2;  // blocks in flight
+  __shared__ v4f sums[kFewWaves][QF][64];
+  __shared__ int32_t ends_s[1024];
+  const int64_t np = (a.N + 15) / 16;
+  const int64_t g = blockIdx.x / np, n0 = (blockIdx.x % np) * 16;
+  int64_t begin = 0, end = a.M;
+  if (a.ends) {
+    monotone_ends_to_lds(a.ends, a.E, a.M, ends_s);
+    begin = g > 0 ? ends_s[g - 1] : 0;
+    end = ends_s[g];
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, gr = lane >> 4;
+  const uint8_t* w = a.w + g * a.w_group + min(n0 + c, (int64_t)a.N - 1) * a.ldw + 16 * gr;
+  const float* ws = a.ws + g * a.ws_group + n0 / kBlkK * a.ldws;
+  const int nb = (a.K + kBlkK - 1) / kBlkK;
+  const auto chunk = [&](const uint8_t* p, int k) {
+    return k < a.K ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  };
+  for (int64_t m0 = begin; m0 < end; m0 += 16 * QF) {
+    v4f acc[QF];
+#pragma unroll
+    for (int q = 0; q < QF; ++q) acc[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint8_t* x[QF];
+    const float* xs[QF];
+#pragma unroll
+    for (int q = 0; q < QF; ++q) {  // rows past the end repeat the last one; not stored
+      const int64_t row = min(m0 + 16 * q + c, end - 1);
+      x[q] = a.a + row * a.lda + 16 * gr;
+      xs[q] = a.as + row;
+    }
+    for (int b0 = wave; b0 < nb; b0 += kFewWaves * kAhead) {
+      uint4 wl[kAhead], wh[kAhead], xl[kAhead][QF], xh[kAhead][QF];
+      float sw[kAhead], sx[kAhead][QF];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int b = b0 + u * kFewWaves, k = b * kBlkK;
+        const bool on = b < nb;
+        wl[u] = on ? chunk(w + k, k + 16 * gr) : make_uint4(0, 0, 0, 0);
+        wh[u] = on ? chunk(w + k + 64, k + 16 * gr + 64) : make_uint4(0, 0, 0, 0);
+        sw[u] = on ? ws[b] : 0.0f;
+#pragma unroll
+        for (int q = 0; q < QF; ++q) {
+          xl[u][q] = on ? chunk(x[q] + k, k + 16 * gr) : make_uint4(0, 0, 0, 0);
+          xh[u][q] = on ? chunk(x[q] + k + 64, k + 16 * gr + 64) : make_uint4(0, 0, 0, 0);
+          sx[u][q] = on ? xs[q][b * a.ldas] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const v8i fw = {(int)wl[u].x, (int)wl[u].y, (int)wl[u].z, (int)wl[u].w,
+                        (int)wh[u].x, (int)wh[u].y, (int)wh[u].z, (int)wh[u].w};
+#pragma unroll
+        for (int q = 0; q < QF; ++q) {
+          const v8i fx = {(int)xl[u][q].x, (int)xl[u][q].y, (int)xl[u][q].z, (int)xl[u][q].w,
+                          (int)xh[u][q].x, (int)xh[u][q].y, (int)xh[u][q].z, (int)xh[u][q].w};
+          const v4f t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              fw, fx, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+          const float f = sw[u] * sx[u][q];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[q][r] = __builtin_fmaf(t[r], f, acc[q][r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < QF; ++q) sums[wave][q][lane] = acc[q];
+    __syncthreads();
+    if (wave < QF) {
+      v4f s = sums[0][wave][lane];
+#pragma unroll
+      for (int u = 1; u < kFewWaves; ++u) s += sums[u][wave][lane];
+      const int64_t row = m0 + 16 * wave + c, n = n0 + 4 * gr;
+      if (row < end) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < a.N) {
+            if (a.out_f32) static_cast<float*>(a.out)[row * a.ldo + n + r] = s[r];
+            else static_cast<uint16_t*>(a.out)[row * a.ldo + n + r] = (uint16_t)pack_bf16x2(s[r], 0.0f);
+          }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Workgroups of a run of tiles: a multiple of 8, for xcd_tile().
+dim3 tile_grid(int64_t tiles) { return dim3((unsigned)((tiles + 7) / 8 * 8)); }
+
+}  // namespace
+
+hipError_t launch_block_mm(const BlockMmArgs& a, hipStream_t stream) {
+  if (a.M == 0 || a.N == 0) return hipSuccess;
+  const int64_t per = (a.M + a.E - 1) / a.E;
+  if (per <= 64) {
+    const dim3 grid((unsigned)((a.N + 15) / 16 * a.E));
+    if (per <= 16)
+      hipLaunchKernelGGL((k_block_few<1>), grid, dim3(64 * kFewWaves), 0, stream, a);
+    else if (per <= 32)
+      hipLaunchKernelGGL((k_block_few<2>), grid, dim3(64 * kFewWaves), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_block_few<4>), grid, dim3(64 * kFewWaves), 0, stream, a);
+    return hipGetLastError();
+  }
+  const auto tiles = [&](int64_t p, int64_t q) {
+    return ((a.M + q - 1) / q + (a.ends ? a.E : 0)) * ((a.N + p - 1) / p);
+  };
+  if (tiles(256, 256) >= device_cu_count())
+    hipLaunchKernelGGL((k_block_fwd<2, 2, 4>), tile_grid(tiles(256, 256)), dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_block_fwd<2, 1, 2>), tile_grid(tiles(128, 128)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_block_wgrad(const BlockWgradArgs& a, hipStream_t stream) {
+  if (a.N == 0 || a.K == 0 || a.E == 0) return hipSuccess;
+  const auto tiles = [&](int64_t p, int64_t q) {
+    return (int64_t)a.E * ((a.K + p - 1) / p) * ((a.N + q - 1) / q);
+  };
+  if (tiles(256, 256) >= device_cu_count())
+    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4>), tile_grid(tiles(256, 256)), dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_block_wgrad<2, 1, 2>), tile_grid(tiles(128, 128)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace mxgg

@@ -5,6 +5,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <vector>
@@ -24,6 +25,11 @@ constexpr int64_t kMaxRowStride = INT64_C(1) << 23;
 // Kernels with one wave per row and four rows per 256-thread workgroup: the
 // grid holds at most 2^32 - 1 work-items.
 constexpr int64_t kMaxWaveRows = 4 * ((INT64_C(1) << 24) - 1);
+
+// Block-scaled products and casts: a tile's 256 rows stay within 2^31 bytes, grids below
+// 2^32 work-items (512 a workgroup).
+constexpr int64_t kMaxBlockWidth = INT64_C(1) << 22;
+constexpr int64_t kMaxBlockGrid = INT64_C(1) << 22;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 }  // namespace
@@ -1344,6 +1350,181 @@ int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const 
                                        static_cast<uint16_t*>(grad_weight),
                                        static_cast<uint8_t*>(workspace),
                                        static_cast<hipStream_t>(stream)), what);
+}
+
+// Shape and x of a cast to blocks of 128.
+static int check_block_cast(const char* what, const void* x, int64_t rows, int64_t cols,
+                            int64_t ldx) {
+  if (rows < 0 || cols < 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: negative size rows=%lld cols=%lld", what,
+                     (long long)rows, (long long)cols);
+  if (cols % 16 != 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: width %lld is not a multiple of 16", what,
+                     (long long)cols);
+  if (rows > INT32_MAX || cols > kMaxBlockWidth)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: rows above 2^31 or width above 2^22", what);
+  if ((rows + 31) / 32 * ((cols + 511) / 512) >= kMaxBlockGrid)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: %lld x %lld elements", what, (long long)rows,
+                     (long long)cols);
+  if (rows == 0 || cols == 0) return MXGG_OK;
+  if (!x) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (ldx < cols)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (!aligned16(x) || ldx % 8 != 0)
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: x must have 16-byte aligned rows", what);
+  return MXGG_OK;
+}
+
+static int check_block_rows(const char* what, const void* q, int64_t ldq, const float* scales,
+                            int64_t lds, int64_t rows, int64_t cols) {
+  if (!q || !scales) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (ldq < cols || lds < rows)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (reinterpret_cast<uintptr_t>(q) % 8 != 0 || ldq % 8 != 0)
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: q must have 8-byte aligned rows", what);
+  return MXGG_OK;
+}
+
+int mxgg_block_quant_dim0(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q,
+                          int64_t ldq, float* scales, int64_t lds, void* stream) {
+  const char* what = "block_quant_dim0";
+  int rc = check_block_cast(what, x, rows, cols, ldx);
+  if (rc != MXGG_OK || rows == 0 || cols == 0) return rc;
+  rc = check_block_rows(what, q, ldq, scales, lds, rows, cols);
+  if (rc != MXGG_OK) return rc;
+  return check_launch(
+      launch_block_rows(static_cast<const uint16_t*>(x), rows, cols, ldx, static_cast<uint8_t*>(q),
+                        ldq, scales, lds, static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_block_quant_dim1(const void* x, int64_t rows, int64_t cols, int64_t ldx,
+                          const int32_t* group_ends, int64_t num_groups, int64_t rows_pad_cap,
+                          void* q, int64_t ldq, float* scales, int64_t lds, void* qt, float* st,
+                          int64_t ldst, int32_t* group_ends_pad, void* stream) {
+  const char* what = "block_quant_dim1";
+  int rc = check_block_cast(what, x, rows, cols, ldx);
+  if (rc != MXGG_OK) return rc;
+  if (group_ends ? num_groups < 1 || num_groups > kMaxGroupsAbi : num_groups != 0)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: num_groups=%lld (1 to 1024 with group_ends, else 0)",
+                     what, (long long)num_groups);
+  const int64_t need = group_ends ? rows + 127 * num_groups : rows;
+  if (rows_pad_cap % 128 != 0 || rows_pad_cap < need / 128 * 128 || rows_pad_cap < rows)
+    return set_error(MXGG_ERR_SHAPE, "%s: rows_pad_cap=%lld for %lld rows in %lld groups", what,
+                     (long long)rows_pad_cap, (long long)rows, (long long)num_groups);
+  if (rows_pad_cap / 128 > 65535)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: rows_pad_cap=%lld", what, (long long)rows_pad_cap);
+  if (group_ends && !group_ends_pad)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (cols > 0 && rows_pad_cap > 0) {
+    if (!qt || !st) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+    if (ldst < cols)
+      return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+    if (!aligned16(qt)) return set_error(MXGG_ERR_ALIGNMENT, "%s: qt 16-byte aligned", what);
+    if (q && rows > 0) {
+      rc = check_block_rows(what, q, ldq, scales, lds, rows, cols);
+      if (rc != MXGG_OK) return rc;
+    }
+  }
+  return check_launch(
+      launch_block_tokens(static_cast<const uint16_t*>(x), rows, cols, ldx, group_ends, num_groups,
+                          rows_pad_cap, static_cast<uint8_t*>(q), ldq, scales, lds,
+                          static_cast<uint8_t*>(qt), st, ldst, group_ends_pad,
+                          static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_block_quant_weight(const void* w, int64_t num_groups, int64_t N, int64_t K, void* q,
+                            float* scales, void* qt, float* st, void* stream) {
+  const char* what = "block_quant_weight";
+  const int rc = check_block_cast(what, w, N, K, K);
+  if (rc != MXGG_OK) return rc;
+  if (num_groups < 0 || num_groups > kMaxGroupsAbi || N / 128 > 65534)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: num_groups=%lld, N=%lld", what,
+                     (long long)num_groups, (long long)N);
+  if (num_groups == 0 || N == 0 || K == 0) return MXGG_OK;
+  if (!q || !scales || (qt && !st))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!aligned16(q) || !aligned16(qt))
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: q and qt 16-byte aligned", what);
+  return check_launch(
+      launch_block_weight(static_cast<const uint16_t*>(w), num_groups, N, K,
+                          static_cast<uint8_t*>(q), scales, static_cast<uint8_t*>(qt), st,
+                          static_cast<hipStream_t>(stream)), what);
+}
+
+// Rows of an e4m3 operand of the block-scaled products.
+static bool block_rows_aligned(const void* p, int64_t ld) { return aligned16(p) && ld % 16 == 0; }
+
+int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t ldas, const void* w,
+                  int64_t w_gstride, int64_t ldw, const float* w_scales, int64_t ws_gstride,
+                  int64_t ldws, const int32_t* group_ends, int64_t num_groups, int64_t M,
+                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* stream) {
+  const char* what = "block_mm";
+  if (out_type != MXGG_OUT_BF16 && out_type != MXGG_OUT_F32)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown out_type %d", what, out_type);
+  if (M < 0 || N < 0 || K < 1 || K % 16 != 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: M=%lld, N=%lld, K=%lld (a positive multiple of 16)", what,
+                     (long long)M, (long long)N, (long long)K);
+  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!group_ends && num_groups != 1))
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: num_groups=%lld (1 to 1024; 1 without group_ends)",
+                     what, (long long)num_groups);
+  if (M > INT32_MAX || N > kMaxBlockWidth || K > kMaxBlockWidth ||
+      ((M + 127) / 128 + num_groups) * ((N + 127) / 128) >= kMaxBlockGrid ||
+      num_groups * ((N + 15) / 16) >= kMaxBlockGrid)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: M=%lld, N=%lld, K=%lld in %lld groups", what,
+                     (long long)M, (long long)N, (long long)K, (long long)num_groups);
+  if (M == 0 || N == 0) return MXGG_OK;
+  if (!a || !a_scales || !w || !w_scales || !out)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const int64_t blocks = (K + 127) / 128;
+  if (lda < K || ldw < K || ldas < M || ldws < blocks || ldo < N ||
+      (num_groups > 1 && (w_gstride < (N - 1) * ldw + K || ws_gstride < 0)))
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (lda > kMaxBlockWidth || ldw > kMaxBlockWidth || blocks * ldas > kMaxBufferBytes / 4 ||
+      (N / 128 + 1) * ldws > kMaxBufferBytes / 4)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: lda=%lld, ldw=%lld, ldas=%lld, ldws=%lld", what,
+                     (long long)lda, (long long)ldw, (long long)ldas, (long long)ldws);
+  if (!block_rows_aligned(a, lda) || !block_rows_aligned(w, ldw) || w_gstride % 16 != 0)
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: a and w must have 16-byte aligned rows", what);
+  const BlockMmArgs g{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w),
+                      w_scales, group_ends, out, lda, ldas, w_gstride, ldw, ws_gstride, ldws, ldo, M,
+                      (int32_t)N, (int32_t)K, (int32_t)num_groups, out_type == MXGG_OUT_F32};
+  return check_launch(launch_block_mm(g, static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_block_wgrad(const void* go_t, int64_t ldgo, const float* go_scales, int64_t ldgos,
+                     const void* ia_t, int64_t ldia, const float* ia_scales, int64_t ldias,
+                     const int32_t* group_ends_pad, int64_t num_groups, int64_t tokens, int64_t N,
+                     int64_t K, void* dw, int out_type, void* stream) {
+  const char* what = "block_wgrad";
+  if (out_type != MXGG_OUT_BF16 && out_type != MXGG_OUT_F32)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown out_type %d", what, out_type);
+  if (tokens < 0 || tokens % 128 != 0 || N < 0 || K < 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld (a multiple of 128), N=%lld, K=%lld", what,
+                     (long long)tokens, (long long)N, (long long)K);
+  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!group_ends_pad && num_groups != 1))
+    return set_error(MXGG_ERR_UNSUPPORTED,
+                     "%s: num_groups=%lld (1 to 1024; 1 without group_ends_pad)", what,
+                     (long long)num_groups);
+  if (tokens > kMaxBlockWidth || N > kMaxBlockWidth || K > kMaxBlockWidth || ldgo > kMaxBlockWidth ||
+      ldia > kMaxBlockWidth ||
+      num_groups * ((N + 127) / 128) * ((K + 127) / 128) >= kMaxBlockGrid)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: tokens=%lld, N=%lld, K=%lld in %lld groups", what,
+                     (long long)tokens, (long long)N, (long long)K, (long long)num_groups);
+  if (N == 0 || K == 0) return MXGG_OK;
+  if (!dw || (tokens > 0 && (!go_t || !go_scales || !ia_t || !ia_scales)))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (tokens > 0 && (ldgo < tokens || ldia < tokens || ldgos < N || ldias < K))
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (tokens / 128 * std::max(ldgos, ldias) > kMaxBufferBytes / 4)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: ldgos=%lld, ldias=%lld", what, (long long)ldgos,
+                     (long long)ldias);
+  if (tokens > 0 && (!block_rows_aligned(go_t, ldgo) || !block_rows_aligned(ia_t, ldia)))
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: operands must have 16-byte aligned rows", what);
+  const BlockWgradArgs g{static_cast<const uint8_t*>(go_t), go_scales,
+                         static_cast<const uint8_t*>(ia_t), ia_scales, group_ends_pad, dw, ldgo,
+                         ldgos, ldia, ldias, tokens, (int32_t)N, (int32_t)K, (int32_t)num_groups,
+                         out_type == MXGG_OUT_F32};
+  return check_launch(launch_block_wgrad(g, static_cast<hipStream_t>(stream)), what);
 }
 
 }  // extern "C"

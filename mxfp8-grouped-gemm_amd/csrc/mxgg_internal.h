@@ -210,6 +210,43 @@ int64_t loss_grad_workspace_bytes(const LossArgs& args, bool need_x, bool need_w
 hipError_t launch_loss_grad(LossArgs args, uint16_t* dx, uint16_t* dw, uint8_t* ws,
                             hipStream_t stream);
 
+// e4m3 with one fp32 scale for each block of 128 (block_cast.hip): rows in blocks of
+// 1 x 128 (s: [ceil(cols / 128)][lds]); tokens in blocks of 128 x 1, transposed to
+// [cols][cap] (st: [cap / 128][ldst]), groups padded to whole blocks, with q and s also by
+// rows unless q is null; weights in tiles of 128 x 128, qt and st transposed or null.
+hipError_t launch_block_rows(const uint16_t* x, int64_t rows, int64_t cols, int64_t ldx,
+                             uint8_t* q, int64_t ldq, float* s, int64_t lds, hipStream_t stream);
+hipError_t launch_block_tokens(const uint16_t* x, int64_t rows, int64_t cols, int64_t ldx,
+                               const int32_t* ends, int64_t E, int64_t cap, uint8_t* q,
+                               int64_t ldq, float* s, int64_t lds, uint8_t* qt, float* st,
+                               int64_t ldst, int32_t* pend, hipStream_t stream);
+hipError_t launch_block_weight(const uint16_t* w, int64_t E, int64_t N, int64_t K, uint8_t* q,
+                               float* s, uint8_t* qt, float* st, hipStream_t stream);
+
+// Their products (block_gemm.hip).
+struct BlockMmArgs {
+  const uint8_t* a;      // [M][lda]
+  const float* as;       // [ceil(K / 128)][ldas]
+  const uint8_t* w;      // [E][N][ldw], w_group bytes a group
+  const float* ws;       // [E][ceil(N / 128)][ldws], ws_group floats a group
+  const int32_t* ends;   // or nullptr: one group of M rows
+  void* out;             // [M][ldo]
+  int64_t lda, ldas, w_group, ldw, ws_group, ldws, ldo, M;
+  int32_t N, K, E, out_f32;
+};
+hipError_t launch_block_mm(const BlockMmArgs& args, hipStream_t stream);
+struct BlockWgradArgs {
+  const uint8_t* go;     // dY^T [N][ldgo]
+  const float* gos;      // [tokens / 128][ldgos]
+  const uint8_t* ia;     // X^T [K][ldia]
+  const float* ias;      // [tokens / 128][ldias]
+  const int32_t* ends;   // padded, or nullptr
+  void* dw;              // [E][N][K]
+  int64_t ldgo, ldgos, ldia, ldias, tokens;
+  int32_t N, K, E, out_f32;
+};
+hipError_t launch_block_wgrad(const BlockWgradArgs& args, hipStream_t stream);
+
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,
                                int32_t* ends, hipStream_t stream);

@@ -53,6 +53,15 @@ from .routing import (
     route_plan,
     route_topk,
 )
+from .block import (
+    FP8BlockLinear,
+    fp8_block_linear,
+    fp8_block_mm,
+    fp8_block_wgrad,
+    to_fp8_block_dim0,
+    to_fp8_block_dim1,
+    to_fp8_block_weight,
+)
 from .loss import LinearCrossEntropy, linear_cross_entropy
 from .optim import AdamW, adamw_state, adamw_step
 from .norm import Norm, layer_norm, rms_norm
@@ -79,5 +88,7 @@ __all__ = [
     "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
     "combine_score_grad", "Norm", "layer_norm", "rms_norm",
+    "to_fp8_block_dim0", "to_fp8_block_dim1", "to_fp8_block_weight", "fp8_block_mm", "fp8_block_wgrad",
+    "fp8_block_linear", "FP8BlockLinear",
     "LinearCrossEntropy", "linear_cross_entropy", "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",
 ]

@@ -46,7 +46,7 @@ OFFS_ENDS = 0
 OFFS_SIZES = 1
 OFFS_AUTO = 2
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 MAX_GROUPS = 1024  # groups of one call
 
 _P = ctypes.c_void_p
@@ -186,6 +186,19 @@ SIGNATURES = {
     "mxgg_linear_cross_entropy_grad_workspace_bytes": (_I64, [_P, _I, _I]),
     "mxgg_linear_cross_entropy_grad": (
         _I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P],
+    ),
+    "mxgg_block_quant_dim0": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "mxgg_block_quant_dim1": (
+        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P],
+    ),
+    "mxgg_block_quant_weight": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "mxgg_block_mm": (
+        _I,
+        [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64,
+         _I, _P],
+    ),
+    "mxgg_block_wgrad": (
+        _I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I, _P],
     ),
     "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
     "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
