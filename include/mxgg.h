@@ -768,6 +768,69 @@ int mxgg_block_wgrad(const void* go_t, int64_t ldgo, const float* go_scales, int
                      const int32_t* group_ends_pad, int64_t num_groups, int64_t tokens, int64_t N,
                      int64_t K, void* dw, int out_type, void* stream);
 
+/*
+ * Root-mean-square norm with the residual's addition:
+ *   h = x + residual (rounded to x's type),  y = h / sqrt(mean(h^2) + eps) * weight
+ * options as mxgg_norm's (center and bias_dtype unused); x, residual, h and y are of its
+ * dtype, rows of any alignment.  stats: fp32 [2, rows] for the gradient (its second half
+ * is written), or NULL.  h and y may not overlap the inputs.
+ */
+int mxgg_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres,
+                      const void* weight, const mxgg_norm_options* options, void* h, int64_t ldh,
+                      void* y, int64_t ldy, float* stats, void* stream);
+
+/*
+ * Its gradients: grad_x (also the residual's) = grad_h + d y / d h applied to grad_y, from
+ * the h and stats of the forward pass; grad_weight of the weight's type.  Either may be
+ * NULL.  workspace: mxgg_norm_grad_workspace_bytes(options), for grad_weight.
+ */
+int mxgg_add_rms_norm_grad(const void* grad_y, int64_t ldg, const void* grad_h, int64_t ldgh,
+                           const void* h, int64_t ldh, const void* weight, const float* stats,
+                           const mxgg_norm_options* options, void* grad_x, int64_t ldgx,
+                           void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
+/*
+ * The same norm (residual and h NULL: of x itself) with its result in e4m3, rounded once
+ * from fp32:
+ *   MXGG_QUANT_MX     one E8M0 byte for each 32 (rule scale_mode), cols % 32 == 0; byte of
+ *                     row m and block b at scales[b * lds + m]
+ *   MXGG_QUANT_BLOCK  one fp32 scale for each 128, max(amax / 448, 2^-126), cols % 16 == 0;
+ *                     scale of row m and block b at ((float*)scales)[b * lds + m]
+ * that is the block-major layout of the row-wise casts.  q: 8-byte aligned rows.
+ */
+typedef enum mxgg_quant_format { MXGG_QUANT_MX = 0, MXGG_QUANT_BLOCK = 1 } mxgg_quant_format;
+
+int mxgg_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldres,
+                        const void* weight, const mxgg_norm_options* options, void* h, int64_t ldh,
+                        void* q, int64_t ldq, void* scales, int64_t lds, int format,
+                        int scale_mode, void* stream);
+
+/*
+ * Global norm of many gradients, sqrt(sum of g^2) in fp64, written to *norm (fp32, on the
+ * device), and clipping in place: g *= min(1, max_norm / (norm + eps)).  A norm that is NaN
+ * makes every gradient NaN; an infinite one makes finite gradients 0.  Tensors are fp32 or
+ * bf16 of any element alignment and must not overlap.  `tensors` is host memory, read during
+ * the call.  workspace: mxgg_grad_norm_workspace_bytes(tensors, count), 8-byte aligned, no
+ * initialisation.  Two kernel launches for every 190 tensors.
+ */
+typedef struct mxgg_grad_tensor {
+  void* data;
+  int64_t n;
+  int32_t dtype;
+} mxgg_grad_tensor;
+
+typedef struct mxgg_clip_options {
+  double max_norm, eps; /* not negative */
+} mxgg_clip_options;
+
+int64_t mxgg_grad_norm_workspace_bytes(const mxgg_grad_tensor* tensors, int64_t count);
+int mxgg_grad_norm(const mxgg_grad_tensor* tensors, int64_t count, float* norm, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int mxgg_clip_grad_norm(const mxgg_grad_tensor* tensors, int64_t count,
+                        const mxgg_clip_options* options, float* norm, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1130,31 +1130,35 @@ int64_t mxgg_norm_grad_workspace_bytes(const mxgg_norm_options* options) {
                                              options->dtype == MXGG_OUT_BF16);
 }
 
-int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
-                   const void* weight, const float* stats, const mxgg_norm_options* options,
-                   void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
-                   void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = check_norm("norm_grad", options);
+// add: a term of grad_x (the residual stream's gradient), or null.
+static int norm_grad(const char* what, const void* grad_y, int64_t ldg, const void* add,
+                     int64_t ldadd, const void* x, int64_t ldx, const void* weight,
+                     const float* stats, const mxgg_norm_options* options, void* grad_x,
+                     int64_t ldgx, void* grad_weight, void* grad_bias, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  const int rc = check_norm(what, options);
   if (rc != MXGG_OK) return rc;
   const mxgg_norm_options& o = *options;
   const bool sums = grad_weight || grad_bias;
   if (o.rows > 0 && (!grad_y || !x || !stats))
-    return set_error(MXGG_ERR_INVALID_ARGUMENT, "norm_grad: null pointer");
-  if (o.rows > 0 && (ldx < o.cols || ldg < o.cols || (grad_x && ldgx < o.cols)))
-    return set_error(MXGG_ERR_SHAPE, "norm_grad: leading dimension smaller than the row");
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (o.rows > 0 && (ldx < o.cols || ldg < o.cols || (grad_x && ldgx < o.cols) || (add && ldadd < o.cols)))
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
   const int64_t need = mxgg_norm_grad_workspace_bytes(options);
   if (sums && workspace_bytes < need)
-    return set_error(MXGG_ERR_SHAPE, "norm_grad: workspace of %lld bytes, %lld needed",
+    return set_error(MXGG_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", what,
                      (long long)workspace_bytes, (long long)need);
   if (sums && need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
     return set_error(workspace ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
-                     "norm_grad: the workspace must be a 4-byte aligned device buffer");
+                     "%s: the workspace must be a 4-byte aligned device buffer", what);
   NormGradArgs a{};
   a.dy = grad_y;
   a.x = x;
   a.w = weight;
   a.stats = stats;
   a.dx = grad_x;
+  a.add = add;
+  a.ldadd = ldadd;
   a.dw = grad_weight;
   a.db = grad_bias;
   a.partial = sums ? static_cast<float*>(workspace) : nullptr;
@@ -1167,7 +1171,161 @@ int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
   a.w_bf16 = o.weight_dtype == MXGG_OUT_BF16;
   a.b_bf16 = o.bias_dtype == MXGG_OUT_BF16;
   a.center = o.center != 0;
-  return check_launch(launch_norm_bwd(a, static_cast<hipStream_t>(stream)), "norm_grad");
+  return check_launch(launch_norm_bwd(a, static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_norm_grad(const void* grad_y, int64_t ldg, const void* x, int64_t ldx,
+                   const void* weight, const float* stats, const mxgg_norm_options* options,
+                   void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+  return norm_grad("norm_grad", grad_y, ldg, nullptr, 0, x, ldx, weight, stats, options, grad_x,
+                   ldgx, grad_weight, grad_bias, workspace, workspace_bytes, stream);
+}
+
+int mxgg_add_rms_norm_grad(const void* grad_y, int64_t ldg, const void* grad_h, int64_t ldgh,
+                           const void* h, int64_t ldh, const void* weight, const float* stats,
+                           const mxgg_norm_options* options, void* grad_x, int64_t ldgx,
+                           void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+  if (options && options->center)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "add_rms_norm_grad: center is not supported");
+  return norm_grad("add_rms_norm_grad", grad_y, ldg, grad_h, ldgh, h, ldh, weight, stats, options,
+                   grad_x, ldgx, grad_weight, nullptr, workspace, workspace_bytes, stream);
+}
+
+// The inputs of a norm with the residual's addition; fills what the outputs share.
+static int check_add_norm(const char* what, const void* x, int64_t ldx, const void* res,
+                          int64_t ldres, const void* weight, const mxgg_norm_options* options,
+                          void* h, int64_t ldh, AddNormArgs& a) {
+  const int rc = check_norm(what, options);
+  if (rc != MXGG_OK) return rc;
+  const mxgg_norm_options& o = *options;
+  if (o.center) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: center is not supported", what);
+  if (o.rows > 0 && (!x || (res != nullptr) != (h != nullptr)))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (o.rows > 0 && (ldx < o.cols || (res && (ldres < o.cols || ldh < o.cols))))
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  a.x = x;
+  a.res = res;
+  a.w = weight;
+  a.h = h;
+  a.rows = o.rows;
+  a.ldx = ldx;
+  a.ldres = ldres;
+  a.ldh = ldh;
+  a.cols = (int32_t)o.cols;
+  a.bf16 = o.dtype == MXGG_OUT_BF16;
+  a.w_bf16 = o.weight_dtype == MXGG_OUT_BF16;
+  a.eps = o.eps;
+  return MXGG_OK;
+}
+
+int mxgg_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres,
+                      const void* weight, const mxgg_norm_options* options, void* h, int64_t ldh,
+                      void* y, int64_t ldy, float* stats, void* stream) {
+  const char* what = "add_rms_norm";
+  AddNormArgs a{};
+  const int rc = check_add_norm(what, x, ldx, residual, ldres, weight, options, h, ldh, a);
+  if (rc != MXGG_OK || a.rows == 0) return rc;
+  if (!y || !residual) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (ldy < a.cols)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  a.y = y;
+  a.ldy = ldy;
+  a.stats = stats;
+  return check_launch(launch_add_norm(a, static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldres,
+                        const void* weight, const mxgg_norm_options* options, void* h, int64_t ldh,
+                        void* q, int64_t ldq, void* scales, int64_t lds, int format,
+                        int scale_mode, void* stream) {
+  const char* what = "rms_norm_quant";
+  AddNormArgs a{};
+  const int rc = check_add_norm(what, x, ldx, residual, ldres, weight, options, h, ldh, a);
+  if (rc != MXGG_OK) return rc;
+  if (format != MXGG_QUANT_MX && format != MXGG_QUANT_BLOCK)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown format %d", what, format);
+  if (scale_mode != MXGG_SCALE_RCEIL && scale_mode != MXGG_SCALE_FLOOR)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown scale_mode %d", what, scale_mode);
+  if (a.cols % (format == MXGG_QUANT_MX ? 32 : 16) != 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: cols=%d is not a multiple of %d", what, a.cols,
+                     format == MXGG_QUANT_MX ? 32 : 16);
+  if (a.rows == 0) return MXGG_OK;
+  if (!q || !scales) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (ldq < a.cols || lds < a.rows)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (reinterpret_cast<uintptr_t>(q) % 8 != 0 || ldq % 8 != 0)
+    return set_error(MXGG_ERR_ALIGNMENT, "%s: q must have 8-byte aligned rows", what);
+  a.q = static_cast<uint8_t*>(q);
+  a.scales = scales;
+  a.ldq = ldq;
+  a.lds = lds;
+  a.mx = format == MXGG_QUANT_MX;
+  a.mode = scale_mode;
+  return check_launch(launch_add_norm(a, static_cast<hipStream_t>(stream)), what);
+}
+
+static int check_grads(const char* what, const mxgg_grad_tensor* tensors, int64_t count) {
+  if (count > 0 && !tensors)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (count < 0 || count > (INT64_C(1) << 24))
+    return set_error(MXGG_ERR_SHAPE, "%s: count=%lld", what, (long long)count);
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const mxgg_grad_tensor& t = tensors[i];
+    if (t.dtype != MXGG_OUT_BF16 && t.dtype != MXGG_OUT_F32)
+      return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: tensor %lld: type %d", what, (long long)i,
+                       t.dtype);
+    if (t.n < 0 || t.n > (INT64_C(1) << 48) || (total += t.n) > (INT64_C(1) << 48))
+      return set_error(MXGG_ERR_SHAPE, "%s: tensor %lld: n=%lld", what, (long long)i,
+                       (long long)t.n);
+    if (t.n > 0 && !t.data)
+      return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: tensor %lld: null pointer", what,
+                       (long long)i);
+    if (reinterpret_cast<uintptr_t>(t.data) % (t.dtype == MXGG_OUT_BF16 ? 2 : 4) != 0)
+      return set_error(MXGG_ERR_ALIGNMENT, "%s: tensor %lld", what, (long long)i);
+  }
+  return MXGG_OK;
+}
+
+int64_t mxgg_grad_norm_workspace_bytes(const mxgg_grad_tensor* tensors, int64_t count) {
+  if (check_grads("grad_norm_workspace_bytes", tensors, count) != MXGG_OK) return -1;
+  return 8 * clip_parts(tensors, count);
+}
+
+// options null: the norm alone.
+static int grad_clip(const char* what, const mxgg_grad_tensor* tensors, int64_t count,
+                     const mxgg_clip_options* options, float* norm, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  const int rc = check_grads(what, tensors, count);
+  if (rc != MXGG_OK) return rc;
+  if (!norm) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (options && !(options->max_norm >= 0 && options->eps >= 0))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: max_norm=%g, eps=%g", what,
+                     options->max_norm, options->eps);
+  const int64_t need = 8 * clip_parts(tensors, count);
+  if (workspace_bytes < need)
+    return set_error(MXGG_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", what,
+                     (long long)workspace_bytes, (long long)need);
+  if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
+    return set_error(workspace ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
+                     "%s: the workspace must be an 8-byte aligned device buffer", what);
+  return check_launch(launch_clip(tensors, count, options, static_cast<double*>(workspace), norm,
+                                  static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_grad_norm(const mxgg_grad_tensor* tensors, int64_t count, float* norm, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  return grad_clip("grad_norm", tensors, count, nullptr, norm, workspace, workspace_bytes, stream);
+}
+
+int mxgg_clip_grad_norm(const mxgg_grad_tensor* tensors, int64_t count,
+                        const mxgg_clip_options* options, float* norm, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (!options) return set_error(MXGG_ERR_INVALID_ARGUMENT, "clip_grad_norm: null options");
+  return grad_clip("clip_grad_norm", tensors, count, options, norm, workspace, workspace_bytes,
+                   stream);
 }
 
 int mxgg_adamw_step(const mxgg_adamw_tensor* tensors, int64_t count,

@@ -154,6 +154,22 @@ struct NormArgs {
   float eps;
 };
 hipError_t launch_norm_fwd(const NormArgs& args, hipStream_t stream);
+// Root-mean-square norm of h = x + residual (or of x), its result in x's type or in 8 bits.
+struct AddNormArgs {
+  const void* x;    // [rows], row stride ldx, fp32 or bf16
+  const void* res;  // or nullptr; of x's type
+  const void* w;    // [cols] or nullptr
+  void* h;          // of x's type; with res only
+  void* y;          // of x's type; or nullptr, and then
+  uint8_t* q;       // e4m3 [rows][ldq]
+  void* scales;     // [block][lds]: E8M0 bytes of 32 (mx), or fp32 of 128
+  float* stats;     // [2][rows] or nullptr: as NormArgs (the second half is written)
+  int64_t rows, ldx, ldres, ldh, ldy, ldq, lds;
+  int32_t cols, bf16, w_bf16, mx, mode;
+  float eps;
+  int32_t run;      // set by the launcher: consecutive rows of a workgroup
+};
+hipError_t launch_add_norm(AddNormArgs args, hipStream_t stream);
 struct NormGradArgs {
   const void* dy;
   const void* x;
@@ -163,7 +179,8 @@ struct NormGradArgs {
   void* dw;        // [cols] or nullptr, of the weight's type
   void* db;
   float* partial;  // [2][norm_grad_parts()][cols], needed for dw or db
-  int64_t rows, lddy, ldx, lddx;
+  const void* add; // [rows] of x's type, added to dx (root-mean-square norm only), or nullptr
+  int64_t rows, lddy, ldx, lddx, ldadd;
   int32_t cols, bf16, w_bf16, b_bf16, center;
 };
 hipError_t launch_norm_bwd(const NormGradArgs& args, hipStream_t stream);
@@ -246,6 +263,12 @@ struct BlockWgradArgs {
   int32_t N, K, E, out_f32;
 };
 hipError_t launch_block_wgrad(const BlockWgradArgs& args, hipStream_t stream);
+
+// Global gradient norm and clipping (clip.hip); part: clip_parts() doubles.
+int64_t clip_parts(const mxgg_grad_tensor* tensors, int64_t count);
+hipError_t launch_clip(const mxgg_grad_tensor* tensors, int64_t count,
+                       const mxgg_clip_options* options, double* part, float* norm,
+                       hipStream_t stream);  // options null: the norm alone
 
 // Group-offset utilities (groups.hip).
 hipError_t launch_offs_to_ends(const int32_t* offs, int64_t E, int64_t tokens, int kind,

@@ -238,13 +238,200 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
   }
 }
 
-template <typename T, int CH, bool CENTER, bool WAVE>
+// Outputs of the norm with the residual's addition.
+enum { kOutSame, kOutMx, kOutBlock };
+constexpr int kScaleRun = 16;  // rows whose scales leave together
+
+// Largest |o| bit pattern of the lanes that hold one block of 32 (MX) or 128 elements.
+template <int OUT, int E>
+__device__ __forceinline__ uint32_t block_amax(uint32_t m) {
+  m = quad_max(m);
+  if (OUT == kOutMx && E == 8) return m;
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, false));  // 8 lanes
+  if (OUT == kOutMx) return m;
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xF, 0xF, false));  // 16
+  if (E == 8) return m;
+  const auto p = __builtin_amdgcn_permlane16_swap(m, m, false, false);             // 32
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+
+// E8M0 byte of a block of fp32 values from the bit pattern of the largest, by the
+// rules of the bf16 casts (e8m0_from_amax16).
+__device__ __forceinline__ uint32_t e8m0_from_amax32(uint32_t amax, int mode) {
+  const int ex = (int)(amax >> 23);
+  const uint32_t mant = amax & 0x7FFFFFu;
+  const int b = ex - 8 + (mode == kModeRceil && mant > 0x600000u ? 1 : 0);
+  if (ex == 255) return mant ? 255u : (mode == kModeRceil ? 254u : 247u);
+  return (uint32_t)(b < 0 ? 0 : b);
+}
+
+// E payload bytes of o under the block's E8M0 byte.
+template <int E>
+__device__ __forceinline__ void mx_payload(const float* o, uint32_t b, int mode, uint32_t* w) {
+#pragma unroll
+  for (int k = 0; k < E / 4; ++k) {
+    const float *f = o + 4 * k;
+    if (mode == kModeRceil)
+      w[k] = __any(b >= 254u) ? encode4_any<kModeRceil, false>(f[0], f[1], f[2], f[3], b)
+                              : encode4_finite<kModeRceil, false>(f[0], f[1], f[2], f[3], b);
+    else
+      w[k] = __any(b == 255u) ? encode4_any<kModeFloor, false>(f[0], f[1], f[2], f[3], b)
+                              : encode4_finite<kModeFloor, false>(f[0], f[1], f[2], f[3], b);
+  }
+}
+
+// Root-mean-square norm of h = x + residual (ADD; rounded to T, as it is kept) or of x.
+//   kOutSame  : y in T, rows dealt out as in k_norm_fwd
+//   kOutMx    : e4m3 and an E8M0 byte for each 32, rounded once from fp32
+//   kOutBlock : e4m3 and an fp32 scale for each 128: max(amax / 448, 2^-126)
+// Scales are laid out block by block, rows next to each other, so the 8-bit outputs
+// are computed for `run` consecutive rows a workgroup, their scales gathered in LDS
+// and written as one run for each block (a byte at a time they would be a memory
+// transaction each: 224 a row of 7168).
+template <typename T, int CH, bool WAVE, int OUT, bool ADD>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add_norm(AddNormArgs a) {
+  constexpr int E = Elems<T>::kCount;
+  constexpr bool kQuant = OUT != kOutSame;
+  constexpr int kMaxBlocks = (WAVE ? 1024 : 32768) / (OUT == kOutMx ? 32 : 128);
+  constexpr int kScaleBytes = kQuant ? kMaxBlocks * kScaleRun * (OUT == kOutMx ? 1 : 4) : 16;
+  __shared__ float slots[2][1][kNormMaxThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint8_t held[kScaleBytes];
+  const T* x = static_cast<const T*>(a.x);
+  const T* res = static_cast<const T*>(a.res);
+  T* h = static_cast<T*>(a.h);
+  T* y = static_cast<T*>(a.y);
+  const RowPlace<WAVE> at_row;
+  const int lane_row = WAVE ? (int)(threadIdx.x >> 6) : 0, rows_at_once = WAVE ? kWaveRows : 1;
+  int n[CH];
+  float w[CH * E];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int at = (at_row.thread + c * at_row.threads) * E;
+    n[c] = min(max(a.cols - at, 0), E);
+#pragma unroll
+    for (int j = 0; j < E; ++j) w[c * E + j] = 1.0f;
+    if (a.w) load_params<E>(a.w, a.w_bf16, at, a.cols, w + c * E);
+  }
+  const float cols = (float)a.cols;
+  uint4 nx[CH], nr[CH];
+  const auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int64_t at = (int64_t)(at_row.thread + c * at_row.threads) * E;
+      nx[c] = load_chunk<false>(x + row * a.ldx + at, n[c]);
+      if (ADD) nr[c] = load_chunk<false>(res + row * a.ldres + at, n[c]);
+    }
+  };
+  const int run = kQuant ? a.run : rows_at_once;
+  int parity = 0;
+  fetch((int64_t)blockIdx.x * run + lane_row);
+  for (int64_t base = (int64_t)blockIdx.x * run; base < a.rows; base += (int64_t)gridDim.x * run) {
+    for (int i = lane_row; i < run; i += rows_at_once) {
+      const int64_t row = base + i;
+      if (row >= a.rows) break;
+      float v[CH * E];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          v[c * E + j] = Elems<T>::get(nx[c], j);
+          if (ADD) v[c * E + j] += Elems<T>::get(nr[c], j);
+        }
+        if (ADD) {
+          const uint4 kept = Elems<T>::pack(v + c * E);
+          store_chunk<T>(h + row * a.ldh + (int64_t)(at_row.thread + c * at_row.threads) * E,
+                         v + c * E, n[c]);
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[c * E + j] = Elems<T>::get(kept, j);
+        }
+      }
+      fetch(i + rows_at_once < run ? row + rows_at_once
+                                   : base + (int64_t)gridDim.x * run + lane_row);
+      float s[1] = {0.0f};
+#pragma unroll
+      for (int k = 0; k < CH * E; ++k) s[0] = __builtin_fmaf(v[k], v[k], s[0]);
+      row_sum<WAVE, 1>(s, slots[parity]);
+      parity ^= 1;
+      const float r = 1.0f / sqrtf(s[0] / cols + a.eps);
+      if (a.stats && at_row.thread == 0) a.stats[a.rows + row] = r;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int chunk = at_row.thread + c * at_row.threads;
+        float o[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] = v[c * E + j] * r * w[c * E + j];
+        if constexpr (!kQuant) {
+          store_chunk<T>(y + row * a.ldy + (int64_t)chunk * E, o, n[c]);
+        } else {
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            m = max(m, j < n[c] ? __float_as_uint(o[j]) & 0x7FFFFFFFu : 0u);
+          m = block_amax<OUT, E>(m);
+          uint32_t p[E / 4];
+          constexpr int kLanes = (OUT == kOutMx ? 32 : 128) / E;
+          const bool first = chunk % kLanes == 0 && n[c] > 0;
+          if constexpr (OUT == kOutMx) {
+            const uint32_t b = e8m0_from_amax32(m, a.mode);
+            mx_payload<E>(o, b, a.mode, p);
+            if (first) held[chunk / kLanes * kScaleRun + i] = (uint8_t)b;
+          } else {
+            float sc = __uint_as_float(m) / 448.0f;
+            sc = sc < 0x1p-126f ? 0x1p-126f : sc;
+            const float f = 1.0f / sc;
+#pragma unroll
+            for (int k = 0; k < E / 4; ++k) {
+              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(o[4 * k] * f, o[4 * k + 1] * f, 0, false);
+              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(o[4 * k + 2] * f, o[4 * k + 3] * f,
+                                                               (int)p[k], true);
+            }
+            if (first) reinterpret_cast<float*>(held)[chunk / kLanes * kScaleRun + i] = sc;
+          }
+          if (n[c] > 0) {  // whole chunks: the width is a multiple of 16
+            uint8_t* q = a.q + row * a.ldq + (int64_t)chunk * E;
+            if constexpr (E == 8) store_stream(q, make_uint2(p[0], p[1]));
+            else __builtin_nontemporal_store(p[0], reinterpret_cast<uint32_t*>(q));
+          }
+        }
+      }
+    }
+    if constexpr (kQuant) {
+      __syncthreads();
+      constexpr int kWidth = OUT == kOutMx ? 32 : 128, kSize = OUT == kOutMx ? 1 : 4;
+      const int blocks = (a.cols + kWidth - 1) / kWidth;
+      const int rows = (int)min((int64_t)run, a.rows - base);
+      uint8_t* out = static_cast<uint8_t*>(a.scales) + base * kSize;
+      if (rows == kScaleRun) {
+        constexpr int kParts = kScaleRun * kSize / 16;  // 16-byte pieces of a block's scales
+        for (int k = threadIdx.x; k < blocks * kParts; k += blockDim.x) {
+          const uint4 v = *reinterpret_cast<const uint4*>(held + 16 * k);
+          __builtin_memcpy(out + (int64_t)(k / kParts) * a.lds * kSize + 16 * (k % kParts), &v, 16);
+        }
+      } else {
+        for (int k = threadIdx.x; k < blocks * kScaleRun; k += blockDim.x) {
+          const int b = k / kScaleRun, i = k % kScaleRun;
+          if (i >= rows) continue;
+          if constexpr (OUT == kOutMx)
+            out[(int64_t)b * a.lds + i] = held[k];
+          else
+            reinterpret_cast<float*>(out)[(int64_t)b * a.lds + i] = reinterpret_cast<float*>(held)[k];
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ADD (root-mean-square norm, no bias): a.add is added to dx.
+template <typename T, int CH, bool CENTER, bool WAVE, bool ADD>
 __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_norm_bwd(NormGradArgs a) {
   constexpr int E = Elems<T>::kCount;
   __shared__ float slots[2][2][kNormMaxThreads / 64];
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   T* dx = static_cast<T*>(a.dx);
+  const T* add = static_cast<const T*>(a.add);
   const RowPlace<WAVE> at_row;
   int n[CH];
   float w[CH * E], dw[CH * E], db[CH * E];
@@ -272,12 +459,15 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
   for (int parity = 0; row < a.rows; row += at_row.step, parity ^= 1) {
     const float mu = CENTER ? a.stats[row] : 0.0f, r = a.stats[a.rows + row];
     // the chunks stay packed; xhat and dy w are formed again after the sums
-    uint4 cx[CH], cg[CH];
+    uint4 cx[CH], cg[CH], ca[CH];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       cx[c] = nx[c];
       cg[c] = ng[c];
+      // of this row, not ahead as the others: there are no registers for both
+      if (ADD) ca[c] = load_chunk<true>(
+          add + row * a.ldadd + (int64_t)(at_row.thread + c * at_row.threads) * E, n[c]);
     }
     const int64_t after = row + at_row.step;
     if (after < a.rows) {
@@ -296,7 +486,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
         // past the end of the row dy is 0, so xhat's value there does not matter
         const float h = (Elems<T>::get(cx[c], j) - mu) * r, g = Elems<T>::get(cg[c], j);
         dw[i] = __builtin_fmaf(g, h, dw[i]);
-        db[i] += g;
+        if (!ADD) db[i] += g;
         const float u = g * w[i];
         s[0] = __builtin_fmaf(u, h, s[0]);
         s[1] += u;
@@ -311,6 +501,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
       for (int j = 0; j < E; ++j) {
         const float h = (Elems<T>::get(cx[c], j) - mu) * r;
         o[j] = r * (Elems<T>::get(cg[c], j) * w[c * E + j] - mg - h * mh);
+        if (ADD) o[j] += Elems<T>::get(ca[c], j);
       }
       store_chunk<T>(dx + row * a.lddx + (int64_t)(at_row.thread + c * at_row.threads) * E, o, n[c]);
     }
@@ -322,7 +513,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
   if constexpr (WAVE) {  // the waves' sums first, in wave order
     __shared__ float part[kWaveRows][64 * CH * E];
     for (int k = 0; k < 2; ++k) {
-      if (k ? !a.db : !a.dw) continue;
+      if (k ? ADD || !a.db : !a.dw) continue;
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < CH * E; ++i)
@@ -344,7 +535,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_nor
     for (int j = 0; j < E; ++j)
       if (j < n[c]) {
         if (a.dw) pw[at + j] = dw[c * E + j];
-        if (a.db) pb[at + j] = db[c * E + j];
+        if (!ADD && a.db) pb[at + j] = db[c * E + j];
       }
   }
 }
@@ -421,7 +612,10 @@ void run_norm(const NormArgs& a, int grid, int threads, hipStream_t stream) {
 }
 template <typename T, bool CENTER, int CH, bool WAVE>
 void run_norm(const NormGradArgs& a, int grid, int threads, hipStream_t stream) {
-  hipLaunchKernelGGL((k_norm_bwd<T, CH, CENTER, WAVE>), dim3(grid), dim3(threads), 0, stream, a);
+  if (!CENTER && a.add)
+    hipLaunchKernelGGL((k_norm_bwd<T, CH, false, WAVE, true>), dim3(grid), dim3(threads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_norm_bwd<T, CH, CENTER, WAVE, false>), dim3(grid), dim3(threads), 0, stream, a);
 }
 // Chunks reached: one wave 1, 2 (bf16: 1024 = 2 * 64 * 8) and 4 (fp32); workgroups
 // 4, 8 (bf16: 32768 = 8 * 512 * 8) and 16 (fp32).
@@ -458,7 +652,44 @@ int norm_grid(int64_t rows, const NormShape& s) {
   return (int)std::min<int64_t>(own, std::max(1, device_cu_count()) * per_cu);
 }
 
+template <typename T, int CH, bool WAVE>
+void run_add_norm(const AddNormArgs& a, int grid, int threads, hipStream_t stream) {
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, stream, a);
+  };
+  if (!a.q) go(k_add_norm<T, CH, WAVE, kOutSame, true>);
+  else if (a.mx) a.res ? go(k_add_norm<T, CH, WAVE, kOutMx, true>) : go(k_add_norm<T, CH, WAVE, kOutMx, false>);
+  else a.res ? go(k_add_norm<T, CH, WAVE, kOutBlock, true>) : go(k_add_norm<T, CH, WAVE, kOutBlock, false>);
+}
+template <typename T>
+void run_add_shape(const AddNormArgs& a, int grid, const NormShape& s, hipStream_t stream) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  if (s.wave) {
+    if (s.ch == 1) run_add_norm<T, 1, true>(a, grid, s.threads, stream);
+    else if (!kF32 || s.ch == 2) run_add_norm<T, 2, true>(a, grid, s.threads, stream);
+    else if constexpr (kF32) run_add_norm<T, 4, true>(a, grid, s.threads, stream);
+  } else {
+    if (s.ch == 4) run_add_norm<T, 4, false>(a, grid, s.threads, stream);
+    else if (!kF32 || s.ch == 8) run_add_norm<T, 8, false>(a, grid, s.threads, stream);
+    else if constexpr (kF32) run_add_norm<T, 16, false>(a, grid, s.threads, stream);
+  }
+}
+
 }  // namespace
+
+hipError_t launch_add_norm(AddNormArgs a, hipStream_t stream) {
+  if (a.rows == 0) return hipSuccess;
+  const NormShape s = norm_shape(a.cols, a.bf16 ? 8 : 4);
+  int grid = norm_grid(a.rows, s);
+  if (a.q) {  // runs of up to 16 rows, as long as every workgroup has one
+    const int64_t unit = s.wave ? kWaveRows : 1, own = (a.rows + unit * grid - 1) / (unit * grid);
+    a.run = (int32_t)(unit * std::min<int64_t>(own, kScaleRun / unit));
+    grid = (int)std::min<int64_t>(grid, (a.rows + a.run - 1) / a.run);
+  }
+  if (a.bf16) run_add_shape<uint16_t>(a, grid, s, stream);
+  else run_add_shape<float>(a, grid, s, stream);
+  return hipGetLastError();
+}
 
 hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;

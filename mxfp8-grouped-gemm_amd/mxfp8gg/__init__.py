@@ -63,8 +63,8 @@ from .block import (
     to_fp8_block_weight,
 )
 from .loss import LinearCrossEntropy, linear_cross_entropy
-from .optim import AdamW, adamw_state, adamw_step
-from .norm import Norm, layer_norm, rms_norm
+from .optim import AdamW, adamw_state, adamw_step, clip_grad_norm_, grad_norm
+from .norm import AddRMSNorm, Norm, add_rms_norm, layer_norm, rms_norm, rms_norm_quant
 from .torchao_compat import (
     apply,
     triton_mxfp8_grouped_mm,
@@ -87,7 +87,8 @@ __all__ = [
     "MXFP8GroupedMM", "mxfp8_grouped_mm", "MXFP8ExpertFFN", "moe_ffn", "moe_ffn_unfused",
     "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
-    "combine_score_grad", "Norm", "layer_norm", "rms_norm",
+    "combine_score_grad", "Norm", "layer_norm", "rms_norm", "add_rms_norm", "AddRMSNorm", "rms_norm_quant",
+    "grad_norm", "clip_grad_norm_",
     "to_fp8_block_dim0", "to_fp8_block_dim1", "to_fp8_block_weight", "fp8_block_mm", "fp8_block_wgrad",
     "fp8_block_linear", "FP8BlockLinear",
     "LinearCrossEntropy", "linear_cross_entropy", "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",

@@ -35,6 +35,9 @@ OUT_F32 = 1
 SCALES_ROW_MAJOR = 0
 SCALES_BLOCK_MAJOR = 1
 
+QUANT_MX = 0
+QUANT_BLOCK = 1
+
 REDUCE_NONE = 0
 REDUCE_SUM = 1
 REDUCE_MEAN = 2
@@ -75,6 +78,18 @@ class AdamwOptions(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + \
                [("step", _I64), ("state_bits", ctypes.c_int32)]
+
+
+class GradTensor(ctypes.Structure):
+    """mxgg_grad_tensor."""
+
+    _fields_ = [("data", _P), ("n", _I64), ("dtype", ctypes.c_int32)]
+
+
+class ClipOptions(ctypes.Structure):
+    """mxgg_clip_options."""
+
+    _fields_ = [(n, ctypes.c_double) for n in ("max_norm", "eps")]
 
 
 class LossOptions(ctypes.Structure):
@@ -200,6 +215,16 @@ SIGNATURES = {
     "mxgg_block_wgrad": (
         _I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I, _P],
     ),
+    "mxgg_add_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P]),
+    "mxgg_add_rms_norm_grad": (
+        _I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _P],
+    ),
+    "mxgg_rms_norm_quant": (
+        _I, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _I, _I, _P],
+    ),
+    "mxgg_grad_norm_workspace_bytes": (_I64, [_P, _I64]),
+    "mxgg_grad_norm": (_I, [_P, _I64, _P, _P, _I64, _P]),
+    "mxgg_clip_grad_norm": (_I, [_P, _I64, _P, _P, _P, _I64, _P]),
     "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
     "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
     "mxgg_norm_grad": (

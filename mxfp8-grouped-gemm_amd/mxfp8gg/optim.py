@@ -1,7 +1,8 @@
-"""AdamW over many tensors at once, with states in 32 or in 8 bits.
+"""AdamW over many tensors at once, with states in 32 or in 8 bits, and the clipping of
+their gradients' global norm.
 
     opt = AdamW(model.parameters(), lr=1e-3, state_bits=8)
-    loss.backward(); opt.step()
+    loss.backward(); opt.clip_grad_norm_(1.0); opt.step()
 
 One kernel launch updates up to 48 tensors (weights and gradients bf16 or fp32).
 8-bit states are MXFP8 as the rest of this package uses it: e4m3 payloads with
@@ -20,7 +21,7 @@ import torch
 from . import _lib
 from .ops import _FP8, _native, _need_gpu, _stream_ptr, _tensors, _took
 
-__all__ = ["AdamW", "adamw_step", "adamw_state"]
+__all__ = ["AdamW", "adamw_step", "adamw_state", "grad_norm", "clip_grad_norm_"]
 
 _TYPES = {torch.float32: _lib.OUT_F32, torch.bfloat16: _lib.OUT_BF16}
 
@@ -113,6 +114,76 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: int, lr: float = 1e-3,
     torch.autograd.graph.increment_version([*params, *exp_avg, *exp_avg_sq, *ms, *vs, *masters])
 
 
+def _own_memory(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one stretch of memory, each once, in any order of its
+    dimensions."""
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _grad_table(grads):
+    """The tensors and their table for the library."""
+    if isinstance(grads, torch.Tensor):
+        grads = [grads]
+    grads = list(grads)
+    table = (_lib.GradTensor * max(len(grads), 1))()
+    seen = set()
+    for i, g in enumerate(grads):
+        _need_gpu(g, f"grads[{i}]")
+        if g.device != grads[0].device:
+            raise ValueError(f"grads[{i}] is on {g.device}, grads[0] on {grads[0].device}")
+        if g.layout != torch.strided or g.dtype not in _TYPES:
+            raise TypeError(f"grads[{i}] must be a dense float32 or bfloat16 tensor, got {g.dtype} "
+                            f"({g.layout})")
+        if not _own_memory(g):
+            raise ValueError(f"grads[{i}] must fill its memory without gaps or overlap, got "
+                             f"{tuple(g.shape)} with strides {g.stride()}")
+        if g.numel() and g.data_ptr() in seen:
+            raise ValueError(f"grads[{i}] is in the list twice")
+        seen.add(g.data_ptr())
+        table[i] = _lib.GradTensor(g.data_ptr(), g.numel(), _TYPES[g.dtype])
+    if not grads:
+        raise ValueError("grads is empty")
+    return grads, table
+
+
+def _clip(grads, what, options=None):
+    grads, table = _grad_table(grads)
+    lib, n = _lib.load(), len(grads)
+    dev = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = lib.mxgg_grad_norm_workspace_bytes(table, n)
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
+    rest = (norm.data_ptr(), ws.data_ptr(), nbytes, _stream_ptr(grads[0]))
+    _lib.check(lib.mxgg_grad_norm(table, n, *rest) if options is None else
+               lib.mxgg_clip_grad_norm(table, n, ctypes.byref(options), *rest), what)
+    return grads, norm
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """sqrt(sum of g^2) over all tensors of the list (bf16 or fp32, on one device), fp32 on
+    the device.  Squares and sums are fp64; the same bits on every run."""
+    return _clip(grads, "grad_norm")[1]
+
+
+def clip_grad_norm_(grads, max_norm: float, eps: float = 1e-6) -> torch.Tensor:
+    """Scale the gradients of the list in place by min(1, max_norm / (norm + eps)), norm being
+    grad_norm(grads), which is returned.  Nothing waits for the device, and where nothing is
+    clipped no gradient is written.  A norm that is NaN makes the gradients NaN, an
+    infinite one makes the finite ones 0.  The tensors may be laid out in any order of
+    their dimensions but must not overlap."""
+    max_norm, eps = float(max_norm), float(eps)
+    if not (max_norm >= 0 and eps >= 0):
+        raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
+    grads, norm = _clip(grads, "clip_grad_norm_", _lib.ClipOptions(max_norm, eps))
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) on adamw_step: a torch optimizer with
     parameter groups, learning-rate schedulers and state_dict as torch's own.
@@ -148,6 +219,13 @@ class AdamW(torch.optim.Optimizer):
             if group["master_weights"] and p.dtype != torch.float32:
                 state["master"] = p.detach().to(torch.float32)
         return state
+
+    def clip_grad_norm_(self, max_norm: float) -> torch.Tensor | None:
+        """clip_grad_norm_ over every parameter's gradient, between backward() and step();
+        None where there is no gradient."""
+        grads = [p.grad for group in self.param_groups for p in group["params"]
+                 if p.grad is not None]
+        return clip_grad_norm_(grads, max_norm) if grads else None
 
     @torch.no_grad()
     def step(self, closure=None):
