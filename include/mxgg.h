@@ -831,6 +831,43 @@ int mxgg_clip_grad_norm(const mxgg_grad_tensor* tensors, int64_t count,
                         const mxgg_clip_options* options, float* norm, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/*
+ * Log probabilities of given tokens from logits z [tokens, vocab] (fp32 or bf16, row
+ * stride ldz, any alignment of the element), p = softmax(z / temperature):
+ *   log_probs [tokens]      log p[target]; 0 for a target of ignore_index, NaN for one
+ *                           that is otherwise outside [0, vocab)
+ *   entropy [tokens]        -sum p log p
+ *   top_ids, top_log_probs  [tokens, topk] (topk up to 64): the largest logits in falling
+ *                           order, equal ones by their index; -1 and -inf where fewer
+ *                           than topk logits are above -inf
+ *   stats                   fp32 [3, tokens], for the gradient
+ * all fp32 (ids int32), each but the alternatives NULL if not wanted; target NULL:
+ * without log_probs.  Logits of -inf have no probability; a row of nothing else has
+ * log_probs -inf and entropy 0.  A row with a NaN or +inf is NaN, with ids -1.  Rows whose
+ * target is ignore_index are not read: 0, 0, -1 and -inf.  workspace:
+ * mxgg_token_log_probs_workspace_bytes(options), 16-byte aligned, no initialisation.
+ */
+typedef struct mxgg_log_prob_options {
+  int64_t tokens, vocab, ldz, ignore_index;
+  int32_t dtype, target_int64, topk;
+  float temperature; /* above 0 */
+} mxgg_log_prob_options;
+
+int64_t mxgg_token_log_probs_workspace_bytes(const mxgg_log_prob_options* options);
+int mxgg_token_log_probs(const void* z, const void* target, const mxgg_log_prob_options* options,
+                         float* log_probs, float* entropy, int32_t* top_ids, float* top_log_probs,
+                         float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The gradient of log_probs, entropy and top_log_probs (the choice of alternatives held
+ * fixed) from theirs, each NULL for none: grad_z [tokens, vocab] of z's type, contiguous.
+ * Rows that are ignored or hold nothing but -inf have a gradient of 0.
+ */
+int mxgg_token_log_probs_grad(const float* grad_log_probs, const float* grad_entropy,
+                              const float* grad_top, const void* z, const void* target,
+                              const int32_t* top_ids, const float* stats,
+                              const mxgg_log_prob_options* options, void* grad_z, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -64,6 +64,23 @@ static int check_launch(hipError_t e, const char* what) {
   return MXGG_OK;
 }
 
+// What both passes of the token log probabilities share.
+template <class Args>
+static void log_prob_args(Args& a, const void* z, const void* target,
+                          const mxgg_log_prob_options& o) {
+  a.z = z;
+  a.target = target;
+  a.T = o.tokens;
+  a.V = o.vocab;
+  a.ldz = o.ldz;
+  a.ignore = o.ignore_index;
+  a.inv_t = 1.0f / o.temperature;
+  a.c = (float)(1.4426950408889634 / o.temperature);
+  a.k = o.topk;
+  a.target64 = o.target_int64 != 0;
+  a.bf16 = o.dtype == MXGG_OUT_BF16;
+}
+
 }  // namespace mxgg
 
 using namespace mxgg;
@@ -1508,6 +1525,78 @@ int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const 
                                        static_cast<uint16_t*>(grad_weight),
                                        static_cast<uint8_t*>(workspace),
                                        static_cast<hipStream_t>(stream)), what);
+}
+
+static int check_log_probs(const char* what, const mxgg_log_prob_options* o) {
+  if (!o) return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null options", what);
+  if (o->dtype != MXGG_OUT_BF16 && o->dtype != MXGG_OUT_F32)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", what, o->dtype);
+  if (!(o->temperature > 0 && o->temperature <= 3.0e38f && 1.0f / o->temperature <= 1.0e38f))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: temperature=%g", what, o->temperature);
+  if (o->tokens < 0 || o->vocab < 1 || o->topk < 0 || o->topk > o->vocab)
+    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld, vocab=%lld, topk=%d", what,
+                     (long long)o->tokens, (long long)o->vocab, o->topk);
+  if (o->tokens > 0 && o->ldz < o->vocab)
+    return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
+  if (o->topk > 64) return set_error(MXGG_ERR_UNSUPPORTED, "%s: topk=%d above 64", what, o->topk);
+  if (!logp_fits(o->tokens, o->vocab))
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: tokens=%lld, vocab=%lld", what,
+                     (long long)o->tokens, (long long)o->vocab);
+  return MXGG_OK;
+}
+
+int64_t mxgg_token_log_probs_workspace_bytes(const mxgg_log_prob_options* options) {
+  if (check_log_probs("token_log_probs_workspace_bytes", options) != MXGG_OK) return -1;
+  LogpArgs a{};
+  log_prob_args(a, nullptr, nullptr, *options);
+  return a.T == 0 ? 0 : logp_workspace_bytes(a);
+}
+
+int mxgg_token_log_probs(const void* z, const void* target, const mxgg_log_prob_options* options,
+                         float* log_probs, float* entropy, int32_t* top_ids, float* top_log_probs,
+                         float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "token_log_probs";
+  const int rc = check_log_probs(what, options);
+  if (rc != MXGG_OK || options->tokens == 0) return rc;
+  if (!z || (log_probs && !target) || (options->topk > 0 && (!top_ids || !top_log_probs)))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  LogpArgs a{};
+  log_prob_args(a, z, target, *options);
+  a.log_probs = log_probs;
+  a.entropy = entropy;
+  a.top_ids = top_ids;
+  a.top_lp = top_log_probs;
+  a.stats = stats;
+  const int64_t need = logp_workspace_bytes(a);
+  if (workspace_bytes < need)
+    return set_error(MXGG_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", what,
+                     (long long)workspace_bytes, (long long)need);
+  if (need > 0 && (!workspace || !aligned16(workspace)))
+    return set_error(workspace ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
+                     "%s: the workspace must be a 16-byte aligned device buffer", what);
+  return check_launch(launch_logp(a, static_cast<uint8_t*>(workspace),
+                                  static_cast<hipStream_t>(stream)), what);
+}
+
+int mxgg_token_log_probs_grad(const float* grad_log_probs, const float* grad_entropy,
+                              const float* grad_top, const void* z, const void* target,
+                              const int32_t* top_ids, const float* stats,
+                              const mxgg_log_prob_options* options, void* grad_z, void* stream) {
+  const char* what = "token_log_probs_grad";
+  const int rc = check_log_probs(what, options);
+  if (rc != MXGG_OK || options->tokens == 0) return rc;
+  if (!z || !stats || !grad_z || (grad_log_probs && !target) ||
+      (grad_top && (options->topk == 0 || !top_ids)))
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  LogpGradArgs a{};
+  log_prob_args(a, z, target, *options);
+  a.top_ids = top_ids;
+  a.stats = stats;
+  a.g_lp = grad_log_probs;
+  a.g_ent = grad_entropy;
+  a.g_top = grad_top;
+  a.dz = grad_z;
+  return check_launch(launch_logp_grad(a, static_cast<hipStream_t>(stream)), what);
 }
 
 // Shape and x of a cast to blocks of 128.

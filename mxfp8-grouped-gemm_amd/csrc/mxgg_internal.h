@@ -264,6 +264,42 @@ struct BlockWgradArgs {
 };
 hipError_t launch_block_wgrad(const BlockWgradArgs& args, hipStream_t stream);
 
+// Token log probabilities (logp.hip).  The launchers fill in the last fields.
+struct LogpArgs {
+  const void* z;        // [T] rows of V, row stride ldz, fp32 or bf16
+  const void* target;   // [T] int32 or int64, or nullptr
+  float* log_probs;     // [T] or nullptr
+  float* entropy;       // [T] or nullptr
+  int32_t* top_ids;     // [T][k]
+  float* top_lp;        // [T][k]
+  float* stats;         // [3][T] or nullptr: maxima, log S, entropies
+  int64_t T, V, ldz, ignore;
+  float c, inv_t;       // log2(e) / temperature, 1 / temperature
+  int32_t k, target64, bf16;
+  int64_t part_len, parts;
+  float4* part_sums;    // [T][parts]
+  uint8_t* part_top;    // [T][parts][k]
+};
+int64_t logp_workspace_bytes(const LogpArgs& args);
+hipError_t launch_logp(LogpArgs args, uint8_t* ws, hipStream_t stream);
+struct LogpGradArgs {
+  const void* z;
+  const void* target;
+  const int32_t* top_ids;
+  const float* stats;
+  const float* g_lp;    // [T], or nullptr
+  const float* g_ent;   // [T], or nullptr
+  const float* g_top;   // [T][k], or nullptr
+  void* dz;             // [T][V]
+  int64_t T, V, ldz, ignore;
+  float c, inv_t;
+  int32_t k, target64, bf16;
+  int64_t part_len, parts;
+};
+hipError_t launch_logp_grad(LogpGradArgs args, hipStream_t stream);
+// Whether the grids of such a call stay below 2^32 work-items (vocab up to 2^24).
+bool logp_fits(int64_t tokens, int64_t vocab);
+
 // Global gradient norm and clipping (clip.hip); part: clip_parts() doubles.
 int64_t clip_parts(const mxgg_grad_tensor* tensors, int64_t count);
 hipError_t launch_clip(const mxgg_grad_tensor* tensors, int64_t count,

@@ -63,6 +63,7 @@ from .block import (
     to_fp8_block_weight,
 )
 from .loss import LinearCrossEntropy, linear_cross_entropy
+from .logprob import TokenLogProbs, token_log_probs
 from .optim import AdamW, adamw_state, adamw_step, clip_grad_norm_, grad_norm
 from .norm import AddRMSNorm, Norm, add_rms_norm, layer_norm, rms_norm, rms_norm_quant
 from .torchao_compat import (
@@ -88,7 +89,7 @@ __all__ = [
     "route_topk", "RouteTopK", "RoutePlan", "route_plan", "gather_rows", "gather_to_mxfp8_dual", "gather_to_mxfp8_dim0",
     "combine",
     "combine_score_grad", "Norm", "layer_norm", "rms_norm", "add_rms_norm", "AddRMSNorm", "rms_norm_quant",
-    "grad_norm", "clip_grad_norm_",
+    "grad_norm", "clip_grad_norm_", "token_log_probs", "TokenLogProbs",
     "to_fp8_block_dim0", "to_fp8_block_dim1", "to_fp8_block_weight", "fp8_block_mm", "fp8_block_wgrad",
     "fp8_block_linear", "FP8BlockLinear",
     "LinearCrossEntropy", "linear_cross_entropy", "AdamW", "adamw_state", "adamw_step", "MXFP8RoutedExpertFFN", "moe_routed_ffn",

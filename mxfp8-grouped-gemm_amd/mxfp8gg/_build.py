@@ -21,7 +21,7 @@ HOST_PATH = PKG_DIR / "_mxgg_host.so"
 
 SOURCES = ["capi.hip", "quant.hip", "swiglu.hip", "route.hip", "groups.hip", "gemm.hip", "topk.hip", "norm.hip",
            "adamw.hip", "loss.hip", "block_cast.hip",
-           "block_gemm.hip", "clip.hip"]
+           "block_gemm.hip", "clip.hip", "logp.hip"]
 HEADERS = ["mxgg_internal.h", "mx_device.h", "gemm_tile.h", "gemm_thin.h", "wgrad_ahead.h"]
 
 ARCH = os.environ.get("MXGG_OFFLOAD_ARCH", "gfx950")

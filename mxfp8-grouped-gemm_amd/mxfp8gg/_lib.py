@@ -92,6 +92,14 @@ class ClipOptions(ctypes.Structure):
     _fields_ = [(n, ctypes.c_double) for n in ("max_norm", "eps")]
 
 
+class LogProbOptions(ctypes.Structure):
+    """mxgg_log_prob_options."""
+
+    _fields_ = [(n, _I64) for n in ("tokens", "vocab", "ldz", "ignore_index")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "target_int64", "topk")] + \
+               [("temperature", ctypes.c_float)]
+
+
 class LossOptions(ctypes.Structure):
     """mxgg_loss_options."""
 
@@ -225,6 +233,9 @@ SIGNATURES = {
     "mxgg_grad_norm_workspace_bytes": (_I64, [_P, _I64]),
     "mxgg_grad_norm": (_I, [_P, _I64, _P, _P, _I64, _P]),
     "mxgg_clip_grad_norm": (_I, [_P, _I64, _P, _P, _P, _I64, _P]),
+    "mxgg_token_log_probs_workspace_bytes": (_I64, [_P]),
+    "mxgg_token_log_probs": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "mxgg_token_log_probs_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "mxgg_norm": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _P, _P]),
     "mxgg_norm_grad_workspace_bytes": (_I64, [_P]),
     "mxgg_norm_grad": (
