@@ -223,3 +223,161 @@ def test_grouped_wgrad(gpu, sizes, N, K):
         if n == 0:
             assert not dw[e].any()
         _near(dw[e], a @ b.t(), a.abs() @ b.abs().t(), 1 + n // 128)
+
+
+def _dequant_rows(x):
+    return _wide(*_ref_rows(x))
+
+
+def _dequant_tokens(x):
+    """Values of x [M, C] in blocks of 128 tokens, transposed: [C, M padded]."""
+    return _wide(*_ref_rows(_pad(x.float(), 0).t()))
+
+
+@pytest.mark.parametrize("sizes,N,K", [(None, 144, 272), (None, 256, 1024), ([40, 0, 129, 300], 272, 144),
+                                       ([0, 0, 5], 128, 128)])
+def test_linear_gradients(gpu, sizes, N, K):
+    M = 333 if sizes is None else sum(sizes) + 4
+    E = 1 if sizes is None else len(sizes)
+    x, dy = _x(gpu, M, K, seed=1), _x(gpu, M, N, seed=2, scale=1e-2)
+    w = _x(gpu, E, N, K, seed=3, scale=K ** -0.5)
+    offs = None if sizes is None else torch.tensor(sizes, device=gpu).cumsum(0).int()
+    leaves = [x.requires_grad_(True), (w[0] if sizes is None else w).detach().requires_grad_(True)]
+    y = mxfp8gg.fp8_block_linear(*leaves, offs)
+    dx, dw = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    dw = dw.view(E, N, K)
+    at = 0
+    for e, n in enumerate([M] if sizes is None else sizes):
+        one = slice(at, at + n)
+        at += n
+        if n == 0:
+            assert not dw[e].any()
+            continue
+        xe, ge = x.detach()[one], dy[one]
+        wq = _wide(*_ref_tiles(w[e]), True)
+        for got, a, b in ((y.detach()[one], _dequant_rows(xe), wq), (dx[one], _dequant_rows(ge), wq.t()),
+                          (dw[e], _dequant_tokens(ge), _dequant_tokens(xe))):
+            _near(got, a @ b.t(), a.abs() @ b.abs().t(), (a.shape[1] + 127) // 128)
+    assert not y[at:].any() and not dx[at:].any()         # rows past the groups
+    # each gradient alone: the same bits
+    assert torch.equal(torch.autograd.grad(y, leaves[0], dy, retain_graph=True)[0], dx)
+    assert torch.equal(torch.autograd.grad(y, leaves[1], dy)[0].view(E, N, K), dw)
+    only = mxfp8gg.fp8_block_linear(leaves[0], leaves[1].detach(), offs)
+    assert torch.equal(only, y) and torch.equal(torch.autograd.grad(only, leaves[0], dy)[0], dx)
+    with torch.no_grad():
+        assert torch.equal(mxfp8gg.fp8_block_linear(*leaves, offs), y)
+
+
+def test_linear_shapes(gpu):
+    x, w = _x(gpu, 12, 64, seed=1), _x(gpu, 32, 64, seed=2)
+    y = mxfp8gg.fp8_block_linear(x, w)
+    assert torch.equal(mxfp8gg.fp8_block_linear(x.view(2, 6, 64), w), y.view(2, 6, 32))
+    assert torch.equal(mxfp8gg.fp8_block_linear(x[0], w), y[0])
+    leaf, wl = x[:0].requires_grad_(True), w.detach().requires_grad_(True)
+    e = mxfp8gg.fp8_block_linear(leaf, wl)
+    dx, dw = torch.autograd.grad(e, (leaf, wl), torch.zeros_like(e))
+    assert e.shape == (0, 32) and dx.shape == (0, 64) and dw.shape == (32, 64) and not dw.any()
+
+
+def test_operand_layouts(gpu):
+    """Row strides, unaligned starts, strided experts and scales of other layouts."""
+    x = _x(gpu, 70, 272, seed=1)
+    q, s = mxfp8gg.to_fp8_block_dim0(x)
+    wq, ws = _weights(gpu, 3, 144, 272, seed=2)
+    offs = torch.tensor([30, 30, 70], dtype=torch.int32, device=gpu)
+    want = mxfp8gg.fp8_block_mm(q, s, wq, ws, offs)
+
+    def bytes_of(t):
+        return t.view(torch.uint8)
+
+    wide = torch.zeros((70, 304), dtype=torch.uint8, device=gpu)
+    wide[:, 16:288] = bytes_of(q)
+    odd = torch.zeros((70, 273), dtype=torch.uint8, device=gpu)
+    odd[:, 1:] = bytes_of(q)
+    two = torch.zeros((6, 144, 272), dtype=torch.uint8, device=gpu)
+    two[::2] = bytes_of(wq)
+    for a in (wide[:, 16:288], odd[:, 1:], bytes_of(q)):
+        for b in (two[::2], bytes_of(wq)):
+            for sa in (s, s.contiguous()):
+                assert torch.equal(mxfp8gg.fp8_block_mm(a, sa, b, ws, offs), want)
+    sc = torch.zeros((3, *ws.shape[1:], 2), device=gpu)
+    sc[..., 1] = ws
+    assert torch.equal(mxfp8gg.fp8_block_mm(q, s, wq, sc[..., 1], offs), want)
+    lead = torch.cat([offs.new_zeros(1), offs]).long()     # [E + 1] with a leading 0, int64
+    assert torch.equal(mxfp8gg.fp8_block_mm(q, s, wq, ws, lead), want)
+
+
+def test_rows_past_the_groups_stay(gpu):
+    """Rows outside every group are not written, whatever their scales hold."""
+    for M, K in ((20, 256), (400, 256), (3000, 128)):
+        x = _x(gpu, M, K, seed=M)
+        q, s = mxfp8gg.to_fp8_block_dim0(x)
+        s = s.clone()
+        s[M // 2:] = float("nan")
+        wq, ws = _weights(gpu, 2, 256, K, seed=2)
+        offs = torch.tensor([M // 4, M // 2], dtype=torch.int32, device=gpu)
+        out = torch.full((M, 256), 7.0, dtype=torch.bfloat16, device=gpu)
+        lib = mxfp8gg.load_library()
+        s = s.t().contiguous()
+        assert lib.mxgg_block_mm(q.data_ptr(), K, s.data_ptr(), M, wq.data_ptr(), 256 * K, K, ws.data_ptr(),
+                                 2 * ws.shape[2], ws.shape[2], offs.data_ptr(), 2, M, 256, K,
+                                 out.data_ptr(), 256, 0, torch.cuda.current_stream().cuda_stream) == 0
+        assert (out[M // 2:] == 7).all() and torch.isfinite(out).all()
+
+
+def test_non_finite_operands(gpu):
+    x = _x(gpu, 40, 256, seed=1).abs()
+    x[3, 200] = float("nan")
+    x[5, 0] = float("inf")
+    w = _x(gpu, 144, 256, seed=2)
+    y = mxfp8gg.fp8_block_linear(x, w)
+    ok = torch.ones(40, dtype=torch.bool, device=gpu)
+    ok[3] = ok[5] = False
+    assert torch.isnan(y[3]).all() and torch.isnan(y[5]).all() and torch.isfinite(y[ok]).all()
+
+
+def test_graph_replays(gpu):
+    x, w = _x(gpu, 30, 256, seed=1), _x(gpu, 144, 256, seed=2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mxfp8gg.fp8_block_linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = mxfp8gg.fp8_block_linear(x, w)
+    for i in range(3):
+        x.copy_(_x(gpu, 30, 256, seed=i + 4))
+        want = mxfp8gg.fp8_block_linear(x, w)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_refusals(gpu):
+    m = mxfp8gg
+    x, w = _x(gpu, 8, 64, seed=1), _x(gpu, 32, 64, seed=2)
+    q, s = m.to_fp8_block_dim0(x)
+    wq, ws = m.to_fp8_block_weight(w)
+    offs = torch.tensor([8], dtype=torch.int32, device=gpu)
+    for call in (lambda: m.to_fp8_block_dim0(x[:, :40]), lambda: m.to_fp8_block_weight(w[:, :40]),
+                 lambda: m.to_fp8_block_dim1(x, offs[:0]),
+                 lambda: m.fp8_block_mm(q, s, wq[:, :48].contiguous(), ws),
+                 lambda: m.fp8_block_mm(q, s[:4], wq, ws), lambda: m.fp8_block_mm(q, s, wq, ws[:, :0]),
+                 lambda: m.fp8_block_mm(q, s.double(), wq, ws), lambda: m.fp8_block_mm(q, s, wq, ws, offs),
+                 lambda: m.fp8_block_mm(q, s, wq[None], ws[None]),
+                 lambda: m.fp8_block_mm(q, s, wq, ws, out_dtype=torch.float16),
+                 lambda: m.fp8_block_mm(q.cpu(), s, wq, ws),
+                 lambda: m.fp8_block_linear(x, w[:20]), lambda: m.fp8_block_linear(x, w[:, :48]),
+                 lambda: m.fp8_block_linear(x, w, offs), lambda: m.fp8_block_linear(x, w[None]),
+                 lambda: m.fp8_block_wgrad(q, s, q, s)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: m.to_fp8_block_dim0(x.float()), lambda: m.to_fp8_block_dim0(x[0]),
+                 lambda: m.to_fp8_block_weight(w.float()), lambda: m.fp8_block_linear(x.float(), w),
+                 lambda: m.fp8_block_mm(x, s, wq, ws)):
+        with pytest.raises(TypeError):
+            call()
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        torch.autograd.grad(m.fp8_block_linear(leaf, w).sum(), leaf, create_graph=True)
