@@ -131,8 +131,9 @@ struct BlockStream {
 // acc[p][q] of the wave: P fragment p = 4 G + i holds rows 64 G + 4 m + i of the wave's
 // part (m = 0..15), Q fragment q rows 4 m + q; D[4g + r][c] is in register r of lane
 // c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i are 16 in a row for every G.
-template <int WP, int GP, int WQ, bool ROWS>
-__device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand& P,
+// ring: two stages in LDS.
+template <int WP, int GP, int WQ, bool ROWS, class Ring>
+__device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P,
                                                const BlockOperand& Q, uint32_t len,
                                                v4f (&acc)[4 * GP][4]) {
   using T = BlockTile<WP, GP, WQ, ROWS>;
@@ -145,10 +146,9 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
   const uint32_t nst = (len + kBlkK - 1) / kBlkK;
   BlockStream<T, ROWS> st;
   st.init(P, Q, len);
-  uint8_t* slot[2] = {ring, ring + T::kStage};
-  st.template load<0, T::kLoads + 1>(slot[0], 0);
+  st.template load<0, T::kLoads + 1>(ring[0], 0);
   if (nst > 1) {
-    st.template load<0, T::kLoads + 1>(slot[1], 1);
+    st.template load<0, T::kLoads + 1>(ring[1], 1);
     wait_barrier<T::kLoads + 1>();
   } else {
     wait_barrier<0>();
@@ -190,10 +190,10 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
   float4 spt[4];
   float sct[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) fb[q] = read_q(slot[0], q);
-  fa[0] = read_p(slot[0], 0);
-  spn[0] = read_sp(slot[0], 0);
-  sqn = *reinterpret_cast<const float4*>(slot[0] + sq_at);
+  for (int q = 0; q < 4; ++q) fb[q] = read_q(ring[0], q);
+  fa[0] = read_p(ring[0], 0);
+  spn[0] = read_sp(ring[0], 0);
+  sqn = *reinterpret_cast<const float4*>(ring[0] + sq_at);
   const auto add = [&](v4f& a, const v4f& x, const float4& sp, float f) __attribute__((always_inline)) {
     if constexpr (ROWS) {
       a[0] = __builtin_fmaf(x[0], sp.x * f, a[0]);
@@ -206,9 +206,12 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
     }
   };
   constexpr int kF = 4 * GP, kN = 4 * kF, kLag = 2;
-  for (uint32_t s = 0; s < nst; ++s) {
-    uint8_t* cur = slot[s & 1u];
-    uint8_t* nxt = slot[(s & 1u) ^ 1u];
+  uint32_t s = 0;
+  // no branch inside: the compiler would move the matrix instructions past it
+  const auto stage = [&](auto loads) __attribute__((always_inline)) {
+    constexpr bool LOADS = decltype(loads)::value;
+    uint8_t* cur = ring[s & 1u];
+    uint8_t* nxt = ring[(s & 1u) ^ 1u];
     sc[0] = sqn.x;
     sc[1] = sqn.y;
     sc[2] = sqn.z;
@@ -226,7 +229,7 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
             // the next stage has landed, every wave has read this one
             wait_barrier<0>();
             MXGG_FENCE();
-            if (s + 2 < nst) st.template load<0, T::kLoads + 1>(cur, s + 2);
+            if constexpr (LOADS) st.template load<0, T::kLoads + 1>(cur, s + 2);
           }
           const uint8_t* from = p == kF - 1 ? nxt : cur;
           const int pn = p == kF - 1 ? 0 : p + 1;
@@ -239,6 +242,7 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
         if (p == kF - 1) fb[q] = read_q(nxt, q);
         sct[n & 3] = sc[q];
         if (ROWS) spt[n & 3] = spn[p & 1];
+        MXGG_FENCE();
       }
       if (n >= kLag) {
         const int o = n - kLag;
@@ -246,7 +250,10 @@ __device__ __forceinline__ void block_mainloop(uint8_t* ring, const BlockOperand
       }
       MXGG_FENCE();
     }
-  }
+  };
+  for (; s + 2 < nst; ++s) stage(std::true_type{});
+  do stage(std::false_type{});
+  while (++s < nst);
   // the slots take the next tile's loads only after every wave's last reads
   release_barrier();
 }
@@ -348,7 +355,7 @@ __device__ __forceinline__ int64_t xcd_tile() {
 template <int WP, int GP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
   using T = BlockTile<WP, GP, WQ, false>;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * T::kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2][T::kStage];
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.N + T::kP - 1) / T::kP;
   GroupTile at{0, 0, a.M, xcd_tile()};
@@ -377,7 +384,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
 template <int WP, int GP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_wgrad(BlockWgradArgs a) {
   using T = BlockTile<WP, GP, WQ, true>;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * T::kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2][T::kStage];
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.K + T::kP - 1) / T::kP, nq = (a.N + T::kQ - 1) / T::kQ;
   const int64_t tile = xcd_tile();
