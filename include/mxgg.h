@@ -749,12 +749,18 @@ int mxgg_block_quant_weight(const void* w, int64_t num_groups, int64_t N, int64_
  * a [M, K] and w [num_groups, N, K] e4m3 (group stride w_gstride bytes), K % 16 == 0,
  * 16-byte aligned rows; a_scales[b * ldas + m]; w_scales[g * ws_gstride + (n / 128) * ldws
  * + b].  Sums are fp32.  out bf16 or fp32 [M, N], row stride ldo elements; rows outside
- * every group are not written.  group_ends NULL: one group (num_groups = 1).
+ * every group are not written.  group_ends NULL: one group (num_groups = 1).  Products of
+ * few tiles are split along K and added in a fixed order: workspace of
+ * mxgg_block_mm_workspace_bytes(group_ends != NULL, ...) bytes for the current device
+ * (0 for most sizes), 16-byte aligned, no initialisation.
  */
+int64_t mxgg_block_mm_workspace_bytes(int grouped, int64_t num_groups, int64_t M, int64_t N,
+                                      int64_t K);
 int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t ldas, const void* w,
                   int64_t w_gstride, int64_t ldw, const float* w_scales, int64_t ws_gstride,
                   int64_t ldws, const int32_t* group_ends, int64_t num_groups, int64_t M,
-                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* stream);
+                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 /*
  * Weight gradient of block-scaled operands: dw[g][n][k] = sum over the tokens t of group g
@@ -762,11 +768,15 @@ int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t lda
  * and their scales as mxgg_block_quant_dim1 writes them.  group_ends_pad: padded ends
  * (multiples of 128; others are rounded down), NULL for one group; tokens % 128 == 0.
  * dw bf16 or fp32 [num_groups, N, K], contiguous; empty groups are written as zeros.
+ * workspace: as mxgg_block_mm's, for sums split along the tokens.
  */
+int64_t mxgg_block_wgrad_workspace_bytes(int grouped, int64_t num_groups, int64_t tokens, int64_t N,
+                                         int64_t K);
 int mxgg_block_wgrad(const void* go_t, int64_t ldgo, const float* go_scales, int64_t ldgos,
                      const void* ia_t, int64_t ldia, const float* ia_scales, int64_t ldias,
                      const int32_t* group_ends_pad, int64_t num_groups, int64_t tokens, int64_t N,
-                     int64_t K, void* dw, int out_type, void* stream);
+                     int64_t K, void* dw, int out_type, void* workspace, int64_t workspace_bytes,
+                     void* stream);
 
 /*
  * Root-mean-square norm with the residual's addition:

@@ -14,9 +14,12 @@
 // own: 8 vector instructions a matrix instruction.
 //
 // Operands stream through two LDS stages of 128 bytes a row by DMA, laid out as in
-// gemm_tile.h; one barrier a stage, seven eighths through it: the next stage has
+// gemm_tile.h; one barrier a stage, three fragments before its end: the next stage has
 // landed and every wave has read the current one, whose slot takes the stage after
-// next; the last matrix instructions of the stage run meanwhile.
+// next, one load after each of the stage's last matrix instructions.
+#include <algorithm>
+#include <utility>
+
 #include "gemm_tile.h"
 
 namespace mxgg {
@@ -41,9 +44,13 @@ struct BlockTile {
   static constexpr int kP = 64 * WP * GP, kQ = 64 * WQ;
   static constexpr int kWavesT = WP * WQ, kThreadsT = 64 * kWavesT;
   static constexpr uint32_t kData = (uint32_t)(kP + kQ) * kBlkK;
-  static constexpr uint32_t kStage = kData + 4u * (kP + kQ);
+  static constexpr uint32_t kScales = 4u * (kP + kQ);     // bytes of a stage's scales
   static constexpr int kLoads = (kP + kQ) / 8 / kWavesT;  // data loads of a wave and stage
   static constexpr int kFrags = 4 * GP;                   // of P
+  struct Ring {
+    uint8_t data[2][kData];
+    uint8_t scales[4][kScales];  // of their own: read until the stage's last products
+  };
   static_assert((kP + kQ) / 64 == kWavesT, "one scale load a wave");
 };
 
@@ -103,38 +110,57 @@ struct BlockStream {
       sstep = 4u;
     }
   }
-  // Loads [FROM, TO) of stage s; the last one of a stage is the scales'.
-  template <int FROM, int TO>
-  __device__ __forceinline__ void load(uint8_t* stage, uint32_t s) const {
-    const uint32_t wave = wave_id(), k0 = s * kBlkK;
+  // Lane offsets of a stage (out of range where its chunk lies past the end).
+  __device__ __forceinline__ void base(uint32_t s, uint32_t& bp, uint32_t& bq) const {
+    const uint32_t k0 = s * kBlkK;
     const bool ok = k0 + kcol < len;
-#pragma unroll
-    for (int j = FROM; j < TO; ++j) {
-      if (j == T::kLoads) {
-        dma_x1(ds, lds_offset(stage) + T::kData + 256u * wave, vs, s * sstep);
-        continue;
-      }
-      const uint32_t run = (uint32_t)T::kWavesT * j + wave;  // 1 KB runs of the stage
+    bp = ok ? vbase_p + k0 : kOobOffset;
+    bq = ok ? vbase_q + k0 : kOobOffset;
+  }
+  // Load J of stage s: data into `slot`, the last one scales into the scales' ring.
+  template <int J, class Ring>
+  __device__ __forceinline__ void load(Ring& ring, uint32_t s, uint32_t bp, uint32_t bq) const {
+    const uint32_t wave = wave_id();
+    if constexpr (J == T::kLoads) {
+      dma_x1(ds, lds_offset(ring.scales[s & 3u]) + 256u * wave, vs, s * sstep);
+    } else {
+      const uint32_t run = (uint32_t)T::kWavesT * J + wave;  // 1 KB runs of the stage
       constexpr uint32_t kRunsP = T::kP / 8;
-      // every run of one load belongs to one operand: kP / 8 is a multiple of kWaves
-      const bool p = (uint32_t)T::kWavesT * j < kRunsP;
+      // every run of one load belongs to one operand: kP / 8 is a multiple of the waves
+      constexpr bool p = (uint32_t)T::kWavesT * J < kRunsP;
       const uint32_t i = (p ? run : run - kRunsP) >> 2;  // 32-slot run of the operand
       const uint32_t row = (i >> 2) * 128u + (i & 3u);
-      const uint32_t v = ok ? (p ? vbase_p : vbase_q) + k0 : kOobOffset;
-      dma_x4(p ? dp : dq, lds_offset(stage) + 1024u * run, v, row * (p ? ldp : ldq));
+      dma_x4(p ? dp : dq, lds_offset(ring.data[s & 1u]) + 1024u * run, p ? bp : bq,
+             row * (p ? ldp : ldq));
     }
+  }
+  template <class Ring, int... J>
+  __device__ __forceinline__ void load_all(Ring& ring, uint32_t s,
+                                           std::integer_sequence<int, J...>) const {
+    uint32_t bp, bq;
+    base(s, bp, bq);
+    (load<J>(ring, s, bp, bq), ...);
+  }
+  template <class Ring>
+  __device__ __forceinline__ void load_all(Ring& ring, uint32_t s) const {
+    load_all(ring, s, std::make_integer_sequence<int, T::kLoads + 1>{});
   }
 };
 
 #define MXGG_FENCE() __builtin_amdgcn_sched_barrier(0)
 
+template <class F, int... N>
+__device__ __forceinline__ void steps(F& f, std::integer_sequence<int, N...>) {
+  (f(std::integral_constant<int, N>{}), ...);
+}
+
 // acc[p][q] of the wave: P fragment p = 4 G + i holds rows 64 G + 4 m + i of the wave's
 // part (m = 0..15), Q fragment q rows 4 m + q; D[4g + r][c] is in register r of lane
 // c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i are 16 in a row for every G.
-// ring: two stages in LDS.
+// qn: rows of Q that are wanted; a wave with none of them only loads.
 template <int WP, int GP, int WQ, bool ROWS, class Ring>
 __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P,
-                                               const BlockOperand& Q, uint32_t len,
+                                               const BlockOperand& Q, uint32_t len, int64_t qn,
                                                v4f (&acc)[4 * GP][4]) {
   using T = BlockTile<WP, GP, WQ, ROWS>;
 #pragma unroll
@@ -146,9 +172,9 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
   const uint32_t nst = (len + kBlkK - 1) / kBlkK;
   BlockStream<T, ROWS> st;
   st.init(P, Q, len);
-  st.template load<0, T::kLoads + 1>(ring[0], 0);
+  st.load_all(ring, 0);
   if (nst > 1) {
-    st.template load<0, T::kLoads + 1>(ring[1], 1);
+    st.load_all(ring, 1);
     wait_barrier<T::kLoads + 1>();
   } else {
     wait_barrier<0>();
@@ -157,6 +183,14 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
 
   const uint32_t lane = threadIdx.x & 63u, wave = wave_id();
   const uint32_t wp = wave % WP, wq = wave / WP;
+  if (uniform((uint32_t)(64 * (int64_t)wq >= qn))) {
+    for (uint32_t s = 0; s < nst; ++s) {
+      wait_barrier<0>();
+      if (s + 2 < nst) st.load_all(ring, s + 2);
+    }
+    release_barrier();
+    return;
+  }
   const uint32_t m = lane & 15u, g = lane >> 4;
   // 64-row part u of an operand: slots 128 (u / 2) + 16 (u % 2) + 32 i + m, i = 0..3
   const auto part = [&](uint32_t u) { return (128u * (u >> 1) + 16u * (u & 1u) + m) * kBlkK; };
@@ -165,8 +199,8 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
 #pragma unroll
   for (int G = 0; G < GP; ++G) pa[G] = part(wp * GP + G);
   const uint32_t qa = T::kP * kBlkK + part(wq);
-  const uint32_t sq_at = T::kData + 4u * (64u * wq + 4u * m);  // Q rows 4 m .. + 3: fragments 0..3
-  const uint32_t sp_at = T::kData + 4u * T::kQ + 256u * wp * GP;
+  const uint32_t sq_at = 4u * (64u * wq + 4u * m);  // Q rows 4 m .. + 3: fragments 0..3
+  const uint32_t sp_at = 4u * T::kQ + 256u * wp * GP;
   const auto read_p = [&](const uint8_t* s, int p) __attribute__((always_inline)) {
     const uint8_t* at = s + pa[p >> 2] + 4096u * (p & 3);
     return lds_v8i(at + lo, at + hi);
@@ -183,17 +217,20 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
       return make_float4(*reinterpret_cast<const float*>(s + sp_at), 0.0f, 0.0f, 0.0f);
   };
 
-  v8i fa[2], fb[4];
+  // P fragments are read kAhead steps before their products
+  constexpr int kF = 4 * GP, kN = 4 * kF, kLag = 2, kAhead = 3, kW = kAhead + 1;
+  v8i fa[kW], fb[4];
   float4 spn[2], sqn;   // scales of the fragments ahead, and of the stage ahead
   float sc[4];          // of the stage: Q's scale (times P's)
   v4f t[4];             // products in flight
   float4 spt[4];
   float sct[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) fb[q] = read_q(ring[0], q);
-  fa[0] = read_p(ring[0], 0);
-  spn[0] = read_sp(ring[0], 0);
-  sqn = *reinterpret_cast<const float4*>(ring[0] + sq_at);
+  for (int q = 0; q < 4; ++q) fb[q] = read_q(ring.data[0], q);
+#pragma unroll
+  for (int p = 0; p < kAhead; ++p) fa[p] = read_p(ring.data[0], p);
+  spn[0] = read_sp(ring.scales[0], 0);
+  sqn = *reinterpret_cast<const float4*>(ring.scales[0] + sq_at);
   const auto add = [&](v4f& a, const v4f& x, const float4& sp, float f) __attribute__((always_inline)) {
     if constexpr (ROWS) {
       a[0] = __builtin_fmaf(x[0], sp.x * f, a[0]);
@@ -205,13 +242,16 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
       for (int r = 0; r < 4; ++r) a[r] = __builtin_fmaf(x[r], f, a[r]);
     }
   };
-  constexpr int kF = 4 * GP, kN = 4 * kF, kLag = 2;
   uint32_t s = 0;
   // no branch inside: the compiler would move the matrix instructions past it
   const auto stage = [&](auto loads) __attribute__((always_inline)) {
     constexpr bool LOADS = decltype(loads)::value;
-    uint8_t* cur = ring[s & 1u];
-    uint8_t* nxt = ring[(s & 1u) ^ 1u];
+    const uint8_t* cur = ring.data[s & 1u];
+    const uint8_t* nxt = ring.data[(s & 1u) ^ 1u];
+    const uint8_t* scales = ring.scales[s & 3u];
+    const uint8_t* scales_nxt = ring.scales[(s + 1) & 3u];
+    uint32_t bp = 0, bq = 0;
+    if constexpr (LOADS) st.base(s + 2, bp, bq);
     sc[0] = sqn.x;
     sc[1] = sqn.y;
     sc[2] = sqn.z;
@@ -220,36 +260,38 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
 #pragma unroll
       for (int q = 0; q < 4; ++q) sc[q] *= spn[0].x;
     }
-#pragma unroll
-    for (int n = 0; n < kN + kLag; ++n) {
-      const int p = n / 4, q = n % 4;
-      if (n < kN) {
-        if (q == 0) {
-          if (p == kF - 1) {
+    const auto step = [&](auto index) __attribute__((always_inline)) {
+      constexpr int n = decltype(index)::value, p = n / 4, q = n % 4;
+      if constexpr (n < kN) {
+        if constexpr (q == 0) {
+          if constexpr (p == kF - kAhead) {
             // the next stage has landed, every wave has read this one
             wait_barrier<0>();
             MXGG_FENCE();
-            if constexpr (LOADS) st.template load<0, T::kLoads + 1>(cur, s + 2);
           }
-          const uint8_t* from = p == kF - 1 ? nxt : cur;
-          const int pn = p == kF - 1 ? 0 : p + 1;
-          fa[(p + 1) & 1] = read_p(from, pn);
-          if (ROWS || p == kF - 1) spn[(p + 1) & 1] = read_sp(from, pn);
-          if (p == kF - 1) sqn = *reinterpret_cast<const float4*>(nxt + sq_at);
+          constexpr int pn = (p + kAhead) % kF;
+          fa[(p + kAhead) % kW] = read_p(p + kAhead < kF ? cur : nxt, pn);
+          if constexpr (ROWS || p == kF - 1)
+            spn[(p + 1) & 1] = read_sp(p + 1 < kF ? scales : scales_nxt, (p + 1) % kF);
+          if constexpr (p == kF - 1) sqn = *reinterpret_cast<const float4*>(scales_nxt + sq_at);
         }
+        // one load after each product: a load holds its wave until it is accepted
+        constexpr int j = n - 4 * (kF - kAhead);
+        if constexpr (LOADS && j >= 0 && j <= T::kLoads) st.template load<j>(ring, s + 2, bp, bq);
         t[n & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            fa[p & 1], fb[q], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
-        if (p == kF - 1) fb[q] = read_q(nxt, q);
+            fa[p % kW], fb[q], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+        if constexpr (p == kF - 1) fb[q] = read_q(nxt, q);
         sct[n & 3] = sc[q];
-        if (ROWS) spt[n & 3] = spn[p & 1];
+        if constexpr (ROWS) spt[n & 3] = spn[p & 1];
         MXGG_FENCE();
       }
-      if (n >= kLag) {
-        const int o = n - kLag;
+      if constexpr (n >= kLag) {
+        constexpr int o = n - kLag;
         add(acc[o / 4][o % 4], t[o & 3], spt[o & 3], sct[o & 3]);
       }
       MXGG_FENCE();
-    }
+    };
+    steps(step, std::make_integer_sequence<int, kN + kLag>{});
   };
   for (; s + 2 < nst; ++s) stage(std::true_type{});
   do stage(std::false_type{});
@@ -308,7 +350,8 @@ struct GroupTile {
   int g;
   int64_t begin, end, tile;
 };
-__device__ __forceinline__ GroupTile find_group(const int32_t* ends_s, int E, int q, int64_t np) {
+__device__ __forceinline__ GroupTile find_group(const int32_t* ends_s, int E, int q, int64_t np,
+                                                uint32_t id) {
   const int lane = threadIdx.x & 63;
   const auto tiles = [&](int g) {
     return g < E ? (int64_t)((ends_s[g] - (g > 0 ? ends_s[g - 1] : 0) + q - 1) / q) * np : 0;
@@ -316,8 +359,8 @@ __device__ __forceinline__ GroupTile find_group(const int32_t* ends_s, int E, in
   int64_t total = 0;
   for (int g = lane; g < E; g += 64) total += tiles(g);
   for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-  const int64_t per = (total + 7) >> 3, t = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || t >= total) return {E, 0, 0, 0};
+  const int64_t per = (total + 7) >> 3, t = (id & 7u) * per + (id >> 3);
+  if ((id >> 3) >= per || t >= total) return {E, 0, 0, 0};
   int64_t before = 0;
   for (int g0 = 0; g0 < E; g0 += 64) {
     const int64_t own = tiles(g0 + lane);
@@ -347,35 +390,49 @@ __device__ __forceinline__ void band(int64_t tile, int64_t nq, int64_t np, int64
   tp = r / h;
 }
 // The same order of tiles where their number is that of the grid.
-__device__ __forceinline__ int64_t xcd_tile() {
-  const int64_t per = gridDim.x >> 3;
-  return (int64_t)(blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+__device__ __forceinline__ int64_t xcd_tile(uint32_t id, uint32_t grid) {
+  return (int64_t)(id & 7u) * (grid >> 3) + (id >> 3);
 }
 
+// Blocks [first, last) of the contraction that part `part` of `parts` adds up.
+struct Part {
+  int64_t first, last;
+  __device__ __forceinline__ Part(int64_t blocks, uint32_t part, uint32_t parts)
+      : first(blocks * part / parts), last(blocks * (part + 1) / parts) {}
+};
+
+// Workgroups [0, grid): tiles, of the first part of the contraction; and so on.
 template <int WP, int GP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
   using T = BlockTile<WP, GP, WQ, false>;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[2][T::kStage];
+  __shared__ __attribute__((aligned(1024))) typename T::Ring ring;
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.N + T::kP - 1) / T::kP;
-  GroupTile at{0, 0, a.M, xcd_tile()};
+  const uint32_t grid = gridDim.x / (uint32_t)a.parts, part = blockIdx.x / grid, id = blockIdx.x % grid;
+  GroupTile at{0, 0, a.M, xcd_tile(id, grid)};
   if (a.ends) {
     monotone_ends_to_lds(a.ends, a.E, a.M, ends_s);
-    at = find_group(ends_s, a.E, T::kQ, np);
+    at = find_group(ends_s, a.E, T::kQ, np, id);
   }
   const int64_t nq = (at.end - at.begin + T::kQ - 1) / T::kQ;
   if (at.g >= a.E || at.tile >= nq * np) return;
   int64_t tq, tp;
   band(at.tile, nq, np, tq, tp);
+  const Part k((a.K + kBlkK - 1) / kBlkK, part, (uint32_t)a.parts);
   const int64_t m0 = at.begin + tq * T::kQ, n0 = tp * T::kP;
-  const BlockOperand P{a.w + at.g * a.w_group + n0 * a.ldw, a.ws + at.g * a.ws_group + n0 / kBlkK * a.ldws,
-                       a.ldw, a.ldws, a.N - n0};
-  const BlockOperand Q{a.a + m0 * a.lda, a.as + m0, a.lda, a.ldas, a.M - m0};
+  const BlockOperand P{a.w + at.g * a.w_group + n0 * a.ldw + k.first * kBlkK,
+                       a.ws + at.g * a.ws_group + n0 / kBlkK * a.ldws + k.first, a.ldw, a.ldws,
+                       a.N - n0};
+  const BlockOperand Q{a.a + m0 * a.lda + k.first * kBlkK, a.as + m0 + k.first * a.ldas, a.lda,
+                       a.ldas, a.M - m0};
   v4f acc[4 * GP][4];
-  block_mainloop<WP, GP, WQ, false>(ring, P, Q, (uint32_t)a.K, acc);
+  block_mainloop<WP, GP, WQ, false>(
+      ring, P, Q, (uint32_t)(min((int64_t)a.K, k.last * kBlkK) - k.first * kBlkK), at.end - m0, acc);
   const uint32_t wave = wave_id();
   const int64_t p0 = n0 + 64 * GP * (wave % WP), q0 = m0 + 64 * (wave / WP);
-  if (a.out_f32)
+  if (a.parts > 1)
+    block_store<GP>(acc, a.partial + part * a.M * a.N, a.N, p0, a.N, q0, at.end);
+  else if (a.out_f32)
     block_store<GP>(acc, static_cast<float*>(a.out), a.ldo, p0, a.N, q0, at.end);
   else
     block_store<GP>(acc, static_cast<uint16_t*>(a.out), a.ldo, p0, a.N, q0, at.end);
@@ -384,33 +441,83 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
 template <int WP, int GP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_wgrad(BlockWgradArgs a) {
   using T = BlockTile<WP, GP, WQ, true>;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[2][T::kStage];
+  __shared__ __attribute__((aligned(1024))) typename T::Ring ring;
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.K + T::kP - 1) / T::kP, nq = (a.N + T::kQ - 1) / T::kQ;
-  const int64_t tile = xcd_tile();
+  const uint32_t grid = gridDim.x / (uint32_t)a.parts, part = blockIdx.x / grid;
+  const int64_t tile = xcd_tile(blockIdx.x % grid, grid);
   const int64_t g = tile / (np * nq);
   if (g >= a.E) return;
-  int64_t t0 = 0, t1 = a.tokens;
+  int64_t b0 = 0, b1 = a.tokens / kBlkK;
   if (a.ends) {
     monotone_ends_to_lds(a.ends, a.E, a.tokens, ends_s);
     // whole blocks: the casts' padded ends are multiples of 128, others are rounded down
-    t0 = (g > 0 ? ends_s[g - 1] : 0) & ~(kBlkK - 1);
-    t1 = ends_s[g] & ~(kBlkK - 1);
+    b0 = (g > 0 ? ends_s[g - 1] : 0) / kBlkK;
+    b1 = ends_s[g] / kBlkK;
   }
+  const Part k(b1 - b0, part, (uint32_t)a.parts);
+  b1 = b0 + k.last;
+  b0 += k.first;
   int64_t tq, tp;
   band(tile % (np * nq), nq, np, tq, tp);
   const int64_t k0 = tp * T::kP, n0 = tq * T::kQ;
-  const int64_t b0 = t0 / kBlkK;
-  const BlockOperand P{a.ia + k0 * a.ldia + t0, a.ias + b0 * a.ldias + k0, a.ldia, a.ldias, a.K - k0};
-  const BlockOperand Q{a.go + n0 * a.ldgo + t0, a.gos + b0 * a.ldgos + n0, a.ldgo, a.ldgos, a.N - n0};
+  const BlockOperand P{a.ia + k0 * a.ldia + b0 * kBlkK, a.ias + b0 * a.ldias + k0, a.ldia, a.ldias,
+                       a.K - k0};
+  const BlockOperand Q{a.go + n0 * a.ldgo + b0 * kBlkK, a.gos + b0 * a.ldgos + n0, a.ldgo, a.ldgos,
+                       a.N - n0};
   v4f acc[4 * GP][4];
-  block_mainloop<WP, GP, WQ, true>(ring, P, Q, (uint32_t)(t1 > t0 ? t1 - t0 : 0), acc);
+  block_mainloop<WP, GP, WQ, true>(ring, P, Q, (uint32_t)((b1 - b0) * kBlkK), a.N - n0, acc);
   const uint32_t wave = wave_id();
   const int64_t p0 = k0 + 64 * GP * (wave % WP), q0 = n0 + 64 * (wave / WP);
-  if (a.out_f32)
-    block_store<GP>(acc, static_cast<float*>(a.dw) + g * a.N * a.K, a.K, p0, a.K, q0, a.N);
+  const int64_t nk = (int64_t)a.N * a.K;
+  if (a.parts > 1)
+    block_store<GP>(acc, a.partial + (part * a.E + g) * nk, a.K, p0, a.K, q0, a.N);
+  else if (a.out_f32)
+    block_store<GP>(acc, static_cast<float*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
   else
-    block_store<GP>(acc, static_cast<uint16_t*>(a.dw) + g * a.N * a.K, a.K, p0, a.K, q0, a.N);
+    block_store<GP>(acc, static_cast<uint16_t*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
+}
+
+// Sums the parts of a split product in their order: out[row][col] of `rows` rows (those
+// below the last group end) from fp32 [parts][rows_all][cols], four columns a thread.
+__global__ __launch_bounds__(256) void k_block_join(const float* __restrict__ partial, int parts,
+                                                    int64_t rows_all, const int32_t* ends, int E,
+                                                    int64_t cols, void* out, int64_t ldo, int f32) {
+  int64_t rows = rows_all;
+  if (ends) {  // the largest end, as the running maximum gives it
+    int32_t top = 0;
+    for (int g = threadIdx.x & 63; g < E; g += 64) top = max(top, ends[g]);
+    for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
+    rows = min(rows, (int64_t)top);
+  }
+  const int64_t wide = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / wide, col = i % wide * 4;
+  if (row >= rows) return;
+  const int n = (int)min((int64_t)4, cols - col);
+  const float* p = partial + row * cols + col;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k = 0; k < parts; ++k, p += rows_all * cols) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n == 4) {
+      __builtin_memcpy(v, p, 16);
+    } else {
+      for (int j = 0; j < n; ++j) v[j] = p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  }
+  if (f32) {
+    float* o = static_cast<float*>(out) + row * ldo + col;
+    if (n == 4) __builtin_memcpy(o, s, 16);
+    else
+      for (int j = 0; j < n; ++j) o[j] = s[j];
+  } else {
+    const uint32_t w[2] = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+    uint16_t* o = static_cast<uint16_t*>(out) + row * ldo + col;
+    if (n == 4) __builtin_memcpy(o, w, 8);
+    else
+      for (int j = 0; j < n; ++j) o[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+  }
 }
 
 // Few rows: a workgroup takes 16 rows of W and all of its group's rows of A, 16 QF at
@@ -504,15 +611,58 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
   }
 }
 
-// Workgroups of a run of tiles: a multiple of 8, for xcd_tile().
-dim3 tile_grid(int64_t tiles) { return dim3((unsigned)((tiles + 7) / 8 * 8)); }
+// How a product is shared out.  256 x 256 tiles where they fill the chip, else 128 x 128
+// ones (two workgroups a compute unit); where those do not fill it either, the
+// contraction is split in parts of at least kMinBlocks blocks.
+struct BlockPlan {
+  bool few, large;
+  int64_t tiles, parts;
+};
+constexpr int64_t kMinBlocks = 4, kMaxSplit = 16;
+BlockPlan plan(int64_t tiles256, int64_t tiles128, int64_t blocks) {
+  const int64_t cus = std::max(1, device_cu_count());
+  if (tiles256 >= cus) return {false, true, tiles256, 1};
+  const int64_t parts = std::min({2 * cus / std::max<int64_t>(tiles128, 1), blocks / kMinBlocks, kMaxSplit});
+  return {false, false, tiles128, std::max<int64_t>(parts, 1)};
+}
+BlockPlan plan_mm(int64_t M, int64_t N, int64_t K, int64_t E, bool grouped) {
+  const int64_t per = (M + E - 1) / E;
+  if (per <= 64) return {true, false, 0, 1};
+  const auto tiles = [&](int64_t t) { return ((M + t - 1) / t + (grouped ? E : 0)) * ((N + t - 1) / t); };
+  return plan(tiles(256), tiles(128), (K + kBlkK - 1) / kBlkK);
+}
+BlockPlan plan_wgrad(int64_t tokens, int64_t N, int64_t K, int64_t E) {
+  const auto tiles = [&](int64_t t) { return E * ((K + t - 1) / t) * ((N + t - 1) / t); };
+  return plan(tiles(256), tiles(128), tokens / kBlkK / E);
+}
+// Workgroups: a multiple of 8 for each part, for xcd_tile().
+dim3 tile_grid(const BlockPlan& p) { return dim3((unsigned)((p.tiles + 7) / 8 * 8 * p.parts)); }
+
+hipError_t join_parts(const float* partial, int64_t parts, int64_t rows, const int32_t* ends, int E,
+                      int64_t cols, void* out, int64_t ldo, int f32, hipStream_t stream) {
+  const int64_t n = rows * ((cols + 3) / 4);
+  hipLaunchKernelGGL(k_block_join, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, partial,
+                     (int)parts, rows, ends, E, cols, out, ldo, f32);
+  return hipGetLastError();
+}
 
 }  // namespace
 
-hipError_t launch_block_mm(const BlockMmArgs& a, hipStream_t stream) {
+int64_t block_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t E, bool grouped) {
+  const BlockPlan p = plan_mm(M, N, K, E, grouped);
+  return p.parts > 1 ? 4 * p.parts * M * N : 0;
+}
+int64_t block_wgrad_workspace_bytes(int64_t tokens, int64_t N, int64_t K, int64_t E) {
+  const BlockPlan p = plan_wgrad(tokens, N, K, E);
+  return p.parts > 1 ? 4 * p.parts * E * N * K : 0;
+}
+
+hipError_t launch_block_mm(BlockMmArgs a, hipStream_t stream) {
   if (a.M == 0 || a.N == 0) return hipSuccess;
-  const int64_t per = (a.M + a.E - 1) / a.E;
-  if (per <= 64) {
+  const BlockPlan p = plan_mm(a.M, a.N, a.K, a.E, a.ends != nullptr);
+  a.parts = (int32_t)p.parts;
+  if (p.few) {
+    const int64_t per = (a.M + a.E - 1) / a.E;
     const dim3 grid((unsigned)((a.N + 15) / 16 * a.E));
     if (per <= 16)
       hipLaunchKernelGGL((k_block_few<1>), grid, dim3(64 * kFewWaves), 0, stream, a);
@@ -522,26 +672,27 @@ hipError_t launch_block_mm(const BlockMmArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL((k_block_few<4>), grid, dim3(64 * kFewWaves), 0, stream, a);
     return hipGetLastError();
   }
-  const auto tiles = [&](int64_t p, int64_t q) {
-    return ((a.M + q - 1) / q + (a.ends ? a.E : 0)) * ((a.N + p - 1) / p);
-  };
-  if (tiles(256, 256) >= device_cu_count())
-    hipLaunchKernelGGL((k_block_fwd<2, 2, 4>), tile_grid(tiles(256, 256)), dim3(512), 0, stream, a);
+  if (p.large)
+    hipLaunchKernelGGL((k_block_fwd<2, 2, 4>), tile_grid(p), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_fwd<2, 1, 2>), tile_grid(tiles(128, 128)), dim3(256), 0, stream, a);
-  return hipGetLastError();
+    hipLaunchKernelGGL((k_block_fwd<2, 1, 2>), tile_grid(p), dim3(256), 0, stream, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || a.parts == 1) return err;
+  return join_parts(a.partial, a.parts, a.M, a.ends, a.E, a.N, a.out, a.ldo, a.out_f32, stream);
 }
 
-hipError_t launch_block_wgrad(const BlockWgradArgs& a, hipStream_t stream) {
+hipError_t launch_block_wgrad(BlockWgradArgs a, hipStream_t stream) {
   if (a.N == 0 || a.K == 0 || a.E == 0) return hipSuccess;
-  const auto tiles = [&](int64_t p, int64_t q) {
-    return (int64_t)a.E * ((a.K + p - 1) / p) * ((a.N + q - 1) / q);
-  };
-  if (tiles(256, 256) >= device_cu_count())
-    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4>), tile_grid(tiles(256, 256)), dim3(512), 0, stream, a);
+  const BlockPlan p = plan_wgrad(a.tokens, a.N, a.K, a.E);
+  a.parts = (int32_t)p.parts;
+  if (p.large)
+    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4>), tile_grid(p), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_wgrad<2, 1, 2>), tile_grid(tiles(128, 128)), dim3(256), 0, stream, a);
-  return hipGetLastError();
+    hipLaunchKernelGGL((k_block_wgrad<2, 1, 2>), tile_grid(p), dim3(256), 0, stream, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || a.parts == 1) return err;
+  return join_parts(a.partial, a.parts, (int64_t)a.E * a.N, nullptr, 0, a.K, a.dw, a.K, a.out_f32,
+                    stream);
 }
 
 }  // namespace mxgg

@@ -1701,17 +1701,13 @@ int mxgg_block_quant_weight(const void* w, int64_t num_groups, int64_t N, int64_
 // Rows of an e4m3 operand of the block-scaled products.
 static bool block_rows_aligned(const void* p, int64_t ld) { return aligned16(p) && ld % 16 == 0; }
 
-int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t ldas, const void* w,
-                  int64_t w_gstride, int64_t ldw, const float* w_scales, int64_t ws_gstride,
-                  int64_t ldws, const int32_t* group_ends, int64_t num_groups, int64_t M,
-                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* stream) {
-  const char* what = "block_mm";
-  if (out_type != MXGG_OUT_BF16 && out_type != MXGG_OUT_F32)
-    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown out_type %d", what, out_type);
+// Sizes of a product of block-scaled operands.
+static int check_block_mm(const char* what, bool grouped, int64_t num_groups, int64_t M, int64_t N,
+                          int64_t K) {
   if (M < 0 || N < 0 || K < 1 || K % 16 != 0)
     return set_error(MXGG_ERR_SHAPE, "%s: M=%lld, N=%lld, K=%lld (a positive multiple of 16)", what,
                      (long long)M, (long long)N, (long long)K);
-  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!group_ends && num_groups != 1))
+  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!grouped && num_groups != 1))
     return set_error(MXGG_ERR_UNSUPPORTED, "%s: num_groups=%lld (1 to 1024; 1 without group_ends)",
                      what, (long long)num_groups);
   if (M > INT32_MAX || N > kMaxBlockWidth || K > kMaxBlockWidth ||
@@ -1719,6 +1715,36 @@ int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t lda
       num_groups * ((N + 15) / 16) >= kMaxBlockGrid)
     return set_error(MXGG_ERR_UNSUPPORTED, "%s: M=%lld, N=%lld, K=%lld in %lld groups", what,
                      (long long)M, (long long)N, (long long)K, (long long)num_groups);
+  return MXGG_OK;
+}
+static int check_block_workspace(const char* what, const void* workspace, int64_t bytes,
+                                 int64_t need) {
+  if (bytes < need)
+    return set_error(MXGG_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", what,
+                     (long long)bytes, (long long)need);
+  if (need > 0 && (!workspace || !aligned16(workspace)))
+    return set_error(workspace ? MXGG_ERR_ALIGNMENT : MXGG_ERR_INVALID_ARGUMENT,
+                     "%s: the workspace must be a 16-byte aligned device buffer", what);
+  return MXGG_OK;
+}
+
+int64_t mxgg_block_mm_workspace_bytes(int grouped, int64_t num_groups, int64_t M, int64_t N,
+                                      int64_t K) {
+  if (check_block_mm("block_mm_workspace_bytes", grouped != 0, num_groups, M, N, K) != MXGG_OK)
+    return -1;
+  return M == 0 || N == 0 ? 0 : block_mm_workspace_bytes(M, N, K, num_groups, grouped != 0);
+}
+
+int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t ldas, const void* w,
+                  int64_t w_gstride, int64_t ldw, const float* w_scales, int64_t ws_gstride,
+                  int64_t ldws, const int32_t* group_ends, int64_t num_groups, int64_t M,
+                  int64_t N, int64_t K, void* out, int64_t ldo, int out_type, void* workspace,
+                  int64_t workspace_bytes, void* stream) {
+  const char* what = "block_mm";
+  if (out_type != MXGG_OUT_BF16 && out_type != MXGG_OUT_F32)
+    return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown out_type %d", what, out_type);
+  int rc = check_block_mm(what, group_ends != nullptr, num_groups, M, N, K);
+  if (rc != MXGG_OK) return rc;
   if (M == 0 || N == 0) return MXGG_OK;
   if (!a || !a_scales || !w || !w_scales || !out)
     return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
@@ -1732,45 +1758,68 @@ int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t lda
                      (long long)lda, (long long)ldw, (long long)ldas, (long long)ldws);
   if (!block_rows_aligned(a, lda) || !block_rows_aligned(w, ldw) || w_gstride % 16 != 0)
     return set_error(MXGG_ERR_ALIGNMENT, "%s: a and w must have 16-byte aligned rows", what);
+  rc = check_block_workspace(what, workspace, workspace_bytes,
+                             block_mm_workspace_bytes(M, N, K, num_groups, group_ends != nullptr));
+  if (rc != MXGG_OK) return rc;
   const BlockMmArgs g{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w),
                       w_scales, group_ends, out, lda, ldas, w_gstride, ldw, ws_gstride, ldws, ldo, M,
-                      (int32_t)N, (int32_t)K, (int32_t)num_groups, out_type == MXGG_OUT_F32};
+                      (int32_t)N, (int32_t)K, (int32_t)num_groups, out_type == MXGG_OUT_F32,
+                      static_cast<float*>(workspace), 1};
   return check_launch(launch_block_mm(g, static_cast<hipStream_t>(stream)), what);
+}
+
+static int check_block_wgrad(const char* what, bool grouped, int64_t num_groups, int64_t tokens,
+                             int64_t N, int64_t K) {
+  if (tokens < 0 || tokens % 128 != 0 || N < 0 || K < 0)
+    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld (a multiple of 128), N=%lld, K=%lld", what,
+                     (long long)tokens, (long long)N, (long long)K);
+  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!grouped && num_groups != 1))
+    return set_error(MXGG_ERR_UNSUPPORTED,
+                     "%s: num_groups=%lld (1 to 1024; 1 without group_ends_pad)", what,
+                     (long long)num_groups);
+  if (tokens > kMaxBlockWidth || N > kMaxBlockWidth || K > kMaxBlockWidth ||
+      num_groups * ((N + 127) / 128) * ((K + 127) / 128) >= kMaxBlockGrid)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: tokens=%lld, N=%lld, K=%lld in %lld groups", what,
+                     (long long)tokens, (long long)N, (long long)K, (long long)num_groups);
+  return MXGG_OK;
+}
+
+int64_t mxgg_block_wgrad_workspace_bytes(int grouped, int64_t num_groups, int64_t tokens, int64_t N,
+                                         int64_t K) {
+  if (check_block_wgrad("block_wgrad_workspace_bytes", grouped != 0, num_groups, tokens, N, K) !=
+      MXGG_OK)
+    return -1;
+  return N == 0 || K == 0 ? 0 : block_wgrad_workspace_bytes(tokens, N, K, num_groups);
 }
 
 int mxgg_block_wgrad(const void* go_t, int64_t ldgo, const float* go_scales, int64_t ldgos,
                      const void* ia_t, int64_t ldia, const float* ia_scales, int64_t ldias,
                      const int32_t* group_ends_pad, int64_t num_groups, int64_t tokens, int64_t N,
-                     int64_t K, void* dw, int out_type, void* stream) {
+                     int64_t K, void* dw, int out_type, void* workspace, int64_t workspace_bytes,
+                     void* stream) {
   const char* what = "block_wgrad";
   if (out_type != MXGG_OUT_BF16 && out_type != MXGG_OUT_F32)
     return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: unknown out_type %d", what, out_type);
-  if (tokens < 0 || tokens % 128 != 0 || N < 0 || K < 0)
-    return set_error(MXGG_ERR_SHAPE, "%s: tokens=%lld (a multiple of 128), N=%lld, K=%lld", what,
-                     (long long)tokens, (long long)N, (long long)K);
-  if (num_groups < 1 || num_groups > kMaxGroupsAbi || (!group_ends_pad && num_groups != 1))
-    return set_error(MXGG_ERR_UNSUPPORTED,
-                     "%s: num_groups=%lld (1 to 1024; 1 without group_ends_pad)", what,
-                     (long long)num_groups);
-  if (tokens > kMaxBlockWidth || N > kMaxBlockWidth || K > kMaxBlockWidth || ldgo > kMaxBlockWidth ||
-      ldia > kMaxBlockWidth ||
-      num_groups * ((N + 127) / 128) * ((K + 127) / 128) >= kMaxBlockGrid)
-    return set_error(MXGG_ERR_UNSUPPORTED, "%s: tokens=%lld, N=%lld, K=%lld in %lld groups", what,
-                     (long long)tokens, (long long)N, (long long)K, (long long)num_groups);
+  int rc = check_block_wgrad(what, group_ends_pad != nullptr, num_groups, tokens, N, K);
+  if (rc != MXGG_OK) return rc;
   if (N == 0 || K == 0) return MXGG_OK;
   if (!dw || (tokens > 0 && (!go_t || !go_scales || !ia_t || !ia_scales)))
     return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (tokens > 0 && (ldgo < tokens || ldia < tokens || ldgos < N || ldias < K))
     return set_error(MXGG_ERR_SHAPE, "%s: leading dimension smaller than the row", what);
-  if (tokens / 128 * std::max(ldgos, ldias) > kMaxBufferBytes / 4)
-    return set_error(MXGG_ERR_UNSUPPORTED, "%s: ldgos=%lld, ldias=%lld", what, (long long)ldgos,
-                     (long long)ldias);
+  if (ldgo > kMaxBlockWidth || ldia > kMaxBlockWidth ||
+      tokens / 128 * std::max(ldgos, ldias) > kMaxBufferBytes / 4)
+    return set_error(MXGG_ERR_UNSUPPORTED, "%s: ldgo=%lld, ldia=%lld, ldgos=%lld, ldias=%lld", what,
+                     (long long)ldgo, (long long)ldia, (long long)ldgos, (long long)ldias);
   if (tokens > 0 && (!block_rows_aligned(go_t, ldgo) || !block_rows_aligned(ia_t, ldia)))
     return set_error(MXGG_ERR_ALIGNMENT, "%s: operands must have 16-byte aligned rows", what);
+  rc = check_block_workspace(what, workspace, workspace_bytes,
+                             block_wgrad_workspace_bytes(tokens, N, K, num_groups));
+  if (rc != MXGG_OK) return rc;
   const BlockWgradArgs g{static_cast<const uint8_t*>(go_t), go_scales,
                          static_cast<const uint8_t*>(ia_t), ia_scales, group_ends_pad, dw, ldgo,
                          ldgos, ldia, ldias, tokens, (int32_t)N, (int32_t)K, (int32_t)num_groups,
-                         out_type == MXGG_OUT_F32};
+                         out_type == MXGG_OUT_F32, static_cast<float*>(workspace), 1};
   return check_launch(launch_block_wgrad(g, static_cast<hipStream_t>(stream)), what);
 }
 

@@ -250,8 +250,11 @@ struct BlockMmArgs {
   void* out;             // [M][ldo]
   int64_t lda, ldas, w_group, ldw, ws_group, ldws, ldo, M;
   int32_t N, K, E, out_f32;
+  float* partial;        // block_mm_workspace_bytes(): sums of a split contraction
+  int32_t parts;         // set by the launcher
 };
-hipError_t launch_block_mm(const BlockMmArgs& args, hipStream_t stream);
+int64_t block_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t E, bool grouped);
+hipError_t launch_block_mm(BlockMmArgs args, hipStream_t stream);
 struct BlockWgradArgs {
   const uint8_t* go;     // dY^T [N][ldgo]
   const float* gos;      // [tokens / 128][ldgos]
@@ -261,8 +264,11 @@ struct BlockWgradArgs {
   void* dw;              // [E][N][K]
   int64_t ldgo, ldgos, ldia, ldias, tokens;
   int32_t N, K, E, out_f32;
+  float* partial;        // block_wgrad_workspace_bytes()
+  int32_t parts;         // set by the launcher
 };
-hipError_t launch_block_wgrad(const BlockWgradArgs& args, hipStream_t stream);
+int64_t block_wgrad_workspace_bytes(int64_t tokens, int64_t N, int64_t K, int64_t E);
+hipError_t launch_block_wgrad(BlockWgradArgs args, hipStream_t stream);
 
 // Token log probabilities (logp.hip).  The launchers fill in the last fields.
 struct LogpArgs {

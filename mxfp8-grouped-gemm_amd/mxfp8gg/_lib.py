@@ -218,11 +218,15 @@ SIGNATURES = {
     "mxgg_block_mm": (
         _I,
         [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64,
-         _I, _P],
+         _I, _P, _I64, _P],
     ),
+    "mxgg_block_mm_workspace_bytes": (_I64, [_I, _I64, _I64, _I64, _I64]),
     "mxgg_block_wgrad": (
-        _I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I, _P],
+        _I,
+        [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I, _P, _I64,
+         _P],
     ),
+    "mxgg_block_wgrad_workspace_bytes": (_I64, [_I, _I64, _I64, _I64, _I64]),
     "mxgg_add_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P]),
     "mxgg_add_rms_norm_grad": (
         _I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _P],

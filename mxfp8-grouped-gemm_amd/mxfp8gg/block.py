@@ -191,13 +191,17 @@ def fp8_block_mm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor,
         ws = ws.contiguous()
     ends = None if offs is None else _group_ends(offs, E, a.device)
     y = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    lib = _lib.load()
+    nbytes = lib.mxgg_block_mm_workspace_bytes(offs is not None, E, M, N, K)
+    ws_buf = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes > 0 else None
     _lib.check(
-        _lib.load().mxgg_block_mm(
+        lib.mxgg_block_mm(
             a.data_ptr(), _ld(a), a_s.data_ptr(), ldas, w.data_ptr(),
             w.stride(0) if w.dim() == 3 and E > 1 else N * K, _ld(w[0] if w.dim() == 3 else w),
             ws.data_ptr(), _blocks(N) * _blocks(K), _blocks(K),
             ends.data_ptr() if ends is not None else None, E, M, N, K, y.data_ptr(), N, out,
-            _stream_ptr(a)), "fp8_block_mm")
+            ws_buf.data_ptr() if ws_buf is not None else None, max(nbytes, 0), _stream_ptr(a)),
+        "fp8_block_mm")
     return y
 
 
@@ -219,11 +223,15 @@ def fp8_block_wgrad(go_t: torch.Tensor, go_scales: torch.Tensor, ia_t: torch.Ten
     ends = None if offs_pad is None else _ends(offs_pad, go)
     E = 1 if ends is None else ends.numel()
     dw = torch.empty((E, N, K), dtype=out_dtype, device=go.device)
+    lib = _lib.load()
+    nbytes = lib.mxgg_block_wgrad_workspace_bytes(ends is not None, E, T, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=go.device) if nbytes > 0 else None
     _lib.check(
-        _lib.load().mxgg_block_wgrad(go.data_ptr(), _ld(go), gs.data_ptr(), ldgs, ia.data_ptr(),
+        lib.mxgg_block_wgrad(go.data_ptr(), _ld(go), gs.data_ptr(), ldgs, ia.data_ptr(),
                                      _ld(ia), xs.data_ptr(), ldxs,
                                      ends.data_ptr() if ends is not None else None, E, T, N, K,
-                                     dw.data_ptr(), out, _stream_ptr(go)), "fp8_block_wgrad")
+                                     dw.data_ptr(), out, ws.data_ptr() if ws is not None else None,
+                                     max(nbytes, 0), _stream_ptr(go)), "fp8_block_wgrad")
     return dw if ends is not None else dw[0]
 
 

@@ -161,7 +161,7 @@ def _weights(gpu, E, N, K, seed):
     return mxfp8gg.to_fp8_block_weight(w)
 
 
-MM = [(1, 16, 16), (1, 4096, 7168), (5, 130, 144), (16, 256, 1024), (17, 48, 2064), (33, 100, 400),
+MM = [(300, 400, 4112), (1003, 2112, 1040), (70, 20, 8192), (1, 16, 16), (1, 4096, 7168), (5, 130, 144), (16, 256, 1024), (17, 48, 2064), (33, 100, 400),
       (64, 272, 512), (65, 128, 128), (100, 130, 1040), (128, 384, 256), (200, 2112, 784),
       (257, 300, 272), (700, 1000, 144), (2049, 4000, 400), (4096, 4096, 256)]
 
@@ -182,7 +182,7 @@ def test_mm(gpu, M, N, K, dtype):
 @pytest.mark.parametrize("sizes,N,K", [([3, 0, 9, 1], 144, 272), ([0, 0, 0, 1], 256, 128),
                                        ([70, 0, 300, 129, 1], 272, 400), ([1000, 0, 24, 300], 520, 144),
                                        ([513, 2000, 0, 255, 1300], 2000, 256), ([0, 0], 16, 16),
-                                       ([5] * 100, 64, 128)])
+                                       ([5] * 100, 64, 128), ([90, 0, 200, 33], 144, 2064)])
 def test_grouped_mm(gpu, sizes, N, K):
     M = sum(sizes) + 5
     x = _x(gpu, M, K, seed=M)
@@ -197,7 +197,8 @@ def test_grouped_mm(gpu, sizes, N, K):
         at += n
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (130, 144, 272), (1000, 256, 512), (300, 4096, 4112)])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (130, 144, 272), (1000, 256, 512), (300, 4096, 4112),
+                                   (5000, 144, 160)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_wgrad(gpu, M, N, K, dtype):
     gt, gs, _ = mxfp8gg.to_fp8_block_dim1(_x(gpu, M, N, seed=M))
@@ -207,7 +208,7 @@ def test_wgrad(gpu, M, N, K, dtype):
     _near(dw, a @ b.t(), a.abs() @ b.abs().t(), gt.shape[1] // 128)
 
 
-@pytest.mark.parametrize("sizes,N,K", [([3, 0, 200, 129], 144, 272), ([700, 0, 0, 1000], 2064, 1024)])
+@pytest.mark.parametrize("sizes,N,K", [([3, 0, 200, 129], 144, 272), ([700, 0, 0, 1000], 2064, 1024), ([3000, 1, 0, 5000], 128, 272)])
 def test_grouped_wgrad(gpu, sizes, N, K):
     M = sum(sizes) + 7
     offs = torch.tensor(sizes, device=gpu).cumsum(0).int()
@@ -309,7 +310,7 @@ def test_operand_layouts(gpu):
 
 def test_rows_past_the_groups_stay(gpu):
     """Rows outside every group are not written, whatever their scales hold."""
-    for M, K in ((20, 256), (400, 256), (3000, 128)):
+    for M, K in ((20, 256), (400, 256), (400, 4096), (3000, 128)):
         x = _x(gpu, M, K, seed=M)
         q, s = mxfp8gg.to_fp8_block_dim0(x)
         s = s.clone()
@@ -319,9 +320,11 @@ def test_rows_past_the_groups_stay(gpu):
         out = torch.full((M, 256), 7.0, dtype=torch.bfloat16, device=gpu)
         lib = mxfp8gg.load_library()
         s = s.t().contiguous()
+        ws_buf = torch.empty(lib.mxgg_block_mm_workspace_bytes(1, 2, M, 256, K), dtype=torch.uint8, device=gpu)
         assert lib.mxgg_block_mm(q.data_ptr(), K, s.data_ptr(), M, wq.data_ptr(), 256 * K, K, ws.data_ptr(),
                                  2 * ws.shape[2], ws.shape[2], offs.data_ptr(), 2, M, 256, K,
-                                 out.data_ptr(), 256, 0, torch.cuda.current_stream().cuda_stream) == 0
+                                 out.data_ptr(), 256, 0, ws_buf.data_ptr(), ws_buf.numel(),
+                                 torch.cuda.current_stream().cuda_stream) == 0
         assert (out[M // 2:] == 7).all() and torch.isfinite(out).all()
 
 
