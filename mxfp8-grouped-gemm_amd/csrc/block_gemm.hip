@@ -38,20 +38,28 @@ struct BlockOperand {
   int64_t rows;
 };
 
-// Workgroup of WP x WQ waves, each 64 GP rows of P by 64 rows of Q.
-template <int WP, int GP, int WQ, bool ROWS>
+// Workgroup of WP x WQ waves, each 64 GP rows of P by 16 FQ rows of Q (FQ = 2: every other
+// pair of a run of 64); operands in a ring of NS stages: two of 64 KB for 256 x 256 tiles,
+// four of 32 KB for 128 x 128 ones.
+template <int WP, int GP, int WQ, int FQ, bool ROWS>
 struct BlockTile {
-  static constexpr int kP = 64 * WP * GP, kQ = 64 * WQ;
+  static constexpr int NS = GP == 2 ? 2 : 4;
+  static constexpr int kP = 64 * WP * GP, kQ = 16 * FQ * WQ;
   static constexpr int kWavesT = WP * WQ, kThreadsT = 64 * kWavesT;
   static constexpr uint32_t kData = (uint32_t)(kP + kQ) * kBlkK;
   static constexpr uint32_t kScales = 4u * (kP + kQ);     // bytes of a stage's scales
   static constexpr int kLoads = (kP + kQ) / 8 / kWavesT;  // data loads of a wave and stage
   static constexpr int kFrags = 4 * GP;                   // of P
   struct Ring {
-    uint8_t data[2][kData];
-    uint8_t scales[4][kScales];  // of their own: read until the stage's last products
+    uint8_t data[NS][kData];
+    uint8_t scales[2 * NS][kScales];  // of their own: read until the stage's last products
   };
-  static_assert((kP + kQ) / 64 == kWavesT, "one scale load a wave");
+  // Two-stage ring: Q's part of a slot is in registers when its stage begins, and takes
+  // its next loads then, half a stage before P's.
+  static constexpr bool kEarlyQ = NS == 2;
+  static constexpr int kLoadsQ = kLoads / 2;
+  static constexpr uint32_t kScaleWaves = (kP + kQ) / 64;  // those beyond repeat their loads
+  static_assert(kWavesT % kScaleWaves == 0, "one scale load a wave");
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) {
@@ -94,8 +102,9 @@ struct BlockStream {
     vbase_p = r * ldp + kcol;
     vbase_q = r * ldq + kcol;
     // scales: the first T::kQ / 64 waves take Q's rows, the others P's
-    const bool of_q = wave < (uint32_t)T::kQ / 64u;
-    const uint32_t w = of_q ? wave : wave - (uint32_t)T::kQ / 64u;
+    const uint32_t sw = wave % T::kScaleWaves;
+    const bool of_q = sw < (uint32_t)T::kQ / 64u;
+    const uint32_t w = of_q ? sw : sw - (uint32_t)T::kQ / 64u;
     if (of_q || ROWS) {
       const BlockOperand& X = of_q ? Q : P;
       // P's floats are kept in the order in which a lane's four rows follow each other
@@ -122,7 +131,7 @@ struct BlockStream {
   __device__ __forceinline__ void load(Ring& ring, uint32_t s, uint32_t bp, uint32_t bq) const {
     const uint32_t wave = wave_id();
     if constexpr (J == T::kLoads) {
-      dma_x1(ds, lds_offset(ring.scales[s & 3u]) + 256u * wave, vs, s * sstep);
+      dma_x1(ds, lds_offset(ring.scales[s % (2 * T::NS)]) + 256u * (wave % T::kScaleWaves), vs, s * sstep);
     } else {
       const uint32_t run = (uint32_t)T::kWavesT * J + wave;  // 1 KB runs of the stage
       constexpr uint32_t kRunsP = T::kP / 8;
@@ -130,20 +139,23 @@ struct BlockStream {
       constexpr bool p = (uint32_t)T::kWavesT * J < kRunsP;
       const uint32_t i = (p ? run : run - kRunsP) >> 2;  // 32-slot run of the operand
       const uint32_t row = (i >> 2) * 128u + (i & 3u);
-      dma_x4(p ? dp : dq, lds_offset(ring.data[s & 1u]) + 1024u * run, p ? bp : bq,
+      dma_x4(p ? dp : dq, lds_offset(ring.data[s % T::NS]) + 1024u * run, p ? bp : bq,
              row * (p ? ldp : ldq));
     }
   }
-  template <class Ring, int... J>
-  __device__ __forceinline__ void load_all(Ring& ring, uint32_t s,
-                                           std::integer_sequence<int, J...>) const {
+  // Loads [FROM, TO) of stage s.
+  template <int FROM, int TO, class Ring>
+  __device__ __forceinline__ void load_range(Ring& ring, uint32_t s, uint32_t bp, uint32_t bq) const {
+    if constexpr (FROM < TO) {
+      load<FROM>(ring, s, bp, bq);
+      load_range<FROM + 1, TO>(ring, s, bp, bq);
+    }
+  }
+  template <int FROM, int TO, class Ring>
+  __device__ __forceinline__ void load_range(Ring& ring, uint32_t s) const {
     uint32_t bp, bq;
     base(s, bp, bq);
-    (load<J>(ring, s, bp, bq), ...);
-  }
-  template <class Ring>
-  __device__ __forceinline__ void load_all(Ring& ring, uint32_t s) const {
-    load_all(ring, s, std::make_integer_sequence<int, T::kLoads + 1>{});
+    load_range<FROM, TO>(ring, s, bp, bq);
   }
 };
 
@@ -155,38 +167,47 @@ __device__ __forceinline__ void steps(F& f, std::integer_sequence<int, N...>) {
 }
 
 // acc[p][q] of the wave: P fragment p = 4 G + i holds rows 64 G + 4 m + i of the wave's
-// part (m = 0..15), Q fragment q rows 4 m + q; D[4g + r][c] is in register r of lane
+// part (m = 0..15), Q fragment q rows 4 m + q (+ 2 for the second wave of a part, FQ = 2); D[4g + r][c] is in register r of lane
 // c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i are 16 in a row for every G.
 // qn: rows of Q that are wanted; a wave with none of them only loads.
-template <int WP, int GP, int WQ, bool ROWS, class Ring>
+template <int WP, int GP, int WQ, int FQ, bool ROWS, class Ring>
 __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P,
                                                const BlockOperand& Q, uint32_t len, int64_t qn,
-                                               v4f (&acc)[4 * GP][4]) {
-  using T = BlockTile<WP, GP, WQ, ROWS>;
+                                               v4f (&acc)[4 * GP][FQ]) {
+  using T = BlockTile<WP, GP, WQ, FQ, ROWS>;
 #pragma unroll
   for (int p = 0; p < 4 * GP; ++p)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[p][q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < FQ; ++q) acc[p][q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   len = uniform(len);
   if (len == 0) return;
   const uint32_t nst = (len + kBlkK - 1) / kBlkK;
   BlockStream<T, ROWS> st;
   st.init(P, Q, len);
-  st.load_all(ring, 0);
-  if (nst > 1) {
-    st.load_all(ring, 1);
-    wait_barrier<T::kLoads + 1>();
-  } else {
-    wait_barrier<0>();
-  }
+  constexpr int NS = T::NS, kAll = T::kLoads + 1;  // loads of a wave and stage
+#pragma unroll
+  for (uint32_t i = 0; i < (uint32_t)NS; ++i)
+    if (i < nst) st.template load_range<0, kAll>(ring, i);
+  // stage 0 has landed, the later ones may be on their way
+  if (NS == 4 && nst > 3) wait_barrier<3 * kAll>();
+  else if (NS == 4 && nst > 2) wait_barrier<2 * kAll>();
+  else if (nst > 1) wait_barrier<kAll>();
+  else wait_barrier<0>();
   MXGG_FENCE();
 
   const uint32_t lane = threadIdx.x & 63u, wave = wave_id();
-  const uint32_t wp = wave % WP, wq = wave / WP;
-  if (uniform((uint32_t)(64 * (int64_t)wq >= qn))) {
+  const uint32_t wp = wave % WP, wq = wave / WP * FQ / 4, wf = wave / WP * FQ % 4;
+  if (uniform((uint32_t)(64 * (int64_t)wq >= qn))) {  // the same barriers and loads, nothing else
     for (uint32_t s = 0; s < nst; ++s) {
-      wait_barrier<0>();
-      if (s + 2 < nst) st.load_all(ring, s + 2);
+      const bool more = s + NS < nst;
+      if (T::kEarlyQ) release_barrier();
+      if (T::kEarlyQ && more) st.template load_range<T::kLoadsQ, T::kLoads>(ring, s + NS);
+      if (T::kEarlyQ && more) wait_barrier<T::kLoadsQ>();
+      else if (!T::kEarlyQ && s + NS <= nst) wait_barrier<(NS - 2) * kAll>();
+      else wait_barrier<0>();
+      if (!more) continue;
+      st.template load_range<0, T::kEarlyQ ? T::kLoadsQ : T::kLoads>(ring, s + NS);
+      st.template load_range<T::kLoads, kAll>(ring, s + NS);
     }
     release_barrier();
     return;
@@ -198,8 +219,8 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
   uint32_t pa[GP];
 #pragma unroll
   for (int G = 0; G < GP; ++G) pa[G] = part(wp * GP + G);
-  const uint32_t qa = T::kP * kBlkK + part(wq);
-  const uint32_t sq_at = 4u * (64u * wq + 4u * m);  // Q rows 4 m .. + 3: fragments 0..3
+  const uint32_t qa = T::kP * kBlkK + part(wq) + 4096u * wf;
+  const uint32_t sq_at = 4u * (64u * wq + 4u * m + wf);  // of the rows of fragments 0, 1, ..
   const uint32_t sp_at = 4u * T::kQ + 256u * wp * GP;
   const auto read_p = [&](const uint8_t* s, int p) __attribute__((always_inline)) {
     const uint8_t* at = s + pa[p >> 2] + 4096u * (p & 3);
@@ -218,19 +239,20 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
   };
 
   // P fragments are read kAhead steps before their products
-  constexpr int kF = 4 * GP, kN = 4 * kF, kLag = 2, kAhead = 3, kW = kAhead + 1;
-  v8i fa[kW], fb[4];
-  float4 spn[2], sqn;   // scales of the fragments ahead, and of the stage ahead
-  float sc[4];          // of the stage: Q's scale (times P's)
+  constexpr int kF = 4 * GP, kN = FQ * kF, kLag = 2, kAhead = 3, kW = kAhead + 1;
+  v8i fa[kW], fb[FQ];
+  float4 spn[2];
+  struct alignas(4 * FQ) Scales { float v[FQ]; } sqn;  // of the stage ahead, as spn of the fragments ahead
+  float sc[FQ];         // of the stage: Q's scale (times P's)
   v4f t[4];             // products in flight
   float4 spt[4];
   float sct[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) fb[q] = read_q(ring.data[0], q);
+  for (int q = 0; q < FQ; ++q) fb[q] = read_q(ring.data[0], q);
 #pragma unroll
   for (int p = 0; p < kAhead; ++p) fa[p] = read_p(ring.data[0], p);
   spn[0] = read_sp(ring.scales[0], 0);
-  sqn = *reinterpret_cast<const float4*>(ring.scales[0] + sq_at);
+  sqn = *reinterpret_cast<const Scales*>(ring.scales[0] + sq_at);
   const auto add = [&](v4f& a, const v4f& x, const float4& sp, float f) __attribute__((always_inline)) {
     if constexpr (ROWS) {
       a[0] = __builtin_fmaf(x[0], sp.x * f, a[0]);
@@ -243,41 +265,46 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
     }
   };
   uint32_t s = 0;
-  // no branch inside: the compiler would move the matrix instructions past it
-  const auto stage = [&](auto loads) __attribute__((always_inline)) {
+  // no branch inside: the compiler would move the matrix instructions past it.
+  // LEFT: loads that may be under way where the next stage has to have landed
+  const auto stage = [&](auto loads, auto left) __attribute__((always_inline)) {
     constexpr bool LOADS = decltype(loads)::value;
-    const uint8_t* cur = ring.data[s & 1u];
-    const uint8_t* nxt = ring.data[(s & 1u) ^ 1u];
-    const uint8_t* scales = ring.scales[s & 3u];
-    const uint8_t* scales_nxt = ring.scales[(s + 1) & 3u];
+    constexpr int LEFT = decltype(left)::value;
+    const uint8_t* cur = ring.data[s % NS];
+    const uint8_t* nxt = ring.data[(s + 1) % NS];
+    const uint8_t* scales = ring.scales[s % (2 * NS)];
+    const uint8_t* scales_nxt = ring.scales[(s + 1) % (2 * NS)];
     uint32_t bp = 0, bq = 0;
-    if constexpr (LOADS) st.base(s + 2, bp, bq);
-    sc[0] = sqn.x;
-    sc[1] = sqn.y;
-    sc[2] = sqn.z;
-    sc[3] = sqn.w;
-    if constexpr (!ROWS) {
+    if constexpr (LOADS) st.base(s + NS, bp, bq);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) sc[q] *= spn[0].x;
-    }
+    for (int q = 0; q < FQ; ++q) sc[q] = ROWS ? sqn.v[q] : sqn.v[q] * spn[0].x;
     const auto step = [&](auto index) __attribute__((always_inline)) {
-      constexpr int n = decltype(index)::value, p = n / 4, q = n % 4;
+      constexpr int n = decltype(index)::value, p = n / FQ, q = n % FQ;
       if constexpr (n < kN) {
         if constexpr (q == 0) {
+          if constexpr (T::kEarlyQ && p == 1) {
+            release_barrier();  // every wave has read Q of this stage
+            MXGG_FENCE();
+          }
           if constexpr (p == kF - kAhead) {
             // the next stage has landed, every wave has read this one
-            wait_barrier<0>();
+            wait_barrier<LEFT>();
             MXGG_FENCE();
           }
           constexpr int pn = (p + kAhead) % kF;
           fa[(p + kAhead) % kW] = read_p(p + kAhead < kF ? cur : nxt, pn);
           if constexpr (ROWS || p == kF - 1)
             spn[(p + 1) & 1] = read_sp(p + 1 < kF ? scales : scales_nxt, (p + 1) % kF);
-          if constexpr (p == kF - 1) sqn = *reinterpret_cast<const float4*>(scales_nxt + sq_at);
+          if constexpr (p == kF - 1) sqn = *reinterpret_cast<const Scales*>(scales_nxt + sq_at);
         }
         // one load after each product: a load holds its wave until it is accepted
-        constexpr int j = n - 4 * (kF - kAhead);
-        if constexpr (LOADS && j >= 0 && j <= T::kLoads) st.template load<j>(ring, s + 2, bp, bq);
+        static_assert(!T::kEarlyQ || FQ >= T::kLoadsQ, "Q's loads follow the products of p = 1");
+        static_assert(FQ * kAhead > (T::kEarlyQ ? T::kLoadsQ : T::kLoads), "a product for each load");
+        constexpr int j0 = n - FQ * (kF - kAhead);
+        constexpr int j = !T::kEarlyQ ? j0 : p == 0 ? -1 : p == 1 ? T::kLoadsQ + q
+                          : j0 < T::kLoadsQ ? j0 : j0 == T::kLoadsQ ? T::kLoads : -1;
+        if constexpr (LOADS && j >= 0 && j <= T::kLoads)
+          st.template load<j>(ring, s + NS, bp, bq);
         t[n & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
             fa[p % kW], fb[q], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
         if constexpr (p == kF - 1) fb[q] = read_q(nxt, q);
@@ -287,57 +314,85 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
       }
       if constexpr (n >= kLag) {
         constexpr int o = n - kLag;
-        add(acc[o / 4][o % 4], t[o & 3], spt[o & 3], sct[o & 3]);
+        add(acc[o / FQ][o % FQ], t[o & 3], spt[o & 3], sct[o & 3]);
       }
       MXGG_FENCE();
     };
     steps(step, std::make_integer_sequence<int, kN + kLag>{});
   };
-  for (; s + 2 < nst; ++s) stage(std::true_type{});
-  do stage(std::false_type{});
-  while (++s < nst);
+  constexpr int kLeft = T::kEarlyQ ? T::kLoadsQ : (NS - 2) * kAll;
+  for (; s + NS < nst; ++s) stage(std::true_type{}, std::integral_constant<int, kLeft>{});
+  if constexpr (NS == 4)  // stages s + 2 and s + 3 on their way
+    if (s + NS == nst) stage(std::false_type{}, std::integral_constant<int, kLeft>{}), ++s;
+  for (; s < nst; ++s) stage(std::false_type{}, std::integral_constant<int, 0>{});
   // the slots take the next tile's loads only after every wave's last reads
   release_barrier();
 }
 
-// The wave's part of a tile to rows of `out` (row = Q row, contiguous along P).
-template <int GP, typename O>
-__device__ __forceinline__ void block_store(const v4f (&acc)[4 * GP][4], O* out, int64_t ldo,
+// The wave's part of a tile to rows of `out` (row = Q row, contiguous along P).  A lane
+// holds 16 elements in a row, its neighbours at 16 lanes' distance the next ones; 16-byte
+// pieces are exchanged between them, so that each store instruction writes whole runs of 64
+// bytes of every row (fp32: pieces (g, e) to lane e; bf16: the high piece to the high half).
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// q0: the row of the wave's first fragment.
+template <int GP, int FQ, typename O>
+__device__ __forceinline__ void block_store(const v4f (&acc)[4 * GP][FQ], O* out, int64_t ldo,
                                             int64_t p0, int64_t pn, int64_t q0, int64_t qn) {
+  constexpr bool kF32 = sizeof(O) == 4;
+  constexpr int kPieces = kF32 ? 4 : 2, kPer = 16 / sizeof(O);  // 16-byte pieces of a lane, elements
   const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < FQ; ++q) {
     const int64_t row = q0 + 4 * c + q;
-    if (row >= qn) continue;
 #pragma unroll
     for (int G = 0; G < GP; ++G) {
-      const int64_t n = p0 + 64 * G + 16 * g;
-      O* o = out + row * ldo + n;
       // element 4 r + i of the lane's 16
       const auto at = [&](int e) { return acc[4 * G + (e & 3)][q][e >> 2]; };
-      if (n + 16 <= pn) {
-        if constexpr (sizeof(O) == 4) {
+      uint32_t w[kPieces][4];
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float f[4] = {at(e), at(e + 1), at(e + 2), at(e + 3)};
-            __builtin_memcpy(o + e, f, 16);
-          }
+      for (int e = 0; e < kPieces; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kF32) w[e][j] = __float_as_uint(at(4 * e + j));
+          else w[e][j] = pack_bf16x2(at(8 * e + 2 * j), at(8 * e + 2 * j + 1));
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kF32) {
+          swap32(w[0][j], w[2][j]);
+          swap32(w[1][j], w[3][j]);
+          swap16(w[0][j], w[1][j]);
+          swap16(w[2][j], w[3][j]);
+        } else {
+          swap32(w[0][j], w[1][j]);
+        }
+      }
+      if (row >= qn) continue;
+#pragma unroll
+      for (int e = 0; e < kPieces; ++e) {
+        // piece e of this lane now: of lane (high bits from e), piece (from the lane)
+        const uint32_t piece = kF32 ? 4u * e + g : 4u * e + 2u * (g & 1u) + (g >> 1);
+        const int64_t n = p0 + 64 * G + (int64_t)(kPer * piece);
+        O* o = out + row * ldo + n;
+        if (n + kPer <= pn) {
+          __builtin_memcpy(o, w[e], 16);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            const uint32_t w[4] = {pack_bf16x2(at(e), at(e + 1)), pack_bf16x2(at(e + 2), at(e + 3)),
-                                   pack_bf16x2(at(e + 4), at(e + 5)),
-                                   pack_bf16x2(at(e + 6), at(e + 7))};
-            __builtin_memcpy(o + e, w, 16);
-          }
+          for (int j = 0; j < kPer; ++j)
+            if (n + j < pn) {
+              if constexpr (kF32) o[j] = __uint_as_float(w[e][j]);
+              else o[j] = (uint16_t)(w[e][j >> 1] >> (16 * (j & 1)));
+            }
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (n + e < pn) {
-            if constexpr (sizeof(O) == 4) o[e] = at(e);
-            else o[e] = (uint16_t)pack_bf16x2(at(e), 0.0f);
-          }
       }
     }
   }
@@ -401,10 +456,16 @@ struct Part {
       : first(blocks * part / parts), last(blocks * (part + 1) / parts) {}
 };
 
+// Row of a tile that a wave's first Q fragment begins with.
+template <int WP, int FQ>
+__device__ __forceinline__ int64_t wave_row(uint32_t wave) {
+  return 64 * (wave / WP * FQ / 4) + wave / WP * FQ % 4;
+}
+
 // Workgroups [0, grid): tiles, of the first part of the contraction; and so on.
-template <int WP, int GP, int WQ>
+template <int WP, int GP, int WQ, int FQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
-  using T = BlockTile<WP, GP, WQ, false>;
+  using T = BlockTile<WP, GP, WQ, FQ, false>;
   __shared__ __attribute__((aligned(1024))) typename T::Ring ring;
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.N + T::kP - 1) / T::kP;
@@ -425,22 +486,22 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
                        a.N - n0};
   const BlockOperand Q{a.a + m0 * a.lda + k.first * kBlkK, a.as + m0 + k.first * a.ldas, a.lda,
                        a.ldas, a.M - m0};
-  v4f acc[4 * GP][4];
-  block_mainloop<WP, GP, WQ, false>(
+  v4f acc[4 * GP][FQ];
+  block_mainloop<WP, GP, WQ, FQ, false>(
       ring, P, Q, (uint32_t)(min((int64_t)a.K, k.last * kBlkK) - k.first * kBlkK), at.end - m0, acc);
   const uint32_t wave = wave_id();
-  const int64_t p0 = n0 + 64 * GP * (wave % WP), q0 = m0 + 64 * (wave / WP);
+  const int64_t p0 = n0 + 64 * GP * (wave % WP), q0 = m0 + wave_row<WP, FQ>(wave);
   if (a.parts > 1)
-    block_store<GP>(acc, a.partial + part * a.M * a.N, a.N, p0, a.N, q0, at.end);
+    block_store<GP, FQ>(acc, a.partial + part * a.M * a.N, a.N, p0, a.N, q0, at.end);
   else if (a.out_f32)
-    block_store<GP>(acc, static_cast<float*>(a.out), a.ldo, p0, a.N, q0, at.end);
+    block_store<GP, FQ>(acc, static_cast<float*>(a.out), a.ldo, p0, a.N, q0, at.end);
   else
-    block_store<GP>(acc, static_cast<uint16_t*>(a.out), a.ldo, p0, a.N, q0, at.end);
+    block_store<GP, FQ>(acc, static_cast<uint16_t*>(a.out), a.ldo, p0, a.N, q0, at.end);
 }
 
-template <int WP, int GP, int WQ>
+template <int WP, int GP, int WQ, int FQ>
 __global__ __launch_bounds__(64 * WP * WQ) void k_block_wgrad(BlockWgradArgs a) {
-  using T = BlockTile<WP, GP, WQ, true>;
+  using T = BlockTile<WP, GP, WQ, FQ, true>;
   __shared__ __attribute__((aligned(1024))) typename T::Ring ring;
   __shared__ int32_t ends_s[1024];
   const int64_t np = (a.K + T::kP - 1) / T::kP, nq = (a.N + T::kQ - 1) / T::kQ;
@@ -465,17 +526,17 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_block_wgrad(BlockWgradArgs a) 
                        a.K - k0};
   const BlockOperand Q{a.go + n0 * a.ldgo + b0 * kBlkK, a.gos + b0 * a.ldgos + n0, a.ldgo, a.ldgos,
                        a.N - n0};
-  v4f acc[4 * GP][4];
-  block_mainloop<WP, GP, WQ, true>(ring, P, Q, (uint32_t)((b1 - b0) * kBlkK), a.N - n0, acc);
+  v4f acc[4 * GP][FQ];
+  block_mainloop<WP, GP, WQ, FQ, true>(ring, P, Q, (uint32_t)((b1 - b0) * kBlkK), a.N - n0, acc);
   const uint32_t wave = wave_id();
-  const int64_t p0 = k0 + 64 * GP * (wave % WP), q0 = n0 + 64 * (wave / WP);
+  const int64_t p0 = k0 + 64 * GP * (wave % WP), q0 = n0 + wave_row<WP, FQ>(wave);
   const int64_t nk = (int64_t)a.N * a.K;
   if (a.parts > 1)
-    block_store<GP>(acc, a.partial + (part * a.E + g) * nk, a.K, p0, a.K, q0, a.N);
+    block_store<GP, FQ>(acc, a.partial + (part * a.E + g) * nk, a.K, p0, a.K, q0, a.N);
   else if (a.out_f32)
-    block_store<GP>(acc, static_cast<float*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
+    block_store<GP, FQ>(acc, static_cast<float*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
   else
-    block_store<GP>(acc, static_cast<uint16_t*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
+    block_store<GP, FQ>(acc, static_cast<uint16_t*>(a.dw) + g * nk, a.K, p0, a.K, q0, a.N);
 }
 
 // Sums the parts of a split product in their order: out[row][col] of `rows` rows (those
@@ -490,33 +551,54 @@ __global__ __launch_bounds__(256) void k_block_join(const float* __restrict__ pa
     for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
     rows = min(rows, (int64_t)top);
   }
-  const int64_t wide = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / wide, col = i % wide * 4;
+  // a split product has fewer elements than 2^32 (a few tiles a compute unit)
+  const uint32_t wide = (uint32_t)(cols + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / wide, col = (int64_t)(i % wide) * 4;
   if (row >= rows) return;
   const int n = (int)min((int64_t)4, cols - col);
   const float* p = partial + row * cols + col;
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = 0; k < parts; ++k, p += rows_all * cols) {
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (n == 4) {
-      __builtin_memcpy(v, p, 16);
-    } else {
-      for (int j = 0; j < n; ++j) v[j] = p[j];
+  constexpr int kJoin = 4;  // parts whose loads are in flight
+  for (int k0 = 0; k0 < parts; k0 += kJoin) {
+    float v[kJoin][4];
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[k][j] = 0.0f;
+      if (k0 + k >= parts) continue;
+      const float* at = p + (int64_t)(k0 + k) * rows_all * cols;
+      if (n == 4) {
+        __builtin_memcpy(v[k], at, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (j < n) v[k][j] = at[j];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] += v[j];
+    for (int k = 0; k < kJoin; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += v[k][j];
   }
   if (f32) {
     float* o = static_cast<float*>(out) + row * ldo + col;
-    if (n == 4) __builtin_memcpy(o, s, 16);
-    else
-      for (int j = 0; j < n; ++j) o[j] = s[j];
+    if (n == 4) {
+      __builtin_memcpy(o, s, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < n) o[j] = s[j];
+    }
   } else {
     const uint32_t w[2] = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
     uint16_t* o = static_cast<uint16_t*>(out) + row * ldo + col;
-    if (n == 4) __builtin_memcpy(o, w, 8);
-    else
-      for (int j = 0; j < n; ++j) o[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    if (n == 4) {
+      __builtin_memcpy(o, w, 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < n) o[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
   }
 }
 
@@ -611,29 +693,45 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
   }
 }
 
-// How a product is shared out.  256 x 256 tiles where they fill the chip, else 128 x 128
-// ones (two workgroups a compute unit); where those do not fill it either, the
-// contraction is split in parts of at least kMinBlocks blocks.
+// How a product is shared out: 256 x 256 or 128 x 128 tiles, those also with the contraction
+// split in parts of at least kMinBlocks blocks, whichever takes less by what a block of a
+// tile was measured to take on a full chip (1.6 and 0.66 us; 0.5 where tiles are few), a
+// second launch (7 us with the partial sums' latency) and the partial sums' way there and
+// back (3 TB/s).  Measured, us: 2048 x 4096 x 7168 small tiles 75, large 83; 4096 x 4096 x
+// 7168 large 99; 256 x 4096 x 7168 in 1, 2, 4 parts 30, 25, 22; 128 x 1024 x 7168 in 1 and 7
+// parts 29 and 15; 512 x 512 x 2048 in 1 and 4 parts 11.5 and 12.5.
 struct BlockPlan {
   bool few, large;
   int64_t tiles, parts;
 };
-constexpr int64_t kMinBlocks = 4, kMaxSplit = 16;
-BlockPlan plan(int64_t tiles256, int64_t tiles128, int64_t blocks) {
+constexpr int64_t kMinBlocks = 2, kMaxSplit = 16;
+BlockPlan plan(int64_t tiles256, int64_t tiles128, int64_t blocks, double out_bytes) {
   const int64_t cus = std::max(1, device_cu_count());
-  if (tiles256 >= cus) return {false, true, tiles256, 1};
-  const int64_t parts = std::min({2 * cus / std::max<int64_t>(tiles128, 1), blocks / kMinBlocks, kMaxSplit});
-  return {false, false, tiles128, std::max<int64_t>(parts, 1)};
+  const auto rounds = [&](int64_t t) { return (double)((t + cus - 1) / cus); };
+  BlockPlan best{false, true, tiles256, 1};
+  double least = rounds(tiles256) * 1.6 * blocks;
+  const int64_t most = std::min({std::max<int64_t>(1, cus / std::max<int64_t>(tiles128, 1)),
+                                 std::max<int64_t>(1, blocks / kMinBlocks), kMaxSplit});
+  for (int64_t parts = 1; parts <= most; ++parts) {
+    const double each = tiles128 * parts > cus ? 0.66 : 0.5;
+    const double us = rounds(tiles128) * each * (double)((blocks + parts - 1) / parts) +
+                      (parts > 1 ? 7.0 + 2.0 * parts * out_bytes / 3e6 : 0.0);
+    if (us < least) {
+      least = us;
+      best = {false, false, tiles128, parts};
+    }
+  }
+  return best;
 }
 BlockPlan plan_mm(int64_t M, int64_t N, int64_t K, int64_t E, bool grouped) {
   const int64_t per = (M + E - 1) / E;
   if (per <= 64) return {true, false, 0, 1};
   const auto tiles = [&](int64_t t) { return ((M + t - 1) / t + (grouped ? E : 0)) * ((N + t - 1) / t); };
-  return plan(tiles(256), tiles(128), (K + kBlkK - 1) / kBlkK);
+  return plan(tiles(256), tiles(128), (K + kBlkK - 1) / kBlkK, 4.0 * M * N);
 }
 BlockPlan plan_wgrad(int64_t tokens, int64_t N, int64_t K, int64_t E) {
   const auto tiles = [&](int64_t t) { return E * ((K + t - 1) / t) * ((N + t - 1) / t); };
-  return plan(tiles(256), tiles(128), tokens / kBlkK / E);
+  return plan(tiles(256), tiles(128), std::max<int64_t>(1, tokens / kBlkK / E), 4.0 * E * N * K);
 }
 // Workgroups: a multiple of 8 for each part, for xcd_tile().
 dim3 tile_grid(const BlockPlan& p) { return dim3((unsigned)((p.tiles + 7) / 8 * 8 * p.parts)); }
@@ -673,9 +771,9 @@ hipError_t launch_block_mm(BlockMmArgs a, hipStream_t stream) {
     return hipGetLastError();
   }
   if (p.large)
-    hipLaunchKernelGGL((k_block_fwd<2, 2, 4>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_fwd<2, 2, 4, 4>), tile_grid(p), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_fwd<2, 1, 2>), tile_grid(p), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((k_block_fwd<2, 1, 4, 2>), tile_grid(p), dim3(512), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.parts == 1) return err;
   return join_parts(a.partial, a.parts, a.M, a.ends, a.E, a.N, a.out, a.ldo, a.out_f32, stream);
@@ -686,9 +784,9 @@ hipError_t launch_block_wgrad(BlockWgradArgs a, hipStream_t stream) {
   const BlockPlan p = plan_wgrad(a.tokens, a.N, a.K, a.E);
   a.parts = (int32_t)p.parts;
   if (p.large)
-    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4, 4>), tile_grid(p), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_wgrad<2, 1, 2>), tile_grid(p), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((k_block_wgrad<2, 1, 4, 2>), tile_grid(p), dim3(512), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.parts == 1) return err;
   return join_parts(a.partial, a.parts, (int64_t)a.E * a.N, nullptr, 0, a.K, a.dw, a.K, a.out_f32,
