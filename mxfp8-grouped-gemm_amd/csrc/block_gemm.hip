@@ -602,95 +602,64 @@ __global__ __launch_bounds__(256) void k_block_join(const float* __restrict__ pa
   }
 }
 
-// Few rows: a workgroup takes 16 rows of W and all of its group's rows of A, 16 QF at
-// a time; its eight waves take blocks of the contraction in turn, straight from memory
-// into registers (W is read once and by nobody else), and their sums are added in wave
-// order.  Bound by W's bytes.
-constexpr int kFewWaves = 8;
-template <int QF>
+// Up to 16 rows of one group: a workgroup takes 16 rows of W; its eight waves take blocks of
+// the contraction in turn, straight from memory into registers (W is read once and by
+// nobody else), and their sums are added in wave order.  Bound by W's bytes: 1 x 4096 x
+// 7168 7.3 us (4.0 TB/s; 9.3 in tiles), 16 rows 9.5 (10.7), 32 rows would take 13.3 (11.8).
+constexpr int kFewWaves = 8, kFewRows = 16;
 __global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
-  constexpr int kAhead = QF == 1 ? 8 : QF == 2 ? 4 : 2;  // blocks in flight
-  __shared__ v4f sums[kFewWaves][QF][64];
-  __shared__ int32_t ends_s[1024];
-  const int64_t np = (a.N + 15) / 16;
-  const int64_t g = blockIdx.x / np, n0 = (blockIdx.x % np) * 16;
-  int64_t begin = 0, end = a.M;
-  if (a.ends) {
-    monotone_ends_to_lds(a.ends, a.E, a.M, ends_s);
-    begin = g > 0 ? ends_s[g - 1] : 0;
-    end = ends_s[g];
-  }
+  constexpr int kAhead = 8;  // blocks in flight
+  __shared__ v4f sums[kFewWaves][64];
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, gr = lane >> 4;
-  const uint8_t* w = a.w + g * a.w_group + min(n0 + c, (int64_t)a.N - 1) * a.ldw + 16 * gr;
-  const float* ws = a.ws + g * a.ws_group + n0 / kBlkK * a.ldws;
+  // rows past the end repeat the last one; not stored
+  const int64_t row = min((int64_t)c, a.M - 1);
+  const uint8_t* w = a.w + min(n0 + c, (int64_t)a.N - 1) * a.ldw + 16 * gr;
+  const uint8_t* x = a.a + row * a.lda + 16 * gr;
+  const float *ws = a.ws + n0 / kBlkK * a.ldws, *xs = a.as + row;
   const int nb = (a.K + kBlkK - 1) / kBlkK;
-  const auto chunk = [&](const uint8_t* p, int k) {
-    return k < a.K ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  const auto chunk = [&](const uint8_t* p, int k) {  // bytes k + 16 gr .. + 15 of a row
+    return k + 16 * gr < a.K ? *reinterpret_cast<const uint4*>(p + k) : make_uint4(0, 0, 0, 0);
   };
-  for (int64_t m0 = begin; m0 < end; m0 += 16 * QF) {
-    v4f acc[QF];
+  const auto fragment = [](const uint4& lo, const uint4& hi) {
+    return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+  };
+  v4f acc{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int b0 = wave; b0 < nb; b0 += kFewWaves * kAhead) {
+    uint4 wl[kAhead], wh[kAhead], xl[kAhead], xh[kAhead];
+    float sw[kAhead], sx[kAhead];
 #pragma unroll
-    for (int q = 0; q < QF; ++q) acc[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint8_t* x[QF];
-    const float* xs[QF];
-#pragma unroll
-    for (int q = 0; q < QF; ++q) {  // rows past the end repeat the last one; not stored
-      const int64_t row = min(m0 + 16 * q + c, end - 1);
-      x[q] = a.a + row * a.lda + 16 * gr;
-      xs[q] = a.as + row;
-    }
-    for (int b0 = wave; b0 < nb; b0 += kFewWaves * kAhead) {
-      uint4 wl[kAhead], wh[kAhead], xl[kAhead][QF], xh[kAhead][QF];
-      float sw[kAhead], sx[kAhead][QF];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int b = b0 + u * kFewWaves, k = b * kBlkK;
-        const bool on = b < nb;
-        wl[u] = on ? chunk(w + k, k + 16 * gr) : make_uint4(0, 0, 0, 0);
-        wh[u] = on ? chunk(w + k + 64, k + 16 * gr + 64) : make_uint4(0, 0, 0, 0);
-        sw[u] = on ? ws[b] : 0.0f;
-#pragma unroll
-        for (int q = 0; q < QF; ++q) {
-          xl[u][q] = on ? chunk(x[q] + k, k + 16 * gr) : make_uint4(0, 0, 0, 0);
-          xh[u][q] = on ? chunk(x[q] + k + 64, k + 16 * gr + 64) : make_uint4(0, 0, 0, 0);
-          sx[u][q] = on ? xs[q][b * a.ldas] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const v8i fw = {(int)wl[u].x, (int)wl[u].y, (int)wl[u].z, (int)wl[u].w,
-                        (int)wh[u].x, (int)wh[u].y, (int)wh[u].z, (int)wh[u].w};
-#pragma unroll
-        for (int q = 0; q < QF; ++q) {
-          const v8i fx = {(int)xl[u][q].x, (int)xl[u][q].y, (int)xl[u][q].z, (int)xl[u][q].w,
-                          (int)xh[u][q].x, (int)xh[u][q].y, (int)xh[u][q].z, (int)xh[u][q].w};
-          const v4f t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              fw, fx, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
-          const float f = sw[u] * sx[u][q];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[q][r] = __builtin_fmaf(t[r], f, acc[q][r]);
-        }
-      }
+    for (int u = 0; u < kAhead; ++u) {
+      const int b = b0 + u * kFewWaves, k = b * kBlkK;
+      wl[u] = chunk(w, k);
+      wh[u] = chunk(w, k + 64);
+      xl[u] = chunk(x, k);
+      xh[u] = chunk(x, k + 64);
+      sw[u] = b < nb ? ws[b] : 0.0f;
+      sx[u] = b < nb ? xs[b * a.ldas] : 0.0f;
     }
 #pragma unroll
-    for (int q = 0; q < QF; ++q) sums[wave][q][lane] = acc[q];
-    __syncthreads();
-    if (wave < QF) {
-      v4f s = sums[0][wave][lane];
+    for (int u = 0; u < kAhead; ++u) {
+      const v4f t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          fragment(wl[u], wh[u]), fragment(xl[u], xh[u]), v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0,
+          0x7F7F7F7F, 0, 0x7F7F7F7F);
+      const float f = sw[u] * sx[u];
 #pragma unroll
-      for (int u = 1; u < kFewWaves; ++u) s += sums[u][wave][lane];
-      const int64_t row = m0 + 16 * wave + c, n = n0 + 4 * gr;
-      if (row < end) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < a.N) {
-            if (a.out_f32) static_cast<float*>(a.out)[row * a.ldo + n + r] = s[r];
-            else static_cast<uint16_t*>(a.out)[row * a.ldo + n + r] = (uint16_t)pack_bf16x2(s[r], 0.0f);
-          }
-      }
+      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(t[r], f, acc[r]);
     }
-    __syncthreads();
   }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || c >= a.M) return;
+#pragma unroll
+  for (int u = 1; u < kFewWaves; ++u) acc += sums[u][lane];
+  const int64_t n = n0 + 4 * gr;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < a.N) {
+      if (a.out_f32) static_cast<float*>(a.out)[row * a.ldo + n + r] = acc[r];
+      else static_cast<uint16_t*>(a.out)[row * a.ldo + n + r] = (uint16_t)pack_bf16x2(acc[r], 0.0f);
+    }
 }
 
 // How a product is shared out: 256 x 256 or 128 x 128 tiles, those also with the contraction
@@ -724,8 +693,7 @@ BlockPlan plan(int64_t tiles256, int64_t tiles128, int64_t blocks, double out_by
   return best;
 }
 BlockPlan plan_mm(int64_t M, int64_t N, int64_t K, int64_t E, bool grouped) {
-  const int64_t per = (M + E - 1) / E;
-  if (per <= 64) return {true, false, 0, 1};
+  if (!grouped && M <= kFewRows) return {true, false, (N + 15) / 16, 1};
   const auto tiles = [&](int64_t t) { return ((M + t - 1) / t + (grouped ? E : 0)) * ((N + t - 1) / t); };
   return plan(tiles(256), tiles(128), (K + kBlkK - 1) / kBlkK, 4.0 * M * N);
 }
@@ -760,14 +728,7 @@ hipError_t launch_block_mm(BlockMmArgs a, hipStream_t stream) {
   const BlockPlan p = plan_mm(a.M, a.N, a.K, a.E, a.ends != nullptr);
   a.parts = (int32_t)p.parts;
   if (p.few) {
-    const int64_t per = (a.M + a.E - 1) / a.E;
-    const dim3 grid((unsigned)((a.N + 15) / 16 * a.E));
-    if (per <= 16)
-      hipLaunchKernelGGL((k_block_few<1>), grid, dim3(64 * kFewWaves), 0, stream, a);
-    else if (per <= 32)
-      hipLaunchKernelGGL((k_block_few<2>), grid, dim3(64 * kFewWaves), 0, stream, a);
-    else
-      hipLaunchKernelGGL((k_block_few<4>), grid, dim3(64 * kFewWaves), 0, stream, a);
+    hipLaunchKernelGGL(k_block_few, dim3((unsigned)p.tiles), dim3(64 * kFewWaves), 0, stream, a);
     return hipGetLastError();
   }
   if (p.large)
