@@ -399,8 +399,11 @@ __device__ __forceinline__ void block_store(const v4f (&acc)[4 * GP][FQ], O* out
 }
 
 // Tile of this workgroup: tiles of group g are ceil(size / q) * np, in group order;
-// consecutive workgroups go to the XCDs in turn, and each XCD takes a run of tiles.
-// g = E for a workgroup past the last tile.
+// consecutive workgroups go to the XCDs in turn, and each XCD takes runs of eight tiles, so
+// that groups' part-filled tiles are dealt out evenly (16384 tokens of 32 uneven experts: an
+// eighth of the tiles in one run 590 us, runs of eight 575).  g = E for a workgroup past
+// the last tile.
+constexpr uint32_t kXcdRun = 8;
 struct GroupTile {
   int g;
   int64_t begin, end, tile;
@@ -414,8 +417,8 @@ __device__ __forceinline__ GroupTile find_group(const int32_t* ends_s, int E, in
   int64_t total = 0;
   for (int g = lane; g < E; g += 64) total += tiles(g);
   for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-  const int64_t per = (total + 7) >> 3, t = (id & 7u) * per + (id >> 3);
-  if ((id >> 3) >= per || t >= total) return {E, 0, 0, 0};
+  const int64_t t = ((int64_t)((id >> 3) / kXcdRun) * 8 + (id & 7u)) * kXcdRun + (id >> 3) % kXcdRun;
+  if (t >= total) return {E, 0, 0, 0};
   int64_t before = 0;
   for (int g0 = 0; g0 < E; g0 += 64) {
     const int64_t own = tiles(g0 + lane);
@@ -701,8 +704,11 @@ BlockPlan plan_wgrad(int64_t tokens, int64_t N, int64_t K, int64_t E) {
   const auto tiles = [&](int64_t t) { return E * ((K + t - 1) / t) * ((N + t - 1) / t); };
   return plan(tiles(256), tiles(128), std::max<int64_t>(1, tokens / kBlkK / E), 4.0 * E * N * K);
 }
-// Workgroups: a multiple of 8 for each part, for xcd_tile().
-dim3 tile_grid(const BlockPlan& p) { return dim3((unsigned)((p.tiles + 7) / 8 * 8 * p.parts)); }
+// Workgroups: whole turns of the XCDs for each part (find_group(), xcd_tile()).
+dim3 tile_grid(const BlockPlan& p, bool grouped) {
+  const int64_t turn = grouped ? 8 * kXcdRun : 8;
+  return dim3((unsigned)((p.tiles + turn - 1) / turn * turn * p.parts));
+}
 
 hipError_t join_parts(const float* partial, int64_t parts, int64_t rows, const int32_t* ends, int E,
                       int64_t cols, void* out, int64_t ldo, int f32, hipStream_t stream) {
@@ -732,9 +738,9 @@ hipError_t launch_block_mm(BlockMmArgs a, hipStream_t stream) {
     return hipGetLastError();
   }
   if (p.large)
-    hipLaunchKernelGGL((k_block_fwd<2, 2, 4, 4>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_fwd<2, 2, 4, 4>), tile_grid(p, a.ends != nullptr), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_fwd<2, 1, 4, 2>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_fwd<2, 1, 4, 2>), tile_grid(p, a.ends != nullptr), dim3(512), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.parts == 1) return err;
   return join_parts(a.partial, a.parts, a.M, a.ends, a.E, a.N, a.out, a.ldo, a.out_f32, stream);
@@ -745,9 +751,9 @@ hipError_t launch_block_wgrad(BlockWgradArgs a, hipStream_t stream) {
   const BlockPlan p = plan_wgrad(a.tokens, a.N, a.K, a.E);
   a.parts = (int32_t)p.parts;
   if (p.large)
-    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4, 4>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_wgrad<2, 2, 4, 4>), tile_grid(p, false), dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_block_wgrad<2, 1, 4, 2>), tile_grid(p), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL((k_block_wgrad<2, 1, 4, 2>), tile_grid(p, false), dim3(512), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.parts == 1) return err;
   return join_parts(a.partial, a.parts, (int64_t)a.E * a.N, nullptr, 0, a.K, a.dw, a.K, a.out_f32,

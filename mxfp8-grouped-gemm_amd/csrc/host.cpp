@@ -17,6 +17,7 @@
 // another ABI version than the header this module was compiled with.
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstring>
 #include <optional>
 #include <stdexcept>
@@ -43,7 +44,11 @@ struct Lib {
   MXGG_FN(route_topk) MXGG_FN(route_topk_grad) MXGG_FN(norm) MXGG_FN(norm_grad)              \
   MXGG_FN(norm_grad_workspace_bytes) MXGG_FN(adamw_step) MXGG_FN(last_error)                 \
   MXGG_FN(linear_cross_entropy) MXGG_FN(linear_cross_entropy_workspace_bytes)                \
-  MXGG_FN(linear_cross_entropy_grad) MXGG_FN(linear_cross_entropy_grad_workspace_bytes)
+  MXGG_FN(linear_cross_entropy_grad) MXGG_FN(linear_cross_entropy_grad_workspace_bytes)      \
+  MXGG_FN(block_quant_dim0) MXGG_FN(block_mm) MXGG_FN(block_mm_workspace_bytes)              \
+  MXGG_FN(add_rms_norm) MXGG_FN(rms_norm_quant) MXGG_FN(token_log_probs)                     \
+  MXGG_FN(token_log_probs_workspace_bytes) MXGG_FN(grad_norm) MXGG_FN(clip_grad_norm)        \
+  MXGG_FN(grad_norm_workspace_bytes)
   MXGG_FNS
 #undef MXGG_FN
 };
@@ -111,6 +116,7 @@ void* st(int64_t stream) { return reinterpret_cast<void*>(stream); }
 using Result = std::variant<std::monostate, int, Tensor, std::tuple<Tensor, Tensor>,
                             std::tuple<Tensor, Tensor, Tensor>,
                             std::tuple<Tensor, Tensor, OptTensor>,
+                            std::tuple<OptTensor, Tensor, OptTensor, OptTensor>,
                             std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>,
                             std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor>,
                             std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor>>;
@@ -685,6 +691,172 @@ Result adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads
   return rc;
 }
 
+// ---------------------------------------------------------------------------
+// Block-scaled products, norms with residual and 8-bit output, log probabilities,
+// gradient clipping: the calls without a gradient of their own.
+// ---------------------------------------------------------------------------
+bool grad_on(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool grad_on(const OptTensor& t) { return t && grad_on(*t); }
+
+// Storage of one fp32 scale for each row and block, block by block.
+Tensor block_scales(int64_t blocks, int64_t rows, const Tensor& like) {
+  return empty({blocks, (rows + 3) / 4 * 4}, like, at::kFloat);
+}
+
+Result block_dim0(const Tensor& x, int64_t stream) {
+  if (!bf16_rows(x) || x.size(1) % 16 != 0) return none();
+  const int64_t M = x.size(0), K = x.size(1);
+  Tensor q = empty({M, K}, x, at::kFloat8_e4m3fn), s = block_scales((K + 127) / 128, M, x);
+  const int rc = lib.block_quant_dim0(cp(x), M, K, x.stride(0), vp(q), K, s.data_ptr<float>(),
+                                      s.stride(0), st(stream));
+  if (rc != MXGG_OK) return rc;
+  return std::make_tuple(q, rows_view(s, M));
+}
+
+// Rows of e4m3 that the kernels read in place.
+bool block_operand(const Tensor& t) {
+  const int64_t d = t.dim();
+  return bytes(t) && d >= 2 && t.stride(d - 1) == 1 && t.stride(d - 2) % 16 == 0 &&
+         t.stride(d - 2) >= t.size(d - 1) && aligned(cp(t), 16);
+}
+Result block_mm(const Tensor& a, const Tensor& as, const Tensor& w, const Tensor& ws,
+                const OptTensor& ends, bool f32, int64_t stream) {
+  if (!block_operand(a) || a.dim() != 2 || !block_operand(w) || w.dim() != (ends ? 3 : 2) ||
+      !w.is_contiguous() || w.device() != a.device() || !ends_ok(ends, a))
+    return none();
+  const int64_t M = a.size(0), K = a.size(1), N = w.size(-2), E = ends ? w.size(0) : 1;
+  const int64_t nb = (N + 127) / 128, kb = (K + 127) / 128;
+  if (w.size(-1) != K || (ends && ends->numel() != E) || !plain(as) || !plain(ws) ||
+      as.scalar_type() != at::kFloat || ws.scalar_type() != at::kFloat ||
+      as.device() != a.device() || ws.device() != a.device() || as.dim() != 2 ||
+      as.size(0) != M || as.size(1) != kb || (as.stride(0) != 1 && M > 1) ||
+      (as.stride(1) < M && kb > 1) || !ws.is_contiguous() || ws.dim() != w.dim() ||
+      ws.size(-2) != nb || ws.size(-1) != kb || (ends && ws.size(0) != E))
+    return none();
+  const int64_t need = lib.block_mm_workspace_bytes(ends.has_value(), E, M, N, K);
+  Tensor buf;
+  if (need > 0) buf = empty({need}, a, at::kByte);
+  Tensor y = empty({M, N}, a, f32 ? at::kFloat : at::kBFloat16);
+  const int rc = lib.block_mm(
+      cp(a), a.stride(0), as.const_data_ptr<float>(), std::max(as.stride(1), M), cp(w), N * K, K,
+      ws.const_data_ptr<float>(), nb * kb, kb, ends_ptr(ends), E, M, N, K, vp(y), N,
+      f32 ? MXGG_OUT_F32 : MXGG_OUT_BF16, need > 0 ? vp(buf) : nullptr,
+      std::max<int64_t>(need, 0), st(stream));
+  if (rc != MXGG_OK) return rc;
+  return y;
+}
+
+// Whether the norm with the residual's addition takes the call as it is.
+bool add_norm_ok(const Tensor& x, const OptTensor& weight, const OptTensor& residual) {
+  if (!plain(x) || !f32_or_bf16(x) || x.dim() < 1 || x.size(-1) > 32768 || row_stride(x) < 0 ||
+      tangent(x) || tangent(weight) || tangent(residual) || grad_on(x) || grad_on(weight) ||
+      grad_on(residual))
+    return false;
+  const int64_t cols = x.size(-1);
+  if (weight && (!plain(*weight) || !f32_or_bf16(*weight) || weight->dim() != 1 ||
+                 weight->size(0) != cols || !weight->is_contiguous() ||
+                 weight->device() != x.device()))
+    return false;
+  return !residual || (plain(*residual) && residual->scalar_type() == x.scalar_type() &&
+                       residual->sizes() == x.sizes() && row_stride(*residual) > 0 &&
+                       residual->device() == x.device());
+}
+mxgg_norm_options add_norm_options(const Tensor& x, const OptTensor& weight, double eps) {
+  return {x.numel() / x.size(-1), x.size(-1), type_of(x),
+          weight ? type_of(*weight) : MXGG_OUT_F32, MXGG_OUT_F32, 0, (float)eps};
+}
+
+Result add_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight, double eps,
+                int64_t stream) {
+  if (!add_norm_ok(x, weight, residual)) return none();
+  const mxgg_norm_options o = add_norm_options(x, weight, eps);
+  Tensor y = empty(x.sizes(), x, x.scalar_type()), h = empty(x.sizes(), x, x.scalar_type());
+  const int rc = lib.add_rms_norm(cp(x), row_stride(x), cp(residual), row_stride(residual),
+                                  weight ? cp(*weight) : nullptr, &o, vp(h), o.cols, vp(y), o.cols,
+                                  nullptr, st(stream));
+  if (rc != MXGG_OK) return rc;
+  return std::make_tuple(y, h);
+}
+
+Result rms_quant(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps,
+                 int format, int mode, int64_t stream) {
+  const bool mx = format == MXGG_QUANT_MX;
+  if (!add_norm_ok(x, weight, residual) || x.size(-1) % (mx ? 32 : 16) != 0) return none();
+  const mxgg_norm_options o = add_norm_options(x, weight, eps);
+  Tensor q = empty({o.rows, o.cols}, x, at::kFloat8_e4m3fn);
+  Tensor s = mx ? block_major(o.rows, o.cols / 32, x) : block_scales((o.cols + 127) / 128, o.rows, x);
+  OptTensor h;
+  if (residual) h = empty(x.sizes(), x, x.scalar_type());
+  const int rc = lib.rms_norm_quant(
+      cp(x), row_stride(x), residual ? cp(*residual) : nullptr,
+      residual ? row_stride(*residual) : 0, weight ? cp(*weight) : nullptr, &o,
+      h ? vp(*h) : nullptr, o.cols, vp(q), o.cols, vp(s), s.stride(0), format, mode, st(stream));
+  if (rc != MXGG_OK) return rc;
+  return std::make_tuple(q, rows_view(s, o.rows), h);
+}
+
+Result log_probs(const Tensor& z, const OptTensor& target, double temperature, int64_t topk,
+                 int64_t ignore_index, int64_t stream) {
+  if (!plain(z) || !f32_or_bf16(z) || z.dim() < 1 || row_stride(z) < 0 || tangent(z) || grad_on(z) ||
+      topk < 0 || topk > std::min<int64_t>(64, z.size(-1)))
+    return none();
+  const auto lead = z.sizes().slice(0, z.dim() - 1);
+  if (target && (!plain(*target) || !target->is_contiguous() || target->sizes() != lead ||
+                 (target->scalar_type() != at::kInt && target->scalar_type() != at::kLong) ||
+                 target->device() != z.device()))
+    return none();
+  const mxgg_log_prob_options o{z.numel() / z.size(-1), z.size(-1), row_stride(z), ignore_index,
+                                type_of(z), target && target->scalar_type() == at::kLong,
+                                (int32_t)topk, (float)temperature};
+  const int64_t need = lib.token_log_probs_workspace_bytes(&o);
+  if (need < 0) return none();
+  OptTensor lp, ids, top;
+  Tensor ent = empty(lead, z, at::kFloat), ws = empty({need}, z, at::kByte);
+  if (target) lp = empty(lead, z, at::kFloat);
+  if (topk > 0) {
+    auto size = lead.vec();
+    size.push_back(topk);
+    ids = empty(size, z, at::kInt);
+    top = empty(size, z, at::kFloat);
+  }
+  const int rc = lib.token_log_probs(
+      cp(z), target ? cp(*target) : nullptr, &o, lp ? lp->data_ptr<float>() : nullptr,
+      ent.data_ptr<float>(), ids ? ids->data_ptr<int32_t>() : nullptr,
+      top ? top->data_ptr<float>() : nullptr, nullptr, vp(ws), need, st(stream));
+  if (rc != MXGG_OK) return rc;
+  return std::make_tuple(lp, ent, ids, top);
+}
+
+// The gradients' norm, and with max_norm not negative their clipping.
+Result clip(const std::vector<Tensor>& grads, double max_norm, double eps, int64_t stream) {
+  const size_t n = grads.size();
+  if (n == 0) return none();
+  std::vector<mxgg_grad_tensor> table(n);
+  std::vector<const void*> at(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& g = grads[i];
+    if (!plain(g) || !g.is_contiguous() || !f32_or_bf16(g) || g.device() != grads[0].device())
+      return none();
+    at[i] = cp(g);
+    table[i] = {const_cast<void*>(at[i]), g.numel(), type_of(g)};
+  }
+  std::sort(at.begin(), at.end());
+  if (std::adjacent_find(at.begin(), at.end()) != at.end()) return none();
+  const int64_t need = lib.grad_norm_workspace_bytes(table.data(), (int64_t)n);
+  if (need < 0) return none();
+  Tensor norm = empty({}, grads[0], at::kFloat), ws = empty({need}, grads[0], at::kByte);
+  const mxgg_clip_options o{max_norm, eps};
+  const int rc = max_norm >= 0
+                     ? lib.clip_grad_norm(table.data(), (int64_t)n, &o, norm.data_ptr<float>(),
+                                          vp(ws), need, st(stream))
+                     : lib.grad_norm(table.data(), (int64_t)n, norm.data_ptr<float>(), vp(ws), need,
+                                     st(stream));
+  if (rc != MXGG_OK) return rc;
+  if (max_norm >= 0)
+    for (const Tensor& g : grads) g.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -704,4 +876,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm", torch::wrap_pybind_function_no_gil(&norm));
   m.def("linear_cross_entropy", torch::wrap_pybind_function_no_gil(&linear_cross_entropy));
   m.def("adamw", torch::wrap_pybind_function_no_gil(&adamw));
+  m.def("block_dim0", torch::wrap_pybind_function_no_gil(&block_dim0));
+  m.def("block_mm", torch::wrap_pybind_function_no_gil(&block_mm));
+  m.def("add_norm", torch::wrap_pybind_function_no_gil(&add_norm));
+  m.def("rms_quant", torch::wrap_pybind_function_no_gil(&rms_quant));
+  m.def("log_probs", torch::wrap_pybind_function_no_gil(&log_probs));
+  m.def("clip", torch::wrap_pybind_function_no_gil(&clip));
 }

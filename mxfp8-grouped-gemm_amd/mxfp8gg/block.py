@@ -17,8 +17,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import (_FP8, _as_u8, _first_order, _group_ends, _mark_ends, _need_gpu, _no_tangent,
-                  _out_code, _stream_ptr, zero_rows_past_groups)
+from .ops import (_FP8, _as_u8, _first_order, _group_ends, _mark_ends, _native, _need_gpu,
+                  _no_tangent, _out_code, _stream_ptr, _tensors, _took, zero_rows_past_groups)
 
 __all__ = ["to_fp8_block_dim0", "to_fp8_block_dim1", "to_fp8_block_weight", "fp8_block_mm",
            "fp8_block_wgrad", "fp8_block_linear", "FP8BlockLinear"]
@@ -56,6 +56,11 @@ def _scale_buffer(blocks: int, rows: int, device) -> torch.Tensor:
 def to_fp8_block_dim0(x: torch.Tensor):
     """(payload e4m3 [M, K], scales fp32 [M, ceil(K / 128)]) of x bf16 [M, K] in blocks
     of 1 x 128 along each row.  The scales are a view of storage laid out block by block."""
+    host = _native(x)
+    if host is not None:
+        r = host.block_dim0(x, _stream_ptr(x))
+        if _took(r, "to_fp8_block_dim0"):
+            return r
     x = _bf16_rows(x, "x")
     M, K = x.shape
     q = torch.empty((M, K), dtype=_FP8, device=x.device)
@@ -169,6 +174,12 @@ def fp8_block_mm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor,
     experts' cumulative row ends (rows past the last one are not written).  K is a
     multiple of 16."""
     out = _out_code(out_dtype)
+    host = _native(a)
+    if host is not None and isinstance(w, torch.Tensor) and isinstance(a_scales, torch.Tensor) \
+            and isinstance(w_scales, torch.Tensor) and _tensors(offs):
+        r = host.block_mm(a, a_scales, w, w_scales, offs, out == _lib.OUT_F32, _stream_ptr(a))
+        if _took(r, "fp8_block_mm"):
+            return r
     a = _payload(a, "a", (2,))
     w = _payload(w, "w", (2, 3))
     M, K = a.shape

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .norm import _ld, _ptr, _rows
-from .ops import _first_order, _need_gpu, _no_tangent, _stream_ptr
+from .ops import _first_order, _native, _need_gpu, _no_tangent, _stream_ptr, _tensors, _took
 
 __all__ = ["token_log_probs", "TokenLogProbs"]
 
@@ -92,6 +92,11 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None,
     alternatives; any other target outside [0, V) has a NaN log probability.
     Differentiable in logits through log_probs, entropy and top_log_probs (the choice of
     alternatives held fixed); ignored and wholly masked rows have gradients of 0."""
+    host = _native(logits)
+    if host is not None and _tensors(targets) and topk.__class__ is int:
+        r = host.log_probs(logits, targets, temperature, topk, ignore_index, _stream_ptr(logits))
+        if _took(r, "token_log_probs"):
+            return TokenLogProbs(*r)
     _need_gpu(logits, "logits")
     if logits.dtype not in _TYPES or logits.dim() < 1:
         raise TypeError("logits must be a float32 or bfloat16 tensor [..., V], got "

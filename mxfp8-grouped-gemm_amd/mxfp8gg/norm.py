@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import (_FP8, _block_major_buffer, _first_order, _mode, _native, _need_gpu, _no_tangent,
+from .ops import (_FP8, _MODES, _block_major_buffer, _first_order, _mode, _native, _need_gpu, _no_tangent,
                   _stream_ptr, _tensors, _took)
 
 __all__ = ["layer_norm", "rms_norm", "Norm", "add_rms_norm", "AddRMSNorm", "rms_norm_quant"]
@@ -229,6 +229,11 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
     """(y, h): h = x + residual, rounded to their type, and y = rms_norm(h, weight, eps), in
     one pass.  x, residual: bf16 or fp32 [..., cols] of one type and shape.  weight: fp32 or
     bf16 [cols], or None.  Differentiable in x, residual and weight, through y and h."""
+    host = _native(x)
+    if host is not None and residual is not None and _tensors(residual, weight):
+        r = host.add_norm(x, residual, weight, eps, _stream_ptr(x))
+        if _took(r, "add_rms_norm"):
+            return r
     opt = _add_checks(x, residual, weight, eps)
     if residual is None:
         raise TypeError("residual must be a torch.Tensor")
@@ -257,6 +262,12 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor | None = None,
     mode is on."""
     if out_format not in _FORMATS:
         raise ValueError(f"out_format must be one of {sorted(_FORMATS)}, got {out_format!r}")
+    host = _native(x, scaling_mode)
+    if host is not None and _tensors(weight, residual):
+        r = host.rms_quant(x, weight, residual, eps, _FORMATS[out_format][0],
+                           _MODES[scaling_mode], _stream_ptr(x))
+        if _took(r, "rms_norm_quant"):
+            return r
     opt = _add_checks(x, residual, weight, eps)
     _no_tangent("rms_norm_quant", x, residual, weight)
     if torch.is_grad_enabled() and any(

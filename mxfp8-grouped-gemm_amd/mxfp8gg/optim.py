@@ -126,10 +126,7 @@ def _own_memory(t: torch.Tensor) -> bool:
 
 
 def _grad_table(grads):
-    """The tensors and their table for the library."""
-    if isinstance(grads, torch.Tensor):
-        grads = [grads]
-    grads = list(grads)
+    """The tensors' table for the library."""
     table = (_lib.GradTensor * max(len(grads), 1))()
     seen = set()
     for i, g in enumerate(grads):
@@ -148,11 +145,18 @@ def _grad_table(grads):
         table[i] = _lib.GradTensor(g.data_ptr(), g.numel(), _TYPES[g.dtype])
     if not grads:
         raise ValueError("grads is empty")
-    return grads, table
+    return table
 
 
 def _clip(grads, what, options=None):
-    grads, table = _grad_table(grads)
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    host = _native(grads[0]) if grads else None
+    if host is not None and all(isinstance(g, torch.Tensor) for g in grads):
+        r = host.clip(grads, -1.0 if options is None else options.max_norm,
+                      0.0 if options is None else options.eps, _stream_ptr(grads[0]))
+        if _took(r, what):
+            return r
+    table = _grad_table(grads)
     lib, n = _lib.load(), len(grads)
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -161,13 +165,15 @@ def _clip(grads, what, options=None):
     rest = (norm.data_ptr(), ws.data_ptr(), nbytes, _stream_ptr(grads[0]))
     _lib.check(lib.mxgg_grad_norm(table, n, *rest) if options is None else
                lib.mxgg_clip_grad_norm(table, n, ctypes.byref(options), *rest), what)
-    return grads, norm
+    if options is not None:
+        torch.autograd.graph.increment_version(grads)
+    return norm
 
 
 def grad_norm(grads) -> torch.Tensor:
     """sqrt(sum of g^2) over all tensors of the list (bf16 or fp32, on one device), fp32 on
     the device.  Squares and sums are fp64; the same bits on every run."""
-    return _clip(grads, "grad_norm")[1]
+    return _clip(grads, "grad_norm")
 
 
 def clip_grad_norm_(grads, max_norm: float, eps: float = 1e-6) -> torch.Tensor:
@@ -179,9 +185,7 @@ def clip_grad_norm_(grads, max_norm: float, eps: float = 1e-6) -> torch.Tensor:
     max_norm, eps = float(max_norm), float(eps)
     if not (max_norm >= 0 and eps >= 0):
         raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
-    grads, norm = _clip(grads, "clip_grad_norm_", _lib.ClipOptions(max_norm, eps))
-    torch.autograd.graph.increment_version(grads)
-    return norm
+    return _clip(grads, "clip_grad_norm_", _lib.ClipOptions(max_norm, eps))
 
 
 class AdamW(torch.optim.Optimizer):
