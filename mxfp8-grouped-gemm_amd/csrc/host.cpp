@@ -707,7 +707,7 @@ Result block_dim0(const Tensor& x, int64_t stream) {
   if (!bf16_rows(x) || x.size(1) % 16 != 0) return none();
   const int64_t M = x.size(0), K = x.size(1);
   Tensor q = empty({M, K}, x, at::kFloat8_e4m3fn), s = block_scales((K + 127) / 128, M, x);
-  const int rc = lib.block_quant_dim0(cp(x), M, K, x.stride(0), vp(q), K, s.data_ptr<float>(),
+  const int rc = lib.block_quant_dim0(cp(x), M, K, M > 1 ? x.stride(0) : K, vp(q), K, s.data_ptr<float>(),
                                       s.stride(0), st(stream));
   if (rc != MXGG_OK) return rc;
   return std::make_tuple(q, rows_view(s, M));
@@ -738,7 +738,7 @@ Result block_mm(const Tensor& a, const Tensor& as, const Tensor& w, const Tensor
   if (need > 0) buf = empty({need}, a, at::kByte);
   Tensor y = empty({M, N}, a, f32 ? at::kFloat : at::kBFloat16);
   const int rc = lib.block_mm(
-      cp(a), a.stride(0), as.const_data_ptr<float>(), std::max(as.stride(1), M), cp(w), N * K, K,
+      cp(a), M > 1 ? a.stride(0) : K, as.const_data_ptr<float>(), std::max(as.stride(1), M), cp(w), N * K, K,
       ws.const_data_ptr<float>(), nb * kb, kb, ends_ptr(ends), E, M, N, K, vp(y), N,
       f32 ? MXGG_OUT_F32 : MXGG_OUT_BF16, need > 0 ? vp(buf) : nullptr,
       std::max<int64_t>(need, 0), st(stream));

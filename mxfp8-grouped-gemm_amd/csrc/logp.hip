@@ -34,7 +34,7 @@ constexpr int kSeg = 64;                   // consecutive logits under one maxim
 constexpr int kMaxSegs = 4096;
 constexpr int64_t kMaxPart = (int64_t)kSeg * kMaxSegs;
 constexpr int64_t kMinPart = 4096;         // elements of a workgroup, at least
-constexpr int kMaxParts = 64;              // of a row, where alternatives are asked for
+constexpr int kMaxParts = 64;              // of a row
 constexpr int kList = 2048;                // candidates
 constexpr int kMaxTop = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -95,21 +95,6 @@ __device__ __forceinline__ void rescale(Sums& a, float m, float c) {
   a.s *= f;
   a.m = m;
 }
-__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
-  const float m = __builtin_fmaxf(a.m, b.m);
-  rescale(a, m, c);
-  rescale(b, m, c);
-  return {m, a.s + b.s, a.w + b.w};
-}
-// Over the wave, in every lane, always in the same order.
-__device__ __forceinline__ Sums wave_join(Sums a, float c) {
-  for (int d = 1; d < 64; d <<= 1) {
-    const Sums b{__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.w, d)};
-    a = (threadIdx.x & d) ? join(b, a, c) : join(a, b, c);
-  }
-  return a;
-}
-
 __device__ __forceinline__ float wave_max(float x) {
   x = __builtin_fmaxf(x, dpp_mov<0xB1>(x));
   x = __builtin_fmaxf(x, dpp_mov<0x4E>(x));
@@ -120,39 +105,96 @@ __device__ __forceinline__ float wave_max(float x) {
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __builtin_fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
-__device__ __forceinline__ int wave_min(int x) {
-  for (int d = 1; d < 64; d <<= 1) x = min(x, __shfl_xor(x, d));
-  return x;
+// Over the wave, in every lane, in an order that does not change.
+__device__ __forceinline__ Sums wave_join(Sums a, float c) {
+  rescale(a, wave_max(a.m), c);
+  return {a.m, wave_sum(a.s), wave_sum(a.w)};
 }
-
+// The same over N parts in LDS, one after the other.
+template <int N>
+__device__ __forceinline__ Sums join_all(const Sums* p, float c) {
+  float m = p[0].m;
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = __builtin_fmaxf(m, p[i].m);
+  Sums t{m, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    Sums a = p[i];
+    rescale(a, m, c);
+    t.s += a.s;
+    t.w += a.w;
+  }
+  return t;
+}
+// A candidate as an integer that orders by value, then by lowest index: the value's bits
+// made monotone (-0 as 0) above the inverted index.  0 is none.
+__device__ __forceinline__ uint64_t key_of(float v, int64_t index) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  const uint32_t o = u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  return (uint64_t)o << 32 | (0xFFFFFFFFu - (uint32_t)index);
+}
 struct Pick {
   float v;
   int32_t i;  // -1: none
 };
-__device__ __forceinline__ bool before(const Pick& a, const Pick& b) {
-  return a.i >= 0 && (b.i < 0 || a.v > b.v || (a.v == b.v && a.i < b.i));
+__device__ __forceinline__ Pick pick_of(uint64_t key) {
+  if (key == 0) return {-kInf, -1};
+  const uint32_t o = (uint32_t)(key >> 32);
+  return {__uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu)),
+          (int32_t)(0xFFFFFFFFu - (uint32_t)key)};
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t x) {
+  for (int d = 1; d < 64; d <<= 1) x = max(x, (uint64_t)__shfl_xor((unsigned long long)x, d));
+  return x;
 }
 
-// The k best of n candidates in LDS (values of -inf are none), by one wave:
-// f(rank, pick) in lane 0.  Candidates are used up.
+// The k-th largest of 64 lanes' values (-inf where fewer are above it).
+__device__ __forceinline__ float kth_of_lanes(float x, int k) {
+  float b = -kInf;
+  for (int r = 0; r < k; ++r) {
+    b = wave_max(x);
+    const uint64_t who = __ballot(x == b);
+    if ((int)(threadIdx.x & 63) == __builtin_ctzll(who ? who : 1)) x = -kInf;
+  }
+  return b;
+}
+
+// The k best of n different keys in LDS (0 is none), in falling order, by every thread of
+// the workgroup: f(rank, key), called by whichever thread has it.  Up to kRanked are
+// ranked against each other at once; more are searched by the first wave for each of
+// the k.
+constexpr int kRanked = 512;
 template <class F>
-__device__ __forceinline__ void pick_best(Pick* list, int n, int k, F f) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void pick_best(uint64_t* list, int n, int k, F f) {
+  if (n <= kRanked) {
+    for (int i = threadIdx.x; i < max(n, k); i += blockDim.x) {
+      const uint64_t own = i < n ? list[i] : 0;
+      int rank = 0, valid = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const uint64_t o = list[j];
+        rank += o > own ? 1 : 0;
+        valid += o != 0 ? 1 : 0;
+      }
+      if (own != 0 && rank < k) f(rank, own);
+      if (i < k && i >= valid) f(i, 0);
+    }
+    return;
+  }
+  if (threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
   const auto best_of_lane = [&] {
-    Pick b{-kInf, -1};
-    for (int j = lane; j < n; j += 64)
-      if (list[j].v > -kInf && before(list[j], b)) b = list[j];
+    uint64_t b = 0;
+    for (int j = lane; j < n; j += 64) b = max(b, list[j]);
     return b;
   };
-  Pick mine = best_of_lane();
+  uint64_t mine = best_of_lane();
   for (int r = 0; r < k; ++r) {
-    const float top = wave_max(mine.i >= 0 ? mine.v : -kInf);
-    const int at = wave_min(mine.i >= 0 && mine.v == top ? mine.i : 0x7FFFFFFF);
-    const Pick got{top, at == 0x7FFFFFFF ? -1 : at};
-    if (lane == 0) f(r, got);
-    if (mine.i == at) {
+    const uint64_t top = wave_max_key(mine);
+    if (lane == 0) f(r, top);
+    if (mine == top && top != 0) {
       for (int j = lane; j < n; j += 64)
-        if (list[j].i == at) list[j].i = -1;
+        if (list[j] == top) list[j] = 0;
       mine = best_of_lane();
     }
   }
@@ -163,20 +205,22 @@ __device__ __forceinline__ int64_t target_of(const LogpArgs& a, int64_t row) {
                     : static_cast<const int32_t*>(a.target)[row];
 }
 
-// A row's results from its sums; rows of nothing but -inf: no alternatives, no entropy.
+// The target's logit, where log probabilities are wanted; read long before it is used.
 template <typename T>
-__device__ __forceinline__ void write_row(const LogpArgs& a, int64_t row, const Sums& t, float log_s) {
+__device__ __forceinline__ float target_logit(const LogpArgs& a, int64_t row, int64_t at) {
+  if (!a.log_probs || at < 0 || at >= a.V) return 0.0f;
+  return Logits<T>::one(static_cast<const T*>(a.z) + row * a.ldz + at);
+}
+// A row's results from its sums; rows of nothing but -inf: no alternatives, no entropy.
+// at, z: the target and its logit.
+__device__ __forceinline__ void write_row(const LogpArgs& a, int64_t row, const Sums& t, float log_s,
+                                          int64_t at, float z) {
   const bool dead = t.m == -kInf && t.s == 0.0f;
   const float ent = dead ? 0.0f : log_s - kLn2 * (t.w / t.s);
   if (a.entropy) a.entropy[row] = ent;
   if (a.log_probs) {
-    const int64_t at = target_of(a, row);
-    float lp = __uint_as_float(0x7FC00000u);
-    if (at >= 0 && at < a.V) {
-      const float z = Logits<T>::one(static_cast<const T*>(a.z) + row * a.ldz + at);
-      lp = dead ? -kInf : (z - t.m) * a.inv_t - log_s;
-    }
-    a.log_probs[row] = lp;
+    const bool in = at >= 0 && at < a.V;
+    a.log_probs[row] = !in ? __uint_as_float(0x7FC00000u) : dead ? -kInf : (z - t.m) * a.inv_t - log_s;
   }
   if (a.stats) {  // log S = inf: p is 0 everywhere
     a.stats[row] = dead ? 0.0f : t.m;
@@ -184,8 +228,9 @@ __device__ __forceinline__ void write_row(const LogpArgs& a, int64_t row, const 
     a.stats[2 * a.T + row] = ent;
   }
 }
-__device__ __forceinline__ void write_pick(const LogpArgs& a, int64_t row, int r, const Pick& p,
+__device__ __forceinline__ void write_pick(const LogpArgs& a, int64_t row, int r, uint64_t key,
                                            const Sums& t, float log_s) {
+  const Pick p = pick_of(key);
   const bool bad = !(t.s == t.s);  // a NaN or an infinity among the logits
   a.top_ids[row * a.k + r] = bad ? -1 : p.i;
   a.top_lp[row * a.k + r] =
@@ -213,16 +258,18 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
   constexpr int kSegLanes = kSeg / E;
   __shared__ Sums parts[kLogpWaves];
   __shared__ float seg_max[TOP ? kMaxSegs : 1];
-  __shared__ Pick list[TOP ? kList : 1];
+  __shared__ uint64_t list[TOP ? kList : 1];
   __shared__ uint16_t segs[TOP ? kMaxSegs : 1];
   __shared__ int counts[2];
   __shared__ float bound;
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (a.target && target_of(a, row) == a.ignore) {
-    if (part == 0 && a.parts == 1) write_ignored(a, row, tid, kLogpThreads);
+  const int64_t target = a.target ? target_of(a, row) : -1;
+  if (a.target && target == a.ignore) {
+    if (a.parts == 1) write_ignored(a, row, tid, kLogpThreads);
     return;
   }
+  const float z_target = a.parts == 1 && tid == 0 ? target_logit<T>(a, row, target) : 0.0f;
   const int64_t first = part * a.part_len;
   const int len = (int)max((int64_t)0, min(a.part_len, a.V - first));
   const T* z = static_cast<const T*>(a.z) + row * a.ldz + first;
@@ -267,13 +314,11 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
   t = wave_join(t, a.c);
   if (lane == 0) parts[wave] = t;
   __syncthreads();
-  t = parts[0];
-#pragma unroll
-  for (int w = 1; w < kLogpWaves; ++w) t = join(t, parts[w], a.c);
+  t = join_all<kLogpWaves>(parts, a.c);
   const float log_s = logf(t.s);
-  Pick* out = reinterpret_cast<Pick*>(a.part_top) + (row * a.parts + part) * a.k;
+  uint64_t* out = a.part_top + (row * a.parts + part) * a.k;
   if (tid == 0) {
-    if (a.parts == 1) write_row<T>(a, row, t, log_s);
+    if (a.parts == 1) write_row(a, row, t, log_s, target, z_target);
     else a.part_sums[row * a.parts + part] = make_float4(t.m, t.s, t.w, 0.0f);
   }
   if constexpr (TOP) {
@@ -281,12 +326,7 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
     if (wave == 0) {
       float best = -kInf;
       for (int s = lane; s < nseg; s += 64) best = __builtin_fmaxf(best, seg_max[s]);
-      float b = -kInf;
-      for (int r = 0; r < a.k; ++r) {  // the k-th largest of the lanes' maxima
-        b = wave_max(best);
-        const uint64_t who = __ballot(best == b);
-        if (lane == __builtin_ctzll(who ? who : 1)) best = -kInf;
-      }
+      const float b = kth_of_lanes(best, a.k);
       if (lane == 0) bound = b;
     }
     __syncthreads();
@@ -313,39 +353,37 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
         int to = 0;
         if (lane == 0) to = atomicAdd(&counts[1], __popcll(who));
         to = __shfl(to, 0) + __popcll(who & ((1ull << lane) - 1));
-        if (in && to < kList) list[to] = Pick{v[u], (int32_t)(first + at[u])};
+        if (in && to < kList) list[to] = key_of(v[u], first + at[u]);
       }
     }
     __syncthreads();
     const int found = counts[1];
-    const auto give = [&](int r, const Pick& p) {
-      if (a.parts == 1) write_pick(a, row, r, p, t, log_s);
-      else out[r] = p;
+    const auto give = [&](int r, uint64_t key) {
+      if (a.parts == 1) write_pick(a, row, r, key, t, log_s);
+      else out[r] = key;
     };
     if (found <= kList) {
-      if (wave == 0) pick_best(list, found, a.k, give);
+      pick_best(list, found, a.k, give);
       return;
     }
     // too many reach the bound: one pass over the part for each of the k
-    Pick last{kInf, -1};
+    uint64_t last = ~0ull;
     for (int r = 0; r < a.k; ++r) {
-      Pick mine{-kInf, -1};
+      uint64_t mine = 0;
       for (int i = tid; i < len; i += kLogpThreads) {
-        const Pick p{Logits<T>::one(z + i), (int32_t)(first + i)};
-        if (p.v > -kInf && (r == 0 || before(last, p)) && before(p, mine)) mine = p;
+        const float v = Logits<T>::one(z + i);
+        const uint64_t key = v > -kInf ? key_of(v, first + i) : 0;
+        if (key < last) mine = max(mine, key);
       }
-      const float top = wave_max(mine.i >= 0 ? mine.v : -kInf);
-      const int at = wave_min(mine.i >= 0 && mine.v == top ? mine.i : 0x7FFFFFFF);
-      if (lane == 0) list[wave] = Pick{top, at == 0x7FFFFFFF ? -1 : at};
+      mine = wave_max_key(mine);
+      if (lane == 0) list[wave] = mine;
       __syncthreads();
-      Pick p{-kInf, -1};
-      for (int w = 0; w < kLogpWaves; ++w)
-        if (before(list[w], p)) p = list[w];
-      if (tid == 0) give(r, p);
-      last = p;
+      last = 0;
+      for (int w = 0; w < kLogpWaves; ++w) last = max(last, list[w]);
+      if (tid == 0) give(r, last);
       __syncthreads();
-      if (p.i < 0) {  // none left
-        for (int q = r + 1 + tid; q < a.k; q += kLogpThreads) give(q, p);
+      if (last == 0) {  // none left
+        for (int q = r + 1 + tid; q < a.k; q += kLogpThreads) give(q, 0);
         return;
       }
     }
@@ -355,26 +393,53 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
 // Joins the parts of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a) {
-  __shared__ Pick list[kMaxParts * kMaxTop];
+  __shared__ uint64_t list[kMaxParts * kMaxTop];
+  __shared__ Sums sums;
+  __shared__ float bound;
+  __shared__ int count;
   const int64_t row = blockIdx.x;
-  if (a.target && target_of(a, row) == a.ignore) {
+  const int64_t target = a.target ? target_of(a, row) : -1;
+  if (a.target && target == a.ignore) {
     write_ignored(a, row, threadIdx.x, blockDim.x);
     return;
   }
-  const int n = a.k > 0 ? (int)a.parts * a.k : 0;
-  const Pick* from = reinterpret_cast<const Pick*>(a.part_top) + row * a.parts * a.k;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) list[i] = from[i];
-  __syncthreads();
-  if (threadIdx.x >= 64) return;
-  Sums t{-kInf, 0.0f, 0.0f};
-  for (int64_t p = threadIdx.x; p < a.parts; p += 64) {
-    const float4 v = a.part_sums[row * a.parts + p];
-    t = join(t, Sums{v.x, v.y, v.z}, a.c);
+  const float z_target = threadIdx.x == 0 ? target_logit<T>(a, row, target) : 0.0f;
+  const int n = (int)a.parts * a.k;
+  const uint64_t* from = a.part_top + row * a.parts * a.k;
+  constexpr int kOwn = kMaxParts * kMaxTop / 256;
+  uint64_t own[kOwn];
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    own[u] = 0;
+    if (u * 256 < n && u * 256 + (int)threadIdx.x < n) own[u] = from[u * 256 + threadIdx.x];
   }
-  t = wave_join(t, a.c);
+  if (threadIdx.x < 64) {  // a lane for each part, at most kMaxParts
+    Sums t{-kInf, 0.0f, 0.0f};
+    float best = -kInf;  // of the part: each part's candidates are in falling order
+    if (threadIdx.x < a.parts) {
+      const float4 v = a.part_sums[row * a.parts + threadIdx.x];
+      t = Sums{v.x, v.y, v.z};
+      if (n > 0) best = pick_of(from[threadIdx.x * a.k]).v;
+    }
+    t = wave_join(t, a.c);
+    const float b = n > 0 ? kth_of_lanes(best, a.k) : 0.0f;
+    if (threadIdx.x == 0) {
+      sums = t;
+      bound = b;
+      count = 0;
+    }
+  }
+  __syncthreads();
+  const Sums t = sums;
   const float log_s = logf(t.s);
-  if (threadIdx.x == 0) write_row<T>(a, row, t, log_s);
-  if (n > 0) pick_best(list, n, a.k, [&](int r, const Pick& p) { write_pick(a, row, r, p, t, log_s); });
+  if (threadIdx.x == 0) write_row(a, row, t, log_s, target, z_target);
+  if (n == 0) return;
+  const float b = bound;
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u)  // in any order: the keys order themselves
+    if (own[u] != 0 && pick_of(own[u]).v >= b) list[atomicAdd(&count, 1)] = own[u];
+  __syncthreads();
+  pick_best(list, count, a.k, [&](int r, uint64_t key) { write_pick(a, row, r, key, t, log_s); });
 }
 
 // dz of one part of a row.  The elements that were chosen (target, alternatives) are
@@ -508,7 +573,7 @@ hipError_t launch_logp(LogpArgs a, uint8_t* ws, hipStream_t stream) {
   a.parts = (a.V + a.part_len - 1) / a.part_len;
   if (a.parts > 1) {
     a.part_sums = reinterpret_cast<float4*>(ws);
-    a.part_top = ws + 16 * a.T * a.parts;
+    a.part_top = reinterpret_cast<uint64_t*>(ws + 16 * a.T * a.parts);
   }
   const dim3 grid((unsigned)(a.T * a.parts));
   const auto go = [&](auto kernel) {

@@ -284,7 +284,7 @@ struct LogpArgs {
   int32_t k, target64, bf16;
   int64_t part_len, parts;
   float4* part_sums;    // [T][parts]
-  uint8_t* part_top;    // [T][parts][k]
+  uint64_t* part_top;   // [T][parts][k]
 };
 int64_t logp_workspace_bytes(const LogpArgs& args);
 hipError_t launch_logp(LogpArgs args, uint8_t* ws, hipStream_t stream);
