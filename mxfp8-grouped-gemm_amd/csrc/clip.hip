@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kClipThreads = 256;
 constexpr int kClipVec = 8;                    // consecutive elements of a thread
-constexpr int kClipRuns = 4;                   // runs of kClipThreads * kClipVec in flight
+constexpr int kClipRuns = 8;                   // runs of kClipThreads * kClipVec in flight
 constexpr int64_t kClipStep = (int64_t)kClipThreads * kClipVec * kClipRuns;
 constexpr int kClipTensors = 190;              // of a launch: the 4 KB of kernel arguments
 constexpr int64_t kClipParts = 2048;           // workgroups of a large call: 8 a compute unit
