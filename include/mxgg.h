@@ -716,7 +716,7 @@ int mxgg_linear_cross_entropy_grad(const float* grad_loss, const void* x, const 
 
 /*
  * e4m3 with one fp32 scale for each block of 128:
- *   s = max(amax / 448, 2^-126),  q = e4m3(x * (1 / s)), nearest even
+ *   s = max(amax (1 / 448), 2^-126),  q = e4m3(x / s), in fp32, nearest even
  * (a block with a NaN has a NaN scale; one with an infinity an infinite one).
  * Widths are multiples of 16; a last block may be narrower than 128.  x is bf16 with
  * 16-byte aligned rows (ldx % 8 == 0), payload rows are 16-byte aligned.
@@ -805,7 +805,7 @@ int mxgg_add_rms_norm_grad(const void* grad_y, int64_t ldg, const void* grad_h, 
  * from fp32:
  *   MXGG_QUANT_MX     one E8M0 byte for each 32 (rule scale_mode), cols % 32 == 0; byte of
  *                     row m and block b at scales[b * lds + m]
- *   MXGG_QUANT_BLOCK  one fp32 scale for each 128, max(amax / 448, 2^-126), cols % 16 == 0;
+ *   MXGG_QUANT_BLOCK  one fp32 scale for each 128, max(amax (1 / 448), 2^-126), cols % 16 == 0;
  *                     scale of row m and block b at ((float*)scales)[b * lds + m]
  * that is the block-major layout of the row-wise casts.  q: 8-byte aligned rows.
  */

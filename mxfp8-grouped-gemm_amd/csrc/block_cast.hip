@@ -1,13 +1,13 @@
 // bf16 -> e4m3 with one fp32 scale for each block of 128.
 //
-//   s = max(amax / 448, 2^-126),  q = e4m3(x * (1 / s))       (nearest even)
+//   s = max(amax (1 / 448), 2^-126),  q = e4m3(x / s)         (fp32; nearest even)
 //
 // A block is 1 x 128 along the row (activations), 128 x 1 along the tokens
 // (operands of the weight gradient, written transposed, restarting at every
 // group) or a 128 x 128 tile (weights).  amax is taken over the bit patterns of
 // |x|, so a NaN makes its block's scale and payload NaN; an infinity makes the
-// scale infinite.  1 / s is one correctly rounded division a block; x * (1 / s)
-// differs from x / s by at most one rounding of fp32.
+// scale infinite.  1 / s is one division a block; a quotient is a product and its
+// correction (BlockDivisor).
 //
 // Memory-bound: 2 bytes read and 1.03 written an element and output.
 #include "mx_device.h"
@@ -17,12 +17,6 @@ namespace mxgg {
 namespace {
 
 constexpr int kBlk = 128;
-
-// Scale of a block from the largest |x| bit pattern, and its reciprocal.
-__device__ __forceinline__ float block_scale(uint32_t amax16) {
-  const float a = bf16_bits_to_f32(amax16) / 448.0f;
-  return a < 0x1p-126f ? 0x1p-126f : a;  // a NaN stays
-}
 
 // Largest value of the 16 lanes of a row, in every one of them.
 __device__ __forceinline__ uint32_t row16_max(uint32_t x) {
@@ -35,9 +29,9 @@ __device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
   const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, (int)w, true);
 }
-__device__ __forceinline__ uint2 cvt_chunk(const uint4& v, float r) {
-  return make_uint2(cvt4(bf16_lo(v.x) * r, bf16_hi(v.x) * r, bf16_lo(v.y) * r, bf16_hi(v.y) * r),
-                    cvt4(bf16_lo(v.z) * r, bf16_hi(v.z) * r, bf16_lo(v.w) * r, bf16_hi(v.w) * r));
+__device__ __forceinline__ uint2 cvt_chunk(const uint4& v, const BlockDivisor& d) {
+  return make_uint2(cvt4(d(bf16_lo(v.x)), d(bf16_hi(v.x)), d(bf16_lo(v.y)), d(bf16_hi(v.y))),
+                    cvt4(d(bf16_lo(v.z)), d(bf16_hi(v.z)), d(bf16_lo(v.w)), d(bf16_hi(v.w))));
 }
 
 // Rows in blocks of 1 x 128: a wave takes one block column of 32 rows, eight loads of
@@ -64,9 +58,9 @@ __global__ __launch_bounds__(256) void k_block_rows(const uint16_t* __restrict__
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = row0 + 4 * i + g;
-    const float sc = block_scale(row16_max(amax16_of_chunk(v[i])));
+    const float sc = block_scale(bf16_bits_to_f32(row16_max(amax16_of_chunk(v[i]))));
     if ((lane & 15) == i) own = sc;
-    const uint2 w = cvt_chunk(v[i], 1.0f / sc);
+    const uint2 w = cvt_chunk(v[i], BlockDivisor(sc));
     if (in && row < rows) store_stream(q + row * ldq + col, w);
   }
   const int64_t row = row0 + 4 * (lane & 15) + g;
@@ -141,27 +135,26 @@ __global__ __launch_bounds__(256) void k_block_tile(CastTile a) {
       m.w = pk_max_u16(m.w, o.w);
     }
   }
-  float tile = 0.0f, rtile = 0.0f;
+  float tile = 1.0f;
   if (TILE) {
-    tile = block_scale(row16_max(amax16_of_chunk(m)));
-    rtile = 1.0f / tile;
+    tile = block_scale(bf16_bits_to_f32(row16_max(amax16_of_chunk(m))));
     if (t == 0) {
       const int64_t nb = (a.rows + kBlk - 1) / kBlk, kb = (a.cols + kBlk - 1) / kBlk;
       a.s[(batch * nb + blockIdx.y) * kb + blockIdx.x] = tile;
       if (COL) a.st[(batch * kb + blockIdx.x) * nb + blockIdx.y] = tile;
     }
   }
+  const BlockDivisor of_tile(tile);
   if (ROW) {
     float own = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float r = rtile;
+      float sc = tile;
       if (!TILE) {
-        const float sc = block_scale(row16_max(amax16_of_chunk(v[i])));
+        sc = block_scale(bf16_bits_to_f32(row16_max(amax16_of_chunk(v[i]))));
         if (c == i) own = sc;
-        r = 1.0f / sc;
       }
-      const uint2 w = cvt_chunk(v[i], r);
+      const uint2 w = cvt_chunk(v[i], TILE ? of_tile : BlockDivisor(sc));
       if (in && 8 * tr + i < ntok)
         store_stream(a.q + (batch * a.rows + tok0 + 8 * tr + i) * a.ldq + col, w);
     }
@@ -173,13 +166,13 @@ __global__ __launch_bounds__(256) void k_block_tile(CastTile a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t top = (j & 1) ? words[j >> 1] >> 16 : words[j >> 1] & 0xFFFFu;
-      sc[j] = TILE ? tile : block_scale(top);
-      const float r = TILE ? rtile : 1.0f / sc[j];
+      sc[j] = TILE ? tile : block_scale(bf16_bits_to_f32(top));
+      const BlockDivisor d = TILE ? of_tile : BlockDivisor(sc[j]);
       float f[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t w = j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w;
-        f[i] = ((j & 1) ? bf16_hi(w) : bf16_lo(w)) * r;
+        f[i] = d((j & 1) ? bf16_hi(w) : bf16_lo(w));
       }
       const uint32_t lo = cvt4(f[0], f[1], f[2], f[3]), hi = cvt4(f[4], f[5], f[6], f[7]);
       bytes[(8 * c + j) * 16 + (tr ^ c)] = (uint64_t)hi << 32 | lo;

@@ -294,6 +294,26 @@ __device__ __forceinline__ float div_nr_finite(float a, float b) {
   return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
 }
 
+// fp32 scale of a block of 128 e4m3 values, from the largest |x|: amax (1 / 448), at least
+// 2^-126 so that its reciprocal is finite.  A NaN stays, an infinity gives an infinite one.
+__device__ __forceinline__ float block_scale(float amax) {
+  const float a = amax * (1.0f / 448.0f);
+  return a < 0x1p-126f ? 0x1p-126f : a;
+}
+// x / s for every x of a block: the product with 1 / s, corrected by its residual as in
+// div_nr_finite.  The quotients of two 8-bit significands often lie on the border between
+// two e4m3 values, where the bare product would fall to either side.  An infinite s gives 0
+// for finite x.
+struct BlockDivisor {
+  float r, s;
+  __device__ __forceinline__ explicit BlockDivisor(float scale)
+      : r(1.0f / scale), s(scale == __builtin_inff() ? 0.0f : scale) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q);
+  }
+};
+
 // exp(x) for |x| <= 88, where neither overflow nor underflow can occur.
 // Cody-Waite reduction: x * log2(e) = n + f, with log2(e) split into a float
 // and the float of the remainder, n = rint, 2^f from v_exp_f32 and n put back

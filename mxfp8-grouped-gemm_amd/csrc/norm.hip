@@ -283,7 +283,7 @@ __device__ __forceinline__ void mx_payload(const float* o, uint32_t b, int mode,
 // Root-mean-square norm of h = x + residual (ADD; rounded to T, as it is kept) or of x.
 //   kOutSame  : y in T, rows dealt out as in k_norm_fwd
 //   kOutMx    : e4m3 and an E8M0 byte for each 32, rounded once from fp32
-//   kOutBlock : e4m3 and an fp32 scale for each 128: max(amax / 448, 2^-126)
+//   kOutBlock : e4m3 and an fp32 scale for each 128 (block_scale)
 // Scales are laid out block by block, rows next to each other, so the 8-bit outputs
 // are computed for `run` consecutive rows a workgroup, their scales gathered in LDS
 // and written as one run for each block (a byte at a time they would be a memory
@@ -377,13 +377,12 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add
             mx_payload<E>(o, b, a.mode, p);
             if (first) held[chunk / kLanes * kScaleRun + i] = (uint8_t)b;
           } else {
-            float sc = __uint_as_float(m) / 448.0f;
-            sc = sc < 0x1p-126f ? 0x1p-126f : sc;
-            const float f = 1.0f / sc;
+            const float sc = block_scale(__uint_as_float(m));
+            const BlockDivisor d(sc);
 #pragma unroll
             for (int k = 0; k < E / 4; ++k) {
-              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(o[4 * k] * f, o[4 * k + 1] * f, 0, false);
-              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(o[4 * k + 2] * f, o[4 * k + 3] * f,
+              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d(o[4 * k]), d(o[4 * k + 1]), 0, false);
+              p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d(o[4 * k + 2]), d(o[4 * k + 3]),
                                                                (int)p[k], true);
             }
             if (first) reinterpret_cast<float*>(held)[chunk / kLanes * kScaleRun + i] = sc;

@@ -8,8 +8,8 @@ the weight gradient in blocks of 128 tokens.
     y = fp8_block_mm(q, s, w, w_scales, offs)    # w e4m3 [N, K] or [E, N, K]
     y = fp8_block_linear(x, w, offs)             # bf16 in, differentiable
 
-A scale is max(amax / 448, 2^-126) and the payload e4m3(x * (1 / scale)), to nearest
-even.  Sums are fp32.  Widths are multiples of 16; the last block of a row may be
+A scale is max(amax * (1 / 448), 2^-126) in fp32 and the payload e4m3(x / scale), to
+nearest even.  Sums are fp32.  Widths are multiples of 16; the last block of a row may be
 narrower than 128.  With `offs` the rows are grouped by expert as in grouped_mm.
 """
 from __future__ import annotations

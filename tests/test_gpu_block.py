@@ -1,7 +1,7 @@
 """GPU parity of the block-scaled e4m3 casts and products.
 
-Casts are compared bit for bit with the definition: scale max(amax / 448, 2^-126) in
-fp32, payload the format's rounding of x * (1 / scale).
+Casts are compared bit for bit with the definition: scale max(amax (1 / 448), 2^-126) in
+fp32, payload the format's rounding of the fp32 quotient x / scale.
 
 Products against 64 bits, S the sum of the products' magnitudes.  The matrix instruction
 aligns each eight consecutive products of e4m3 values to the largest of them and cuts what
@@ -41,9 +41,8 @@ def _pad(x, *dims):
 def _cast(b, dims):
     """(payload, scale) of fp32 blocks spanning `dims` of b."""
     a = b.abs().amax(dim=dims, keepdim=True)
-    # a quotient of tensors: by a number torch multiplies with its reciprocal
-    s = torch.clamp(a / torch.full_like(a, 448.0), min=2.0 ** -126)
-    return (b * (1 / s)).to(FP8), s
+    s = torch.clamp(a * (torch.ones_like(a) / torch.full_like(a, 448.0)), min=2.0 ** -126)
+    return (b / s).to(FP8), s
 
 
 def _ref_rows(x):
