@@ -45,7 +45,10 @@ struct Lib {
   MXGG_FN(norm_grad_workspace_bytes) MXGG_FN(adamw_step) MXGG_FN(last_error)                 \
   MXGG_FN(linear_cross_entropy) MXGG_FN(linear_cross_entropy_workspace_bytes)                \
   MXGG_FN(linear_cross_entropy_grad) MXGG_FN(linear_cross_entropy_grad_workspace_bytes)      \
-  MXGG_FN(block_quant_dim0) MXGG_FN(block_mm) MXGG_FN(block_mm_workspace_bytes)              \
+  MXGG_FN(block_quant_dim0) MXGG_FN(block_quant_dim1) MXGG_FN(block_quant_weight)            \
+  MXGG_FN(block_mm) MXGG_FN(block_mm_workspace_bytes) MXGG_FN(block_wgrad)                   \
+  MXGG_FN(block_wgrad_workspace_bytes) MXGG_FN(add_rms_norm_grad)                            \
+  MXGG_FN(token_log_probs_grad)                                                              \
   MXGG_FN(add_rms_norm) MXGG_FN(rms_norm_quant) MXGG_FN(token_log_probs)                     \
   MXGG_FN(token_log_probs_workspace_bytes) MXGG_FN(grad_norm) MXGG_FN(clip_grad_norm)        \
   MXGG_FN(grad_norm_workspace_bytes)
@@ -692,8 +695,8 @@ Result adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads
 }
 
 // ---------------------------------------------------------------------------
-// Block-scaled products, norms with residual and 8-bit output, log probabilities,
-// gradient clipping: the calls without a gradient of their own.
+// Block-scaled products, norms with residual and 8-bit output, log probabilities and
+// gradient clipping.
 // ---------------------------------------------------------------------------
 bool grad_on(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool grad_on(const OptTensor& t) { return t && grad_on(*t); }
@@ -703,14 +706,56 @@ Tensor block_scales(int64_t blocks, int64_t rows, const Tensor& like) {
   return empty({blocks, (rows + 3) / 4 * 4}, like, at::kFloat);
 }
 
+// A cast: payload and scales by rows (q, s) and by columns of tokens (qt, st), the scales as
+// they are stored.
+struct BlockCast {
+  Tensor q, s, qt, st, pad;
+};
+int64_t rows_ld(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+int cast_rows(const Tensor& x, BlockCast& c, int64_t stream) {
+  const int64_t M = x.size(0), K = x.size(1);
+  c.q = empty({M, K}, x, at::kFloat8_e4m3fn);
+  c.s = block_scales((K + 127) / 128, M, x);
+  return lib.block_quant_dim0(cp(x), M, K, rows_ld(x), vp(c.q), K, c.s.data_ptr<float>(),
+                              c.s.stride(0), st(stream));
+}
+int cast_tokens(const Tensor& x, const OptTensor& ends, bool rows, BlockCast& c, int64_t stream) {
+  const int64_t M = x.size(0), C = x.size(1), E = ends ? ends->numel() : 0;
+  const int64_t cap = (M + 127 * E + 127) / 128 * 128;
+  if (rows) {
+    c.q = empty({M, C}, x, at::kFloat8_e4m3fn);
+    c.s = block_scales((C + 127) / 128, M, x);
+  }
+  c.qt = empty({C, cap}, x, at::kFloat8_e4m3fn);
+  c.st = block_scales(cap / 128, C, x);
+  if (ends) c.pad = empty({E}, x, at::kInt);
+  return lib.block_quant_dim1(
+      cp(x), M, C, rows_ld(x), ends_ptr(ends), E, cap, vp_or_null(c.q), C,
+      static_cast<float*>(vp_or_null(c.s)), rows ? c.s.stride(0) : 0, vp(c.qt),
+      c.st.data_ptr<float>(), c.st.stride(0), static_cast<int32_t*>(vp_or_null(c.pad)), st(stream));
+}
+
 Result block_dim0(const Tensor& x, int64_t stream) {
   if (!bf16_rows(x) || x.size(1) % 16 != 0) return none();
-  const int64_t M = x.size(0), K = x.size(1);
-  Tensor q = empty({M, K}, x, at::kFloat8_e4m3fn), s = block_scales((K + 127) / 128, M, x);
-  const int rc = lib.block_quant_dim0(cp(x), M, K, M > 1 ? x.stride(0) : K, vp(q), K, s.data_ptr<float>(),
-                                      s.stride(0), st(stream));
+  BlockCast c;
+  const int rc = cast_rows(x, c, stream);
   if (rc != MXGG_OK) return rc;
-  return std::make_tuple(q, rows_view(s, M));
+  return std::make_tuple(c.q, rows_view(c.s, x.size(0)));
+}
+
+// y of operands whose layout has been checked; ld of a and of its scales.
+int product(const Tensor& a, int64_t lda, const Tensor& as, int64_t ldas, const Tensor& w,
+            const Tensor& ws, const OptTensor& ends, bool f32, Tensor& y, int64_t stream) {
+  const int64_t M = a.size(0), K = a.size(1), N = w.size(-2), E = ends ? w.size(0) : 1;
+  const int64_t nb = (N + 127) / 128, kb = (K + 127) / 128;
+  const int64_t need = lib.block_mm_workspace_bytes(ends.has_value(), E, M, N, K);
+  Tensor buf;
+  if (need > 0) buf = empty({need}, a, at::kByte);
+  y = empty({M, N}, a, f32 ? at::kFloat : at::kBFloat16);
+  return lib.block_mm(cp(a), lda, as.const_data_ptr<float>(), ldas, cp(w), N * K, K,
+                      ws.const_data_ptr<float>(), nb * kb, kb, ends_ptr(ends), E, M, N, K, vp(y), N,
+                      f32 ? MXGG_OUT_F32 : MXGG_OUT_BF16, need > 0 ? vp(buf) : nullptr,
+                      std::max<int64_t>(need, 0), st(stream));
 }
 
 // Rows of e4m3 that the kernels read in place.
@@ -733,24 +778,105 @@ Result block_mm(const Tensor& a, const Tensor& as, const Tensor& w, const Tensor
       (as.stride(1) < M && kb > 1) || !ws.is_contiguous() || ws.dim() != w.dim() ||
       ws.size(-2) != nb || ws.size(-1) != kb || (ends && ws.size(0) != E))
     return none();
-  const int64_t need = lib.block_mm_workspace_bytes(ends.has_value(), E, M, N, K);
-  Tensor buf;
-  if (need > 0) buf = empty({need}, a, at::kByte);
-  Tensor y = empty({M, N}, a, f32 ? at::kFloat : at::kBFloat16);
-  const int rc = lib.block_mm(
-      cp(a), M > 1 ? a.stride(0) : K, as.const_data_ptr<float>(), std::max(as.stride(1), M), cp(w), N * K, K,
-      ws.const_data_ptr<float>(), nb * kb, kb, ends_ptr(ends), E, M, N, K, vp(y), N,
-      f32 ? MXGG_OUT_F32 : MXGG_OUT_BF16, need > 0 ? vp(buf) : nullptr,
-      std::max<int64_t>(need, 0), st(stream));
+  Tensor y;
+  const int rc = product(a, rows_ld(a), as, std::max(as.stride(1), M), w, ws, ends, f32, y, stream);
   if (rc != MXGG_OK) return rc;
   return y;
+}
+
+// fp8_block_linear: x [M, K], w [N, K] or [E, N, K] with ends.
+struct BlockLinear : torch::autograd::Function<BlockLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const OptTensor& ends, bool need_x, bool need_w, int64_t stream) {
+    const char* what = "fp8_block_linear";
+    BlockCast c;
+    check(need_w ? cast_tokens(x, ends, true, c, stream) : cast_rows(x, c, stream), what);
+    const int64_t N = w.size(-2), K = w.size(-1), E = ends ? w.size(0) : 1;
+    const int64_t nb = (N + 127) / 128, kb = (K + 127) / 128;
+    const auto shape = [&](int64_t r, int64_t n) {
+      return ends ? std::vector<int64_t>{E, r, n} : std::vector<int64_t>{r, n};
+    };
+    Tensor q = empty(w.sizes(), w, at::kFloat8_e4m3fn), s = empty(shape(nb, kb), w, at::kFloat), qt, t;
+    if (need_x) {
+      qt = empty(shape(K, N), w, at::kFloat8_e4m3fn);
+      t = empty(shape(kb, nb), w, at::kFloat);
+    }
+    check(lib.block_quant_weight(cp(w), E, N, K, vp(q), s.data_ptr<float>(), vp_or_null(qt),
+                                 static_cast<float*>(vp_or_null(t)), st(stream)),
+          what);
+    Tensor y;
+    check(product(c.q, K, c.s, c.s.stride(0), q, s, ends, false, y, stream), what);
+    if (ends)
+      check(lib.zero_rows_past_groups(vp(y), y.size(0), 2 * N, 2 * N, ends_ptr(ends), E, st(stream)),
+            what);
+    if (need_x || need_w) {
+      ctx->save_for_backward({c.qt, c.st, c.pad, ends.value_or(Tensor()), qt, t});
+      ctx->saved_data["need"] = (int64_t)(need_x | (int)need_w << 1);
+      ctx->saved_data["stream"] = stream;
+      ctx->saved_data["inputs"] = K;
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const char* what = "fp8_block_linear";
+    first_order(what);
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &xt = saved[0], &xts = saved[1], &pad = saved[2];
+    const OptTensor ends = saved[3].defined() ? OptTensor(saved[3]) : OptTensor();
+    const int64_t need = ctx->saved_data["need"].toInt(), stream = ctx->saved_data["stream"].toInt();
+    const int64_t K = ctx->saved_data["inputs"].toInt();
+    Tensor dy = grads[0].to(at::kBFloat16);
+    if (!bf16_rows(dy)) dy = dy.clone(at::MemoryFormat::Contiguous);
+    const int64_t N = dy.size(1), E = ends ? ends->numel() : 1;
+    BlockCast c;
+    check(need & 2 ? cast_tokens(dy, ends, need & 1, c, stream) : cast_rows(dy, c, stream), what);
+    Tensor dx, dw;
+    if (need & 2) {
+      const int64_t T = c.qt.size(1);
+      const int64_t bytes = lib.block_wgrad_workspace_bytes(ends.has_value(), E, T, N, K);
+      Tensor ws;
+      if (bytes > 0) ws = empty({bytes}, dy, at::kByte);
+      dw = ends ? empty({E, N, K}, dy, at::kBFloat16) : empty({N, K}, dy, at::kBFloat16);
+      check(lib.block_wgrad(vp(c.qt), T, c.st.const_data_ptr<float>(), c.st.stride(0), cp(xt), T,
+                            xts.const_data_ptr<float>(), xts.stride(0),
+                            ends ? pad.const_data_ptr<int32_t>() : nullptr, E, T, N, K, vp(dw),
+                            MXGG_OUT_BF16, vp_or_null(ws), std::max<int64_t>(bytes, 0), st(stream)),
+            what);
+    }
+    if (need & 1) {
+      check(product(c.q, N, c.s, c.s.stride(0), saved[4], saved[5], ends, false, dx, stream), what);
+      if (ends)
+        check(lib.zero_rows_past_groups(vp(dx), dx.size(0), 2 * K, 2 * K, ends_ptr(ends), E,
+                                        st(stream)),
+              what);
+    }
+    return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Result block_linear(const Tensor& x, const Tensor& w, const OptTensor& ends, int64_t stream) {
+  if (!plain(x) || !plain(w) || x.scalar_type() != at::kBFloat16 ||
+      w.scalar_type() != at::kBFloat16 || w.device() != x.device() || tangent(x) || tangent(w) ||
+      w.dim() != (ends ? 3 : 2) || !w.is_contiguous() || !aligned(cp(w), 16) || x.dim() < 1 ||
+      (ends && x.dim() != 2) || x.size(-1) != w.size(-1) || w.size(-1) % 16 != 0 ||
+      w.size(-2) % 16 != 0 || w.size(-1) == 0 || w.size(-2) == 0 || !ends_ok(ends, x) ||
+      (ends && ends->numel() != w.size(0)))
+    return none();
+  const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  if (!bf16_rows(x2)) return none();
+  const bool grad = at::GradMode::is_enabled();
+  const Tensor y =
+      BlockLinear::apply(x2, w, ends, grad && x.requires_grad(), grad && w.requires_grad(), stream);
+  if (x.dim() == 2) return y;
+  auto size = x.sizes().vec();
+  size.back() = w.size(-2);
+  return y.view(size);
 }
 
 // Whether the norm with the residual's addition takes the call as it is.
 bool add_norm_ok(const Tensor& x, const OptTensor& weight, const OptTensor& residual) {
   if (!plain(x) || !f32_or_bf16(x) || x.dim() < 1 || x.size(-1) > 32768 || row_stride(x) < 0 ||
-      tangent(x) || tangent(weight) || tangent(residual) || grad_on(x) || grad_on(weight) ||
-      grad_on(residual))
+      tangent(x) || tangent(weight) || tangent(residual))
     return false;
   const int64_t cols = x.size(-1);
   if (weight && (!plain(*weight) || !f32_or_bf16(*weight) || weight->dim() != 1 ||
@@ -766,22 +892,79 @@ mxgg_norm_options add_norm_options(const Tensor& x, const OptTensor& weight, dou
           weight ? type_of(*weight) : MXGG_OUT_F32, MXGG_OUT_F32, 0, (float)eps};
 }
 
+// (y, h, stats)
+variable_list add_norm_forward(const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                               const mxgg_norm_options& o, bool keep_stats, int64_t stream) {
+  Tensor y = empty(x.sizes(), x, x.scalar_type()), h = empty(x.sizes(), x, x.scalar_type()), stats;
+  if (keep_stats) stats = empty({2, o.rows}, x, at::kFloat);
+  check(lib.add_rms_norm(cp(x), row_stride(x), cp(residual), row_stride(residual),
+                         weight ? cp(*weight) : nullptr, &o, vp(h), o.cols, vp(y), o.cols,
+                         static_cast<float*>(vp_or_null(stats)), st(stream)),
+        "add_rms_norm");
+  return {y, h, stats};
+}
+
+struct AddNorm : torch::autograd::Function<AddNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual,
+                               const OptTensor& weight, const mxgg_norm_options& o, int64_t stream) {
+    const variable_list r = add_norm_forward(x, residual, weight, o, true, stream);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r[1], weight.value_or(Tensor()), r[2]});
+    keep(ctx, "options", o);
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["need"] =
+        (int64_t)((x.requires_grad() || residual.requires_grad()) | (int)grad_needed(weight) << 1);
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_order("add_rms_norm");
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1], &stats = saved[2];
+    const auto o = kept<mxgg_norm_options>(ctx, "options");
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const auto type = o.weight_dtype == MXGG_OUT_BF16 ? at::kBFloat16 : at::kFloat;
+    const auto rows = [&](const Tensor& g) {
+      const Tensor d = g.to(h.scalar_type());
+      return row_stride(d) < 0 ? d.contiguous() : d;
+    };
+    if (!grads[0].defined()) {  // only h was used
+      const Tensor dh = grads[1].defined() && need & 1 ? grads[1].to(h.scalar_type()) : Tensor();
+      return {dh, dh, need & 2 ? at::zeros({o.cols}, h.options().dtype(type)) : Tensor(), Tensor(),
+              Tensor()};
+    }
+    const Tensor dy = rows(grads[0]), dh = grads[1].defined() ? rows(grads[1]) : Tensor();
+    Tensor dx, dw, ws;
+    if (need & 1) dx = empty(h.sizes(), h, h.scalar_type());
+    if (need & 2) {
+      dw = empty({o.cols}, h, type);
+      ws = empty({lib.norm_grad_workspace_bytes(&o)}, h, at::kByte);
+    }
+    check(lib.add_rms_norm_grad(cp(dy), row_stride(dy), cp_or_null(dh),
+                                dh.defined() ? row_stride(dh) : 0, cp(h), o.cols, cp_or_null(w),
+                                stats.const_data_ptr<float>(), &o, vp_or_null(dx), o.cols,
+                                vp_or_null(dw), vp_or_null(ws), ws.defined() ? ws.numel() : 0,
+                                st(ctx->saved_data["stream"].toInt())),
+          "add_rms_norm_grad");
+    return {dx, dx, dw, Tensor(), Tensor()};
+  }
+};
+
 Result add_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight, double eps,
                 int64_t stream) {
   if (!add_norm_ok(x, weight, residual)) return none();
   const mxgg_norm_options o = add_norm_options(x, weight, eps);
-  Tensor y = empty(x.sizes(), x, x.scalar_type()), h = empty(x.sizes(), x, x.scalar_type());
-  const int rc = lib.add_rms_norm(cp(x), row_stride(x), cp(residual), row_stride(residual),
-                                  weight ? cp(*weight) : nullptr, &o, vp(h), o.cols, vp(y), o.cols,
-                                  nullptr, st(stream));
-  if (rc != MXGG_OK) return rc;
-  return std::make_tuple(y, h);
+  const variable_list r = grad_on(x) || grad_on(residual) || grad_on(weight)
+                              ? AddNorm::apply(x, residual, weight, o, stream)
+                              : add_norm_forward(x, residual, weight, o, false, stream);
+  return std::make_tuple(r[0], r[1]);
 }
 
 Result rms_quant(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps,
                  int format, int mode, int64_t stream) {
   const bool mx = format == MXGG_QUANT_MX;
-  if (!add_norm_ok(x, weight, residual) || x.size(-1) % (mx ? 32 : 16) != 0) return none();
+  if (!add_norm_ok(x, weight, residual) || grad_on(x) || grad_on(weight) || grad_on(residual) ||
+      x.size(-1) % (mx ? 32 : 16) != 0)
+    return none();
   const mxgg_norm_options o = add_norm_options(x, weight, eps);
   Tensor q = empty({o.rows, o.cols}, x, at::kFloat8_e4m3fn);
   Tensor s = mx ? block_major(o.rows, o.cols / 32, x) : block_scales((o.cols + 127) / 128, o.rows, x);
@@ -795,10 +978,78 @@ Result rms_quant(const Tensor& x, const OptTensor& weight, const OptTensor& resi
   return std::make_tuple(q, rows_view(s, o.rows), h);
 }
 
+// Entropy, then log probabilities (with targets), ids and log probabilities of the top
+// (with topk), then the statistics.
+variable_list log_prob_forward(const Tensor& z, const OptTensor& target,
+                               const mxgg_log_prob_options& o, bool keep_stats, int64_t stream) {
+  const auto lead = z.sizes().slice(0, z.dim() - 1);
+  Tensor ent = empty(lead, z, at::kFloat), lp, ids, top, stats;
+  if (target) lp = empty(lead, z, at::kFloat);
+  if (o.topk > 0) {
+    auto size = lead.vec();
+    size.push_back(o.topk);
+    ids = empty(size, z, at::kInt);
+    top = empty(size, z, at::kFloat);
+  }
+  if (keep_stats) stats = empty({3, o.tokens}, z, at::kFloat);
+  const int64_t need = lib.token_log_probs_workspace_bytes(&o);
+  const Tensor ws = empty({std::max<int64_t>(need, 0)}, z, at::kByte);
+  check(lib.token_log_probs(cp(z), target ? cp(*target) : nullptr, &o,
+                            static_cast<float*>(vp_or_null(lp)), ent.data_ptr<float>(),
+                            static_cast<int32_t*>(vp_or_null(ids)),
+                            static_cast<float*>(vp_or_null(top)),
+                            static_cast<float*>(vp_or_null(stats)), vp(ws), need, st(stream)),
+        "token_log_probs");
+  variable_list r{ent};
+  if (target) r.push_back(lp);
+  if (o.topk > 0) {
+    r.push_back(ids);
+    r.push_back(top);
+  }
+  r.push_back(stats);
+  return r;
+}
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const OptTensor& target,
+                               const mxgg_log_prob_options& o, int64_t stream) {
+    variable_list r = log_prob_forward(z, target, o, true, stream);
+    const Tensor stats = r.back();
+    r.pop_back();
+    const Tensor ids = o.topk > 0 ? r[r.size() - 2] : Tensor();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({z, target.value_or(Tensor()), ids, stats});
+    if (ids.defined()) ctx->mark_non_differentiable({ids});
+    keep(ctx, "options", o);
+    ctx->saved_data["stream"] = stream;
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_order("token_log_probs");
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &target = saved[1], &ids = saved[2], &stats = saved[3];
+    const auto o = kept<mxgg_log_prob_options>(ctx, "options");
+    const auto grad = [&](size_t i) {
+      return i < grads.size() && grads[i].defined() ? grads[i].to(at::kFloat).contiguous() : Tensor();
+    };
+    const Tensor ge = grad(0), gl = target.defined() ? grad(1) : Tensor();
+    const Tensor gt = o.topk > 0 ? grad(grads.size() - 1) : Tensor();
+    Tensor dz = empty(z.sizes(), z, z.scalar_type());
+    check(lib.token_log_probs_grad(static_cast<const float*>(cp_or_null(gl)),
+                                   static_cast<const float*>(cp_or_null(ge)),
+                                   static_cast<const float*>(cp_or_null(gt)), cp(z),
+                                   cp_or_null(target), static_cast<const int32_t*>(cp_or_null(ids)),
+                                   stats.const_data_ptr<float>(), &o, vp(dz),
+                                   st(ctx->saved_data["stream"].toInt())),
+          "token_log_probs_grad");
+    return {dz, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 Result log_probs(const Tensor& z, const OptTensor& target, double temperature, int64_t topk,
                  int64_t ignore_index, int64_t stream) {
-  if (!plain(z) || !f32_or_bf16(z) || z.dim() < 1 || row_stride(z) < 0 || tangent(z) || grad_on(z) ||
-      topk < 0 || topk > std::min<int64_t>(64, z.size(-1)))
+  if (!plain(z) || !f32_or_bf16(z) || z.dim() < 1 || row_stride(z) < 0 || tangent(z) || topk < 0 ||
+      topk > std::min<int64_t>(64, z.size(-1)))
     return none();
   const auto lead = z.sizes().slice(0, z.dim() - 1);
   if (target && (!plain(*target) || !target->is_contiguous() || target->sizes() != lead ||
@@ -808,23 +1059,17 @@ Result log_probs(const Tensor& z, const OptTensor& target, double temperature, i
   const mxgg_log_prob_options o{z.numel() / z.size(-1), z.size(-1), row_stride(z), ignore_index,
                                 type_of(z), target && target->scalar_type() == at::kLong,
                                 (int32_t)topk, (float)temperature};
-  const int64_t need = lib.token_log_probs_workspace_bytes(&o);
-  if (need < 0) return none();
+  if (lib.token_log_probs_workspace_bytes(&o) < 0) return none();
+  const variable_list r = grad_on(z) ? LogProbs::apply(z, target, o, stream)
+                                     : log_prob_forward(z, target, o, false, stream);
   OptTensor lp, ids, top;
-  Tensor ent = empty(lead, z, at::kFloat), ws = empty({need}, z, at::kByte);
-  if (target) lp = empty(lead, z, at::kFloat);
+  size_t i = 1;
+  if (target) lp = r[i++];
   if (topk > 0) {
-    auto size = lead.vec();
-    size.push_back(topk);
-    ids = empty(size, z, at::kInt);
-    top = empty(size, z, at::kFloat);
+    ids = r[i++];
+    top = r[i++];
   }
-  const int rc = lib.token_log_probs(
-      cp(z), target ? cp(*target) : nullptr, &o, lp ? lp->data_ptr<float>() : nullptr,
-      ent.data_ptr<float>(), ids ? ids->data_ptr<int32_t>() : nullptr,
-      top ? top->data_ptr<float>() : nullptr, nullptr, vp(ws), need, st(stream));
-  if (rc != MXGG_OK) return rc;
-  return std::make_tuple(lp, ent, ids, top);
+  return std::make_tuple(lp, r[0], ids, top);
 }
 
 // The gradients' norm, and with max_norm not negative their clipping.
@@ -878,6 +1123,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw", torch::wrap_pybind_function_no_gil(&adamw));
   m.def("block_dim0", torch::wrap_pybind_function_no_gil(&block_dim0));
   m.def("block_mm", torch::wrap_pybind_function_no_gil(&block_mm));
+  m.def("block_linear", torch::wrap_pybind_function_no_gil(&block_linear));
   m.def("add_norm", torch::wrap_pybind_function_no_gil(&add_norm));
   m.def("rms_quant", torch::wrap_pybind_function_no_gil(&rms_quant));
   m.def("log_probs", torch::wrap_pybind_function_no_gil(&log_probs));

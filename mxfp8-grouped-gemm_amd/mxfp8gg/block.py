@@ -291,6 +291,11 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor,
     gradients of 0).  N and K are multiples of 16.  Differentiable in x and w: the
     gradients' products are block-scaled as well, dy in blocks along N for x's and in
     blocks of tokens, as x, for w's."""
+    host = _native(x)
+    if host is not None and isinstance(w, torch.Tensor) and _tensors(offs):
+        r = host.block_linear(x, w, offs, _stream_ptr(x))
+        if _took(r, "fp8_block_linear"):
+            return r
     _need_gpu(x, "x")
     _need_gpu(w, "w")
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
