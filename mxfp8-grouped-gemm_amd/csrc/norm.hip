@@ -288,6 +288,10 @@ __device__ __forceinline__ void mx_payload(const float* o, uint32_t b, int mode,
 // are computed for `run` consecutive rows a workgroup, their scales gathered in LDS
 // and written as one run for each block (a byte at a time they would be a memory
 // transaction each: 224 a row of 7168).
+// Memory-bound, 16384 x 7168 bf16: both sums and the norm 168-177 us (5.5 TB/s of two
+// streams in and two out), its backward pass with the residual stream's gradient 166
+// (5.7); 8-bit results 170-174 us, without a residual 86 (fp32 scales) and 100 (E8M0: the
+// encoding's vector instructions).
 template <typename T, int CH, bool WAVE, int OUT, bool ADD>
 __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add_norm(AddNormArgs a) {
   constexpr int E = Elems<T>::kCount;
