@@ -3,9 +3,10 @@
 bf16 -> MXFP8 casts, a forward grouped GEMM and a weight-gradient grouped GEMM
 over ragged expert groups, the expert FFN's fused SwiGLU casts, the token
 routing (decision, dispatch plan, gather, combine), norms, the loss of a linear
-layer over a vocabulary and the optimizer step around them, all as hand-written
-HIP kernels in libmxgg.so behind a C ABI (include/mxgg.h).  This package is the
-host side: it takes torch tensors, allocates outputs, and calls the library on
+layer over a vocabulary and the optimizer step around them, products of e4m3
+operands in blocks of 128, log probabilities of tokens and gradient clipping, all
+as hand-written HIP kernels in libmxgg.so behind a C ABI (include/mxgg.h).  This
+package is the host side: it takes torch tensors, allocates outputs, and calls the library on
 the current stream.
 """
 from ._lib import MxggError, load as load_library
