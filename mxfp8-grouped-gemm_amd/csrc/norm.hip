@@ -287,11 +287,10 @@ __device__ __forceinline__ void mx_payload(const float* o, uint32_t b, int mode,
 // Scales are laid out block by block, rows next to each other, so the 8-bit outputs
 // are computed for `run` consecutive rows a workgroup, their scales gathered in LDS
 // and written as one run for each block (a byte at a time they would be a memory
-// transaction each: 224 a row of 7168).
+// transaction each: 224 a row of 7168); runs of one row write theirs at once.
 // Memory-bound, 16384 x 7168 bf16: both sums and the norm 168-177 us (5.5 TB/s of two
 // streams in and two out), its backward pass with the residual stream's gradient 166
-// (5.7); 8-bit results 170-174 us, without a residual 86 (fp32 scales) and 100 (E8M0: the
-// encoding's vector instructions).
+// (5.7); 8-bit results 167-169 us.
 template <typename T, int CH, bool WAVE, int OUT, bool ADD>
 __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add_norm(AddNormArgs a) {
   constexpr int E = Elems<T>::kCount;
@@ -379,7 +378,8 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add
           if constexpr (OUT == kOutMx) {
             const uint32_t b = e8m0_from_amax32(m, a.mode);
             mx_payload<E>(o, b, a.mode, p);
-            if (first) held[chunk / kLanes * kScaleRun + i] = (uint8_t)b;
+            if (first && run == 1) static_cast<uint8_t*>(a.scales)[chunk / kLanes * a.lds + row] = (uint8_t)b;
+            else if (first) held[chunk / kLanes * kScaleRun + i] = (uint8_t)b;
           } else {
             const float sc = block_scale(__uint_as_float(m));
             const BlockDivisor d(sc);
@@ -389,7 +389,8 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add
               p[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(d(o[4 * k + 2]), d(o[4 * k + 3]),
                                                                (int)p[k], true);
             }
-            if (first) reinterpret_cast<float*>(held)[chunk / kLanes * kScaleRun + i] = sc;
+            if (first && run == 1) static_cast<float*>(a.scales)[chunk / kLanes * a.lds + row] = sc;
+            else if (first) reinterpret_cast<float*>(held)[chunk / kLanes * kScaleRun + i] = sc;
           }
           if (n[c] > 0) {  // whole chunks: the width is a multiple of 16
             uint8_t* q = a.q + row * a.ldq + (int64_t)chunk * E;
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kNormMaxThreads) void k_add
         }
       }
     }
-    if constexpr (kQuant) {
+    if (kQuant && run > 1) {
       __syncthreads();
       constexpr int kWidth = OUT == kOutMx ? 32 : 128, kSize = OUT == kOutMx ? 1 : 4;
       const int blocks = (a.cols + kWidth - 1) / kWidth;
@@ -655,6 +656,19 @@ int norm_grid(int64_t rows, const NormShape& s) {
   return (int)std::min<int64_t>(own, std::max(1, device_cu_count()) * per_cu);
 }
 
+// The norm with the residual's addition has more work an element than k_norm_fwd, and rows of
+// a workgroup take two chunks a thread where they fit, as long as the sum and the norm leave
+// as they are only up to 2^26 elements.  7168 bf16, two chunks against four, us, sum and norm
+// / E8M0 / fp32 scales: 64 rows 3.5 / 4.6 / 4.4 and 4.7 / 7.5 / 6.2, 1024 8.0 / 11.0 / 9.8 and
+// 9.0 / 12.9 / 11.3, 4096 35.2 / 36.8 / 35.0 and 36.7 / 40.2 / 37.9, 16384 174 / 169 / 167
+// and 169 / 173 / 170.
+NormShape add_norm_shape(const AddNormArgs& a) {
+  const int per_chunk = a.bf16 ? 8 : 4, chunks = (a.cols + per_chunk - 1) / per_chunk;
+  const NormShape s = norm_shape(a.cols, per_chunk);
+  if (s.wave || chunks > 2 * kNormMaxThreads || (!a.q && a.rows * a.cols > INT64_C(1) << 26)) return s;
+  return {2, ((chunks + 1) / 2 + 63) / 64 * 64, false};
+}
+
 template <typename T, int CH, bool WAVE>
 void run_add_norm(const AddNormArgs& a, int grid, int threads, hipStream_t stream) {
   const auto go = [&](auto kernel) {
@@ -672,7 +686,8 @@ void run_add_shape(const AddNormArgs& a, int grid, const NormShape& s, hipStream
     else if (!kF32 || s.ch == 2) run_add_norm<T, 2, true>(a, grid, s.threads, stream);
     else if constexpr (kF32) run_add_norm<T, 4, true>(a, grid, s.threads, stream);
   } else {
-    if (s.ch == 4) run_add_norm<T, 4, false>(a, grid, s.threads, stream);
+    if (s.ch == 2) run_add_norm<T, 2, false>(a, grid, s.threads, stream);
+    else if (s.ch == 4) run_add_norm<T, 4, false>(a, grid, s.threads, stream);
     else if (!kF32 || s.ch == 8) run_add_norm<T, 8, false>(a, grid, s.threads, stream);
     else if constexpr (kF32) run_add_norm<T, 16, false>(a, grid, s.threads, stream);
   }
@@ -682,7 +697,7 @@ void run_add_shape(const AddNormArgs& a, int grid, const NormShape& s, hipStream
 
 hipError_t launch_add_norm(AddNormArgs a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;
-  const NormShape s = norm_shape(a.cols, a.bf16 ? 8 : 4);
+  const NormShape s = add_norm_shape(a);
   int grid = norm_grid(a.rows, s);
   if (a.q) {  // runs of up to 16 rows, as long as every workgroup has one
     const int64_t unit = s.wave ? kWaveRows : 1, own = (a.rows + unit * grid - 1) / (unit * grid);
