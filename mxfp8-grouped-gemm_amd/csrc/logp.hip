@@ -12,9 +12,9 @@
 // kept apart, so nothing is lost where the logits share a large offset.
 //
 // The k best: the pass leaves the maximum of every 64 consecutive logits in LDS.  The
-// k-th largest of 64 interleaved groups' maxima bounds the k-th best from below; the few
-// runs of 64 that reach it are read again and what reaches it is collected, a few
-// more than k values, among which k are picked by value, then lowest index.  Rows
+// k-th largest of 64 interleaved groups' maxima (of 256 where k is large) bounds the k-th
+// best from below; the few runs of 64 that reach it are read again and what reaches it is
+// collected, a few more than k values, among which k are picked by value, then lowest index.  Rows
 // where more reach the bound than the list holds (thousands of equal logits) are searched
 // again for each of the k.
 //
@@ -22,8 +22,8 @@
 //
 // Measured: 4096 x 131072 bf16 191-200 us (5.4-5.6 TB/s), with 8 alternatives 205, their
 // gradient 379 (5.7 TB/s read and written); 1000 x 50021 fp32 34 us (6.0), with 20
-// alternatives 41; 16 x 131072 with 8 in 32 parts each 10 us and 7 for the join, where the
-// chain of dependent steps counts, not the 4 MB.
+// alternatives 41; 16 x 131072 with 8 alternatives 11.7 us (with 64 23.8), 16 x 32000 8.2,
+// where the chain of dependent steps counts, not the 4 MB.
 #include <algorithm>
 
 #include "mx_device.h"
@@ -38,10 +38,14 @@ constexpr int kAhead = 4;                  // 16-byte loads of a thread in fligh
 constexpr int kSeg = 64;                   // consecutive logits under one maximum
 constexpr int kMaxSegs = 4096;
 constexpr int64_t kMaxPart = (int64_t)kSeg * kMaxSegs;
-constexpr int64_t kMinPart = 4096;         // elements of a workgroup, at least
+constexpr int64_t kMinPart = 8192;         // elements of a workgroup, at least
+constexpr int64_t kWholeBytes = 128 << 10; // rows of up to this many stay whole
 constexpr int kMaxParts = 64;              // of a row
 constexpr int kList = 2048;                // candidates
 constexpr int kMaxTop = 64;
+// Alternatives up to which 64 groups bound well: 64 of 64 leave 300 candidates and more,
+// 16 x 131072 with 64 alternatives 107 us (23.8 with 256 groups), with 20 13.7.
+constexpr int kCoarse = 32;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kFar = -1e6f;              // an exponent whose power of two is 0
@@ -153,15 +157,32 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t x) {
   return x;
 }
 
-// The k-th largest of 64 lanes' values (-inf where fewer are above it).
+// The k-th largest of 64 lanes' values (-inf where fewer are above it): the smallest of those
+// that fewer than k others are above.
 __device__ __forceinline__ float kth_of_lanes(float x, int k) {
-  float b = -kInf;
-  for (int r = 0; r < k; ++r) {
-    b = wave_max(x);
-    const uint64_t who = __ballot(x == b);
-    if ((int)(threadIdx.x & 63) == __builtin_ctzll(who ? who : 1)) x = -kInf;
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 64; ++j)
+    above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), j)) > x ? 1 : 0;
+  return -wave_max(above < k ? -x : -kInf);
+}
+// The same of the first 256 threads' values, for the workgroup; held: 256 values, low: 4.
+__device__ __forceinline__ float kth_of_group(float x, int k, float* held, float* low) {
+  const int tid = threadIdx.x;
+  if (tid < 256) held[tid] = x;
+  __syncthreads();
+  if (tid < 256) {
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 256; j += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(held + j);
+      above += (o.x > x ? 1 : 0) + (o.y > x ? 1 : 0) + (o.z > x ? 1 : 0) + (o.w > x ? 1 : 0);
+    }
+    const float m = -wave_max(above < k ? -x : -kInf);
+    if ((tid & 63) == 0) low[tid >> 6] = m;
   }
-  return b;
+  __syncthreads();
+  return __builtin_fminf(__builtin_fminf(low[0], low[1]), __builtin_fminf(low[2], low[3]));
 }
 
 // The k best of n different keys in LDS (0 is none), in falling order, by every thread of
@@ -263,10 +284,10 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
   constexpr int kSegLanes = kSeg / E;
   __shared__ Sums parts[kLogpWaves];
   __shared__ float seg_max[TOP ? kMaxSegs : 1];
-  __shared__ uint64_t list[TOP ? kList : 1];
+  __shared__ __attribute__((aligned(16))) uint64_t list[TOP ? kList : 1];
   __shared__ uint16_t segs[TOP ? kMaxSegs : 1];
   __shared__ int counts[2];
-  __shared__ float bound;
+  __shared__ float bound, low[4];
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t target = a.target ? target_of(a, row) : -1;
@@ -328,14 +349,22 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
   }
   if constexpr (TOP) {
     const int nseg = (len + kSeg - 1) / kSeg;
-    if (wave == 0) {
+    const auto best_of = [&](int from, int step) {
       float best = -kInf;
-      for (int s = lane; s < nseg; s += 64) best = __builtin_fmaxf(best, seg_max[s]);
-      const float b = kth_of_lanes(best, a.k);
-      if (lane == 0) bound = b;
+      for (int s = from; s < nseg; s += step) best = __builtin_fmaxf(best, seg_max[s]);
+      return best;
+    };
+    float b;
+    if (a.k <= kCoarse) {
+      if (wave == 0) {
+        b = kth_of_lanes(best_of(lane, 64), a.k);
+        if (lane == 0) bound = b;
+      }
+      __syncthreads();
+      b = bound;
+    } else {
+      b = kth_of_group(tid < 256 ? best_of(tid, 256) : -kInf, a.k, reinterpret_cast<float*>(list), low);
     }
-    __syncthreads();
-    const float b = bound;
     for (int s = tid; s < nseg; s += kLogpThreads)
       if (seg_max[s] >= b && seg_max[s] > -kInf) segs[atomicAdd(&counts[0], 1)] = (uint16_t)s;
     __syncthreads();
@@ -398,9 +427,9 @@ __global__ __launch_bounds__(kLogpThreads) void k_logp(LogpArgs a) {
 // Joins the parts of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a) {
-  __shared__ uint64_t list[kMaxParts * kMaxTop];
+  __shared__ __attribute__((aligned(16))) uint64_t list[kMaxParts * kMaxTop];
   __shared__ Sums sums;
-  __shared__ float bound;
+  __shared__ float bound, low[4];
   __shared__ int count;
   const int64_t row = blockIdx.x;
   const int64_t target = a.target ? target_of(a, row) : -1;
@@ -418,16 +447,17 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a) {
     own[u] = 0;
     if (u * 256 < n && u * 256 + (int)threadIdx.x < n) own[u] = from[u * 256 + threadIdx.x];
   }
+  // the first candidates of every part (they are in falling order), as many as threads hold
+  const int p = (int)(threadIdx.x % (uint32_t)a.parts), r = (int)(threadIdx.x / (uint32_t)a.parts);
+  const float best = r < a.k ? pick_of(from[p * a.k + r]).v : -kInf;
   if (threadIdx.x < 64) {  // a lane for each part, at most kMaxParts
     Sums t{-kInf, 0.0f, 0.0f};
-    float best = -kInf;  // of the part: each part's candidates are in falling order
     if (threadIdx.x < a.parts) {
       const float4 v = a.part_sums[row * a.parts + threadIdx.x];
       t = Sums{v.x, v.y, v.z};
-      if (n > 0) best = pick_of(from[threadIdx.x * a.k]).v;
     }
     t = wave_join(t, a.c);
-    const float b = n > 0 ? kth_of_lanes(best, a.k) : 0.0f;
+    const float b = n > 0 && a.k <= kCoarse ? kth_of_lanes(best, a.k) : 0.0f;
     if (threadIdx.x == 0) {
       sums = t;
       bound = b;
@@ -439,7 +469,8 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a) {
   const float log_s = logf(t.s);
   if (threadIdx.x == 0) write_row(a, row, t, log_s, target, z_target);
   if (n == 0) return;
-  const float b = bound;
+  const float b = a.k <= kCoarse ? bound
+                                 : kth_of_group(best, a.k, reinterpret_cast<float*>(list), low);
 #pragma unroll
   for (int u = 0; u < kOwn; ++u)  // in any order: the keys order themselves
     if (own[u] != 0 && pick_of(own[u]).v >= b) list[atomicAdd(&count, 1)] = own[u];
@@ -553,11 +584,17 @@ __global__ __launch_bounds__(kGradThreads) void k_logp_grad(LogpGradArgs a) {
   }
 }
 
-// Parts of a row: one where the rows fill the chip twice over, else as many as do, of
-// kMinPart elements at least; at most kMaxPart (the maxima held in LDS) each.
+// Parts of a row: one where there is a row for each compute unit or rows are short, else as
+// many as fill the chip twice over, of kMinPart elements at least; at most kMaxPart (the
+// maxima held in LDS) each.  Whole against split, us, without and with 8 alternatives: 256 x
+// 131072 bf16 14.9 / 21.8 and 17.5 / 26.1, 128 rows of it 12.8 / 19.9 and 11.4 / 19.4; 16 x
+// 65536 7.3 / 12.1 and 7.2 / 13.3, 16 x 32000 4.9 / 8.8 and 7.2 / 13.7; fp32 with 8, 16 x
+// 65536 13.6 and 12.4, 16 x 32000 9.3 and 12.6.  Parts of 4096, 8192 and 16384 (16 x 131072
+// bf16 with 8): 14.1, 12.2, 12.4.
 int64_t logp_part_len(const LogpArgs& a) {
   const int64_t cus = std::max(1, device_cu_count());
-  int64_t parts = a.T >= 2 * cus ? 1 : (2 * cus + a.T - 1) / std::max<int64_t>(a.T, 1);
+  const bool whole = a.T >= cus || a.V * (a.bf16 ? 2 : 4) <= kWholeBytes;
+  int64_t parts = whole ? 1 : (2 * cus + a.T - 1) / std::max<int64_t>(a.T, 1);
   parts = std::min(parts, (a.V + kMinPart - 1) / kMinPart);
   parts = std::min<int64_t>(parts, kMaxParts);
   parts = std::max(parts, (a.V + kMaxPart - 1) / kMaxPart);
