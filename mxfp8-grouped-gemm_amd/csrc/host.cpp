@@ -993,12 +993,13 @@ variable_list log_prob_forward(const Tensor& z, const OptTensor& target,
   }
   if (keep_stats) stats = empty({3, o.tokens}, z, at::kFloat);
   const int64_t need = lib.token_log_probs_workspace_bytes(&o);
-  const Tensor ws = empty({std::max<int64_t>(need, 0)}, z, at::kByte);
+  Tensor ws;
+  if (need > 0) ws = empty({need}, z, at::kByte);
   check(lib.token_log_probs(cp(z), target ? cp(*target) : nullptr, &o,
                             static_cast<float*>(vp_or_null(lp)), ent.data_ptr<float>(),
                             static_cast<int32_t*>(vp_or_null(ids)),
                             static_cast<float*>(vp_or_null(top)),
-                            static_cast<float*>(vp_or_null(stats)), vp(ws), need, st(stream)),
+                            static_cast<float*>(vp_or_null(stats)), vp_or_null(ws), need, st(stream)),
         "token_log_probs");
   variable_list r{ent};
   if (target) r.push_back(lp);
