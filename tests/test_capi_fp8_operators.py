@@ -259,13 +259,17 @@ def test_log_probs(lib):
     for kw in (dict(options=None), dict(z=None), dict(target=None), dict(ids=None),
                dict(stats=None), dict(dz=None)):
         assert _call(lib.mxgg_token_log_probs_grad, LOGP_GRAD, kw) == INVALID
+    none = _logp(tokens=0)
+    assert _call(lib.mxgg_token_log_probs, LOGP, dict(options=none, z=None)) == _lib.OK
+    assert _call(lib.mxgg_token_log_probs_grad, LOGP_GRAD, dict(options=none, z=None)) == _lib.OK
+    assert lib.mxgg_token_log_probs_workspace_bytes(none) == 0
+
+
+@pytest.mark.gpu  # which rows are shared out depends on the card
+def test_log_probs_workspace(gpu, lib):
     long = dict(tokens=1, vocab=1 << 17, ldz=1 << 17)
     need = lib.mxgg_token_log_probs_workspace_bytes(_logp(**long))
     assert need > 0
     for status, kw in ((SHAPE, dict(workspace_bytes=need - 1)), (INVALID, dict(workspace=None)),
                        (ALIGNMENT, dict(workspace=P + 4))):
         assert _call(lib.mxgg_token_log_probs, LOGP, {"options": _logp(**long), **kw}) == status
-    none = _logp(tokens=0)
-    assert _call(lib.mxgg_token_log_probs, LOGP, dict(options=none, z=None)) == _lib.OK
-    assert _call(lib.mxgg_token_log_probs_grad, LOGP_GRAD, dict(options=none, z=None)) == _lib.OK
-    assert lib.mxgg_token_log_probs_workspace_bytes(none) == 0
