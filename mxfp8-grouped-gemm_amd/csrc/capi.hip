@@ -1658,7 +1658,7 @@ int mxgg_block_quant_dim1(const void* x, int64_t rows, int64_t cols, int64_t ldx
   if (rows_pad_cap % 128 != 0 || rows_pad_cap < need / 128 * 128 || rows_pad_cap < rows)
     return set_error(MXGG_ERR_SHAPE, "%s: rows_pad_cap=%lld for %lld rows in %lld groups", what,
                      (long long)rows_pad_cap, (long long)rows, (long long)num_groups);
-  if (rows_pad_cap / 128 > 65535)
+  if (rows_pad_cap > kMaxBlockWidth)  // what mxgg_block_wgrad takes
     return set_error(MXGG_ERR_UNSUPPORTED, "%s: rows_pad_cap=%lld", what, (long long)rows_pad_cap);
   if (group_ends && !group_ends_pad)
     return set_error(MXGG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);

@@ -51,7 +51,8 @@ DIM1 = dict(x=P, rows=200, cols=64, ldx=64, ends=P, groups=2, cap=512, q=P, ldq=
     (SHAPE, dict(cap=128, ends=None, groups=0)), (INVALID, dict(ends_pad=None)),
     (INVALID, dict(qt=None)), (INVALID, dict(st=None)), (SHAPE, dict(ldst=63)),
     (ALIGNMENT, dict(qt=P + 8)), (ALIGNMENT, dict(q=P + 4)), (INVALID, dict(scales=None)),
-    (SHAPE, dict(lds=199)), (UNSUPPORTED, dict(cap=128 << 16))])
+    (SHAPE, dict(lds=199)), (UNSUPPORTED, dict(cap=128 << 16)),
+    (UNSUPPORTED, dict(cap=(1 << 22) + 128))])
 def test_block_quant_dim1(lib, status, kw):
     assert _call(lib.mxgg_block_quant_dim1, DIM1, kw) == status
     assert lib.mxgg_last_error()
