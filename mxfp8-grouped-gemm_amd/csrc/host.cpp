@@ -705,6 +705,11 @@ bool grad_on(const OptTensor& t) { return t && grad_on(*t); }
 Tensor block_scales(int64_t blocks, int64_t rows, const Tensor& like) {
   return empty({blocks, (rows + 3) / 4 * 4}, like, at::kFloat);
 }
+// The same as the caller sees it, [rows, blocks]: a view would take as long as the allocation.
+Tensor block_scales_of_rows(int64_t rows, int64_t blocks, const Tensor& like) {
+  return at::empty_strided({rows, blocks}, {1, (rows + 3) / 4 * 4},
+                           like.options().dtype(at::kFloat).requires_grad(false));
+}
 
 // A cast: payload and scales by rows (q, s) and by columns of tokens (qt, st), the scales as
 // they are stored.
@@ -737,10 +742,12 @@ int cast_tokens(const Tensor& x, const OptTensor& ends, bool rows, BlockCast& c,
 
 Result block_dim0(const Tensor& x, int64_t stream) {
   if (!bf16_rows(x) || x.size(1) % 16 != 0) return none();
-  BlockCast c;
-  const int rc = cast_rows(x, c, stream);
+  const int64_t M = x.size(0), K = x.size(1);
+  Tensor q = empty({M, K}, x, at::kFloat8_e4m3fn), s = block_scales_of_rows(M, (K + 127) / 128, x);
+  const int rc = lib.block_quant_dim0(cp(x), M, K, rows_ld(x), vp(q), K, s.data_ptr<float>(),
+                                      s.stride(1), st(stream));
   if (rc != MXGG_OK) return rc;
-  return std::make_tuple(c.q, rows_view(c.s, x.size(0)));
+  return std::make_tuple(q, s);
 }
 
 // y of operands whose layout has been checked; ld of a and of its scales.
@@ -967,15 +974,16 @@ Result rms_quant(const Tensor& x, const OptTensor& weight, const OptTensor& resi
     return none();
   const mxgg_norm_options o = add_norm_options(x, weight, eps);
   Tensor q = empty({o.rows, o.cols}, x, at::kFloat8_e4m3fn);
-  Tensor s = mx ? block_major(o.rows, o.cols / 32, x) : block_scales((o.cols + 127) / 128, o.rows, x);
+  Tensor s = mx ? rows_view(block_major(o.rows, o.cols / 32, x), o.rows)
+                : block_scales_of_rows(o.rows, (o.cols + 127) / 128, x);
   OptTensor h;
   if (residual) h = empty(x.sizes(), x, x.scalar_type());
   const int rc = lib.rms_norm_quant(
       cp(x), row_stride(x), residual ? cp(*residual) : nullptr,
       residual ? row_stride(*residual) : 0, weight ? cp(*weight) : nullptr, &o,
-      h ? vp(*h) : nullptr, o.cols, vp(q), o.cols, vp(s), s.stride(0), format, mode, st(stream));
+      h ? vp(*h) : nullptr, o.cols, vp(q), o.cols, vp(s), s.stride(1), format, mode, st(stream));
   if (rc != MXGG_OK) return rc;
-  return std::make_tuple(q, rows_view(s, o.rows), h);
+  return std::make_tuple(q, s, h);
 }
 
 // Entropy, then log probabilities (with targets), ids and log probabilities of the top
