@@ -1089,7 +1089,8 @@ Result clip(const std::vector<Tensor>& grads, double max_norm, double eps, int64
   std::vector<const void*> at(n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
-    if (!plain(g) || !g.is_contiguous() || !f32_or_bf16(g) || g.device() != grads[0].device())
+    if (!plain(g) || !g.is_contiguous() || !f32_or_bf16(g) || g.device() != grads[0].device() ||
+        (max_norm >= 0 && g.requires_grad() && g.is_leaf()))  // a parameter in place of its gradient
       return none();
     at[i] = cp(g);
     table[i] = {const_cast<void*>(at[i]), g.numel(), type_of(g)};

@@ -125,8 +125,8 @@ def _own_memory(t: torch.Tensor) -> bool:
     return True
 
 
-def _grad_table(grads):
-    """The tensors' table for the library."""
+def _grad_table(grads, written):
+    """The tensors' table for the library; written: it scales them."""
     table = (_lib.GradTensor * max(len(grads), 1))()
     seen = set()
     for i, g in enumerate(grads):
@@ -136,6 +136,9 @@ def _grad_table(grads):
         if g.layout != torch.strided or g.dtype not in _TYPES:
             raise TypeError(f"grads[{i}] must be a dense float32 or bfloat16 tensor, got {g.dtype} "
                             f"({g.layout})")
+        if written and g.requires_grad and g.is_leaf:
+            raise ValueError(f"grads[{i}] is a parameter (a leaf that requires grad) and would be "
+                             "scaled itself: pass the parameters' gradients")
         if not _own_memory(g):
             raise ValueError(f"grads[{i}] must fill its memory without gaps or overlap, got "
                              f"{tuple(g.shape)} with strides {g.stride()}")
@@ -156,7 +159,7 @@ def _clip(grads, what, options=None):
                       0.0 if options is None else options.eps, _stream_ptr(grads[0]))
         if _took(r, what):
             return r
-    table = _grad_table(grads)
+    table = _grad_table(grads, options is not None)
     lib, n = _lib.load(), len(grads)
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -181,7 +184,9 @@ def clip_grad_norm_(grads, max_norm: float, eps: float = 1e-6) -> torch.Tensor:
     grad_norm(grads), which is returned.  Nothing waits for the device, and where nothing is
     clipped no gradient is written.  A norm that is NaN makes the gradients NaN, an
     infinite one makes the finite ones 0.  The tensors may be laid out in any order of
-    their dimensions but must not overlap."""
+    their dimensions but must not overlap.  Parameters themselves (leaves that require
+    grad, which torch's function of the name takes) are refused; the scaling is not
+    recorded by autograd."""
     max_norm, eps = float(max_norm), float(eps)
     if not (max_norm >= 0 and eps >= 0):
         raise ValueError(f"max_norm and eps must not be negative, got {max_norm} and {eps}")
