@@ -248,11 +248,12 @@ def fp8_block_wgrad(go_t: torch.Tensor, go_scales: torch.Tensor, ia_t: torch.Ten
 
 class FP8BlockLinear(torch.autograd.Function):
     """fp8_block_linear with both gradients.  Kept for the backward pass: the transposed
-    casts of x (for w's gradient) and of w (for x's)."""
+    casts of x (for w's gradient) and of w (for x's).  grad: grad mode where it is applied
+    (needs_input_grad does not know it, and in here it is off)."""
 
     @staticmethod
-    def forward(ctx, x, w, ends):
-        need_x, need_w = ctx.needs_input_grad[:2]
+    def forward(ctx, x, w, ends, grad=True):
+        need_x, need_w = (grad and n for n in ctx.needs_input_grad[:2])
         x2 = _bf16_rows(x, "x")
         if need_w:
             q, s, qt, st, pad = _dim1(x2, ends, True)
@@ -281,7 +282,7 @@ class FP8BlockLinear(torch.autograd.Function):
             dx = fp8_block_mm(q, s, wt, wts, ends)
             if ends is not None:
                 zero_rows_past_groups(dx, ends)
-        return dx, dw, None
+        return dx, dw, None, None
 
 
 def fp8_block_linear(x: torch.Tensor, w: torch.Tensor,
@@ -312,5 +313,5 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor,
         raise ValueError(f"N={N} and K={K} must be positive multiples of 16")
     _no_tangent("fp8_block_linear", x, w)
     ends = None if offs is None else _group_ends(offs, w.shape[0], x.device)
-    y = FP8BlockLinear.apply(x.reshape(-1, K), w, ends)
+    y = FP8BlockLinear.apply(x.reshape(-1, K), w, ends, torch.is_grad_enabled())
     return y.view(*x.shape[:-1], N)
