@@ -741,7 +741,7 @@ int cast_tokens(const Tensor& x, const OptTensor& ends, bool rows, BlockCast& c,
 }
 
 Result block_dim0(const Tensor& x, int64_t stream) {
-  if (!bf16_rows(x) || x.size(1) % 16 != 0) return none();
+  if (!bf16_rows(x) || x.size(1) % 16 != 0 || tangent(x)) return none();
   const int64_t M = x.size(0), K = x.size(1);
   Tensor q = empty({M, K}, x, at::kFloat8_e4m3fn), s = block_scales_of_rows(M, (K + 127) / 128, x);
   const int rc = lib.block_quant_dim0(cp(x), M, K, rows_ld(x), vp(q), K, s.data_ptr<float>(),
@@ -774,7 +774,8 @@ bool block_operand(const Tensor& t) {
 Result block_mm(const Tensor& a, const Tensor& as, const Tensor& w, const Tensor& ws,
                 const OptTensor& ends, bool f32, int64_t stream) {
   if (!block_operand(a) || a.dim() != 2 || !block_operand(w) || w.dim() != (ends ? 3 : 2) ||
-      !w.is_contiguous() || w.device() != a.device() || !ends_ok(ends, a))
+      !w.is_contiguous() || w.device() != a.device() || !ends_ok(ends, a) || tangent(a) ||
+      tangent(as) || tangent(w) || tangent(ws))
     return none();
   const int64_t M = a.size(0), K = a.size(1), N = w.size(-2), E = ends ? w.size(0) : 1;
   const int64_t nb = (N + 127) / 128, kb = (K + 127) / 128;
@@ -1090,7 +1091,7 @@ Result clip(const std::vector<Tensor>& grads, double max_norm, double eps, int64
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     if (!plain(g) || !g.is_contiguous() || !f32_or_bf16(g) || g.device() != grads[0].device() ||
-        (max_norm >= 0 && g.requires_grad() && g.is_leaf()))  // a parameter in place of its gradient
+        tangent(g) || (max_norm >= 0 && g.requires_grad() && g.is_leaf()))  // a parameter itself
       return none();
     at[i] = cp(g);
     table[i] = {const_cast<void*>(at[i]), g.numel(), type_of(g)};

@@ -10,7 +10,9 @@ the weight gradient in blocks of 128 tokens.
 
 A scale is max(amax * (1 / 448), 2^-126) in fp32 and the payload e4m3(x / scale), to
 nearest even.  Sums are fp32.  Widths are multiples of 16; the last block of a row may be
-narrower than 128.  With `offs` the rows are grouped by expert as in grouped_mm.
+narrower than 128.  With `offs` the rows are grouped by expert as in grouped_mm.  Inputs
+that carry a tangent of forward-mode differentiation are refused; casts of inputs that
+require grad are not recorded by autograd.
 """
 from __future__ import annotations
 
@@ -61,6 +63,8 @@ def to_fp8_block_dim0(x: torch.Tensor):
         r = host.block_dim0(x, _stream_ptr(x))
         if _took(r, "to_fp8_block_dim0"):
             return r
+    _need_gpu(x, "x")
+    _no_tangent("to_fp8_block_dim0", x)
     x = _bf16_rows(x, "x")
     M, K = x.shape
     q = torch.empty((M, K), dtype=_FP8, device=x.device)
@@ -95,6 +99,8 @@ def to_fp8_block_dim1(x: torch.Tensor, offs: torch.Tensor | None = None):
     """(payload e4m3 [C, T], scales fp32 [C, T / 128], padded ends or None) of x bf16
     [M, C] in blocks of 128 tokens of a column, transposed.  The tokens of every group of
     `offs` (all of them without) are padded with zeros to whole blocks."""
+    _need_gpu(x, "x")
+    _no_tangent("to_fp8_block_dim1", x)
     x = _bf16_rows(x, "x")
     ends = None if offs is None else _ends(offs, x)
     return _dim1(x, ends, False)[2:]
@@ -117,6 +123,7 @@ def to_fp8_block_weight(w: torch.Tensor, dual: bool = False):
     N, K = w.shape[-2:]
     if K % 16 != 0 or (dual and N % 16 != 0):
         raise ValueError(f"w {tuple(w.shape)}: K (and N with dual) must be multiples of 16")
+    _no_tangent("to_fp8_block_weight", w)
     w = w.detach().contiguous()
     if w.data_ptr() % 16:
         w = w.clone()
@@ -137,7 +144,6 @@ def to_fp8_block_weight(w: torch.Tensor, dual: bool = False):
 
 def _payload(t: torch.Tensor, name: str, dims) -> torch.Tensor:
     """An e4m3 (or raw byte) operand with 16-byte aligned rows."""
-    _need_gpu(t, name)
     if t.dim() not in dims:
         raise ValueError(f"{name} must have {' or '.join(map(str, dims))} dimensions, "
                          f"got {tuple(t.shape)}")
@@ -153,7 +159,6 @@ def _payload(t: torch.Tensor, name: str, dims) -> torch.Tensor:
 
 def _row_scales(s: torch.Tensor, shape, name: str, device):
     """(scales of one a row and block, stride from block to block), rows consecutive."""
-    _need_gpu(s, name)
     if s.dtype != torch.float32 or tuple(s.shape) != shape or s.device != device:
         raise ValueError(f"{name} must be float32 {shape} on {device}, got {s.dtype} "
                          f"{tuple(s.shape)} on {s.device}")
@@ -180,6 +185,9 @@ def fp8_block_mm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor,
         r = host.block_mm(a, a_scales, w, w_scales, offs, out == _lib.OUT_F32, _stream_ptr(a))
         if _took(r, "fp8_block_mm"):
             return r
+    for t, name in ((a, "a"), (a_scales, "a_scales"), (w, "w"), (w_scales, "w_scales")):
+        _need_gpu(t, name)
+    _no_tangent("fp8_block_mm", a, a_scales, w, w_scales)
     a = _payload(a, "a", (2,))
     w = _payload(w, "w", (2, 3))
     M, K = a.shape
@@ -191,7 +199,6 @@ def fp8_block_mm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor,
     if (offs is None) != (w.dim() == 2):
         raise ValueError("offs goes with weights [E, N, K]")
     a_s, ldas = _row_scales(a_scales, (M, _blocks(K)), "a_scales", a.device)
-    _need_gpu(w_scales, "w_scales")
     shape = (*w.shape[:-2], _blocks(N), _blocks(K))
     if w_scales.dtype != torch.float32 or tuple(w_scales.shape) != shape \
             or w_scales.device != a.device:
@@ -223,6 +230,9 @@ def fp8_block_wgrad(go_t: torch.Tensor, go_scales: torch.Tensor, ia_t: torch.Ten
     scales [N, T / 128], ia_t [K, T] with [K, T / 128].  Returns [N, K], or [E, N, K] for
     the padded ends that the casts return (every entry a multiple of 128)."""
     out = _out_code(out_dtype)
+    for t, name in ((go_t, "go_t"), (go_scales, "go_scales"), (ia_t, "ia_t"), (ia_scales, "ia_scales")):
+        _need_gpu(t, name)
+    _no_tangent("fp8_block_wgrad", go_t, go_scales, ia_t, ia_scales)
     go, ia = _payload(go_t, "go_t", (2,)), _payload(ia_t, "ia_t", (2,))
     N, T = go.shape
     K = ia.shape[0]

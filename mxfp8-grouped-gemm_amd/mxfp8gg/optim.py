@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _FP8, _native, _need_gpu, _stream_ptr, _tensors, _took
+from .ops import _FP8, _native, _need_gpu, _no_tangent, _stream_ptr, _tensors, _took
 
 __all__ = ["AdamW", "adamw_step", "adamw_state", "grad_norm", "clip_grad_norm_"]
 
@@ -160,6 +160,7 @@ def _clip(grads, what, options=None):
         if _took(r, what):
             return r
     table = _grad_table(grads, options is not None)
+    _no_tangent(what, *grads)
     lib, n = _lib.load(), len(grads)
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
