@@ -17,6 +17,8 @@
 // another ABI version than the header this module was compiled with.
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
+
 #include <algorithm>
 #include <cstring>
 #include <optional>
@@ -432,9 +434,13 @@ void* vp_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr;
 const void* cp_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 // Refuses a backward pass under create_graph: the gradients would be constants in its
-// graph, and second derivatives would leave their part out unnoticed.
-void first_order(const char* what) {
+// graph, and second derivatives would leave their part out unnoticed.  The same where an
+// incoming gradient carries a forward-mode tangent.
+void first_order(const char* what, const variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " cannot be differentiated twice (create_graph)");
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& g : grads)
+    TORCH_CHECK(!g.defined() || !tangent(g), "the gradient of ", what, " has no forward-mode derivative");
 }
 
 // (expert_idx, weights) and, for the gradient, what it needs of the chosen.
@@ -464,7 +470,7 @@ struct RouteTopK : torch::autograd::Function<RouteTopK> {
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    first_order("route_topk");
+    first_order("route_topk", grads);
     const variable_list saved = ctx->get_saved_variables();
     const auto o = kept<mxgg_route_options>(ctx, "options");
     const Tensor d = grads[1].to(at::kFloat).contiguous();
@@ -529,7 +535,7 @@ struct Norm : torch::autograd::Function<Norm> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    first_order("norm");
+    first_order("norm", grads);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const auto o = kept<mxgg_norm_options>(ctx, "options");
@@ -605,7 +611,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    first_order("linear_cross_entropy");
+    first_order("linear_cross_entropy", grads);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &target = saved[2], &stats = saved[3];
     const auto o = kept<mxgg_loss_options>(ctx, "options");
@@ -827,7 +833,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const char* what = "fp8_block_linear";
-    first_order(what);
+    first_order(what, grads);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &xt = saved[0], &xts = saved[1], &pad = saved[2];
     const OptTensor ends = saved[3].defined() ? OptTensor(saved[3]) : OptTensor();
@@ -925,7 +931,8 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    first_order("add_rms_norm");
+    // where only h was used, dh passes through as it is
+    first_order("add_rms_norm", grads[0].defined() ? grads : variable_list());
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &w = saved[1], &stats = saved[2];
     const auto o = kept<mxgg_norm_options>(ctx, "options");
@@ -1035,7 +1042,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    first_order("token_log_probs");
+    first_order("token_log_probs", grads);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &z = saved[0], &target = saved[1], &ids = saved[2], &stats = saved[3];
     const auto o = kept<mxgg_log_prob_options>(ctx, "options");

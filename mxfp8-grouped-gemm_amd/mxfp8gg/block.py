@@ -278,7 +278,7 @@ class FP8BlockLinear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _first_order("fp8_block_linear")
+        _first_order("fp8_block_linear", dy)
         qt, st, pad, ends, wt, wts = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         dy = _bf16_rows(dy.to(torch.bfloat16), "dy")

@@ -63,7 +63,7 @@ class _TokenLogProbs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, glp, gent, _, gtop):
-        _first_order("token_log_probs")
+        _first_order("token_log_probs", glp, gent, gtop)
         z, target, ids, stats = ctx.saved_tensors
         g = [t.to(torch.float32).contiguous() if t is not None else None for t in (glp, gent, gtop)]
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)

@@ -63,7 +63,7 @@ class LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
-        _first_order("linear_cross_entropy")
+        _first_order("linear_cross_entropy", dloss)
         x, w, target, stats = ctx.saved_tensors
         opt, dev = ctx.opt, x.device
         need_x, need_w = ctx.needs_input_grad[:2]

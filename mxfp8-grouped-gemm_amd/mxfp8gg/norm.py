@@ -66,7 +66,7 @@ class Norm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _first_order("norm")
+        _first_order("norm", dy)
         x2, w, stats = ctx.saved_tensors
         opt, dev = ctx.opt, x2.device
         dy2 = _rows(dy.to(x2.dtype), opt.cols)
@@ -197,7 +197,8 @@ class AddRMSNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh):
-        _first_order("add_rms_norm")
+        # where only h was used, dh passes through as it is
+        _first_order("add_rms_norm", *((dy, dh) if dy is not None else ()))
         h, w, stats = ctx.saved_tensors
         opt, dev = ctx.opt, h.device
         need_w = ctx.needs_input_grad[2]

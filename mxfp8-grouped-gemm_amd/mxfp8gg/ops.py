@@ -73,13 +73,6 @@ def _need_gpu(t: torch.Tensor, name: str) -> None:
         )
 
 
-def _first_order(what: str) -> None:
-    """Refuses a backward pass under create_graph: the gradients would be constants in
-    its graph, and second derivatives would leave their part out unnoticed."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what} cannot be differentiated twice (create_graph)")
-
-
 def _no_tangent(what: str, *ts) -> None:
     """Refuses inputs that carry a tangent of forward-mode differentiation: the result
     would come without one, which reads as a derivative of zero."""
@@ -87,6 +80,15 @@ def _no_tangent(what: str, *ts) -> None:
             t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
             for t in ts):
         raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
+def _first_order(what: str, *grads) -> None:
+    """Refuses a backward pass under create_graph: the gradients would be constants in
+    its graph, and second derivatives would leave their part out unnoticed.  The same where
+    an incoming gradient carries a forward-mode tangent."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} cannot be differentiated twice (create_graph)")
+    _no_tangent(f"the gradient of {what}", *grads)
 
 
 def _mode(scaling_mode) -> int:

@@ -75,7 +75,7 @@ class RouteTopK(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, _, dscores):
-        _first_order("route_topk")
+        _first_order("route_topk", dscores)
         idx, selected, *x = ctx.saved_tensors
         shape, dtype = ctx.like
         d = dscores.to(torch.float32).contiguous()
