@@ -819,8 +819,9 @@ int mxgg_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_
 /*
  * Global norm of many gradients, sqrt(sum of g^2) in fp64, written to *norm (fp32, on the
  * device), and clipping in place: g *= min(1, max_norm / (norm + eps)).  A norm that is NaN
- * makes every gradient NaN; an infinite one makes finite gradients 0.  Tensors are fp32 or
- * bf16 of any element alignment and must not overlap.  `tensors` is host memory, read during
+ * makes every gradient NaN; an infinite one makes finite gradients 0, unless max_norm is
+ * infinite too, which clips nothing; nor does a norm of 0, whatever the bound.  Tensors are
+ * fp32 or bf16 of any element alignment and must not overlap.  `tensors` is host memory, read during
  * the call.  workspace: mxgg_grad_norm_workspace_bytes(tensors, count), 8-byte aligned, no
  * initialisation.  Two kernel launches for every 190 tensors.
  */

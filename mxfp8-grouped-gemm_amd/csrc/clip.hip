@@ -175,6 +175,9 @@ __global__ __launch_bounds__(kClipThreads) void k_clip_scale(ClipTable a, int cl
   const double norm = sqrt(group_sum(s, slots));
   if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
   if (!clip || a.count == 0) return;
+  // no factor where there is nothing to clip: an infinite bound (inf / inf), or zeros under a
+  // bound of zero (0 / 0)
+  if (norm == norm && (a.max_norm == __builtin_inf() || norm + a.eps == 0.0)) return;
   const float f = (float)(a.max_norm / (norm + a.eps));
   if (f >= 1.0f) return;  // a NaN goes on: its gradients become NaN
   const int b = (int)(gridDim.x - 1 - blockIdx.x), at = tensor_of(a, b);

@@ -183,8 +183,9 @@ def grad_norm(grads) -> torch.Tensor:
 def clip_grad_norm_(grads, max_norm: float, eps: float = 1e-6) -> torch.Tensor:
     """Scale the gradients of the list in place by min(1, max_norm / (norm + eps)), norm being
     grad_norm(grads), which is returned.  Nothing waits for the device, and where nothing is
-    clipped no gradient is written.  A norm that is NaN makes the gradients NaN, an
-    infinite one makes the finite ones 0.  The tensors may be laid out in any order of
+    clipped no gradient is written: nothing ever is where max_norm is infinite, whatever the
+    norm short of NaN.  A norm that is NaN makes the gradients NaN, an infinite one makes
+    the finite ones 0.  The tensors may be laid out in any order of
     their dimensions but must not overlap.  Parameters themselves (leaves that require
     grad, which torch's function of the name takes) are refused; the scaling is not
     recorded by autograd."""

@@ -46,3 +46,37 @@ def test_gradients_with_a_graph_are_clipped(gpu, host):
     assert abs(float(norm) - float(want.norm())) < 1e-4
     assert torch.allclose(p.grad, want * (0.5 / float(want.norm())), rtol=1e-5, atol=0)
     p.grad = None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("max_norm,eps,worst", [
+    (float("inf"), 1e-6, 2.0), (float("inf"), 1e-6, float("inf")), (float("inf"), 0.0, 0.0),
+    (float("inf"), 0.0, float("inf")), (float("inf"), float("inf"), 2.0), (0.0, 0.0, 0.0),
+    (1.0, 0.0, 0.0), (0.0, 1e-6, 0.0)])
+def test_nothing_to_clip(gpu, host, dtype, max_norm, eps, worst):
+    """An infinite bound, whatever the norm, and gradients of zero, whatever the bound:
+    the factors inf / inf and 0 / 0 do not exist, and nothing is written."""
+    grads = [torch.zeros(5000, device=gpu, dtype=dtype), torch.zeros(3, device=gpu, dtype=dtype)]
+    grads[1][1], grads[0][7] = worst, -0.0
+    if worst:
+        grads[0][100:200] = torch.linspace(-1, 1, 100)
+    before = [g.clone() for g in grads]
+    norm = mxfp8gg.clip_grad_norm_(grads, max_norm, eps)
+    assert torch.equal(norm, mxfp8gg.grad_norm(before))
+    for g, b in zip(grads, before):
+        assert torch.equal(g.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("max_norm,eps,factor", [(0.0, 0.0, 0.0), (0.0, 1e-6, 0.0),
+                                                 (2.0, float("inf"), 0.0), (2.5, 0.0, 0.5)])
+def test_extreme_bounds_of_a_finite_norm(gpu, host, max_norm, eps, factor):
+    g = torch.tensor([3.0, -4.0], device=gpu)
+    assert float(mxfp8gg.clip_grad_norm_([g], max_norm, eps)) == 5.0
+    assert g.tolist() == [3.0 * factor, -4.0 * factor]
+
+
+def test_a_nan_stays_under_an_infinite_bound(gpu, host):
+    g = [torch.ones(9, device=gpu), torch.ones(9, device=gpu, dtype=torch.bfloat16)]
+    g[0][3] = float("nan")
+    assert torch.isnan(mxfp8gg.clip_grad_norm_(g, float("inf")))
+    assert all(torch.isnan(t).all() for t in g)
