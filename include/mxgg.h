@@ -748,9 +748,12 @@ int mxgg_block_quant_weight(const void* w, int64_t num_groups, int64_t N, int64_
  *               * sum over k in b of a[m][k] w[g][n][k]        (m in group g)
  * a [M, K] and w [num_groups, N, K] e4m3 (group stride w_gstride bytes), K % 16 == 0,
  * 16-byte aligned rows; a_scales[b * ldas + m]; w_scales[g * ws_gstride + (n / 128) * ldws
- * + b].  Sums are fp32.  out bf16 or fp32 [M, N], row stride ldo elements; rows outside
- * every group are not written.  group_ends NULL: one group (num_groups = 1).  Products of
- * few tiles are split along K and added in a fixed order: workspace of
+ * + b].  Sums are fp32, but for those of eight consecutive products inside the matrix
+ * instruction, which are cut 13 bits below the largest of the eight: at most 7 * 2^-13 of the
+ * sum of magnitudes, 2e-5 of the result in the root mean square of normal data.  out bf16 or
+ * fp32 [M, N], row stride ldo elements; rows outside every group are not written.
+ * group_ends NULL: one group (num_groups = 1).  Products of few tiles are split along K and
+ * added in a fixed order: workspace of
  * mxgg_block_mm_workspace_bytes(group_ends != NULL, ...) bytes for the current device
  * (0 for most sizes), 16-byte aligned, no initialisation.
  */
@@ -767,8 +770,8 @@ int mxgg_block_mm(const void* a, int64_t lda, const float* a_scales, int64_t lda
  * of dY[t][n] X[t][k], from the transposed payloads go_t [N, tokens] and ia_t [K, tokens]
  * and their scales as mxgg_block_quant_dim1 writes them.  group_ends_pad: padded ends
  * (multiples of 128; others are rounded down), NULL for one group; tokens % 128 == 0.
- * dw bf16 or fp32 [num_groups, N, K], contiguous; empty groups are written as zeros.
- * workspace: as mxgg_block_mm's, for sums split along the tokens.
+ * Sums as mxgg_block_mm's.  dw bf16 or fp32 [num_groups, N, K], contiguous; empty groups are
+ * written as zeros.  workspace: as mxgg_block_mm's, for sums split along the tokens.
  */
 int64_t mxgg_block_wgrad_workspace_bytes(int grouped, int64_t num_groups, int64_t tokens, int64_t N,
                                          int64_t K);
