@@ -21,9 +21,13 @@
 // first fragment's end, takes its loads behind a second barrier half a stage earlier.
 //
 // Bound by the matrix unit's share of the cycles and, in long runs, by power: 16384 x 4096
-// x 7168 393-397 us (2420-2450 TFLOP/s; the library's product with one scale a tensor
-// 2630), 8192^3 431-450 us (2440-2550), weight gradient of 8192^3 521-550 us (2000-2110).
-// 32 uneven groups of 16384 tokens (4096 x 7168) 571-600 us: part-filled tiles.
+// x 7168 378-397 us (2420-2550 TFLOP/s; the library's product with one scale a tensor
+// 2630), 8192^3 425-450 us (2440-2580), weight gradient of 8192^3 521-550 us (2000-2110).
+// 16384 tokens in 32 uneven groups (4096 x 7168): part-filled tiles, 497 us where the groups
+// make 79 row tiles of 256 and 530-557 where they make 81 to 83.  Weight gradient of such
+// groups 1135 us (850 TFLOP/s): four blocks of 128 tokens a group on the average, and 1.9 GB
+// of bf16 results.  Few rows of many groups are not split along K: one row 26 us, a row for
+// each of 8 groups 41, of 32 163 (5.8 TB/s of weights).
 #include <algorithm>
 #include <utility>
 
@@ -418,8 +422,8 @@ __device__ __forceinline__ void block_store(const v4f (&acc)[4 * GP][FQ], O* out
 // Tile of this workgroup: tiles of group g are ceil(size / q) * np, in group order;
 // consecutive workgroups go to the XCDs in turn, and each XCD takes runs of eight tiles, so
 // that groups' part-filled tiles are dealt out evenly (16384 tokens of 32 uneven experts: an
-// eighth of the tiles in one run 590 us, runs of eight 575).  g = E for a workgroup past
-// the last tile.
+// eighth of the tiles in one run 590 us, runs of eight 575, both while rows of the next group
+// were still fetched).  g = E for a workgroup past the last tile.
 constexpr uint32_t kXcdRun = 8;
 struct GroupTile {
   int g;
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void k_block_fwd(BlockMmArgs a) {
                        a.ws + at.g * a.ws_group + n0 / kBlkK * a.ldws + k.first, a.ldw, a.ldws,
                        a.N - n0};
   // rows of the next group read as zero: nothing to fetch, less power (16384 tokens of 32
-  // uneven groups 509 -> 501 us, 512 tokens 188 -> 167)
+  // uneven groups, 80 row tiles, 509 -> 501 us, 512 tokens 188 -> 167)
   const BlockOperand Q{a.a + m0 * a.lda + k.first * kBlkK, a.as + m0 + k.first * a.ldas, a.lda,
                        a.ldas, at.end - m0};
   v4f acc[4 * GP][FQ];

@@ -3,16 +3,18 @@
 //   norm = sqrt(sum over all tensors of g^2),  g <- g min(1, max_norm / (norm + eps))
 //
 // Two passes.  The first leaves one sum of squares a workgroup; squares and sums are
-// fp64 (exact for fp32 and bf16 values: no overflow at 1e19, nothing lost below 1e-23),
-// which the vector units do many times faster than memory delivers.  In the second
+// fp64, which the vector units do many times faster than memory delivers: a square of an
+// fp32 or bf16 value is exact (48 bits; no overflow at 1e19, nothing lost below 1e-23), and
+// each addition rounds to 2^-53, so the norm is the fp32 rounding of the true one but next
+// to a border between two.  In the second
 // every workgroup adds all of the partial sums in the same order, so the factor is the
 // same in each and from run to run, and ends without touching its gradients where
 // nothing is clipped.
 //
 // Memory-bound: each gradient is read twice and written once.  The second pass goes
 // through the tensors backwards and finds what the first read last in the cache.  235 M
-// bf16 gradients: 89-101 us (4.7-5.3 TB/s) and 146 (6.4, part of it from the cache); fp32
-// 163 us (5.8) for the norm.
+// bf16 gradients: 85-101 us (4.7-5.5 TB/s) and 146 (6.4, part of it from the cache); fp32
+// 163-165 us (5.8) for the norm.
 #include <algorithm>
 
 #include "mx_device.h"
